@@ -34,7 +34,9 @@ HIP_SOURCES = [
     "spmm_rowscalar.hip",
     "preprocess.hip",
     "preprocess_windows.hip",
+    "layer_norm.hip",
 ]
+EXT_SOURCES = ["custom_op.cpp", "dense_ops.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # Packed-FP32 instructions (v_pk_*_f32) are disabled for all device code:
@@ -90,17 +92,27 @@ def build_extension() -> str:
         "/opt/rocm/include",
     ]
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    tmp = EXTENSION + ".tmp"
-    cmd = [
-        "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+    flags = [
+        "-O2", "-std=c++17", "-fPIC",
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
         "-DTORCH_EXTENSION_NAME=custom_ops_lib",
         "-DTORCH_API_INCLUDE_EXTENSION_H",
         "-D__HIP_PLATFORM_AMD__=1",
         "-DUSE_ROCM=1",
         *[f"-I{p}" for p in includes],
-        os.path.join(CSRC, "torch_ext", "custom_op.cpp"),
-        "-o", tmp,
+    ]
+
+    def compile_one(src: str) -> str:
+        obj = os.path.join(BUILD, "ext_" + os.path.splitext(src)[0] + ".o")
+        _run(["g++", *flags, "-c", os.path.join(CSRC, "torch_ext", src), "-o", obj])
+        return obj
+
+    os.makedirs(BUILD, exist_ok=True)
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(EXT_SOURCES)) as pool:
+        objs = list(pool.map(compile_one, EXT_SOURCES))
+    tmp = EXTENSION + ".tmp"
+    cmd = [
+        "g++", "-shared", *objs, "-o", tmp,
         f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
         f"-L{HERE}", "-lspmm_mi355x",
         "-Wl,-rpath,$ORIGIN",

@@ -7,26 +7,16 @@
 // its tensors, allocates the output on the tensor's device and calls the C ABI
 // of libspmm_mi355x.so on the current HIP stream.  There is no host compute
 // path: tensors that are not on a GPU are rejected.
-#include <torch/extension.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
+#include "ext_common.h"
 
 #include <map>
-#include <stdexcept>
-#include <string>
 
 #include <ATen/hip/HIPContext.h>
-
-#include "../../../include/spmm_mi355x.h"
 
 namespace {
 
 constexpr int64_t kSpmmHalfMaxDenseWidth = 1024;
 constexpr int64_t kSpmmFloatMaxDenseWidth = 512;
-
-inline bool is_gpu(const at::Tensor& tensor) { return tensor.device().is_cuda(); }
-#define TORCH_CHECK_GPU(tensor) \
-  TORCH_CHECK(is_gpu(tensor), #tensor " must be a GPU tensor (MI355X build; reference: NPU tensor)")
 
 // Same checks and messages as the reference (extension/custom_op.cpp:39-64).
 void check_dense_contract(const at::Tensor& dense, int64_t alignment, const char* op_name) {
@@ -50,33 +40,8 @@ void check_value_contract(const at::Tensor& value, const at::Tensor& dense, cons
   TORCH_CHECK(value.is_contiguous(), name, " must be contiguous");
 }
 
-int32_t index_type_of(const at::Tensor& t, const char* name) {
-  if (t.scalar_type() == at::kInt) return SPMM_INDEX_I32;
-  if (t.scalar_type() == at::kLong) return SPMM_INDEX_I64;
-  TORCH_CHECK(false, name, " must be an int32 or int64 tensor, but got ", t.scalar_type());
-  return -1;
-}
-
 int32_t value_type_of(const at::Tensor& dense) {
   return dense.scalar_type() == at::kHalf ? SPMM_VALUE_F16 : SPMM_VALUE_F32;
-}
-
-// Maps a library status to the exception type the reference raises for the
-// same condition (pybind11 turns these into ValueError / IndexError /
-// OverflowError / RuntimeError).
-void raise_status(spmm_status st, const char* what) {
-  if (st == SPMM_OK) return;
-  const std::string msg = std::string(what) + ": " + spmm_last_error();
-  switch (st) {
-    case SPMM_ERR_INVALID_ARGUMENT: throw std::invalid_argument(msg);
-    case SPMM_ERR_OUT_OF_RANGE: throw std::out_of_range(msg);
-    case SPMM_ERR_OVERFLOW: throw std::overflow_error(msg);
-    default: TORCH_CHECK(false, msg);
-  }
-}
-
-spmm_stream current_stream(const at::Tensor& t) {
-  return reinterpret_cast<spmm_stream>(c10::hip::getCurrentHIPStream(t.device().index()).stream());
 }
 
 void check_same_device(const at::Tensor& a, const at::Tensor& b, const char* name) {
@@ -87,10 +52,6 @@ void check_same_device(const at::Tensor& a, const at::Tensor& b, const char* nam
 // that is not a multiple of 16 bytes is copied.
 at::Tensor aligned(const at::Tensor& t) {
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone();
-}
-
-at::Tensor workspace(const at::Tensor& like, size_t bytes) {
-  return at::empty({static_cast<int64_t>(bytes > 0 ? bytes : 1)}, like.options().dtype(at::kByte));
 }
 
 }  // namespace
@@ -656,5 +617,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "Split CSR into (16,1)-BSR + CSR hybrid dict by block density (GPU)");
   m.def("pack_rows", &pack_rows, "packed[inv[i]] = tensor[i]; other rows zero (GPU)");
   m.def("restore_rows", &restore_rows, "out[i] = packed[inv[i]] (GPU)");
+  bind_dense_ops(m);
   m.def("library_version", []() { return std::string(spmm_version()); });
 }

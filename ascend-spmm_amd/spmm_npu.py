@@ -23,6 +23,7 @@ from custom_ops_lib import (  # noqa: E402
     block_level_split,
     csr_to_ascend_cube,
     csr_to_bcsr,
+    layer_norm,
     pack_rows as _pack_rows,
     preprocess,
     restore_rows as _restore_rows,
@@ -201,6 +202,7 @@ __all__ = [
     "block_level_split",
     "csr_to_ascend_cube",
     "csr_to_bcsr",
+    "layer_norm",
     "make_start",
     "pack_node_tensor",
     "preprocess",

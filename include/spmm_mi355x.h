@@ -49,7 +49,13 @@ typedef enum spmm_status {
 } spmm_status;
 
 typedef enum spmm_index_type { SPMM_INDEX_I32 = 0, SPMM_INDEX_I64 = 1 } spmm_index_type;
-typedef enum spmm_value_type { SPMM_VALUE_F16 = 0, SPMM_VALUE_F32 = 1, SPMM_VALUE_F64 = 2 } spmm_value_type;
+/* BF16: the dense operators only (layer norm, grouped products, orthogonalised updates). */
+typedef enum spmm_value_type {
+  SPMM_VALUE_F16 = 0,
+  SPMM_VALUE_F32 = 1,
+  SPMM_VALUE_F64 = 2,
+  SPMM_VALUE_BF16 = 3
+} spmm_value_type;
 
 /* Opaque HIP stream (hipStream_t); NULL is the default stream. */
 typedef void* spmm_stream;
@@ -405,6 +411,43 @@ spmm_status spmm_taskmap_fill_record(const spmm_csr_matrix* m, int64_t window_si
  * estimated aic, aiv and max cost. */
 spmm_status spmm_taskmap_scalars(const spmm_taskmap_info* info, int64_t* const* ints,
                                  double* const* doubles, spmm_stream stream);
+
+/* ------------------------------------------------------------------------
+ * Dense operators of a graph layer with typed nodes, for training on the
+ * graphs that the operators above multiply with.  No counterpart in the
+ * reference.  Values are F16, BF16 or F32; every sum is held in fp32 or more
+ * and each output is rounded once.  Row strides are in elements, the last
+ * dimension is contiguous, and no alignment beyond the element's is required.
+ * ---------------------------------------------------------------------- */
+
+/* layer_norm: y = (x - mean) * rstd * weight + bias over each row of x, with
+ * rstd = 1 / sqrt(var + eps) and the biased variance.  weight and bias hold
+ * `width` values of param_type (value_type or F32); NULL stands for 1 and 0.
+ * mean and rstd (fp32, one per row) are written where not NULL; the gradient
+ * takes them. */
+typedef struct spmm_norm_desc {
+  int64_t rows;
+  int64_t width;
+  int64_t x_stride;     /* elements between rows of x                      */
+  int64_t grad_stride;  /* elements between rows of grad (gradient only)   */
+  double eps;
+  int32_t value_type;   /* x, y, grad, dx                                  */
+  int32_t param_type;   /* weight, bias, dweight, dbias                    */
+} spmm_norm_desc;
+
+spmm_status spmm_layer_norm_run(const spmm_norm_desc* desc, const void* x, const void* weight,
+                                const void* bias, void* y, float* mean, float* rstd,
+                                spmm_stream stream);
+
+/* Gradient of layer_norm with respect to x, weight and bias, from the
+ * incoming gradient `grad` and the forward call's mean and rstd; each of dx,
+ * dweight and dbias may be NULL.  The sums over rows are added in an order
+ * that depends on the sizes alone, so results repeat exactly. */
+spmm_status spmm_layer_norm_grad_workspace(const spmm_norm_desc* desc, size_t* bytes);
+spmm_status spmm_layer_norm_grad_run(const spmm_norm_desc* desc, const void* x, const void* weight,
+                                     const float* mean, const float* rstd, const void* grad,
+                                     void* dx, void* dweight, void* dbias, void* workspace,
+                                     size_t workspace_bytes, spmm_stream stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */
