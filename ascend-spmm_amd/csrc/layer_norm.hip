@@ -7,6 +7,7 @@
 // which keeps its digits where the mean is large against the spread.
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "numeric.h"
 
@@ -14,6 +15,10 @@ namespace spmm {
 namespace {
 
 constexpr int kThreads = 256;
+
+// Most work-groups of the register kernels: two of four waves per CU.  Each
+// leaves one row of partial sums of the parameters' gradients.
+constexpr int64_t kNormGroups = 512;
 
 struct NormArgs {
   int64_t rows, width, x_stride, grad_stride;
@@ -62,13 +67,209 @@ __device__ inline void block_sum(float (&v)[K]) {
   }
 }
 
-// One work-group per row, the row read once per statistic.
+// Sums of K values over the L lanes that share a row: a part of a wave, or
+// the whole work-group.
+template <int L, int K>
+__device__ inline void row_sum(float (&v)[K]) {
+  if constexpr (L > 64) {
+    block_sum(v);
+  } else {
+#pragma unroll
+    for (int d = L / 2; d > 0; d >>= 1)
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], d);
+  }
+}
+
+// The register kernels.  L lanes share a row (threads / L rows of a
+// work-group at once) and each holds I pieces of 16 bytes of it, so x (and
+// grad) is read once.  A group walks rows a grid apart and loads the next
+// row's pieces before it reduces the current one.
+template <typename T, int L, int I>
+struct RowTile {
+  static constexpr int V = kPiece<T>;
+  static constexpr int kBlock = L > kThreads ? L : kThreads;
+  static constexpr int kGroups = kBlock / L;
+
+  __device__ static inline int64_t column(int i) { return static_cast<int64_t>((i * L + threadIdx.x % L)) * V; }
+
+  __device__ static inline void load(const T* row, int64_t width, float (&v)[I][V]) {
+#pragma unroll
+    for (int i = 0; i < I; ++i) load_piece(row + column(i), width - column(i), v[i]);
+  }
+};
+
+template <typename T, int L, int I>
+__global__ __launch_bounds__((RowTile<T, L, I>::kBlock)) void norm_forward(NormArgs a, const T* __restrict__ x,
+                                                                           const void* __restrict__ w,
+                                                                           const void* __restrict__ b,
+                                                                           T* __restrict__ y, float* mean, float* rstd) {
+  using Tile = RowTile<T, L, I>;
+  constexpr int V = Tile::V;
+  const float count = static_cast<float>(a.width);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * Tile::kGroups;
+  int64_t r = static_cast<int64_t>(blockIdx.x) * Tile::kGroups + threadIdx.x / L;
+  float wv[I][V], bv[I][V], next[I][V];
+  if (r < a.rows) Tile::load(x + r * a.x_stride, a.width, next);
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    load_param<T>(w, a.param_f32, Tile::column(i), a.width, 1.0f, wv[i]);
+    load_param<T>(b, a.param_f32, Tile::column(i), a.width, 0.0f, bv[i]);
+  }
+  // Groups of a work-group stay together (block_sum's barriers).
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * Tile::kGroups; r0 < a.rows; r0 += step, r += step) {
+    float v[I][V], s[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[i][j] = next[i][j];
+    if (r + step < a.rows) Tile::load(x + (r + step) * a.x_stride, a.width, next);
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[0] += v[i][j];
+    row_sum<L>(s);
+    const float m = s[0] / count;
+    s[0] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        v[i][j] = Tile::column(i) + j < a.width ? v[i][j] - m : 0.0f;
+        s[0] += v[i][j] * v[i][j];
+      }
+    row_sum<L>(s);
+    const float rs = 1.0f / sqrtf(s[0] / count + a.eps);
+    if (r >= a.rows) continue;
+    if (threadIdx.x % L == 0 && mean != nullptr) mean[r] = m;
+    if (threadIdx.x % L == 0 && rstd != nullptr) rstd[r] = rs;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[i][j] = v[i][j] * rs * wv[i][j] + bv[i][j];
+      store_piece(y + r * a.width + Tile::column(i), a.width - Tile::column(i), v[i]);
+    }
+  }
+}
+
+// dx of each row, and the column sums of dy z and dy over the rows of the
+// work-group: part[group][2][width].
+template <typename T, int L, int I>
+__global__ __launch_bounds__((RowTile<T, L, I>::kBlock)) void norm_backward(NormArgs a, const T* __restrict__ x,
+                                                                            const void* __restrict__ w,
+                                                                            const float* __restrict__ mean,
+                                                                            const float* __restrict__ rstd,
+                                                                            const T* __restrict__ grad,
+                                                                            T* __restrict__ dx, float* part) {
+  using Tile = RowTile<T, L, I>;
+  constexpr int V = Tile::V;
+  const float count = static_cast<float>(a.width);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * Tile::kGroups;
+  int64_t r = static_cast<int64_t>(blockIdx.x) * Tile::kGroups + threadIdx.x / L;
+  float wv[I][V], dw[I][V] = {}, db[I][V] = {}, nx[I][V], ng[I][V], nm = 0.0f, nrs = 0.0f;
+  auto fetch = [&](int64_t row) {
+    Tile::load(x + row * a.x_stride, a.width, nx);
+    Tile::load(grad + row * a.grad_stride, a.width, ng);
+    nm = mean[row];
+    nrs = rstd[row];
+  };
+  if (r < a.rows) fetch(r);
+#pragma unroll
+  for (int i = 0; i < I; ++i) load_param<T>(w, a.param_f32, Tile::column(i), a.width, 1.0f, wv[i]);
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * Tile::kGroups; r0 < a.rows; r0 += step, r += step) {
+    float z[I][V], g[I][V], s[2] = {0.0f, 0.0f};
+    const float m = nm, rs = nrs;
+    const bool live = r < a.rows;
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        z[i][j] = nx[i][j];
+        g[i][j] = ng[i][j];
+      }
+    if (r + step < a.rows) fetch(r + step);
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const bool in = Tile::column(i) + j < a.width;
+          z[i][j] = in ? (z[i][j] - m) * rs : 0.0f;
+          dw[i][j] += g[i][j] * z[i][j];
+          db[i][j] += g[i][j];
+          g[i][j] = in ? g[i][j] * wv[i][j] : 0.0f;
+          s[0] += g[i][j];
+          s[1] += g[i][j] * z[i][j];
+        }
+    }
+    if (dx == nullptr) continue;
+    row_sum<L>(s);
+    if (!live) continue;
+    const float g0 = s[0] / count, g1 = s[1] / count;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) g[i][j] = rs * (g[i][j] - g0 - z[i][j] * g1);
+      store_piece(dx + r * a.width + Tile::column(i), a.width - Tile::column(i), g[i]);
+    }
+  }
+  if (part == nullptr) return;
+  // The work-group's groups in turn: within a wave by lane exchange, then the
+  // waves through LDS.
+  float* p = part + static_cast<int64_t>(blockIdx.x) * 2 * a.width;
+  if constexpr (L <= 64) {
+    constexpr int W = Tile::kBlock / 64;
+    __shared__ float lds[W][2][64 * V];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+#pragma unroll
+        for (int d = L; d < 64; d <<= 1) {
+          dw[i][j] += __shfl_xor(dw[i][j], d);
+          db[i][j] += __shfl_xor(db[i][j], d);
+        }
+      }
+      __syncthreads();
+      if (lane < L)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          lds[wave][0][lane * V + j] = dw[i][j];
+          lds[wave][1][lane * V + j] = db[i][j];
+        }
+      __syncthreads();
+      for (int k = threadIdx.x; k < 2 * L * V; k += Tile::kBlock) {
+        const int which = k / (L * V), c = k % (L * V);
+        const int64_t col = static_cast<int64_t>(i) * L * V + c;
+        float sum = 0.0f;
+#pragma unroll
+        for (int q = 0; q < W; ++q) sum += lds[q][which][c];
+        if (col < a.width) p[which * a.width + col] = sum;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int64_t col = Tile::column(i) + j;
+        if (col < a.width) {
+          p[col] = dw[i][j];
+          p[a.width + col] = db[i][j];
+        }
+      }
+  }
+}
+
+// Wider rows than the registers of a work-group hold: one work-group per row,
+// the row read once per statistic.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void norm_forward_wide(NormArgs a, const T* __restrict__ x,
                                                               const void* __restrict__ w, const void* __restrict__ b,
                                                               T* __restrict__ y, float* mean, float* rstd) {
   constexpr int V = kPiece<T>;
-  const float inv = 1.0f / static_cast<float>(a.width);
+  const float count = static_cast<float>(a.width);
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* xr = x + r * a.x_stride;
     float s[1] = {0.0f};
@@ -79,7 +280,7 @@ __global__ __launch_bounds__(kThreads) void norm_forward_wide(NormArgs a, const 
       for (int i = 0; i < V; ++i) s[0] += v[i];
     }
     block_sum(s);
-    const float m = s[0] * inv;
+    const float m = s[0] / count;
     s[0] = 0.0f;
     for (int64_t c = threadIdx.x * V; c < a.width; c += kThreads * V) {
       float v[V];
@@ -89,7 +290,7 @@ __global__ __launch_bounds__(kThreads) void norm_forward_wide(NormArgs a, const 
         if (c + i < a.width) s[0] += (v[i] - m) * (v[i] - m);
     }
     block_sum(s);
-    const float rs = 1.0f / sqrtf(s[0] * inv + a.eps);
+    const float rs = 1.0f / sqrtf(s[0] / count + a.eps);
     if (threadIdx.x == 0 && mean != nullptr) mean[r] = m;
     if (threadIdx.x == 0 && rstd != nullptr) rstd[r] = rs;
     for (int64_t c = threadIdx.x * V; c < a.width; c += kThreads * V) {
@@ -112,7 +313,7 @@ __global__ __launch_bounds__(kThreads) void norm_backward_wide(NormArgs a, const
                                                                const float* __restrict__ rstd,
                                                                const T* __restrict__ grad, T* __restrict__ dx) {
   constexpr int V = kPiece<T>;
-  const float inv = 1.0f / static_cast<float>(a.width);
+  const float count = static_cast<float>(a.width);
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* xr = x + r * a.x_stride;
     const T* gr = grad + r * a.grad_stride;
@@ -131,7 +332,7 @@ __global__ __launch_bounds__(kThreads) void norm_backward_wide(NormArgs a, const
         }
     }
     block_sum(s);
-    const float g0 = s[0] * inv, g1 = s[1] * inv;
+    const float g0 = s[0] / count, g1 = s[1] / count;
     for (int64_t c = threadIdx.x * V; c < a.width; c += kThreads * V) {
       float v[V], d[V], wv[V];
       load_piece(xr + c, a.width - c, v);
@@ -221,9 +422,54 @@ NormArgs norm_args(const spmm_norm_desc* d) {
   return {d->rows, d->width, d->x_stride, d->grad_stride, static_cast<float>(d->eps), d->param_type == SPMM_VALUE_F32};
 }
 
+// Calls f(L, I) with the lanes per row and pieces per lane for rows of
+// `width`: the fewest lanes that hold the row in one piece each, then up to
+// four pieces each of a wave, 256 and 1024 threads.  False where the row is
+// wider than that.
+template <typename T, typename F>
+bool with_tile(int64_t width, F f) {
+  const int64_t pieces = ceil_div(width, kPiece<T>);
+#define SPMM_TILE(L, I) \
+  if (pieces <= (L) * (I)) return f(std::integral_constant<int, L>(), std::integral_constant<int, I>()), true
+  SPMM_TILE(8, 1);
+  SPMM_TILE(16, 1);
+  SPMM_TILE(32, 1);
+  SPMM_TILE(64, 1);
+  SPMM_TILE(64, 2);
+  SPMM_TILE(64, 4);
+  SPMM_TILE(256, 2);
+  SPMM_TILE(256, 4);
+  SPMM_TILE(1024, 2);
+  SPMM_TILE(1024, 4);
+#undef SPMM_TILE
+  return false;
+}
+
+int64_t tile_groups(int64_t width, int64_t piece) {
+  const int64_t pieces = ceil_div(width, piece);
+  for (int64_t lanes = 8; lanes <= 64; lanes *= 2)
+    if (pieces <= lanes) return kThreads / lanes;
+  return pieces <= 256 ? kThreads / 64 : 1;
+}
+
+// Work-groups of the backward kernel: each has four rows per group at least,
+// so that its partial sums cost little against its rows.
+int64_t backward_blocks(int64_t rows, int64_t groups) {
+  const int64_t want = ceil_div(rows, 4 * groups);
+  return want < kNormGroups ? want : kNormGroups;
+}
+
 template <typename T>
 spmm_status run_forward(const spmm_norm_desc* d, const void* x, const void* w, const void* b, void* y, float* mean,
                         float* rstd, hipStream_t s) {
+  const bool tiled = with_tile<T>(d->width, [&](auto L, auto I) {
+    using Tile = RowTile<T, decltype(L)::value, decltype(I)::value>;
+    const int64_t blocks = ceil_div(d->rows, Tile::kGroups), most = 4 * kNormGroups;
+    hipLaunchKernelGGL((norm_forward<T, decltype(L)::value, decltype(I)::value>),
+                       dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(Tile::kBlock), 0, s,
+                       norm_args(d), static_cast<const T*>(x), w, b, static_cast<T*>(y), mean, rstd);
+  });
+  if (tiled) return check_launch("layer_norm");
   hipLaunchKernelGGL(norm_forward_wide<T>, dim3(row_blocks(d->rows)), dim3(kThreads), 0, s, norm_args(d),
                      static_cast<const T*>(x), w, b, static_cast<T*>(y), mean, rstd);
   return check_launch("layer_norm");
@@ -235,13 +481,23 @@ spmm_status run_backward(const spmm_norm_desc* d, const void* x, const void* w, 
   const NormArgs a = norm_args(d);
   const T *tx = static_cast<const T*>(x), *tg = static_cast<const T*>(grad);
   int64_t chunks = 0;
-  if (d->rows > 0 && dx != nullptr) {
+  const bool sums = dw != nullptr || db != nullptr;
+  const bool tiled = d->rows > 0 && with_tile<T>(d->width, [&](auto L, auto I) {
+    using Tile = RowTile<T, decltype(L)::value, decltype(I)::value>;
+    chunks = backward_blocks(d->rows, Tile::kGroups);
+    hipLaunchKernelGGL((norm_backward<T, decltype(L)::value, decltype(I)::value>),
+                       dim3(static_cast<unsigned>(chunks)), dim3(Tile::kBlock), 0, s, a, tx, w, mean, rstd, tg,
+                       static_cast<T*>(dx), sums ? part : nullptr);
+  });
+  if (tiled)
+    if (spmm_status st = check_launch("layer_norm_grad")) return st;
+  if (!tiled && d->rows > 0 && dx != nullptr) {
     hipLaunchKernelGGL(norm_backward_wide<T>, dim3(row_blocks(d->rows)), dim3(kThreads), 0, s, a, tx, w, mean, rstd,
                        tg, static_cast<T*>(dx));
     if (spmm_status st = check_launch("layer_norm_grad")) return st;
   }
-  if (dw == nullptr && db == nullptr) return SPMM_OK;
-  if (d->rows > 0) {
+  if (!sums) return SPMM_OK;
+  if (!tiled && d->rows > 0) {
     const int64_t chunk = ceil_div(d->rows, column_chunks(d->rows, d->width));
     chunks = ceil_div(d->rows, chunk);
     hipLaunchKernelGGL(norm_columns_wide<T>,
@@ -260,7 +516,11 @@ spmm_status run_backward(const spmm_norm_desc* d, const void* x, const void* w, 
 }
 
 size_t grad_workspace_bytes(const spmm_norm_desc* d) {
-  return static_cast<size_t>(column_chunks(d->rows, d->width)) * 2 * static_cast<size_t>(d->width) * sizeof(float);
+  const int64_t piece = 16 / dense_type_bytes(d->value_type);
+  const bool tiled = ceil_div(d->width, piece) <= 4096;  // the widest tile
+  const int64_t chunks = tiled ? backward_blocks(d->rows, tile_groups(d->width, piece))
+                               : column_chunks(d->rows, d->width);
+  return static_cast<size_t>(chunks) * 2 * static_cast<size_t>(d->width) * sizeof(float);
 }
 
 }  // namespace
@@ -301,9 +561,9 @@ spmm_status spmm_layer_norm_grad_run(const spmm_norm_desc* d, const void* x, con
   if (dx == nullptr && dweight == nullptr && dbias == nullptr) return SPMM_OK;
   if (d->rows > 0 && (x == nullptr || mean == nullptr || rstd == nullptr || grad == nullptr))
     return fail(SPMM_ERR_INVALID_ARGUMENT, "layer_norm: null device pointer");
-  if ((dweight != nullptr || dbias != nullptr) && (workspace == nullptr || workspace_bytes < grad_workspace_bytes(d)))
-    return fail(SPMM_ERR_CONTRACT, "layer_norm: workspace too small: need " + std::to_string(grad_workspace_bytes(d)) +
-                                       " bytes");
+  const size_t need = dweight != nullptr || dbias != nullptr ? grad_workspace_bytes(d) : 0;
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(SPMM_ERR_CONTRACT, "layer_norm: workspace too small: need " + std::to_string(need) + " bytes");
   float* part = static_cast<float*>(workspace);
   hipStream_t s = as_stream(stream);
   switch (d->value_type) {
