@@ -35,6 +35,7 @@ HIP_SOURCES = [
     "preprocess.hip",
     "preprocess_windows.hip",
     "layer_norm.hip",
+    "grouped_matmul.hip",
 ]
 EXT_SOURCES = ["custom_op.cpp", "dense_ops.cpp"]
 

@@ -1,5 +1,5 @@
 // The dense operators of a graph layer with typed nodes, as differentiable
-// torch operators over the C ABI: layer_norm.  They check their tensors,
+// torch operators over the C ABI: layer_norm and grouped_matmul.  They check their tensors,
 // allocate outputs and workspace on the tensors' device and launch on its
 // current stream.  Gradients are not differentiable themselves.
 #include "ext_common.h"
@@ -26,11 +26,14 @@ int32_t dense_type_of(const at::Tensor& t, const char* op) {
 // evenly apart, else a copy.
 at::Tensor as_rows(const at::Tensor& t) {
   const int64_t width = t.size(-1);
+  if (t.dim() == 2 && t.numel() == 0) return t;
   if (t.dim() == 2 && (t.stride(1) == 1 || width == 1) && (t.stride(0) >= width || t.size(0) <= 1)) return t;
-  return t.contiguous().view({width > 0 ? t.numel() / width : 0, width});
+  return t.contiguous().view({t.numel() / width, width});
 }
 
-int64_t row_stride(const at::Tensor& rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+int64_t row_stride(const at::Tensor& rows) {
+  return rows.size(0) > 1 && rows.numel() > 0 ? rows.stride(0) : rows.size(1);
+}
 
 bool wants_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 bool wants_grad(const c10::optional<at::Tensor>& t) { return t.has_value() && wants_grad(*t); }
@@ -133,10 +136,107 @@ at::Tensor layer_norm(const at::Tensor& x, const c10::optional<at::Tensor>& weig
   return layer_norm_forward(x, weight, bias, eps, false, nullptr, nullptr);
 }
 
+// ---------------------------------------------------------- grouped_matmul
+
+// weight [groups, inner, width] whose matrices are contiguous, either as they
+// are or transposed; a copy where they are neither.
+at::Tensor grouped_weight(const at::Tensor& w, bool* transposed) {
+  const int64_t k = w.size(1), n = w.size(2);
+  const bool apart = w.size(0) <= 1 || w.stride(0) >= k * n;
+  *transposed = false;
+  if (apart && (w.stride(2) == 1 || n <= 1) && (w.stride(1) == n || k <= 1)) return w;
+  if (apart && (w.stride(1) == 1 || k <= 1) && (w.stride(2) == k || n <= 1)) {
+    *transposed = true;
+    return w;
+  }
+  return w.contiguous();
+}
+
+void check_grouped(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& offsets) {
+  TORCH_CHECK_GPU(x);
+  TORCH_CHECK_GPU(weight);
+  TORCH_CHECK_GPU(offsets);
+  TORCH_CHECK(x.dim() == 2, "grouped_matmul: x must be a 2D Tensor, but got: ", x.dim());
+  TORCH_CHECK(weight.dim() == 3, "grouped_matmul: weight must be a 3D Tensor, but got: ", weight.dim());
+  TORCH_CHECK(offsets.dim() == 1, "grouped_matmul: offsets must be a 1D Tensor, but got: ", offsets.dim());
+  dense_type_of(x, "grouped_matmul");
+  TORCH_CHECK(weight.scalar_type() == x.scalar_type(), "grouped_matmul: weight must have the dtype of x");
+  TORCH_CHECK(weight.size(1) == x.size(1), "grouped_matmul: x has ", x.size(1), " columns, but weight takes ",
+              weight.size(1));
+  TORCH_CHECK(offsets.size(0) == weight.size(0) + 1, "grouped_matmul: offsets must hold one entry more than weight has "
+              "matrices (", weight.size(0) + 1, "), but got ", offsets.size(0));
+  index_type_of(offsets, "offsets");
+  TORCH_CHECK(weight.device() == x.device() && offsets.device() == x.device(),
+              "grouped_matmul: weight and offsets must be on the same device as x");
+}
+
+spmm_grouped_desc grouped_desc(const at::Tensor& rows, const at::Tensor& weight, bool transposed,
+                               const at::Tensor& offsets) {
+  const int64_t k = weight.size(1), n = weight.size(2);
+  return {rows.size(0), weight.size(0), k, n, row_stride(rows), n, weight.size(0) > 1 ? weight.stride(0) : k * n,
+          transposed ? 1 : 0, index_type_of(offsets, "offsets"), dense_type_of(rows, "grouped_matmul")};
+}
+
+at::Tensor grouped_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& offsets) {
+  c10::DeviceGuard guard(x.device());
+  bool transposed;
+  const at::Tensor rows = as_rows(x), w = grouped_weight(weight, &transposed), off = offsets.contiguous();
+  const spmm_grouped_desc d = grouped_desc(rows, w, transposed, off);
+  at::Tensor out = at::empty({d.rows, d.width}, x.options());
+  size_t bytes = 0;
+  raise_status(spmm_grouped_workspace(&d, &bytes), "grouped_matmul");
+  at::Tensor ws = workspace(x, bytes);
+  raise_status(spmm_grouped_run(&d, rows.data_ptr(), w.data_ptr(), off.data_ptr(), out.data_ptr(), ws.data_ptr(), bytes,
+                                current_stream(x)),
+               "grouped_matmul");
+  return out;
+}
+
+struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
+                            const at::Tensor& offsets) {
+    ctx->save_for_backward({x, weight, offsets});
+    return grouped_forward(x, weight, offsets);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "grouped_matmul: its gradient is not differentiable");
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &weight = saved[1];
+    c10::DeviceGuard guard(x.device());
+    bool transposed;
+    const at::Tensor rows = as_rows(x), grad = as_rows(grads[0]), w = grouped_weight(weight, &transposed);
+    const at::Tensor off = saved[2].contiguous();
+    spmm_grouped_desc d = grouped_desc(rows, w, transposed, off);
+    d.grad_stride = row_stride(grad);
+    at::Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) dx = at::empty(x.sizes(), x.options());
+    // In weight's storage order, as its gradient is added to it.
+    if (ctx->needs_input_grad(1))
+      dw = transposed ? at::empty({d.groups, d.width, d.inner}, x.options()).transpose(1, 2)
+                      : at::empty({d.groups, d.inner, d.width}, x.options());
+    size_t bytes = 0;
+    raise_status(spmm_grouped_grad_workspace(&d, &bytes), "grouped_matmul");
+    at::Tensor ws = workspace(x, bytes);
+    raise_status(spmm_grouped_grad_run(&d, rows.data_ptr(), w.data_ptr(), off.data_ptr(), grad.data_ptr(),
+                                       dx.defined() ? dx.data_ptr() : nullptr, dw.defined() ? dw.data_ptr() : nullptr,
+                                       ws.data_ptr(), bytes, current_stream(x)),
+                 "grouped_matmul");
+    return {dx, dw, at::Tensor()};
+  }
+};
+
+at::Tensor grouped_matmul(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& offsets) {
+  check_grouped(x, weight, offsets);
+  if (wants_grad(x) || wants_grad(weight)) return GroupedMatmul::apply(x, weight, offsets);
+  return grouped_forward(x, weight, offsets);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(myops, m) {
   m.def("layer_norm(Tensor x, Tensor? weight=None, Tensor? bias=None, float eps=1e-05) -> Tensor", &layer_norm);
+  m.def("grouped_matmul(Tensor x, Tensor weight, Tensor offsets) -> Tensor", &grouped_matmul);
 }
 
 void bind_dense_ops(pybind11::module_& m) {
@@ -149,4 +249,14 @@ void bind_dense_ops(pybind11::module_& m) {
     )doc",
         pybind11::arg("x"), pybind11::arg("weight") = pybind11::none(), pybind11::arg("bias") = pybind11::none(),
         pybind11::arg("eps") = 1e-5);
+  m.def("grouped_matmul", &grouped_matmul,
+        R"doc(
+    Products of row groups with their own matrices, on the GPU: out[r] = x[r] @
+    weight[g] for offsets[g] <= r < offsets[g + 1].  x [rows, inner], weight
+    [groups, inner, width] (its matrices contiguous or transposed), offsets
+    [groups + 1] int32 or int64, ascending, on the GPU; groups may be empty, and
+    rows outside of all groups become zero.  FP16, BF16 or FP32, sums in FP32.
+    Differentiable with respect to x and weight.
+    )doc",
+        pybind11::arg("x"), pybind11::arg("weight"), pybind11::arg("offsets"));
 }

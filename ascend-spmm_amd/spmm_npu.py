@@ -23,6 +23,7 @@ from custom_ops_lib import (  # noqa: E402
     block_level_split,
     csr_to_ascend_cube,
     csr_to_bcsr,
+    grouped_matmul,
     layer_norm,
     pack_rows as _pack_rows,
     preprocess,
@@ -202,6 +203,7 @@ __all__ = [
     "block_level_split",
     "csr_to_ascend_cube",
     "csr_to_bcsr",
+    "grouped_matmul",
     "layer_norm",
     "make_start",
     "pack_node_tensor",

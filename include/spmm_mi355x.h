@@ -449,6 +449,38 @@ spmm_status spmm_layer_norm_grad_run(const spmm_norm_desc* desc, const void* x, 
                                      void* dx, void* dweight, void* dbias, void* workspace,
                                      size_t workspace_bytes, spmm_stream stream);
 
+/* grouped_matmul: out[r] = x[r] * weight[g] for the rows r of group g, that
+ * is offsets[g] <= r < offsets[g + 1].  offsets (device memory, `groups` + 1
+ * ascending entries of index_type) may leave groups empty; rows before
+ * offsets[0] and from offsets[groups] on become zero.  weight[g] is
+ * inner x width, at weight + g * weight_stride; transposed: stored as
+ * width x inner, each group's matrix contiguous either way. */
+typedef struct spmm_grouped_desc {
+  int64_t rows;           /* of x, out and grad                            */
+  int64_t groups;
+  int64_t inner;          /* columns of x                                  */
+  int64_t width;          /* columns of out                                */
+  int64_t x_stride;       /* elements between rows of x                    */
+  int64_t grad_stride;    /* elements between rows of grad (gradients only) */
+  int64_t weight_stride;  /* elements between the groups' matrices         */
+  int32_t weight_transposed;
+  int32_t index_type;
+  int32_t value_type;
+} spmm_grouped_desc;
+
+spmm_status spmm_grouped_workspace(const spmm_grouped_desc* desc, size_t* bytes);
+spmm_status spmm_grouped_run(const spmm_grouped_desc* desc, const void* x, const void* weight,
+                             const void* offsets, void* out, void* workspace,
+                             size_t workspace_bytes, spmm_stream stream);
+
+/* Its gradients: dx[r] = grad[r] * weight[g]^T (zero outside the groups), and
+ * dweight[g] = x_g^T * grad_g (zero for an empty group), contiguous and in
+ * weight's storage order.  dx or dweight may be NULL. */
+spmm_status spmm_grouped_grad_workspace(const spmm_grouped_desc* desc, size_t* bytes);
+spmm_status spmm_grouped_grad_run(const spmm_grouped_desc* desc, const void* x, const void* weight,
+                                  const void* offsets, const void* grad, void* dx, void* dweight,
+                                  void* workspace, size_t workspace_bytes, spmm_stream stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
