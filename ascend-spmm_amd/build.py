@@ -36,6 +36,7 @@ HIP_SOURCES = [
     "preprocess_windows.hip",
     "layer_norm.hip",
     "grouped_matmul.hip",
+    "orthogonalize.hip",
 ]
 EXT_SOURCES = ["custom_op.cpp", "dense_ops.cpp"]
 

@@ -232,6 +232,30 @@ at::Tensor grouped_matmul(const at::Tensor& x, const at::Tensor& weight, const a
   return grouped_forward(x, weight, offsets);
 }
 
+// ----------------------------------------------------------- orthogonalize
+
+// coefficients: a, b, c of every step.
+at::Tensor orthogonalize(const at::Tensor& update, const std::vector<double>& coefficients, double eps) {
+  TORCH_CHECK_GPU(update);
+  TORCH_CHECK(update.dim() >= 2, "orthogonalize: update must have at least two dimensions, but got: ", update.dim());
+  TORCH_CHECK(coefficients.size() % 3 == 0, "orthogonalize: coefficients must hold three values for each step");
+  TORCH_CHECK(!wants_grad(update), "orthogonalize is not differentiable: call it under torch.no_grad()");
+  c10::DeviceGuard guard(update.device());
+  const at::Tensor u = update.contiguous();
+  const int64_t rows = u.size(-2), width = u.size(-1);
+  int64_t batch = 1;
+  for (int64_t i = 0; i + 2 < u.dim(); ++i) batch *= u.size(i);
+  const spmm_orthogonalize_desc d{batch, rows, width, static_cast<int64_t>(coefficients.size() / 3),
+                                  coefficients.data(), eps, dense_type_of(u, "orthogonalize")};
+  at::Tensor out = at::empty(u.sizes(), u.options());
+  size_t bytes = 0;
+  raise_status(spmm_orthogonalize_workspace(&d, &bytes), "orthogonalize");
+  at::Tensor ws = workspace(u, bytes);
+  raise_status(spmm_orthogonalize_run(&d, u.data_ptr(), out.data_ptr(), ws.data_ptr(), bytes, current_stream(u)),
+               "orthogonalize");
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(myops, m) {
@@ -259,4 +283,6 @@ void bind_dense_ops(pybind11::module_& m) {
     Differentiable with respect to x and weight.
     )doc",
         pybind11::arg("x"), pybind11::arg("weight"), pybind11::arg("offsets"));
+  m.def("orthogonalize", &orthogonalize, "Newton-Schulz steps on matrix updates (GPU)", pybind11::arg("update"),
+        pybind11::arg("coefficients"), pybind11::arg("eps"));
 }

@@ -25,6 +25,7 @@ from custom_ops_lib import (  # noqa: E402
     csr_to_bcsr,
     grouped_matmul,
     layer_norm,
+    orthogonalize as _orthogonalize,
     pack_rows as _pack_rows,
     preprocess,
     restore_rows as _restore_rows,
@@ -198,6 +199,29 @@ class PackedGraph:
         return restore_node_tensor(y_packed, self.inv_permutation)
 
 
+def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """``steps`` Newton-Schulz steps on each matrix of ``update`` (the last two
+    dimensions; FP16, BF16 or FP32 on the GPU), as an optimiser applies them to
+    a momentum before the weight update.
+
+    ``X = update / (|update|_F + eps)``, then each step replaces ``X`` by
+    ``a X + (b A + c A A) X`` with ``A = X X^T``; matrices with more rows than
+    columns take the same polynomial from the right.  ``coefficients`` is one
+    ``(a, b, c)`` for all steps, or a sequence of ``steps`` of them.  The default
+    sends singular values to about [0.7, 1.2] without changing their vectors.
+    Returns a new tensor of the shape and type of ``update``.
+    """
+    steps = int(steps)
+    if steps < 0:
+        raise ValueError("steps must not be negative")
+    flat = [float(v) for c in coefficients for v in (c if isinstance(c, (tuple, list)) else (c,))]
+    if len(flat) == 3 and not isinstance(coefficients[0], (tuple, list)):
+        flat *= steps
+    if len(flat) != 3 * steps:
+        raise ValueError("coefficients must be one (a, b, c), or one for each step")
+    return _orthogonalize(update, flat, eps)
+
+
 __all__ = [
     "PackedGraph",
     "block_level_split",
@@ -206,6 +230,7 @@ __all__ = [
     "grouped_matmul",
     "layer_norm",
     "make_start",
+    "orthogonalize",
     "pack_node_tensor",
     "preprocess",
     "restore_node_tensor",

@@ -481,6 +481,26 @@ spmm_status spmm_grouped_grad_run(const spmm_grouped_desc* desc, const void* x, 
                                   const void* offsets, const void* grad, void* dx, void* dweight,
                                   void* workspace, size_t workspace_bytes, spmm_stream stream);
 
+/* orthogonalize: `steps` Newton-Schulz steps on each of `batch` matrices of
+ * rows x width (contiguous).  X = update / (|update|_F + eps), then each step
+ * replaces X by a X + (b A + c A A) X with A = X X^T (for more rows than
+ * columns the same polynomial from the right).  coefficients: 3 * steps host
+ * values (a, b, c of each step).  out may be update itself. */
+typedef struct spmm_orthogonalize_desc {
+  int64_t batch;
+  int64_t rows;
+  int64_t width;
+  int64_t steps;
+  const double* coefficients;
+  double eps;
+  int32_t value_type;
+} spmm_orthogonalize_desc;
+
+spmm_status spmm_orthogonalize_workspace(const spmm_orthogonalize_desc* desc, size_t* bytes);
+spmm_status spmm_orthogonalize_run(const spmm_orthogonalize_desc* desc, const void* update,
+                                   void* out, void* workspace, size_t workspace_bytes,
+                                   spmm_stream stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
