@@ -1,10 +1,24 @@
 // Matrix products grouped by row ranges: out[r] = x[r] W[g] for the rows r of
 // group g, with dx[r] = grad[r] W[g]^T and dW[g] = x_g^T grad_g.
+//
+// All three are products of operands as they lie in memory: x and grad are
+// read along their rows for out and dx and across them for dW, W either way,
+// so nothing is turned first.  Tiles are those of mma_256.h (fp16 and bf16,
+// 16-byte aligned, large) and mma_128.h (the rest).
+//
+// out and dx: one work-group per tile, none across a group's end; which group
+// a tile belongs to is found on the device by one wave-wide scan of offsets.
+//
+// dW: groups differ in length and there may be few tiles, so the steps of all
+// tiles' sums are counted through and cut into equal parts, one for each
+// work-group.  A tile inside one part is written at once; the pieces of one
+// that is cut go to the workspace in fp32 and are added in order.
 #include <climits>
 #include <type_traits>
 #include <utility>
 
-#include "fma_tile.h"
+#include "mma_128.h"
+#include "mma_256.h"
 
 namespace spmm {
 namespace {
@@ -13,90 +27,256 @@ struct GroupedArgs {
   int64_t rows, groups;
   int64_t inner, width;  // of the product at hand: depth and output columns
   int64_t in_stride;     // rows of its left operand
-  int64_t weight_stride, w_depth, w_col;
+  int64_t weight_stride;
+  const void* offsets;
+  bool wide;             // offsets are int64
 };
 
-template <typename I>
-__device__ inline int64_t edge(const I* offsets, int64_t g, int64_t rows) {
-  const int64_t v = static_cast<int64_t>(offsets[g]);
-  return v < 0 ? 0 : v > rows ? rows : v;
+__device__ inline int64_t edge(const GroupedArgs& a, int64_t g) {
+  const int64_t v = a.wide ? static_cast<const int64_t*>(a.offsets)[g] : static_cast<const int32_t*>(a.offsets)[g];
+  return v < 0 ? 0 : v > a.rows ? a.rows : v;
 }
 
-// The `tile`-th tile of `height` rows, none across a group's end.  Segment 0
-// is the rows before the first group, segment groups + 1 those behind the
-// last; both are `group` -1.  False past the last tile.  Every lane of a wave
-// calls it and gets the same answer.
-struct RowRange {
-  int64_t first, rows, group;
-};
-template <typename I>
-__device__ inline bool find_rows(const I* offsets, int64_t groups, int64_t rows, int64_t height, int64_t tile,
-                                 RowRange& found) {
+// Finds the segment of [0, segments) that holds `at`, where segment s takes
+// size(s) places: sets `before` to the places ahead of it.  Past the last,
+// returns `segments` and their total.  Every lane of a wave calls it and gets
+// the same answer.
+template <typename F>
+__device__ inline int64_t find_segment(int64_t segments, int64_t at, F size, int64_t& before) {
   const int lane = threadIdx.x & 63;
-  int64_t before = 0;
-  for (int64_t s0 = 0; s0 < groups + 2; s0 += 64) {
-    const int64_t s = s0 + lane;
-    int64_t lo = 0, hi = 0;
-    if (s < groups + 2) {
-      lo = s == 0 ? 0 : edge(offsets, s - 1, rows);
-      hi = s == groups + 1 ? rows : edge(offsets, s, rows);
-    }
-    const int64_t mine = hi > lo ? (hi - lo + height - 1) / height : 0;
+  before = 0;
+  for (int64_t s0 = 0; s0 < segments; s0 += 64) {
+    const int64_t mine = s0 + lane < segments ? size(s0 + lane) : 0;
     int64_t upto = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int64_t o = __shfl_up(upto, d);
       if (lane >= d) upto += o;
     }
-    const unsigned long long past = __ballot(before + upto > tile);
+    const unsigned long long past = __ballot(before + upto > at);
     if (past != 0) {
-      const int at = __ffsll(past) - 1;
-      const int64_t start = __shfl(lo, at) + (tile - before - __shfl(upto - mine, at)) * height;
-      const int64_t end = __shfl(hi, at);
-      found.first = start;
-      found.rows = end - start < height ? end - start : height;
-      found.group = s0 + at == 0 || s0 + at == groups + 1 ? -1 : s0 + at - 1;
-      return true;
+      const int found = __ffsll(past) - 1;
+      before += __shfl(upto - mine, found);
+      return s0 + found;
     }
     before += __shfl(upto, 63);
   }
-  return false;
+  return segments;
 }
 
-// Row tiles times column tiles, the latter fastest.
-template <typename T, typename I>
-__global__ __launch_bounds__(kThreads) void grouped_rows(GroupedArgs a, const T* __restrict__ in,
-                                                         const T* __restrict__ weight,
-                                                         const I* __restrict__ offsets, T* __restrict__ out) {
-  const int64_t across = (a.width + kTile - 1) / kTile;
+__device__ inline int64_t uniform(int64_t v) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v));
+  const unsigned hi = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v >> 32));
+  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// The `tile`-th range of at most `height` rows, none across a group's end.
+// Segment 0 is the rows before the first group, segment groups + 1 those
+// behind the last; both are `group` -1.  False past the last range.
+struct RowRange {
+  int64_t first, rows, group;
+};
+__device__ inline bool find_rows(const GroupedArgs& a, int64_t height, int64_t tile, RowRange& r) {
+  auto low = [&](int64_t s) { return s == 0 ? 0 : edge(a, s - 1); };
+  auto high = [&](int64_t s) { return s == a.groups + 1 ? a.rows : edge(a, s); };
+  int64_t before;
+  const int64_t s = find_segment(a.groups + 2, tile, [&](int64_t t) {
+    const int64_t n = high(t) - low(t);
+    return n > 0 ? (n + height - 1) / height : 0;
+  }, before);
+  if (s == a.groups + 2) return false;
+  r.first = uniform(low(s) + (tile - before) * height);
+  const int64_t left = uniform(high(s)) - r.first;
+  r.rows = left < height ? left : height;
+  r.group = uniform(s == 0 || s == a.groups + 1 ? -1 : s - 1);
+  return true;
+}
+
+// Four sums of one row, rounded; `cols`: of the row from the first of them.
+template <typename T>
+__device__ inline void store_four(T* to, int64_t cols, f32x4 v) {
+  typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  if (cols >= 4) {
+    *reinterpret_cast<four*>(to) =
+        four{static_cast<T>(v[0]), static_cast<T>(v[1]), static_cast<T>(v[2]), static_cast<T>(v[3])};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < cols) to[e] = static_cast<T>(v[e]);
+  }
+}
+
+// Work-groups run on the XCDs in turn; each XCD gets one run of the tiles, so
+// that neighbours share its L2.
+__device__ inline int64_t run_of_xcd(int64_t block, int64_t blocks) {
+  const int64_t each = blocks / kXcds, rest = blocks % kXcds, x = block % kXcds;
+  return x * each + (x < rest ? x : rest) + block / kXcds;
+}
+
+// Tile `n` of down x across: blocks of four tile rows, down them first, so
+// that the tiles at work together share rows of both operands.
+__device__ inline void place_tile(int64_t n, int64_t down, int64_t across, int64_t& i, int64_t& j) {
+  const int64_t block = n / (4 * across), first = 4 * block, high = down - first < 4 ? down - first : 4;
+  const int64_t m = n - block * 4 * across;
+  i = first + m % high;
+  j = m / high;
+}
+
+// The engines of one product: Large of mma_256.h, Small of mma_128.h.
+template <typename T, bool kAC, bool kBC>
+struct Large {
+  typedef T Value;
+  static constexpr int kRows = mma::kTile, kCols = mma::kTile, kThreads = mma::kThreads, kStep = mma::kDepth;
+  static constexpr int kLds = mma::kLdsBytes, kPerCu = 1;
+  mma::Sums s;
+  __device__ inline void sum(const mma::Operand<T>& a, const mma::Operand<T>& b, char* lds) {
+    mma::multiply_tile<T, kAC, kBC, 1>(a, b, lds, s);
+  }
+  template <typename F>
+  __device__ inline void each(F f) const {
+    mma::for_sums(s, f);
+  }
+};
+
+template <typename T, bool kAC, bool kBC, int kHeight, bool kAligned>
+struct Small {
+  typedef T Value;
+  typedef mma::Tile128<T, kAC, kBC, kHeight, kAligned> Tile;
+  static constexpr int kRows = kHeight, kCols = mma::kCols128, kThreads = mma::kThreads128,
+                       kStep = mma::Step<T>::kDepth;
+  // fp32's parts take registers for 256 a thread
+  static constexpr int kLds = Tile::kLdsBytes, kPerCu = std::is_same_v<T, float> ? 2 : 3;
+  mma::Sums128<kHeight> s;
+  __device__ inline void sum(const mma::Operand<T>& a, const mma::Operand<T>& b, char* lds) {
+    s.clear();
+    Tile::template add<1>(a, b, lds, 0, (a.depth + kStep - 1) / kStep, s);
+  }
+  template <typename F>
+  __device__ inline void each(F f) const {
+    s.each(f);
+  }
+};
+
+// out or dx; kTurned: the weights' depth is their contiguous extent.
+template <typename E, bool kTurned>
+__global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void grouped_rows(
+    GroupedArgs a, const typename E::Value* __restrict__ in, const typename E::Value* __restrict__ weight,
+    typename E::Value* __restrict__ out, int64_t down) {
+  typedef typename E::Value T;
+  __shared__ __align__(1024) char lds[E::kLds];
+  const int64_t across = (a.width + E::kCols - 1) / E::kCols;
+  int64_t i, j;
+  place_tile(run_of_xcd(blockIdx.x, gridDim.x), down, across, i, j);
   RowRange r;
-  if (!find_rows(offsets, a.groups, a.rows, kTile, blockIdx.x / across, r)) return;
-  const int64_t c0 = blockIdx.x % across * kTile;
-  const int64_t cols = a.width - c0 < kTile ? a.width - c0 : kTile;
-  float acc[4][4] = {};
-  if (r.group >= 0)
-    multiply_tile<T>({in + r.first * a.in_stride, a.in_stride, 1},
-                     {weight + r.group * a.weight_stride + c0 * a.w_col, a.w_col, a.w_depth}, r.rows, cols, a.inner, acc);
-  store_tile(out + r.first * a.width + c0, a.width, r.rows, cols, acc);
+  if (!find_rows(a, E::kRows, i, r)) return;
+  const int64_t c0 = j * E::kCols;
+  const int64_t cols = a.width - c0 < E::kCols ? a.width - c0 : E::kCols;
+  T* to = out + r.first * a.width + c0;
+  auto store = [&](int row, int col, f32x4 v) {
+    if (row < r.rows && col < cols) store_four(to + row * a.width + col, cols - col, v);
+  };
+  E e;
+  const T* w = weight + (r.group < 0 ? 0 : r.group) * a.weight_stride + (kTurned ? c0 * a.inner : c0);
+  // outside the groups: an empty sum
+  e.sum({in + r.first * a.in_stride, nullptr, a.in_stride, r.rows, r.group < 0 ? 0 : a.inner},
+        {w, nullptr, kTurned ? a.inner : a.width, cols, r.group < 0 ? 0 : a.inner}, lds);
+  e.each(store);
 }
 
-// dW[g]: `left` columns by `right` columns, summed over the group's rows.
-template <typename T, typename I>
-__global__ __launch_bounds__(kThreads) void grouped_weights(GroupedArgs a, const T* __restrict__ left,
-                                                            int64_t left_stride, const T* __restrict__ right,
-                                                            int64_t right_stride, const I* __restrict__ offsets,
-                                                            T* __restrict__ dweight) {
-  const int64_t across = (a.width + kTile - 1) / kTile, down = (a.inner + kTile - 1) / kTile;
-  const int64_t g = blockIdx.x / (across * down);
-  const int64_t i0 = blockIdx.x / across % down * kTile, c0 = blockIdx.x % across * kTile;
-  const int64_t rows = a.inner - i0 < kTile ? a.inner - i0 : kTile;
-  const int64_t cols = a.width - c0 < kTile ? a.width - c0 : kTile;
-  const int64_t lo = edge(offsets, g, a.rows), hi = edge(offsets, g + 1, a.rows);
-  float acc[4][4] = {};
-  multiply_tile<T>({left + lo * left_stride + i0, 1, left_stride}, {right + lo * right_stride + c0, 1, right_stride},
-                   rows, cols, hi > lo ? hi - lo : 0, acc);
-  store_tile(dweight + (g * a.inner + i0) * a.width + c0, a.width, rows, cols, acc);
+// Steps of the sums of all tiles of dW, counted group by group and tile by
+// tile; an empty group's tiles have one step each, which adds nothing.
+struct Steps {
+  int64_t tiles, depth;  // tiles of a matrix; rows of a step
+  __device__ inline int64_t of(const GroupedArgs& a, int64_t g) const {
+    const int64_t n = edge(a, g + 1) - edge(a, g);
+    return n > 0 ? (n + depth - 1) / depth : 1;
+  }
+  __device__ inline int64_t find(const GroupedArgs& a, int64_t at, int64_t& before) const {
+    return find_segment(a.groups, at, [&](int64_t g) { return tiles * of(a, g); }, before);
+  }
+};
+__device__ __host__ inline int64_t part_start(int64_t total, int64_t part, int64_t parts) {
+  return total / parts * part + total % parts * part / parts;
 }
+
+// pieces: [parts][2][tile] fp32; a part's first piece goes to its first
+// place, a later one to its second.
+template <typename E>
+__global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void grouped_weights(
+    GroupedArgs a, const typename E::Value* __restrict__ left, int64_t left_stride,
+    const typename E::Value* __restrict__ right, int64_t right_stride, typename E::Value* __restrict__ dweight,
+    float* __restrict__ pieces) {
+  typedef typename E::Value T;
+  __shared__ __align__(1024) char lds[E::kLds];
+  const int64_t across = (a.width + E::kCols - 1) / E::kCols, down = (a.inner + E::kRows - 1) / E::kRows;
+  const Steps steps{across * down, E::kStep};
+  int64_t total;
+  steps.find(a, INT64_MAX, total);
+  total = uniform(total);
+  const int64_t part = run_of_xcd(blockIdx.x, gridDim.x);
+  const int64_t u0 = part_start(total, part, gridDim.x), u1 = part_start(total, part + 1, gridDim.x);
+  for (int64_t u = u0; u < u1;) {
+    int64_t before;
+    const int64_t g = uniform(steps.find(a, u, before));
+    before = uniform(before);
+    const int64_t lo = uniform(edge(a, g)), hi = uniform(edge(a, g + 1)), n = uniform(steps.of(a, g));
+    const int64_t tile = (u - before) / n, s0 = (u - before) % n;
+    const int64_t s1 = n - s0 < u1 - u ? n : s0 + (u1 - u);
+    int64_t i, j;
+    place_tile(tile, down, across, i, j);
+    const int64_t i0 = i * E::kRows, j0 = j * E::kCols;
+    const int64_t rows = a.inner - i0 < E::kRows ? a.inner - i0 : E::kRows;
+    const int64_t cols = a.width - j0 < E::kCols ? a.width - j0 : E::kCols;
+    const int64_t first = lo + s0 * E::kStep, last = lo + s1 * E::kStep < hi ? lo + s1 * E::kStep : hi;
+    const int64_t depth = last > first ? last - first : 0;
+    E e;
+    e.sum({left + first * left_stride + i0, nullptr, left_stride, rows, depth},
+          {right + first * right_stride + j0, nullptr, right_stride, cols, depth}, lds);
+    if (s0 == 0 && s1 == n) {
+      T* to = dweight + (g * a.inner + i0) * a.width + j0;
+      e.each([&](int row, int col, f32x4 v) {
+        if (row < rows && col < cols) store_four(to + row * a.width + col, cols - col, v);
+      });
+    } else {
+      float* to = pieces + (2 * part + (u == u0 ? 0 : 1)) * E::kRows * E::kCols;
+      e.each([&](int row, int col, f32x4 v) { *reinterpret_cast<f32x4*>(to + row * E::kCols + col) = v; });
+    }
+    u += s1 - s0;
+  }
+}
+
+// Adds the pieces of the tiles that were cut; a work-group takes 1024 sums.
+template <typename T>
+__global__ __launch_bounds__(256) void join_pieces(GroupedArgs a, int64_t tile_rows, int64_t tile_cols, int64_t step,
+                                                   int64_t parts, const float* __restrict__ pieces,
+                                                   T* __restrict__ dweight) {
+  const int64_t across = (a.width + tile_cols - 1) / tile_cols, down = (a.inner + tile_rows - 1) / tile_rows;
+  const Steps steps{across * down, step};
+  const int64_t slices = tile_rows * tile_cols / 1024;
+  const int64_t g = blockIdx.x / (slices * steps.tiles), tile = blockIdx.x / slices % steps.tiles;
+  int64_t total, before;
+  steps.find(a, INT64_MAX, total);
+  find_segment(a.groups, INT64_MAX, [&](int64_t s) { return s < g ? steps.tiles * steps.of(a, s) : 0; }, before);
+  const int64_t n = steps.of(a, g), u0 = before + tile * n, u1 = u0 + n;
+  // the part that holds the tile's first step
+  int64_t part = static_cast<int64_t>(static_cast<double>(u0) / static_cast<double>(total) * static_cast<double>(parts));
+  while (part > 0 && part_start(total, part, parts) > u0) --part;
+  while (part_start(total, part + 1, parts) <= u0) ++part;
+  if (part_start(total, part + 1, parts) >= u1) return;  // written whole
+  const int64_t e = blockIdx.x % slices * 1024 + threadIdx.x * 4;
+  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (; part < parts && part_start(total, part, parts) < u1; ++part) {
+    const int64_t at = part_start(total, part, parts);
+    if (at == part_start(total, part + 1, parts)) continue;
+    s += *reinterpret_cast<const f32x4*>(pieces + (2 * part + (at >= u0 ? 0 : 1)) * tile_rows * tile_cols + e);
+  }
+  int64_t i, j;
+  place_tile(tile, down, across, i, j);
+  const int64_t row = i * tile_rows + e / tile_cols, col = j * tile_cols + e % tile_cols;
+  if (row < a.inner && col < a.width) store_four(dweight + (g * a.inner + row) * a.width + col, a.width - col, s);
+}
+
+constexpr int64_t kMostStride = int64_t(1) << 22;
 
 spmm_status check_grouped_desc(const spmm_grouped_desc* d, const char* op) {
   if (d == nullptr) return fail(SPMM_ERR_INVALID_ARGUMENT, "null descriptor");
@@ -106,8 +286,9 @@ spmm_status check_grouped_desc(const spmm_grouped_desc* d, const char* op) {
     return fail(SPMM_ERR_CONTRACT, std::string(op) + " supports only FP16, BF16 and FP32 tensors");
   if (d->rows < 0 || d->groups < 0 || d->inner < 0 || d->width < 0)
     return fail(SPMM_ERR_CONTRACT, std::string(op) + ": negative extent");
-  if (d->inner > INT32_MAX || d->width > INT32_MAX)
-    return fail(SPMM_ERR_CONTRACT, std::string(op) + ": inner and width must be below 2^31");
+  // offsets inside a tile are 32-bit
+  if (d->inner >= kMostStride || d->width >= kMostStride || (d->rows > 1 && d->x_stride >= kMostStride))
+    return fail(SPMM_ERR_CONTRACT, std::string(op) + ": inner, width and row strides must be below 2^22");
   if (d->rows > 1 && d->x_stride < d->inner) return fail(SPMM_ERR_CONTRACT, std::string(op) + ": rows of x overlap");
   if (d->groups > 1 && d->weight_stride < d->inner * d->width)
     return fail(SPMM_ERR_CONTRACT, std::string(op) + ": matrices of weight overlap");
@@ -120,57 +301,136 @@ spmm_status check_grid(int64_t blocks, const char* op) {
   return SPMM_OK;
 }
 
-// The weight's steps along the depth and the columns of the product x W, or
-// of grad W^T where `back`.
-GroupedArgs rows_args(const spmm_grouped_desc* d, bool back) {
-  const int64_t inner_step = d->weight_transposed ? 1 : d->width, width_step = d->weight_transposed ? d->inner : 1;
-  if (back)
-    return {d->rows, d->groups, d->width, d->inner, d->grad_stride, d->weight_stride, width_step, inner_step};
-  return {d->rows, d->groups, d->inner, d->width, d->x_stride, d->weight_stride, inner_step, width_step};
+// Whether 16-byte pieces of the operands can be copied as they lie.
+bool pieces_aligned(const spmm_grouped_desc* d, const void* x, const void* weight, const void* grad) {
+  const int64_t size = dense_type_bytes(d->value_type);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(grad);
+  return at % 16 == 0 && d->inner % 8 == 0 && d->width % 8 == 0 && (d->rows <= 1 || d->x_stride * size % 16 == 0) &&
+         (grad == nullptr || d->rows <= 1 || d->grad_stride * size % 16 == 0) &&
+         (d->groups <= 1 || d->weight_stride * size % 16 == 0);
 }
 
-template <typename T, typename I>
-spmm_status run_rows(const GroupedArgs& a, const void* in, const void* weight, const void* offsets, void* out,
-                     hipStream_t s, const char* op) {
-  if (a.rows == 0 || a.width == 0) return SPMM_OK;
-  const int64_t blocks = (ceil_div(a.rows, kTile) + a.groups + 1) * ceil_div(a.width, kTile);
-  if (spmm_status st = check_grid(blocks, op)) return st;
-  hipLaunchKernelGGL((grouped_rows<T, I>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, s, a,
-                     static_cast<const T*>(in), static_cast<const T*>(weight), static_cast<const I*>(offsets),
-                     static_cast<T*>(out));
-  return check_launch(op);
+constexpr int64_t kCus = 256;
+
+// The large tile for out and dx: a matrix must fit the copies' 32-bit count of
+// pieces; at least three quarters of the CUs get a tile, and the groups'
+// average fills half of one.  65536 x 1024 x 2048 bf16 in 8 groups: 289 us
+// with it, 413 with the small tile.
+bool large_rows(const GroupedArgs& a) {
+  return a.width > mma::kCols128 && a.inner * a.width < (int64_t(1) << 33) && a.inner >= 2 * mma::kDepth && a.rows / mma::kTile * ceil_div(a.width, mma::kTile) >= kCus * 3 / 4 &&
+         a.rows >= a.groups * mma::kTile / 2;
 }
 
-template <typename T, typename I>
-spmm_status run_weights(const spmm_grouped_desc* d, const void* x, const void* grad, const void* offsets, void* dweight,
-                        hipStream_t s, const char* op) {
-  if (d->groups == 0 || d->inner == 0 || d->width == 0) return SPMM_OK;
-  const T *tx = static_cast<const T*>(x), *tg = static_cast<const T*>(grad);
-  GroupedArgs a{d->rows, d->groups, d->inner, d->width, 0, 0, 0, 0};
-  if (d->weight_transposed) std::swap(a.inner, a.width);
-  const int64_t blocks = ceil_div(a.inner, kTile) * ceil_div(a.width, kTile) * a.groups;
-  if (spmm_status st = check_grid(blocks, op)) return st;
-  hipLaunchKernelGGL((grouped_weights<T, I>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, s, a,
-                     d->weight_transposed ? tg : tx, d->weight_transposed ? d->grad_stride : d->x_stride,
-                     d->weight_transposed ? tx : tg, d->weight_transposed ? d->x_stride : d->grad_stride,
-                     static_cast<const I*>(offsets), static_cast<T*>(dweight));
-  return check_launch(op);
+// The low tile where the groups' average leaves most of a tile of 128 empty.
+bool low_rows(const GroupedArgs& a) { return a.rows <= 48 * a.groups; }
+
+bool large_weights(const GroupedArgs& a, int64_t stride, int64_t other) {
+  return a.inner > mma::kCols128 && a.width > mma::kCols128 &&
+         a.rows * (stride > other ? stride : other) < (int64_t(1) << 33) && a.rows >= 4 * mma::kDepth * a.groups;
 }
 
-// Calls f with null pointers of the value and index types.
+// Parts of dW's steps: one round of work-groups, each with eight steps or more
+// on average, so that pieces cost little beside their sums.
+template <typename E>
+int64_t weight_parts(const GroupedArgs& a) {
+  const int64_t tiles = ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols);
+  const int64_t steps = (a.rows / E::kStep + a.groups) * tiles;
+  const int64_t most = kCus * E::kPerCu, want = ceil_div(steps, 8);
+  return want < most ? want : most;
+}
+template <typename E>
+size_t weight_bytes(const GroupedArgs& a) {
+  return static_cast<size_t>(weight_parts<E>(a)) * 2 * E::kRows * E::kCols * sizeof(float);
+}
+
+// Calls f with null pointers of the value type.
 template <typename F>
-spmm_status with_types(const spmm_grouped_desc* d, F f) {
-  auto indexed = [&](auto* t) {
-    return d->index_type == SPMM_INDEX_I32 ? f(t, static_cast<int32_t*>(nullptr)) : f(t, static_cast<int64_t*>(nullptr));
-  };
-  switch (d->value_type) {
-    case SPMM_VALUE_F16: return indexed(static_cast<_Float16*>(nullptr));
-    case SPMM_VALUE_BF16: return indexed(static_cast<__bf16*>(nullptr));
-    default: return indexed(static_cast<float*>(nullptr));
+spmm_status with_type(int32_t value_type, F f) {
+  switch (value_type) {
+    case SPMM_VALUE_F16: return f(static_cast<_Float16*>(nullptr));
+    case SPMM_VALUE_BF16: return f(static_cast<__bf16*>(nullptr));
+    default: return f(static_cast<float*>(nullptr));
   }
 }
 template <typename P>
 using value_of = std::remove_pointer_t<P>;
+
+template <typename E, bool kTurned>
+spmm_status launch_rows(const GroupedArgs& a, const void* in, const void* weight, void* out, hipStream_t s,
+                        const char* op) {
+  typedef typename E::Value T;
+  const int64_t down = ceil_div(a.rows, E::kRows) + a.groups + 1;
+  const int64_t blocks = down * ceil_div(a.width, E::kCols);
+  if (spmm_status st = check_grid(blocks, op)) return st;
+  hipLaunchKernelGGL((grouped_rows<E, kTurned>), dim3(static_cast<unsigned>(blocks)), dim3(E::kThreads), 0, s, a,
+                     static_cast<const T*>(in), static_cast<const T*>(weight), static_cast<T*>(out), down);
+  return check_launch(op);
+}
+
+// in [rows, depth] times each group's matrix, whose depth is contiguous where
+// kTurned.
+template <typename T, bool kTurned>
+spmm_status run_rows(const GroupedArgs& a, bool aligned, const void* in, const void* weight, void* out, hipStream_t s,
+                     const char* op) {
+  if (a.rows == 0 || a.width == 0) return SPMM_OK;
+  if constexpr (sizeof(T) == 2)
+    if (aligned && large_rows(a)) return launch_rows<Large<T, false, !kTurned>, kTurned>(a, in, weight, out, s, op);
+  if (low_rows(a))
+    return aligned ? launch_rows<Small<T, false, !kTurned, 32, true>, kTurned>(a, in, weight, out, s, op)
+                   : launch_rows<Small<T, false, !kTurned, 32, false>, kTurned>(a, in, weight, out, s, op);
+  return aligned ? launch_rows<Small<T, false, !kTurned, 128, true>, kTurned>(a, in, weight, out, s, op)
+                 : launch_rows<Small<T, false, !kTurned, 128, false>, kTurned>(a, in, weight, out, s, op);
+}
+
+template <typename E>
+spmm_status launch_weights(const GroupedArgs& a, const void* left, int64_t left_stride, const void* right,
+                           int64_t right_stride, void* dweight, void* ws, size_t ws_bytes, hipStream_t s,
+                           const char* op) {
+  typedef typename E::Value T;
+  const size_t need = weight_bytes<E>(a);
+  if (ws == nullptr || ws_bytes < need)
+    return fail(SPMM_ERR_CONTRACT, std::string(op) + ": workspace too small: need " + std::to_string(need) + " bytes");
+  const int64_t parts = weight_parts<E>(a);
+  const int64_t slices =
+      a.groups * ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols) * (E::kRows * E::kCols / 1024);
+  if (spmm_status st = check_grid(slices, op)) return st;
+  hipLaunchKernelGGL(grouped_weights<E>, dim3(static_cast<unsigned>(parts)), dim3(E::kThreads), 0, s, a,
+                     static_cast<const T*>(left), left_stride, static_cast<const T*>(right), right_stride,
+                     static_cast<T*>(dweight), static_cast<float*>(ws));
+  if (spmm_status st = check_launch(op)) return st;
+  hipLaunchKernelGGL(join_pieces<T>, dim3(static_cast<unsigned>(slices)), dim3(256), 0, s, a,
+                     static_cast<int64_t>(E::kRows), static_cast<int64_t>(E::kCols), static_cast<int64_t>(E::kStep),
+                     parts, static_cast<const float*>(ws), static_cast<T*>(dweight));
+  return check_launch(op);
+}
+
+GroupedArgs grouped_args(const spmm_grouped_desc* d, const void* offsets) {
+  return {d->rows, d->groups, d->inner, d->width, d->x_stride, d->weight_stride, offsets,
+          d->index_type == SPMM_INDEX_I64};
+}
+
+// dW's operands, in the order of weight's storage.
+struct WeightSides {
+  GroupedArgs a;
+  const void *left, *right;
+  int64_t left_stride, right_stride;
+  WeightSides(const spmm_grouped_desc* d, const void* offsets, const void* x, const void* grad)
+      : a(grouped_args(d, offsets)), left(x), right(grad), left_stride(d->x_stride), right_stride(d->grad_stride) {
+    if (d->weight_transposed) {
+      std::swap(a.inner, a.width);
+      std::swap(left, right);
+      std::swap(left_stride, right_stride);
+    }
+  }
+};
+
+template <typename T, typename F>
+spmm_status with_weight_engine(const GroupedArgs& a, bool aligned, int64_t stride, int64_t other, F f) {
+  if constexpr (sizeof(T) == 2)
+    if (aligned && large_weights(a, stride, other)) return f(static_cast<Large<T, true, true>*>(nullptr));
+  if (aligned) return f(static_cast<Small<T, true, true, 128, true>*>(nullptr));
+  return f(static_cast<Small<T, true, true, 128, false>*>(nullptr));
+}
 
 }  // namespace
 }  // namespace spmm
@@ -197,38 +457,68 @@ spmm_status spmm_grouped_run(const spmm_grouped_desc* d, const void* x, const vo
     return fail(SPMM_ERR_INVALID_ARGUMENT, "grouped_matmul: null device pointer");
   (void)workspace;
   (void)workspace_bytes;
-  return with_types(d, [&](auto* t, auto* i) {
-    return run_rows<value_of<decltype(t)>, value_of<decltype(i)>>(rows_args(d, false), x, weight, offsets, out,
-                                                                  as_stream(stream), "grouped_matmul");
+  const GroupedArgs a = grouped_args(d, offsets);
+  const bool aligned = pieces_aligned(d, x, weight, nullptr);
+  hipStream_t s = as_stream(stream);
+  return with_type(d->value_type, [&](auto* t) {
+    using T = value_of<decltype(t)>;
+    return d->weight_transposed ? run_rows<T, true>(a, aligned, x, weight, out, s, "grouped_matmul")
+                                : run_rows<T, false>(a, aligned, x, weight, out, s, "grouped_matmul");
   });
 }
 
 spmm_status spmm_grouped_grad_workspace(const spmm_grouped_desc* d, size_t* bytes) {
-  return spmm_grouped_workspace(d, bytes);
+  clear_error();
+  if (bytes == nullptr) return fail(SPMM_ERR_INVALID_ARGUMENT, "null argument");
+  if (spmm_status st = check_grouped_desc(d, "grouped_matmul")) return st;
+  // of whichever engine the pointers' alignment leads to
+  const WeightSides w(d, nullptr, nullptr, nullptr);
+  return with_type(d->value_type, [&](auto* t) {
+    size_t most = 0;
+    for (bool aligned : {false, true})
+      with_weight_engine<value_of<decltype(t)>>(w.a, aligned, w.left_stride, w.right_stride, [&](auto* e) {
+        const size_t need = weight_bytes<value_of<decltype(e)>>(w.a);
+        most = need > most ? need : most;
+        return SPMM_OK;
+      });
+    *bytes = most;
+    return SPMM_OK;
+  });
 }
 
 spmm_status spmm_grouped_grad_run(const spmm_grouped_desc* d, const void* x, const void* weight, const void* offsets,
                                   const void* grad, void* dx, void* dweight, void* workspace, size_t workspace_bytes,
                                   spmm_stream stream) {
+  const char* op = "grouped_matmul gradient";
   clear_error();
   if (spmm_status st = check_grouped_desc(d, "grouped_matmul")) return st;
   if (d->rows > 1 && d->grad_stride < d->width)
     return fail(SPMM_ERR_CONTRACT, "grouped_matmul: rows of grad overlap");
+  if (d->rows > 1 && d->grad_stride >= kMostStride)
+    return fail(SPMM_ERR_CONTRACT, "grouped_matmul: inner, width and row strides must be below 2^22");
   if (offsets == nullptr || (d->rows > 0 && d->width > 0 && grad == nullptr) ||
       (dx != nullptr && d->groups > 0 && d->inner > 0 && d->width > 0 && weight == nullptr) ||
       (dweight != nullptr && d->rows > 0 && d->inner > 0 && x == nullptr))
     return fail(SPMM_ERR_INVALID_ARGUMENT, "grouped_matmul: null device pointer");
-  (void)workspace;
-  (void)workspace_bytes;
-  return with_types(d, [&](auto* t, auto* i) {
+  const bool aligned = pieces_aligned(d, x, weight, grad);
+  hipStream_t s = as_stream(stream);
+  return with_type(d->value_type, [&](auto* t) {
     using T = value_of<decltype(t)>;
-    using I = value_of<decltype(i)>;
-    if (dx != nullptr)
-      if (spmm_status st = run_rows<T, I>(rows_args(d, true), grad, weight, offsets, dx, as_stream(stream),
-                                          "grouped_matmul gradient"))
+    if (dx != nullptr) {
+      GroupedArgs a = grouped_args(d, offsets);
+      std::swap(a.inner, a.width);
+      a.in_stride = d->grad_stride;
+      // W^T: its depth is W's columns, contiguous unless W is transposed
+      if (spmm_status st = d->weight_transposed ? run_rows<T, false>(a, aligned, grad, weight, dx, s, op)
+                                                : run_rows<T, true>(a, aligned, grad, weight, dx, s, op))
         return st;
-    if (dweight == nullptr) return SPMM_OK;
-    return run_weights<T, I>(d, x, grad, offsets, dweight, as_stream(stream), "grouped_matmul gradient");
+    }
+    if (dweight == nullptr || d->groups == 0 || d->inner == 0 || d->width == 0) return SPMM_OK;
+    const WeightSides w(d, offsets, x, grad);
+    return with_weight_engine<T>(w.a, aligned, w.left_stride, w.right_stride, [&](auto* e) {
+      return launch_weights<value_of<decltype(e)>>(w.a, w.left, w.left_stride, w.right, w.right_stride, dweight,
+                                                   workspace, workspace_bytes, s, op);
+    });
   });
 }
 

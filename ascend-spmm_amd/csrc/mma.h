@@ -1,0 +1,54 @@
+// Operands and matrix instructions of the product tiles (mma_256.h, mma_128.h).
+#pragma once
+
+#include "numeric.h"
+
+namespace spmm {
+namespace mma {
+
+// threadIdx.x, computed anew: in a loop over tiles, addresses made from it are
+// not kept in registers across the other tiles' sums.
+__device__ inline int thread_here() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+
+// An operand of the product: element (i, k) of the tile.  Where C is false k
+// is the contiguous one, at p[i * ld + k]; where true i is, at p[k * ld + i].
+// p and ld are multiples of 16 bytes, and so is `depth` where C is false.
+// Rows i >= valid and k >= depth are not read and count as zeros, but where C
+// is true: memory up to the 16-byte piece of the last valid element is read
+// there, and sums with i >= valid hold anything.  `lo` is the second plane of
+// an operand held as the sum of two, else null.
+template <typename T>
+struct Operand {
+  const T* p;
+  const T* lo;
+  int64_t ld;
+  int64_t valid;
+  int64_t depth;
+};
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+__device__ inline unsigned lds_address(const void* p) {
+  return static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_ptr)p));
+}
+
+// The 16 x 16 x 32 matrix instruction: lane (i = lane % 16, q = lane / 16) holds
+// k = 8 q .. 8 q + 7 of row i of either operand, and gets the sums of b's row i
+// with a's rows 4 q .. 4 q + 3.
+template <typename T>
+__device__ inline f32x4 multiply(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (std::is_same_v<T, _Float16>)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+}
+
+}  // namespace mma
+}  // namespace spmm

@@ -1,0 +1,276 @@
+// kRows x 128 tiles of matrix products, four waves, for operands of any
+// alignment and for fp32.
+//
+// Operands pass through registers into LDS, one step of the sum at a time; the
+// next step's loads are under way during the matrix instructions, and three to
+// four work-groups of a CU hide each other's barriers.
+//
+// fp32 operands are split into three bf16 parts on the way, each the leading
+// eight digits of what the ones before leave over, so their sum is the fp32
+// value; all their products but that of the last two, which is below 2^-28 of
+// the whole, are added in fp32.  That is the precision of fp32 products at 8 of
+// the 16 matrix cycles that fp32 instructions take.
+#pragma once
+
+#include "mma.h"
+
+namespace spmm {
+namespace mma {
+
+constexpr int kCols128 = 128;
+constexpr int kThreads128 = 256;
+
+template <typename T>
+struct Step {
+  static constexpr int kParts = std::is_same_v<T, float> ? 3 : 1;
+  static constexpr int kDepth = std::is_same_v<T, float> ? 32 : 64;
+  typedef std::conditional_t<std::is_same_v<T, float>, __bf16, T> Part;
+};
+
+// Three bf16 parts of fp32 values, by truncation: all parts of a value have its
+// sign, and what the last one leaves is below 2^-24 of it.  Parts that would be
+// zero are 2^-126 where the value is 2^-60 or more: nothing against the sum,
+// and the product with an infinity stays infinite.
+__device__ inline void split(float x, unsigned& hi, unsigned& mid, unsigned& lo) {
+  const unsigned sign = __builtin_bit_cast(unsigned, x) & 0x80000000u;
+  const unsigned least = (__builtin_bit_cast(unsigned, x) & 0x7f800000u) >= 0x21800000u ? sign | 0x00800000u : 0u;
+  hi = __builtin_bit_cast(unsigned, x) & 0xffff0000u;
+  const float high = __builtin_bit_cast(float, hi);
+  const float rest = x == high ? 0.0f : x - high;
+  mid = __builtin_bit_cast(unsigned, rest) & 0xffff0000u;
+  const float last = rest - __builtin_bit_cast(float, mid);
+  lo = __builtin_bit_cast(unsigned, last) & 0xffff0000u;
+  mid = (mid & 0x7fffffffu) == 0u ? least : mid;
+  lo = (lo & 0x7fffffffu) == 0u ? least : lo;
+}
+
+// One operand's kRows x depth of a step in LDS and its way there.  Layouts as
+// the 256 tile's halves: where k is contiguous, lines of kDepth elements whose
+// 16-byte pieces are exchanged by the line; else lines of kRows elements whose
+// 32-byte units are exchanged by k.  A thread's pieces lie whole rounds of
+// lines apart, which leaves the exchange alike: one offset serves them all.
+template <typename T, bool C, int kRows, bool kAligned>
+struct Stage {
+  typedef Step<T> S;
+  static constexpr int kPieces = kRows * S::kDepth / 8;  // of eight elements
+  static constexpr int kEach = (kPieces + kThreads128 - 1) / kThreads128;
+  static constexpr bool kWhole = kPieces % kThreads128 == 0;  // else the last threads have none
+  static constexpr int kBytes = kRows * S::kDepth * 2;        // of one part
+  static constexpr int kAcross = (C ? kRows : S::kDepth) / 8;
+  static constexpr int kLines = kThreads128 / kAcross;        // of a round
+  static constexpr int kLineBytes = kAcross * 16;
+  static constexpr int kVectors = sizeof(T) / 2;
+  static_assert(!C || kRows == 128, "low tiles are of contiguous k");
+  static_assert(kLines % 16 == 0, "the exchange repeats every 16 lines");
+
+  u32x4 held[kEach][kVectors];
+  int line, piece;   // of the thread's first piece
+  unsigned from;     // its offset in the operand, in elements
+  unsigned round;    // offset between rounds
+  int to;            // its place in LDS
+
+  // The exchange: place of a 16-byte piece of a line.
+  __device__ static inline int place(int line, int piece) {
+    if constexpr (C)
+      return line * kLineBytes + (piece ^ (((line & 3) | ((line >> 3 & 1) << 2)) << 1)) * 16;
+    else if constexpr (S::kDepth == 64)
+      return line * kLineBytes + (piece ^ (line & 7)) * 16;
+    else
+      return line * kLineBytes + (piece ^ (line >> 1 & 3)) * 16;
+  }
+
+  __device__ inline Stage(int64_t ld, int thread) {
+    line = thread / kAcross;
+    piece = thread % kAcross;
+    from = static_cast<unsigned>(line * ld) + piece * 8;
+    round = static_cast<unsigned>(kLines * ld);
+    to = place(line, piece);
+    if (!kWhole && line >= (C ? S::kDepth : kRows)) line = 1 << 28;  // none
+  }
+
+  // Loads the step at p, with `left` of the sum's depth, into registers; zeros
+  // outside the operand.
+  __device__ inline void load(const T* p, int valid, int left) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int l = line + e * kLines, c = piece * 8;
+      const bool in = l < (C ? left : valid) && c < (C ? valid : left);
+      const T* at = p + (in ? from + e * round : 0u);
+      if constexpr (kAligned) {  // p itself can always be read
+#pragma unroll
+        for (int h = 0; h < kVectors; ++h) {
+          const u32x4 v = reinterpret_cast<const u32x4*>(at)[h];
+          held[e][h] = in ? v : u32x4{0u, 0u, 0u, 0u};
+        }
+      } else {
+        const int count = in ? (C ? valid : left) - c : 0;
+        if (count >= 8) {
+#pragma unroll
+          for (int h = 0; h < kVectors; ++h)
+            held[e][h] = __builtin_bit_cast(u32x4, *reinterpret_cast<const piece_t<T>*>(at + kPiece<T> * h));
+        } else {
+          T some[8];
+#pragma unroll
+          for (int m = 0; m < 8; ++m) some[m] = m < count ? at[m] : static_cast<T>(0.0f);
+          __builtin_memcpy(&held[e], some, sizeof(some));
+        }
+      }
+    }
+  }
+
+  __device__ inline void store(char* lds) const {
+    if (!kWhole && line == 1 << 28) return;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      char* at = lds + to + e * kLines * kLineBytes;
+      if constexpr (S::kParts == 1) {
+        *reinterpret_cast<u32x4*>(at) = held[e][0];
+      } else {
+        u32x4 parts[3];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          unsigned a[3], b[3];
+          split(__builtin_bit_cast(float, static_cast<unsigned>(held[e][m / 2][m % 2 * 2])), a[0], a[1], a[2]);
+          split(__builtin_bit_cast(float, static_cast<unsigned>(held[e][m / 2][m % 2 * 2 + 1])), b[0], b[1], b[2]);
+#pragma unroll
+          for (int q = 0; q < 3; ++q) parts[q][m] = a[q] >> 16 | b[q];
+        }
+#pragma unroll
+        for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x4*>(at + q * kBytes) = parts[q];
+      }
+    }
+  }
+};
+
+// Reads kCount fragments of 16 rows, from row `first`: one address for each
+// that the exchange tells apart, the rest by constant offsets.
+template <typename T, bool C, int kRows, int kCount>
+struct Reader128 {
+  typedef Stage<T, C, kRows, true> G;
+  static constexpr int kDepth = Step<T>::kDepth;
+  static constexpr int kAddresses = C ? kCount : kDepth / 32;
+  int at[kAddresses];
+
+  __device__ inline Reader128(int first, int thread) {
+    const int lane = thread & 63, q = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < kAddresses; ++i) {
+      if constexpr (C)
+        at[i] = G::place(8 * q + ((lane & 15) >> 2), first / 8 + 2 * i + ((lane & 3) >> 1)) + (lane & 1) * 8;
+      else
+        at[i] = G::place(first + (lane & 15), 4 * i + q);
+    }
+  }
+
+  // Fragment r for 32 k from 32 * kk, of a part.
+  __device__ inline u32x4 read(const char* lds, int r, int kk, int part) const {
+    if constexpr (!C) {
+      return *reinterpret_cast<const u32x4*>(lds + at[kk] + r * 16 * G::kLineBytes + part * G::kBytes);
+    } else {
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+      u32x2 h[2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+        h[m] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                             (lds_s16x4)(lds + at[r] + (kk * 32 + m * 4) * G::kLineBytes + part * G::kBytes)));
+      return __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3);
+    }
+  }
+};
+
+// The tile's sums: wave (w / kAlong, w % kAlong) holds kA x kB fragments.
+template <int kRows>
+struct Sums128 {
+  static constexpr int kAlong = kRows == 128 ? 2 : 4;  // waves along the columns
+  static constexpr int kA = kRows == 128 ? 4 : 2;
+  static constexpr int kB = kRows == 128 ? 4 : 2;
+  f32x4 c[kA][kB];
+
+  __device__ inline void clear() {
+#pragma unroll
+    for (int i = 0; i < kA; ++i)
+#pragma unroll
+      for (int j = 0; j < kB; ++j) c[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  // f(row, column, four sums of neighbouring columns)
+  template <typename F>
+  __device__ inline void each(F f) const {
+    const int thread = thread_here(), lane = thread & 63, wave = thread >> 6;
+    const int row = wave / kAlong * kA * 16 + (lane & 15), col = wave % kAlong * kB * 16 + (lane >> 4) * 4;
+#pragma unroll
+    for (int i = 0; i < kA; ++i)
+#pragma unroll
+      for (int j = 0; j < kB; ++j) f(row + i * 16, col + j * 16, c[i][j]);
+  }
+};
+
+template <typename T, bool kAC, bool kBC, int kRows, bool kAligned>
+struct Tile128 {
+  typedef Step<T> S;
+  typedef Stage<T, kAC, kRows, kAligned> StageA;
+  typedef Stage<T, kBC, kCols128, kAligned> StageB;
+  static constexpr int kLdsBytes = S::kParts * (StageA::kBytes + StageB::kBytes);
+
+  // Adds the steps [from, to) of the sum over k of A(i, k) B(j, k).
+  template <int kPlanes>
+  __device__ static inline void add(const Operand<T>& a, const Operand<T>& b, char* lds, int64_t from, int64_t to,
+                                    Sums128<kRows>& s) {
+    const int thread = thread_here(), wave = thread >> 6;
+    StageA sa(a.ld, thread);
+    StageB sb(b.ld, thread);
+    char* lb = lds + S::kParts * StageA::kBytes;
+    typedef Sums128<kRows> Sums;
+    const Reader128<T, kAC, kRows, Sums::kA> ra(wave / Sums::kAlong * Sums::kA * 16, thread);
+    const Reader128<T, kBC, kCols128, Sums::kB> rb(wave % Sums::kAlong * Sums::kB * 16, thread);
+    const int64_t steps = (a.depth + S::kDepth - 1) / S::kDepth;  // of one plane
+    const int va = static_cast<int>(a.valid), vb = static_cast<int>(b.valid);
+    auto load = [&](int64_t t) {
+      const int64_t plane = kPlanes == 1 ? 0 : t / steps, k0 = (t - plane * steps) * S::kDepth;
+      const int64_t left = a.depth - k0;
+      const int most = static_cast<int>(left < S::kDepth ? left : S::kDepth);
+      sa.load((plane == 2 ? a.lo : a.p) + k0 * (kAC ? a.ld : 1), va, most);
+      sb.load((plane == 1 ? b.lo : b.p) + k0 * (kBC ? b.ld : 1), vb, most);
+    };
+    if (from < to) load(from);
+    for (int64_t t = from; t < to; ++t) {
+      __syncthreads();  // the last step's fragments have been read
+      sa.store(lds);
+      sb.store(lb);
+      if (t + 1 < to) load(t + 1);
+      __syncthreads();
+#pragma unroll
+      for (int kk = 0; kk < S::kDepth / 32; ++kk) {
+        u32x4 fa[Sums::kA][S::kParts];
+#pragma unroll
+        for (int i = 0; i < Sums::kA; ++i)
+#pragma unroll
+          for (int q = 0; q < S::kParts; ++q) fa[i][q] = ra.read(lds, i, kk, q);
+#pragma unroll
+        for (int j = 0; j < Sums::kB; ++j) {
+          u32x4 fb[S::kParts];
+#pragma unroll
+          for (int q = 0; q < S::kParts; ++q) fb[q] = rb.read(lb, j, kk, q);
+          if constexpr (S::kParts == 1) {
+#pragma unroll
+            for (int i = 0; i < Sums::kA; ++i)
+              s.c[i][j] = multiply<T>(fb[0], fa[i][0], s.c[i][j]);
+          } else {
+            // the smallest products first
+            constexpr int kOrder[8][2] = {{2, 1}, {1, 2}, {2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
+#pragma unroll
+            for (int o = 0; o < 8; ++o)
+#pragma unroll
+              for (int i = 0; i < Sums::kA; ++i)
+                s.c[i][j] = multiply<__bf16>(fb[kOrder[o][1]], fa[i][kOrder[o][0]], s.c[i][j]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+};
+
+}  // namespace mma
+}  // namespace spmm

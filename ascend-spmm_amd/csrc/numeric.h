@@ -2,6 +2,8 @@
 // orthogonalised updates): fp16, bf16 and fp32, with all arithmetic in fp32.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace spmm {

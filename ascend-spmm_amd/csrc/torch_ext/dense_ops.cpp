@@ -152,6 +152,12 @@ at::Tensor grouped_weight(const at::Tensor& w, bool* transposed) {
   return w.contiguous();
 }
 
+// Rows for the grouped products, whose row strides are below 2^22.
+at::Tensor as_grouped_rows(const at::Tensor& t) {
+  const at::Tensor rows = as_rows(t);
+  return row_stride(rows) < (int64_t(1) << 22) ? rows : rows.contiguous();
+}
+
 void check_grouped(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& offsets) {
   TORCH_CHECK_GPU(x);
   TORCH_CHECK_GPU(weight);
@@ -180,7 +186,7 @@ spmm_grouped_desc grouped_desc(const at::Tensor& rows, const at::Tensor& weight,
 at::Tensor grouped_forward(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& offsets) {
   c10::DeviceGuard guard(x.device());
   bool transposed;
-  const at::Tensor rows = as_rows(x), w = grouped_weight(weight, &transposed), off = offsets.contiguous();
+  const at::Tensor rows = as_grouped_rows(x), w = grouped_weight(weight, &transposed), off = offsets.contiguous();
   const spmm_grouped_desc d = grouped_desc(rows, w, transposed, off);
   at::Tensor out = at::empty({d.rows, d.width}, x.options());
   size_t bytes = 0;
@@ -205,7 +211,7 @@ struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
     const at::Tensor &x = saved[0], &weight = saved[1];
     c10::DeviceGuard guard(x.device());
     bool transposed;
-    const at::Tensor rows = as_rows(x), grad = as_rows(grads[0]), w = grouped_weight(weight, &transposed);
+    const at::Tensor rows = as_grouped_rows(x), grad = as_grouped_rows(grads[0]), w = grouped_weight(weight, &transposed);
     const at::Tensor off = saved[2].contiguous();
     spmm_grouped_desc d = grouped_desc(rows, w, transposed, off);
     d.grad_stride = row_stride(grad);

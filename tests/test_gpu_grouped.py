@@ -167,6 +167,28 @@ def test_one_group_of_many_rows(spmm_npu, dtype):
         check(got, ref, m, n, dtype, what)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("sizes,inner,width", [([9000, 0, 16001, 300], 264, 520), ([24999, 130, 3], 512, 264),
+                                               ([700, 1000, 24001], 192, 776)])
+def test_large_tiles(spmm_npu, sizes, inner, width, turned, dtype):
+    """Enough rows for the 256 x 256 tiles, whose last steps, rows and columns
+    are parts of one; rows before and behind the groups."""
+    before, after = 300, 77
+    rows = before + sum(sizes) + after
+    x, w, dy = make(rows, len(sizes), inner, width, dtype)
+    if turned:
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    inside = slice(before, before + sum(sizes))
+    want, mag, terms = plain(x[inside], w, edges_of(sizes), dy[inside])
+    y, dx, dw = run_all(spmm_npu.grouped_matmul, x, w, edges_of(sizes, before), dy)
+    check(y[inside], want[0], mag[0], terms[0], dtype, "y")
+    check(dx[inside], want[1], mag[1], terms[1], dtype, "dx")
+    check(dw, want[2], mag[2], terms[2], dtype, "dw")
+    for t in (y, dx):
+        assert not t[:before].any() and not t[before + sum(sizes):].any()
+
+
 def test_offsets_past_32_bits(spmm_npu):
     """x of more than 2^31 elements: its last rows are where they should be."""
     rows, inner, width = 270_000, 8192, 16
