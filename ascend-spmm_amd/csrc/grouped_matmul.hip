@@ -106,22 +106,6 @@ __device__ inline void store_four(T* to, int64_t cols, f32x4 v) {
   }
 }
 
-// Work-groups run on the XCDs in turn; each XCD gets one run of the tiles, so
-// that neighbours share its L2.
-__device__ inline int64_t run_of_xcd(int64_t block, int64_t blocks) {
-  const int64_t each = blocks / kXcds, rest = blocks % kXcds, x = block % kXcds;
-  return x * each + (x < rest ? x : rest) + block / kXcds;
-}
-
-// Tile `n` of down x across: blocks of four tile rows, down them first, so
-// that the tiles at work together share rows of both operands.
-__device__ inline void place_tile(int64_t n, int64_t down, int64_t across, int64_t& i, int64_t& j) {
-  const int64_t block = n / (4 * across), first = 4 * block, high = down - first < 4 ? down - first : 4;
-  const int64_t m = n - block * 4 * across;
-  i = first + m % high;
-  j = m / high;
-}
-
 // The engines of one product: Large of mma_256.h, Small of mma_128.h.
 template <typename T, bool kAC, bool kBC>
 struct Large {
@@ -149,7 +133,7 @@ struct Small {
   mma::Sums128<kHeight> s;
   __device__ inline void sum(const mma::Operand<T>& a, const mma::Operand<T>& b, char* lds) {
     s.clear();
-    Tile::template add<1>(a, b, lds, 0, (a.depth + kStep - 1) / kStep, s);
+    Tile::add(a, b, lds, 0, (a.depth + kStep - 1) / kStep, s);
   }
   template <typename F>
   __device__ inline void each(F f) const {
@@ -166,7 +150,7 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
   __shared__ __align__(1024) char lds[E::kLds];
   const int64_t across = (a.width + E::kCols - 1) / E::kCols;
   int64_t i, j;
-  place_tile(run_of_xcd(blockIdx.x, gridDim.x), down, across, i, j);
+  mma::place_tile(mma::run_of_xcd(blockIdx.x, gridDim.x), down, across, i, j);
   RowRange r;
   if (!find_rows(a, E::kRows, i, r)) return;
   const int64_t c0 = j * E::kCols;
@@ -213,7 +197,7 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
   int64_t total;
   steps.find(a, INT64_MAX, total);
   total = uniform(total);
-  const int64_t part = run_of_xcd(blockIdx.x, gridDim.x);
+  const int64_t part = mma::run_of_xcd(blockIdx.x, gridDim.x);
   const int64_t u0 = part_start(total, part, gridDim.x), u1 = part_start(total, part + 1, gridDim.x);
   for (int64_t u = u0; u < u1;) {
     int64_t before;
@@ -223,7 +207,7 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
     const int64_t tile = (u - before) / n, s0 = (u - before) % n;
     const int64_t s1 = n - s0 < u1 - u ? n : s0 + (u1 - u);
     int64_t i, j;
-    place_tile(tile, down, across, i, j);
+    mma::place_tile(tile, down, across, i, j);
     const int64_t i0 = i * E::kRows, j0 = j * E::kCols;
     const int64_t rows = a.inner - i0 < E::kRows ? a.inner - i0 : E::kRows;
     const int64_t cols = a.width - j0 < E::kCols ? a.width - j0 : E::kCols;
@@ -271,7 +255,7 @@ __global__ __launch_bounds__(256) void join_pieces(GroupedArgs a, int64_t tile_r
     s += *reinterpret_cast<const f32x4*>(pieces + (2 * part + (at >= u0 ? 0 : 1)) * tile_rows * tile_cols + e);
   }
   int64_t i, j;
-  place_tile(tile, down, across, i, j);
+  mma::place_tile(tile, down, across, i, j);
   const int64_t row = i * tile_rows + e / tile_cols, col = j * tile_cols + e % tile_cols;
   if (row < a.inner && col < a.width) store_four(dweight + (g * a.inner + row) * a.width + col, a.width - col, s);
 }

@@ -38,6 +38,22 @@ __device__ inline unsigned lds_address(const void* p) {
   return static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_ptr)p));
 }
 
+// Work-groups run on the XCDs in turn; each XCD gets one run of the tiles, so
+// that neighbours share its L2.
+__device__ inline int64_t run_of_xcd(int64_t block, int64_t blocks) {
+  const int64_t each = blocks / kXcds, rest = blocks % kXcds, x = block % kXcds;
+  return x * each + (x < rest ? x : rest) + block / kXcds;
+}
+
+// Tile `n` of down x across: blocks of four tile rows, down them first, so
+// that the tiles at work together share rows of both operands.
+__device__ inline void place_tile(int64_t n, int64_t down, int64_t across, int64_t& i, int64_t& j) {
+  const int64_t block = n / (4 * across), first = 4 * block, high = down - first < 4 ? down - first : 4;
+  const int64_t m = n - block * 4 * across;
+  i = first + m % high;
+  j = m / high;
+}
+
 // The 16 x 16 x 32 matrix instruction: lane (i = lane % 16, q = lane / 16) holds
 // k = 8 q .. 8 q + 7 of row i of either operand, and gets the sums of b's row i
 // with a's rows 4 q .. 4 q + 3.

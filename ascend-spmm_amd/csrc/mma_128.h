@@ -20,11 +20,11 @@ namespace mma {
 constexpr int kCols128 = 128;
 constexpr int kThreads128 = 256;
 
-template <typename T>
+// kPair: fp16 operands held as the sum of two planes in memory.
+template <typename T, bool kPair = false>
 struct Step {
-  static constexpr int kParts = std::is_same_v<T, float> ? 3 : 1;
+  static constexpr int kParts = std::is_same_v<T, float> ? 3 : kPair ? 2 : 1;
   static constexpr int kDepth = std::is_same_v<T, float> ? 32 : 64;
-  typedef std::conditional_t<std::is_same_v<T, float>, __bf16, T> Part;
 };
 
 // Three bf16 parts of fp32 values, by truncation: all parts of a value have its
@@ -49,9 +49,9 @@ __device__ inline void split(float x, unsigned& hi, unsigned& mid, unsigned& lo)
 // 16-byte pieces are exchanged by the line; else lines of kRows elements whose
 // 32-byte units are exchanged by k.  A thread's pieces lie whole rounds of
 // lines apart, which leaves the exchange alike: one offset serves them all.
-template <typename T, bool C, int kRows, bool kAligned>
+template <typename T, bool C, int kRows, bool kAligned, bool kPair = false>
 struct Stage {
-  typedef Step<T> S;
+  typedef Step<T, kPair> S;
   static constexpr int kPieces = kRows * S::kDepth / 8;  // of eight elements
   static constexpr int kEach = (kPieces + kThreads128 - 1) / kThreads128;
   static constexpr bool kWhole = kPieces % kThreads128 == 0;  // else the last threads have none
@@ -79,7 +79,7 @@ struct Stage {
       return line * kLineBytes + (piece ^ (line >> 1 & 3)) * 16;
   }
 
-  __device__ inline Stage(int64_t ld, int thread) {
+  __device__ inline void start(int64_t ld, int thread) {
     line = thread / kAcross;
     piece = thread % kAcross;
     from = static_cast<unsigned>(line * ld) + piece * 8;
@@ -123,7 +123,7 @@ struct Stage {
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       char* at = lds + to + e * kLines * kLineBytes;
-      if constexpr (S::kParts == 1) {
+      if constexpr (S::kParts < 3) {
         *reinterpret_cast<u32x4*>(at) = held[e][0];
       } else {
         u32x4 parts[3];
@@ -147,7 +147,7 @@ struct Stage {
 template <typename T, bool C, int kRows, int kCount>
 struct Reader128 {
   typedef Stage<T, C, kRows, true> G;
-  static constexpr int kDepth = Step<T>::kDepth;
+  static constexpr int kDepth = G::S::kDepth;
   static constexpr int kAddresses = C ? kCount : kDepth / 32;
   int at[kAddresses];
 
@@ -206,38 +206,47 @@ struct Sums128 {
   }
 };
 
-template <typename T, bool kAC, bool kBC, int kRows, bool kAligned>
+template <typename T, bool kAC, bool kBC, int kRows, bool kAligned, bool kPair = false>
 struct Tile128 {
-  typedef Step<T> S;
-  typedef Stage<T, kAC, kRows, kAligned> StageA;
-  typedef Stage<T, kBC, kCols128, kAligned> StageB;
+  typedef Step<T, kPair> S;
+  typedef Stage<T, kAC, kRows, kAligned, kPair> StageA;
+  typedef Stage<T, kBC, kCols128, kAligned, kPair> StageB;
   static constexpr int kLdsBytes = S::kParts * (StageA::kBytes + StageB::kBytes);
 
   // Adds the steps [from, to) of the sum over k of A(i, k) B(j, k).
-  template <int kPlanes>
   __device__ static inline void add(const Operand<T>& a, const Operand<T>& b, char* lds, int64_t from, int64_t to,
                                     Sums128<kRows>& s) {
+    constexpr int kPlanes = kPair ? 2 : 1;
     const int thread = thread_here(), wave = thread >> 6;
-    StageA sa(a.ld, thread);
-    StageB sb(b.ld, thread);
     char* lb = lds + S::kParts * StageA::kBytes;
     typedef Sums128<kRows> Sums;
     const Reader128<T, kAC, kRows, Sums::kA> ra(wave / Sums::kAlong * Sums::kA * 16, thread);
     const Reader128<T, kBC, kCols128, Sums::kB> rb(wave % Sums::kAlong * Sums::kB * 16, thread);
-    const int64_t steps = (a.depth + S::kDepth - 1) / S::kDepth;  // of one plane
     const int va = static_cast<int>(a.valid), vb = static_cast<int>(b.valid);
+    StageA sa[kPlanes];
+    StageB sb[kPlanes];
+#pragma unroll
+    for (int q = 0; q < kPlanes; ++q) {
+      sa[q].start(a.ld, thread);
+      sb[q].start(b.ld, thread);
+    }
     auto load = [&](int64_t t) {
-      const int64_t plane = kPlanes == 1 ? 0 : t / steps, k0 = (t - plane * steps) * S::kDepth;
-      const int64_t left = a.depth - k0;
+      const int64_t k0 = t * S::kDepth, left = a.depth - k0;
       const int most = static_cast<int>(left < S::kDepth ? left : S::kDepth);
-      sa.load((plane == 2 ? a.lo : a.p) + k0 * (kAC ? a.ld : 1), va, most);
-      sb.load((plane == 1 ? b.lo : b.p) + k0 * (kBC ? b.ld : 1), vb, most);
+#pragma unroll
+      for (int q = 0; q < kPlanes; ++q) {
+        sa[q].load((q == 0 ? a.p : a.lo) + k0 * (kAC ? a.ld : 1), va, most);
+        sb[q].load((q == 0 ? b.p : b.lo) + k0 * (kBC ? b.ld : 1), vb, most);
+      }
     };
     if (from < to) load(from);
     for (int64_t t = from; t < to; ++t) {
       __syncthreads();  // the last step's fragments have been read
-      sa.store(lds);
-      sb.store(lb);
+#pragma unroll
+      for (int q = 0; q < kPlanes; ++q) {
+        sa[q].store(lds + q * StageA::kBytes);
+        sb[q].store(lb + q * StageB::kBytes);
+      }
       if (t + 1 < to) load(t + 1);
       __syncthreads();
 #pragma unroll
@@ -252,19 +261,15 @@ struct Tile128 {
           u32x4 fb[S::kParts];
 #pragma unroll
           for (int q = 0; q < S::kParts; ++q) fb[q] = rb.read(lb, j, kk, q);
-          if constexpr (S::kParts == 1) {
+          // products of parts, the smallest first
+          constexpr int kProducts = S::kParts == 1 ? 1 : S::kParts == 2 ? 3 : 8;
+          constexpr int kOrder[8][2] = {{0, 0}, {0, 1}, {1, 0}, {1, 1}, {0, 2}, {2, 0}, {1, 2}, {2, 1}};
+          typedef std::conditional_t<S::kParts == 3, __bf16, T> Part;
+#pragma unroll
+          for (int o = kProducts - 1; o >= 0; --o)
 #pragma unroll
             for (int i = 0; i < Sums::kA; ++i)
-              s.c[i][j] = multiply<T>(fb[0], fa[i][0], s.c[i][j]);
-          } else {
-            // the smallest products first
-            constexpr int kOrder[8][2] = {{2, 1}, {1, 2}, {2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
-#pragma unroll
-            for (int o = 0; o < 8; ++o)
-#pragma unroll
-              for (int i = 0; i < Sums::kA; ++i)
-                s.c[i][j] = multiply<__bf16>(fb[kOrder[o][1]], fa[i][kOrder[o][0]], s.c[i][j]);
-          }
+              s.c[i][j] = multiply<Part>(fb[kOrder[o][1]], fa[i][kOrder[o][0]], s.c[i][j]);
         }
       }
     }

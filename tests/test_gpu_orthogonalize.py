@@ -83,6 +83,14 @@ def test_stacks(spmm_npu, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(49, 300, 257), (25, 250, 900), (200, 130, 130)])
+def test_large_tiles(spmm_npu, shape, dtype):
+    """Enough tiles of 256 x 256 for the chip, whole and in part."""
+    u = make(shape, dtype)
+    check(spmm_npu.orthogonalize(u), plain(u), dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("steps,coefficients", [
     (0, ABC), (1, ABC), (2, (1.5, -0.5, 0.0)), (10, (1.5, -0.5, 0.0)), (3, (2.0, -1.5, 0.5)),
     (3, [(8.2, -23.5, 17.3), (4.1, -2.9, 0.5), (3.9, -2.8, 0.5)]), (1, (0.0, 0.0, 0.0)), (2, (30.0, 5.0, 2.0))])
