@@ -9,16 +9,16 @@
 // out and dx: one work-group per tile, none across a group's end; which group
 // a tile belongs to is found on the device by one wave-wide scan of offsets.
 //
-// dW: groups differ in length and there may be few tiles, so the steps of all
-// tiles' sums are counted through and cut into equal parts, one for each
-// work-group.  A tile inside one part is written at once; the pieces of one
-// that is cut go to the workspace in fp32 and are added in order.
+// dW: groups differ in length and there may be few tiles, so the rows of all
+// groups are counted through and cut into equal ranges, and a work-group sums
+// one tile over one range, group after group.  A group inside one range is
+// written at once; the pieces of one that is cut go to the workspace in fp32
+// and are added in order.
 #include <climits>
 #include <type_traits>
 #include <utility>
 
-#include "mma_128.h"
-#include "mma_256.h"
+#include "mma_ring.h"
 
 namespace spmm {
 namespace {
@@ -141,6 +141,23 @@ struct Small {
   }
 };
 
+template <typename T, bool kAC, bool kBC>
+struct Middle {
+  typedef T Value;
+  typedef mma::Ring<T, kAC, kBC, false> Tile;
+  static constexpr int kRows = 128, kCols = mma::kCols128, kThreads = mma::kThreads128, kStep = Tile::kDepth;
+  static constexpr int kLds = Tile::kLdsBytes, kPerCu = 2;
+  mma::Sums128<128> s;
+  __device__ inline void sum(const mma::Operand<T>& a, const mma::Operand<T>& b, char* lds) {
+    s.clear();
+    Tile::add(a, b, lds, 0, static_cast<int>((a.depth + kStep - 1) / kStep), s);
+  }
+  template <typename F>
+  __device__ inline void each(F f) const {
+    s.each(f);
+  }
+};
+
 // out or dx; kTurned: the weights' depth is their contiguous extent.
 template <typename E, bool kTurned>
 __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void grouped_rows(
@@ -167,51 +184,48 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
   e.each(store);
 }
 
-// Steps of the sums of all tiles of dW, counted group by group and tile by
-// tile; an empty group's tiles have one step each, which adds nothing.
-struct Steps {
-  int64_t tiles, depth;  // tiles of a matrix; rows of a step
-  __device__ inline int64_t of(const GroupedArgs& a, int64_t g) const {
-    const int64_t n = edge(a, g + 1) - edge(a, g);
-    return n > 0 ? (n + depth - 1) / depth : 1;
-  }
-  __device__ inline int64_t find(const GroupedArgs& a, int64_t at, int64_t& before) const {
-    return find_segment(a.groups, at, [&](int64_t g) { return tiles * of(a, g); }, before);
-  }
-};
-__device__ __host__ inline int64_t part_start(int64_t total, int64_t part, int64_t parts) {
-  return total / parts * part + total % parts * part / parts;
+// dW's sums run over the rows of all groups, counted in steps of 64 (an empty
+// group has one, which adds nothing) and cut into `parts` equal ranges.  The
+// cuts depend on sizes alone, so every engine adds in the same order.
+constexpr int kRowStep = 64;
+__device__ inline int64_t steps_of(const GroupedArgs& a, int64_t g) {
+  const int64_t n = edge(a, g + 1) - edge(a, g);
+  return n > 0 ? (n + kRowStep - 1) / kRowStep : 1;
 }
+__device__ inline int64_t find_step(const GroupedArgs& a, int64_t at, int64_t& before) {
+  return find_segment(a.groups, at, [&](int64_t g) { return steps_of(a, g); }, before);
+}
+__device__ inline int64_t part_start(int64_t total, int64_t part, int64_t parts) { return total * part / parts; }
 
-// pieces: [parts][2][tile] fp32; a part's first piece goes to its first
-// place, a later one to its second.
+// A work-group sums one tile over one range; tiles of a range are neighbours,
+// which share its rows in their XCD's L2.  The pieces of groups that a range
+// cuts go to pieces [parts][tiles][2][tile] in fp32: a range's first group to
+// the first place, its last one to the second.
 template <typename E>
 __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void grouped_weights(
     GroupedArgs a, const typename E::Value* __restrict__ left, int64_t left_stride,
     const typename E::Value* __restrict__ right, int64_t right_stride, typename E::Value* __restrict__ dweight,
-    float* __restrict__ pieces) {
+    int64_t parts, float* __restrict__ pieces) {
   typedef typename E::Value T;
   __shared__ __align__(1024) char lds[E::kLds];
   const int64_t across = (a.width + E::kCols - 1) / E::kCols, down = (a.inner + E::kRows - 1) / E::kRows;
-  const Steps steps{across * down, E::kStep};
   int64_t total;
-  steps.find(a, INT64_MAX, total);
+  find_step(a, INT64_MAX, total);
   total = uniform(total);
-  const int64_t part = mma::run_of_xcd(blockIdx.x, gridDim.x);
-  const int64_t u0 = part_start(total, part, gridDim.x), u1 = part_start(total, part + 1, gridDim.x);
+  const int64_t block = mma::run_of_xcd(blockIdx.x, gridDim.x);
+  const int64_t part = block / (across * down);
+  int64_t i, j;
+  mma::place_tile(block % (across * down), down, across, i, j);
+  const int64_t i0 = i * E::kRows, j0 = j * E::kCols;
+  const int64_t rows = a.inner - i0 < E::kRows ? a.inner - i0 : E::kRows;
+  const int64_t cols = a.width - j0 < E::kCols ? a.width - j0 : E::kCols;
+  const int64_t u0 = part_start(total, part, parts), u1 = part_start(total, part + 1, parts);
   for (int64_t u = u0; u < u1;) {
     int64_t before;
-    const int64_t g = uniform(steps.find(a, u, before));
-    before = uniform(before);
-    const int64_t lo = uniform(edge(a, g)), hi = uniform(edge(a, g + 1)), n = uniform(steps.of(a, g));
-    const int64_t tile = (u - before) / n, s0 = (u - before) % n;
-    const int64_t s1 = n - s0 < u1 - u ? n : s0 + (u1 - u);
-    int64_t i, j;
-    mma::place_tile(tile, down, across, i, j);
-    const int64_t i0 = i * E::kRows, j0 = j * E::kCols;
-    const int64_t rows = a.inner - i0 < E::kRows ? a.inner - i0 : E::kRows;
-    const int64_t cols = a.width - j0 < E::kCols ? a.width - j0 : E::kCols;
-    const int64_t first = lo + s0 * E::kStep, last = lo + s1 * E::kStep < hi ? lo + s1 * E::kStep : hi;
+    const int64_t g = uniform(find_step(a, u, before));
+    const int64_t lo = uniform(edge(a, g)), hi = uniform(edge(a, g + 1)), n = uniform(steps_of(a, g));
+    const int64_t s0 = u - uniform(before), s1 = n - s0 < u1 - u ? n : s0 + (u1 - u);
+    const int64_t first = lo + s0 * kRowStep, last = lo + s1 * kRowStep < hi ? lo + s1 * kRowStep : hi;
     const int64_t depth = last > first ? last - first : 0;
     E e;
     e.sum({left + first * left_stride + i0, nullptr, left_stride, rows, depth},
@@ -222,38 +236,37 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
         if (row < rows && col < cols) store_four(to + row * a.width + col, cols - col, v);
       });
     } else {
-      float* to = pieces + (2 * part + (u == u0 ? 0 : 1)) * E::kRows * E::kCols;
+      float* to = pieces + (2 * block + (u == u0 ? 0 : 1)) * E::kRows * E::kCols;
       e.each([&](int row, int col, f32x4 v) { *reinterpret_cast<f32x4*>(to + row * E::kCols + col) = v; });
     }
     u += s1 - s0;
   }
 }
 
-// Adds the pieces of the tiles that were cut; a work-group takes 1024 sums.
+// Adds the pieces of the groups that were cut; a work-group takes 1024 sums.
 template <typename T>
-__global__ __launch_bounds__(256) void join_pieces(GroupedArgs a, int64_t tile_rows, int64_t tile_cols, int64_t step,
-                                                   int64_t parts, const float* __restrict__ pieces,
-                                                   T* __restrict__ dweight) {
+__global__ __launch_bounds__(256) void join_pieces(GroupedArgs a, int64_t tile_rows, int64_t tile_cols, int64_t parts,
+                                                   const float* __restrict__ pieces, T* __restrict__ dweight) {
   const int64_t across = (a.width + tile_cols - 1) / tile_cols, down = (a.inner + tile_rows - 1) / tile_rows;
-  const Steps steps{across * down, step};
-  const int64_t slices = tile_rows * tile_cols / 1024;
-  const int64_t g = blockIdx.x / (slices * steps.tiles), tile = blockIdx.x / slices % steps.tiles;
+  const int64_t tiles = across * down, size = tile_rows * tile_cols, slices = size / 1024;
+  const int64_t g = blockIdx.x / (slices * tiles), tile = blockIdx.x / slices % tiles;
   int64_t total, before;
-  steps.find(a, INT64_MAX, total);
-  find_segment(a.groups, INT64_MAX, [&](int64_t s) { return s < g ? steps.tiles * steps.of(a, s) : 0; }, before);
-  const int64_t n = steps.of(a, g), u0 = before + tile * n, u1 = u0 + n;
-  // the part that holds the tile's first step
-  int64_t part = static_cast<int64_t>(static_cast<double>(u0) / static_cast<double>(total) * static_cast<double>(parts));
+  find_step(a, INT64_MAX, total);
+  find_segment(a.groups, INT64_MAX, [&](int64_t s) { return s < g ? steps_of(a, s) : 0; }, before);
+  const int64_t u0 = before, u1 = u0 + steps_of(a, g);
+  // the range that holds the group's first step
+  int64_t part = u0 * parts / total;
   while (part > 0 && part_start(total, part, parts) > u0) --part;
   while (part_start(total, part + 1, parts) <= u0) ++part;
   if (part_start(total, part + 1, parts) >= u1) return;  // written whole
   const int64_t e = blockIdx.x % slices * 1024 + threadIdx.x * 4;
-  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (; part < parts && part_start(total, part, parts) < u1; ++part) {
-    const int64_t at = part_start(total, part, parts);
-    if (at == part_start(total, part + 1, parts)) continue;
-    s += *reinterpret_cast<const f32x4*>(pieces + (2 * part + (at >= u0 ? 0 : 1)) * tile_rows * tile_cols + e);
-  }
+  const float* from = pieces + tile * 2 * size + e;
+  f32x4 s = *reinterpret_cast<const f32x4*>(from + (part * tiles * 2 + (part_start(total, part, parts) < u0)) * size);
+  // ranges that start inside the group
+  int64_t end = part + 1;
+  while (end < parts && part_start(total, end, parts) < u1) ++end;
+#pragma unroll 4
+  for (++part; part < end; ++part) s += *reinterpret_cast<const f32x4*>(from + part * tiles * 2 * size);
   int64_t i, j;
   mma::place_tile(tile, down, across, i, j);
   const int64_t row = i * tile_rows + e / tile_cols, col = j * tile_cols + e % tile_cols;
@@ -296,35 +309,56 @@ bool pieces_aligned(const spmm_grouped_desc* d, const void* x, const void* weigh
 
 constexpr int64_t kCus = 256;
 
-// The large tile for out and dx: a matrix must fit the copies' 32-bit count of
-// pieces; at least three quarters of the CUs get a tile, and the groups'
+// The large tile for out and dx: at least three quarters of the CUs get a tile, and the groups'
 // average fills half of one.  65536 x 1024 x 2048 bf16 in 8 groups: 289 us
 // with it, 413 with the small tile.
 bool large_rows(const GroupedArgs& a) {
-  return a.width > mma::kCols128 && a.inner * a.width < (int64_t(1) << 33) && a.inner >= 2 * mma::kDepth && a.rows / mma::kTile * ceil_div(a.width, mma::kTile) >= kCus * 3 / 4 &&
+  return a.width > mma::kCols128 && a.inner >= 2 * mma::kDepth && a.rows / mma::kTile * ceil_div(a.width, mma::kTile) >= kCus * 3 / 4 &&
          a.rows >= a.groups * mma::kTile / 2;
 }
 
 // The low tile where the groups' average leaves most of a tile of 128 empty.
 bool low_rows(const GroupedArgs& a) { return a.rows <= 48 * a.groups; }
 
-bool large_weights(const GroupedArgs& a, int64_t stride, int64_t other) {
-  return a.inner > mma::kCols128 && a.width > mma::kCols128 &&
-         a.rows * (stride > other ? stride : other) < (int64_t(1) << 33) && a.rows >= 4 * mma::kDepth * a.groups;
+// Copies count an operand's pieces in 32 bits.
+bool small_counts(const GroupedArgs& a, int64_t stride, int64_t other) {
+  return a.rows * (stride > other ? stride : other) < (int64_t(1) << 33);
 }
 
-// Parts of dW's steps: one round of work-groups, each with eight steps or more
-// on average, so that pieces cost little beside their sums.
-template <typename E>
+bool large_weights(const GroupedArgs& a) {
+  return a.inner > mma::kCols128 && a.width > mma::kCols128 && a.rows >= 4 * mma::kDepth * a.groups;
+}
+
+// Ranges that dW's rows are cut into: the number that takes the least time by
+// this count, in microseconds.  A round of work-groups takes its steps (1 each
+// for the large tile, 0.5 for two of the small one on a CU); a cut costs a
+// piece of each tile written and read at 4 TB/s, and joining a launch.
 int64_t weight_parts(const GroupedArgs& a) {
-  const int64_t tiles = ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols);
-  const int64_t steps = (a.rows / E::kStep + a.groups) * tiles;
-  const int64_t most = kCus * E::kPerCu, want = ceil_div(steps, 8);
-  return want < most ? want : most;
+  const bool large = large_weights(a);
+  const int64_t side = large ? mma::kTile : 128, at_once = kCus * (large ? 1 : 2);
+  const int64_t tiles = ceil_div(a.inner, side) * ceil_div(a.width, side);
+  const int64_t steps = a.rows / kRowStep + a.groups;
+  if (tiles == 0 || steps == 0) return 1;
+  const double step = large ? 1.0 : 0.5, piece = static_cast<double>(tiles * side * side) * 8.0 / 4e6;
+  int64_t best = 1;
+  double least = 1e300;
+  auto consider = [&](int64_t parts) {
+    if (parts < 1 || parts > steps) return;
+    const double time = static_cast<double>(ceil_div(parts * tiles, at_once) * ceil_div(steps, parts)) * step +
+                        (parts > 1 ? static_cast<double>(parts) * piece + 4.0 : 0.0);
+    if (time < least) {
+      least = time;
+      best = parts;
+    }
+  };
+  for (int64_t p = 1; p <= 4; ++p) consider(p);
+  for (int64_t k = 1; k <= 32; ++k) consider(at_once * k / (8 * tiles));
+  return best;
 }
 template <typename E>
 size_t weight_bytes(const GroupedArgs& a) {
-  return static_cast<size_t>(weight_parts<E>(a)) * 2 * E::kRows * E::kCols * sizeof(float);
+  const int64_t parts = weight_parts(a), tiles = ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols);
+  return parts == 1 ? 0 : static_cast<size_t>(parts * tiles) * 2 * E::kRows * E::kCols * sizeof(float);
 }
 
 // Calls f with null pointers of the value type.
@@ -357,13 +391,18 @@ template <typename T, bool kTurned>
 spmm_status run_rows(const GroupedArgs& a, bool aligned, const void* in, const void* weight, void* out, hipStream_t s,
                      const char* op) {
   if (a.rows == 0 || a.width == 0) return SPMM_OK;
+  // (copies count a matrix's pieces in 32 bits)
+  aligned = aligned && a.inner * a.width < (int64_t(1) << 33);
   if constexpr (sizeof(T) == 2)
     if (aligned && large_rows(a)) return launch_rows<Large<T, false, !kTurned>, kTurned>(a, in, weight, out, s, op);
   if (low_rows(a))
     return aligned ? launch_rows<Small<T, false, !kTurned, 32, true>, kTurned>(a, in, weight, out, s, op)
                    : launch_rows<Small<T, false, !kTurned, 32, false>, kTurned>(a, in, weight, out, s, op);
-  return aligned ? launch_rows<Small<T, false, !kTurned, 128, true>, kTurned>(a, in, weight, out, s, op)
-                 : launch_rows<Small<T, false, !kTurned, 128, false>, kTurned>(a, in, weight, out, s, op);
+  if constexpr (sizeof(T) == 2)
+    if (aligned) return launch_rows<Middle<T, false, !kTurned>, kTurned>(a, in, weight, out, s, op);
+  if constexpr (sizeof(T) == 4)
+    if (aligned) return launch_rows<Small<T, false, !kTurned, 128, true>, kTurned>(a, in, weight, out, s, op);
+  return launch_rows<Small<T, false, !kTurned, 128, false>, kTurned>(a, in, weight, out, s, op);
 }
 
 template <typename E>
@@ -372,19 +411,19 @@ spmm_status launch_weights(const GroupedArgs& a, const void* left, int64_t left_
                            const char* op) {
   typedef typename E::Value T;
   const size_t need = weight_bytes<E>(a);
-  if (ws == nullptr || ws_bytes < need)
+  if (need > 0 && (ws == nullptr || ws_bytes < need))
     return fail(SPMM_ERR_CONTRACT, std::string(op) + ": workspace too small: need " + std::to_string(need) + " bytes");
-  const int64_t parts = weight_parts<E>(a);
-  const int64_t slices =
-      a.groups * ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols) * (E::kRows * E::kCols / 1024);
-  if (spmm_status st = check_grid(slices, op)) return st;
-  hipLaunchKernelGGL(grouped_weights<E>, dim3(static_cast<unsigned>(parts)), dim3(E::kThreads), 0, s, a,
+  const int64_t parts = weight_parts(a), tiles = ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols);
+  const int64_t slices = a.groups * tiles * (E::kRows * E::kCols / 1024);
+  if (spmm_status st = check_grid(slices > parts * tiles ? slices : parts * tiles, op)) return st;
+  hipLaunchKernelGGL(grouped_weights<E>, dim3(static_cast<unsigned>(parts * tiles)), dim3(E::kThreads), 0, s, a,
                      static_cast<const T*>(left), left_stride, static_cast<const T*>(right), right_stride,
-                     static_cast<T*>(dweight), static_cast<float*>(ws));
+                     static_cast<T*>(dweight), parts, static_cast<float*>(ws));
   if (spmm_status st = check_launch(op)) return st;
+  if (parts == 1) return SPMM_OK;
   hipLaunchKernelGGL(join_pieces<T>, dim3(static_cast<unsigned>(slices)), dim3(256), 0, s, a,
-                     static_cast<int64_t>(E::kRows), static_cast<int64_t>(E::kCols), static_cast<int64_t>(E::kStep),
-                     parts, static_cast<const float*>(ws), static_cast<T*>(dweight));
+                     static_cast<int64_t>(E::kRows), static_cast<int64_t>(E::kCols), parts,
+                     static_cast<const float*>(ws), static_cast<T*>(dweight));
   return check_launch(op);
 }
 
@@ -411,8 +450,11 @@ struct WeightSides {
 template <typename T, typename F>
 spmm_status with_weight_engine(const GroupedArgs& a, bool aligned, int64_t stride, int64_t other, F f) {
   if constexpr (sizeof(T) == 2)
-    if (aligned && large_weights(a, stride, other)) return f(static_cast<Large<T, true, true>*>(nullptr));
-  if (aligned) return f(static_cast<Small<T, true, true, 128, true>*>(nullptr));
+    if (aligned && small_counts(a, stride, other))
+      return large_weights(a) ? f(static_cast<Large<T, true, true>*>(nullptr))
+                              : f(static_cast<Middle<T, true, true>*>(nullptr));
+  if constexpr (sizeof(T) == 4)
+    if (aligned) return f(static_cast<Small<T, true, true, 128, true>*>(nullptr));
   return f(static_cast<Small<T, true, true, 128, false>*>(nullptr));
 }
 

@@ -26,8 +26,7 @@
 #include <type_traits>
 #include <utility>
 
-#include "mma_128.h"
-#include "mma_256.h"
+#include "mma_ring.h"
 
 namespace spmm {
 namespace {
@@ -200,8 +199,8 @@ __global__ __launch_bounds__(mma::kThreads, 2) void product_large(Product p, Fin
 }
 
 template <typename T, bool kTurned, bool kPair>
-__global__ __launch_bounds__(mma::kThreads128, kPair ? 2 : 3) void product_small(Product p, Finish f) {
-  typedef mma::Tile128<half, false, kTurned, 128, true, kPair> Tile;
+__global__ __launch_bounds__(mma::kThreads128, kPair ? 1 : 2) void product_small(Product p, Finish f) {
+  typedef mma::Ring<half, false, kTurned, kPair> Tile;
   __shared__ __align__(1024) char lds[Tile::kLdsBytes];
   const int64_t down = (p.m + 127) / 128, across = (p.n + 127) / 128;
   const int64_t block = mma::run_of_xcd(blockIdx.x, gridDim.x);
@@ -209,11 +208,11 @@ __global__ __launch_bounds__(mma::kThreads128, kPair ? 2 : 3) void product_small
   int64_t i, j;
   mma::place_tile(block % (down * across), down, across, i, j);
   const int64_t r0 = i * 128, c0 = j * 128;
-  const int64_t steps = (p.depth + mma::kDepth - 1) / mma::kDepth;
+  const int64_t steps = (p.depth + Tile::kDepth - 1) / Tile::kDepth;
   mma::Sums128<128> s;
   s.clear();
   Tile::add(operand(p.left, batch, r0, 128, p.m, p.depth, false), operand(p.right, batch, c0, 128, p.n, p.depth, kTurned),
-            lds, steps * split / p.splits, steps * (split + 1) / p.splits, s);
+            lds, static_cast<int>(steps * split / p.splits), static_cast<int>(steps * (split + 1) / p.splits), s);
   const int64_t batches = gridDim.x / (down * across * p.splits);
   float* to = p.sums + (split * batches + batch) * p.m * p.n;
   s.each([&](int row, int col, f32x4 v) {
