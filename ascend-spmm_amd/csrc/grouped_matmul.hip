@@ -106,6 +106,15 @@ __device__ inline void store_four(T* to, int64_t cols, f32x4 v) {
   }
 }
 
+// Calls f(row, column, four sums of neighbouring columns) for the lane's part
+// of a tile.
+template <typename S, typename F>
+__device__ inline void each_four(S& s, F f) {
+  s.place();
+#pragma unroll
+  for (int k = 0; k < S::kFours; ++k) f(s.row(k), s.col(k), s.four(k));
+}
+
 // The engines of one product: Large of mma_256.h, Small of mma_128.h.
 template <typename T, bool kAC, bool kBC>
 struct Large {
@@ -117,8 +126,8 @@ struct Large {
     mma::multiply_tile<T, kAC, kBC, 1>(a, b, lds, s);
   }
   template <typename F>
-  __device__ inline void each(F f) const {
-    mma::for_sums(s, f);
+  __device__ inline void each(F f) {
+    each_four(s, f);
   }
 };
 
@@ -136,8 +145,8 @@ struct Small {
     Tile::add(a, b, lds, 0, (a.depth + kStep - 1) / kStep, s);
   }
   template <typename F>
-  __device__ inline void each(F f) const {
-    s.each(f);
+  __device__ inline void each(F f) {
+    each_four(s, f);
   }
 };
 
@@ -153,8 +162,8 @@ struct Middle {
     Tile::add(a, b, lds, 0, static_cast<int>((a.depth + kStep - 1) / kStep), s);
   }
   template <typename F>
-  __device__ inline void each(F f) const {
-    s.each(f);
+  __device__ inline void each(F f) {
+    each_four(s, f);
   }
 };
 

@@ -20,10 +20,9 @@ namespace mma {
 constexpr int kCols128 = 128;
 constexpr int kThreads128 = 256;
 
-// kPair: fp16 operands held as the sum of two planes in memory.
-template <typename T, bool kPair = false>
+template <typename T>
 struct Step {
-  static constexpr int kParts = std::is_same_v<T, float> ? 3 : kPair ? 2 : 1;
+  static constexpr int kParts = std::is_same_v<T, float> ? 3 : 1;
   static constexpr int kDepth = std::is_same_v<T, float> ? 32 : 64;
 };
 
@@ -49,9 +48,9 @@ __device__ inline void split(float x, unsigned& hi, unsigned& mid, unsigned& lo)
 // 16-byte pieces are exchanged by the line; else lines of kRows elements whose
 // 32-byte units are exchanged by k.  A thread's pieces lie whole rounds of
 // lines apart, which leaves the exchange alike: one offset serves them all.
-template <typename T, bool C, int kRows, bool kAligned, bool kPair = false>
+template <typename T, bool C, int kRows, bool kAligned>
 struct Stage {
-  typedef Step<T, kPair> S;
+  typedef Step<T> S;
   static constexpr int kPieces = kRows * S::kDepth / 8;  // of eight elements
   static constexpr int kEach = (kPieces + kThreads128 - 1) / kThreads128;
   static constexpr bool kWhole = kPieces % kThreads128 == 0;  // else the last threads have none
@@ -123,7 +122,7 @@ struct Stage {
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       char* at = lds + to + e * kLines * kLineBytes;
-      if constexpr (S::kParts < 3) {
+      if constexpr (S::kParts == 1) {
         *reinterpret_cast<u32x4*>(at) = held[e][0];
       } else {
         u32x4 parts[3];
@@ -194,59 +193,50 @@ struct Sums128 {
       for (int j = 0; j < kB; ++j) c[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  // f(row, column, four sums of neighbouring columns)
-  template <typename F>
-  __device__ inline void each(F f) const {
+  // The lane's sums as fours of neighbouring columns; place() comes first.
+  static constexpr int kFours = kA * kB;
+  int row0, col0;
+  __device__ inline void place() {
     const int thread = thread_here(), lane = thread & 63, wave = thread >> 6;
-    const int row = wave / kAlong * kA * 16 + (lane & 15), col = wave % kAlong * kB * 16 + (lane >> 4) * 4;
-#pragma unroll
-    for (int i = 0; i < kA; ++i)
-#pragma unroll
-      for (int j = 0; j < kB; ++j) f(row + i * 16, col + j * 16, c[i][j]);
+    row0 = wave / kAlong * kA * 16 + (lane & 15);
+    col0 = wave % kAlong * kB * 16 + (lane >> 4) * 4;
   }
+  __device__ inline int row(int k) const { return k / kB * 16 + row0; }
+  __device__ inline int col(int k) const { return k % kB * 16 + col0; }
+  __device__ inline f32x4 four(int k) const { return c[k / kB][k % kB]; }
 };
 
-template <typename T, bool kAC, bool kBC, int kRows, bool kAligned, bool kPair = false>
+template <typename T, bool kAC, bool kBC, int kRows, bool kAligned>
 struct Tile128 {
-  typedef Step<T, kPair> S;
-  typedef Stage<T, kAC, kRows, kAligned, kPair> StageA;
-  typedef Stage<T, kBC, kCols128, kAligned, kPair> StageB;
+  typedef Step<T> S;
+  typedef Stage<T, kAC, kRows, kAligned> StageA;
+  typedef Stage<T, kBC, kCols128, kAligned> StageB;
   static constexpr int kLdsBytes = S::kParts * (StageA::kBytes + StageB::kBytes);
 
   // Adds the steps [from, to) of the sum over k of A(i, k) B(j, k).
   __device__ static inline void add(const Operand<T>& a, const Operand<T>& b, char* lds, int64_t from, int64_t to,
                                     Sums128<kRows>& s) {
-    constexpr int kPlanes = kPair ? 2 : 1;
     const int thread = thread_here(), wave = thread >> 6;
     char* lb = lds + S::kParts * StageA::kBytes;
     typedef Sums128<kRows> Sums;
     const Reader128<T, kAC, kRows, Sums::kA> ra(wave / Sums::kAlong * Sums::kA * 16, thread);
     const Reader128<T, kBC, kCols128, Sums::kB> rb(wave % Sums::kAlong * Sums::kB * 16, thread);
     const int va = static_cast<int>(a.valid), vb = static_cast<int>(b.valid);
-    StageA sa[kPlanes];
-    StageB sb[kPlanes];
-#pragma unroll
-    for (int q = 0; q < kPlanes; ++q) {
-      sa[q].start(a.ld, thread);
-      sb[q].start(b.ld, thread);
-    }
+    StageA sa;
+    StageB sb;
+    sa.start(a.ld, thread);
+    sb.start(b.ld, thread);
     auto load = [&](int64_t t) {
       const int64_t k0 = t * S::kDepth, left = a.depth - k0;
       const int most = static_cast<int>(left < S::kDepth ? left : S::kDepth);
-#pragma unroll
-      for (int q = 0; q < kPlanes; ++q) {
-        sa[q].load((q == 0 ? a.p : a.lo) + k0 * (kAC ? a.ld : 1), va, most);
-        sb[q].load((q == 0 ? b.p : b.lo) + k0 * (kBC ? b.ld : 1), vb, most);
-      }
+      sa.load(a.p + k0 * (kAC ? a.ld : 1), va, most);
+      sb.load(b.p + k0 * (kBC ? b.ld : 1), vb, most);
     };
     if (from < to) load(from);
     for (int64_t t = from; t < to; ++t) {
       __syncthreads();  // the last step's fragments have been read
-#pragma unroll
-      for (int q = 0; q < kPlanes; ++q) {
-        sa[q].store(lds + q * StageA::kBytes);
-        sb[q].store(lb + q * StageB::kBytes);
-      }
+      sa.store(lds);
+      sb.store(lb);
       if (t + 1 < to) load(t + 1);
       __syncthreads();
 #pragma unroll
@@ -262,7 +252,7 @@ struct Tile128 {
 #pragma unroll
           for (int q = 0; q < S::kParts; ++q) fb[q] = rb.read(lb, j, kk, q);
           // products of parts, the smallest first
-          constexpr int kProducts = S::kParts == 1 ? 1 : S::kParts == 2 ? 3 : 8;
+          constexpr int kProducts = S::kParts == 1 ? 1 : 8;
           constexpr int kOrder[8][2] = {{0, 0}, {0, 1}, {1, 0}, {1, 1}, {0, 2}, {2, 0}, {1, 2}, {2, 1}};
           typedef std::conditional_t<S::kParts == 3, __bf16, T> Part;
 #pragma unroll

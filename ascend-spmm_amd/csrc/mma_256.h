@@ -248,6 +248,19 @@ struct Copier {
 // The sums of a tile: quadrant [h][g] of the wave.
 struct Sums {
   Quadrant c[2][2];
+
+  // The lane's sums as fours of neighbouring columns; place() comes first.
+  static constexpr int kFours = 32;
+  int row0, col0;
+  __device__ inline void place() {
+    const int thread = thread_here(), lane = thread & 63, wave = thread >> 6;
+    row0 = (wave >> 2) * 64 + (lane & 15);
+    col0 = (wave & 3) * 32 + (lane >> 4) * 4;
+  }
+  // k: row half, row, column half, column
+  __device__ inline int row(int k) const { return (k >> 4) * 128 + (k >> 2 & 3) * 16 + row0; }
+  __device__ inline int col(int k) const { return (k >> 1 & 1) * 128 + (k & 1) * 16 + col0; }
+  __device__ inline f32x4 four(int k) const { return c[k >> 4][k >> 1 & 1][k >> 2 & 3][k & 1]; }
 };
 
 // sum over k of A(i, k) B(j, k).  kPlanes 3: operands held as sums of two
@@ -331,22 +344,6 @@ __device__ inline void multiply_tile(const Operand<T>& a, const Operand<T>& b, c
   // No copy outlives the loop: LDS is free again.
   wait_copies<0>();
   barrier();
-}
-
-// Calls f(row, column, four sums of neighbouring columns) for the lane's part
-// of the tile.
-template <typename F>
-__device__ inline void for_sums(const Sums& s, F f) {
-  const int thread = thread_here(), lane = thread & 63, wave = thread >> 6;
-  const int row = (wave >> 2) * 64 + (lane & 15), col = (wave & 3) * 32 + (lane >> 4) * 4;
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) f(h * 128 + i * 16 + row, g * 128 + j * 16 + col, s.c[h][g][i][j]);
 }
 
 }  // namespace mma

@@ -108,62 +108,103 @@ struct Planes {
 };
 
 // What is done with the sums of a product: v = alpha * sum + (beta + alpha *
-// (left[i] + right[j])) * E(i, j), E the planes `add` (and left[i] on the
-// diagonal, where right is used), then stored as planes, or as the result.
+// rest[i]) * E(i, j), E the planes `add`; stored as planes or as the result.
+// rest, on one plane's products, is what the high planes leave of the left
+// factor's diagonal: of the polynomial for the update of X; of A for the
+// polynomial, where it counts on both sides and E lacks it on the diagonal.
+enum Kind { kGram, kPoly, kUpdate, kLast };
+
 struct Finish {
   float alpha, beta;
-  Planes add;          // hi null: none
-  const float* left;   // [batch][rows], what the high planes leave of a diagonal, or null
-  bool both;           // right is left, and E lacks it on the diagonal
-  Planes to;
-  float* diagonal;     // [batch][rows]: what to.hi leaves of the diagonal, or null
-  int64_t diagonal_rows;
-  void* out;           // the result, [rows][cols] of the update's type and shape, or null
+  Planes add;           // not for kGram
+  const float* rest;    // [batch][rest_rows]
+  Planes to;            // not for kLast
+  float* diagonal;      // [batch][rest_rows]: what to.hi leaves of the diagonal (one plane's products)
+  int64_t rest_rows;
+  void* out;            // kLast: the result, [rows][cols] of the update's type and shape
   int64_t rows, cols;
   bool tall;
 };
 
-template <typename T>
-__device__ inline void finish_four(const Finish& f, int64_t batch, int64_t row, int64_t col, f32x4 sum) {
-  f32x4 v = sum * f.alpha;
-  if (f.add.hi != nullptr) {
+// Four neighbouring columns of a row of E, as they are loaded.
+struct Addend {
+  f16x4 hi, lo;
+  float rest, across[4];
+};
+
+template <Kind kKind, bool kPair>
+__device__ inline Addend load_addend(const Finish& f, int64_t batch, int64_t row, int64_t col) {
+  Addend a = {};
+  if constexpr (kKind != kGram) {
     const int64_t at = batch * f.add.size + row * f.add.ld + col;
-    const f16x4 h = *reinterpret_cast<const f16x4*>(f.add.hi + at);
-    f16x4 l = {};
-    if (f.add.lo != nullptr) l = *reinterpret_cast<const f16x4*>(f.add.lo + at);
-    const float* d = f.left == nullptr ? nullptr : f.left + batch * f.diagonal_rows;
-    const float r = d == nullptr ? 0.0f : d[row];
+    a.hi = *reinterpret_cast<const f16x4*>(f.add.hi + at);
+    if constexpr (kPair || kKind != kPoly) a.lo = *reinterpret_cast<const f16x4*>(f.add.lo + at);
+    if constexpr (!kPair) {
+      a.rest = f.rest[batch * f.rest_rows + row];
+      if constexpr (kKind == kPoly)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a.across[e] = f.rest[batch * f.rest_rows + col + e];
+    }
+  }
+  return a;
+}
+
+template <typename T, Kind kKind, bool kPair>
+__device__ inline void finish_four(const Finish& f, const Addend& a, int64_t batch, int64_t row, int64_t col, f32x4 sum) {
+  f32x4 v = sum * f.alpha;
+  if constexpr (kKind != kGram)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      float x = static_cast<float>(h[e]) + static_cast<float>(l[e]);
-      float w = f.beta + f.alpha * r;
-      if (f.both) {
-        w += f.alpha * d[col + e];
-        if (row == col + e) x += r;
+      float x = static_cast<float>(a.hi[e]) + static_cast<float>(a.lo[e]);
+      float w = f.beta + f.alpha * a.rest;
+      if constexpr (kKind == kPoly && !kPair) {
+        w += f.alpha * a.across[e];
+        if (row == col + e) x += a.rest;
       }
       v[e] += w * x;
     }
-  }
-  if (f.out != nullptr) {
+  if constexpr (kKind == kLast) {
     T* out = static_cast<T*>(f.out) + batch * f.rows * f.cols;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int64_t i = f.tall ? col + e : row, j = f.tall ? row : col + e;
       if (i < f.rows && j < f.cols) out[i * f.cols + j] = static_cast<T>(v[e]);
     }
-    return;
-  }
-  f16x4 h, l;
+  } else {
+    f16x4 h, l;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    h[e] = static_cast<half>(v[e]);
-    l[e] = static_cast<half>(v[e] - static_cast<float>(h[e]));
-    if (f.diagonal != nullptr && row == col + e)
-      f.diagonal[batch * f.diagonal_rows + row] = v[e] - static_cast<float>(h[e]);
+    for (int e = 0; e < 4; ++e) {
+      h[e] = static_cast<half>(v[e]);
+      l[e] = static_cast<half>(v[e] - static_cast<float>(h[e]));
+      if constexpr (!kPair && kKind != kUpdate)
+        if (row == col + e) f.diagonal[batch * f.rest_rows + row] = v[e] - static_cast<float>(h[e]);
+    }
+    const int64_t at = batch * f.to.size + row * f.to.ld + col;
+    *reinterpret_cast<f16x4*>(f.to.hi + at) = h;
+    if constexpr (kPair || kKind == kUpdate) *reinterpret_cast<f16x4*>(f.to.lo + at) = l;
   }
-  const int64_t at = batch * f.to.size + row * f.to.ld + col;
-  *reinterpret_cast<f16x4*>(f.to.hi + at) = h;
-  if (f.to.lo != nullptr) *reinterpret_cast<f16x4*>(f.to.lo + at) = l;
+}
+
+// Finishes a tile's sums, kCount at a time: all of a batch's addends are
+// loaded before the first is used.
+template <typename T, Kind kKind, bool kPair, int kCount, typename S>
+__device__ inline void finish_tile(const Finish& f, const S& s, int64_t batch, int64_t r0, int64_t c0, int64_t m,
+                                   int64_t n) {
+#pragma unroll
+  for (int b = 0; b < S::kFours / kCount; ++b) {
+    Addend a[kCount];
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) {
+      const int64_t row = r0 + s.row(b * kCount + k), col = c0 + s.col(b * kCount + k);
+      const bool in = row < m && col < n;
+      a[k] = load_addend<kKind, kPair>(f, batch, in ? row : 0, in ? col : 0);
+    }
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) {
+      const int64_t row = r0 + s.row(b * kCount + k), col = c0 + s.col(b * kCount + k);
+      if (row < m && col < n) finish_four<T, kKind, kPair>(f, a[k], batch, row, col, s.four(b * kCount + k));
+    }
+  }
 }
 
 // The product of `left` [m][depth] with `right`, [n][depth], or [depth][n]
@@ -181,9 +222,9 @@ __device__ inline mma::Operand<half> operand(const Planes& p, int64_t batch, int
   return {p.hi + at, p.lo == nullptr ? nullptr : p.lo + at, p.ld, rows - first < most ? rows - first : most, depth};
 }
 
-// Tiles of a work-group in order: splits fastest outside a matrix's tiles.
-template <typename T, bool kTurned, int kPlanes>
+template <typename T, Kind kKind, bool kPair>
 __global__ __launch_bounds__(mma::kThreads, 2) void product_large(Product p, Finish f) {
+  constexpr bool kTurned = kKind == kUpdate || kKind == kLast;
   __shared__ __align__(1024) char lds[mma::kLdsBytes];
   const int64_t down = (p.m + mma::kTile - 1) / mma::kTile, across = (p.n + mma::kTile - 1) / mma::kTile;
   const int64_t block = mma::run_of_xcd(blockIdx.x, gridDim.x), batch = block / (down * across);
@@ -191,15 +232,17 @@ __global__ __launch_bounds__(mma::kThreads, 2) void product_large(Product p, Fin
   mma::place_tile(block % (down * across), down, across, i, j);
   const int64_t r0 = i * mma::kTile, c0 = j * mma::kTile;
   mma::Sums s;
-  mma::multiply_tile<half, false, kTurned, kPlanes>(operand(p.left, batch, r0, mma::kTile, p.m, p.depth, false),
-                                                    operand(p.right, batch, c0, mma::kTile, p.n, p.depth, kTurned), lds, s);
-  mma::for_sums(s, [&](int row, int col, f32x4 v) {
-    if (r0 + row < p.m && c0 + col < p.n) finish_four<T>(f, batch, r0 + row, c0 + col, v);
-  });
+  mma::multiply_tile<half, false, kTurned, kPair ? 3 : 1>(
+      operand(p.left, batch, r0, mma::kTile, p.m, p.depth, false),
+      operand(p.right, batch, c0, mma::kTile, p.n, p.depth, kTurned), lds, s);
+  s.place();
+  finish_tile<T, kKind, kPair, 16>(f, s, batch, r0, c0, p.m, p.n);
 }
 
-template <typename T, bool kTurned, bool kPair>
+// Splits of a matrix are further apart than its tiles.
+template <typename T, Kind kKind, bool kPair>
 __global__ __launch_bounds__(mma::kThreads128, kPair ? 1 : 2) void product_small(Product p, Finish f) {
+  constexpr bool kTurned = kKind == kUpdate || kKind == kLast;
   typedef mma::Ring<half, false, kTurned, kPair> Tile;
   __shared__ __align__(1024) char lds[Tile::kLdsBytes];
   const int64_t down = (p.m + 127) / 128, across = (p.n + 127) / 128;
@@ -213,25 +256,32 @@ __global__ __launch_bounds__(mma::kThreads128, kPair ? 1 : 2) void product_small
   s.clear();
   Tile::add(operand(p.left, batch, r0, 128, p.m, p.depth, false), operand(p.right, batch, c0, 128, p.n, p.depth, kTurned),
             lds, static_cast<int>(steps * split / p.splits), static_cast<int>(steps * (split + 1) / p.splits), s);
+  s.place();
+  if (p.splits == 1) {
+    finish_tile<T, kKind, kPair, 16>(f, s, batch, r0, c0, p.m, p.n);
+    return;
+  }
   const int64_t batches = gridDim.x / (down * across * p.splits);
   float* to = p.sums + (split * batches + batch) * p.m * p.n;
-  s.each([&](int row, int col, f32x4 v) {
-    if (r0 + row >= p.m || c0 + col >= p.n) return;
-    if (p.splits > 1) *reinterpret_cast<f32x4*>(to + (r0 + row) * p.n + c0 + col) = v;
-    else finish_four<T>(f, batch, r0 + row, c0 + col, v);
-  });
+#pragma unroll
+  for (int k = 0; k < s.kFours; ++k) {
+    const int64_t row = r0 + s.row(k), col = c0 + s.col(k);
+    if (row < p.m && col < p.n) *reinterpret_cast<f32x4*>(to + row * p.n + col) = s.four(k);
+  }
 }
 
 // Adds the splits' sums in order and finishes them.
-template <typename T>
+template <typename T, Kind kKind, bool kPair>
 __global__ __launch_bounds__(kThreads) void finish_sums(Product p, Finish f, int64_t batches) {
   const int64_t fours = p.m * p.n / 4, n = fours * batches;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
        i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t batch = i / fours, e = i % fours * 4, row = e / p.n, col = e % p.n;
+    const Addend a = load_addend<kKind, kPair>(f, batch, row, col);
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
     for (int64_t k = 0; k < p.splits; ++k) s += *reinterpret_cast<const f32x4*>(p.sums + (k * n + i) * 4);
-    const int64_t e = i % fours * 4;
-    finish_four<T>(f, i / fours, e / p.n, e % p.n, s);
+    finish_four<T, kKind, kPair>(f, a, batch, row, col, s);
   }
 }
 
@@ -240,8 +290,212 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void store_planes(Finish f, int64_t mp, int64_t batches) {
   const int64_t fours = mp * f.add.ld / 4;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < fours * batches;
-       i += static_cast<int64_t>(gridDim.x) * kThreads)
-    finish_four<T>(f, i / fours, i % fours * 4 / f.add.ld, i % fours * 4 % f.add.ld, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t batch = i / fours, row = i % fours * 4 / f.add.ld, col = i % fours * 4 % f.add.ld;
+    finish_four<T, kLast, true>(f, load_addend<kLast, true>(f, batch, row, col), batch, row, col,
+                                f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+  }
+}
+
+// A whole matrix in one work-group, its planes in LDS: no launch between the
+// products.  X lies in lines of np + 8 elements, A and its polynomial (in A's
+// place) in lines of mp + 8: an odd number of 16-byte pieces, so that the same
+// piece of neighbouring lines lies in different banks.  A wave sums blocks of
+// 32 x 32.  What bounds it is the LDS reads of one CU (8 KB for 12 matrix
+// instructions) and the barriers.
+constexpr int kInnerThreads = 512;
+constexpr int kInnerWaves = kInnerThreads / 64;
+constexpr int kInnerSteps = 16;   // most steps
+// Most blocks of a wave: 40 of 1024 sums, and 16 where little LDS leaves room
+// for a second work-group on a CU.
+constexpr int kInnerBlocks = 5, kInnerBlocksFew = 2;
+constexpr int kInnerLds = 160 * 1024 - 512, kInnerLdsFew = 40 * 1024;
+
+struct InnerArgs {
+  int64_t rows, cols;
+  int m, n, mp, np;  // extents and padded ones, multiples of 32
+  bool tall;
+  int steps;
+  double eps, scale;
+  float gram[kInnerSteps], poly[kInnerSteps], poly_a[kInnerSteps], update[kInnerSteps], update_x[kInnerSteps];
+};
+
+__host__ __device__ constexpr int64_t inner_bytes(int64_t mp, int64_t np) {
+  return 4 * mp * (np + 8) + 4 * mp * (mp + 8);
+}
+
+// Two planes of a matrix in LDS.
+struct InnerPlanes {
+  half* hi;
+  half* lo;
+  int ld;
+};
+
+// Fragment for 32 k from k0 of 16 lines from `first` (k along them).
+__device__ inline u32x4 inner_along(const half* p, int ld, int first, int k0, int lane) {
+  return *reinterpret_cast<const u32x4*>(p + (first + (lane & 15)) * ld + k0 + (lane >> 4) * 8);
+}
+// The same of 16 columns from `first` (k across lines).
+__device__ inline u32x4 inner_across(const half* p, int ld, int first, int k0, int lane) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+  mma::u32x2 h[2];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+    h[m] = __builtin_bit_cast(
+        mma::u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(
+                        p + (k0 + (lane >> 4) * 8 + m * 4 + ((lane & 15) >> 2)) * ld + first + (lane & 3) * 4)));
+  return __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3);
+}
+
+typedef f32x4 InnerBlock[2][2];
+
+// The wave's blocks of left times right (turned: k across right's lines).
+template <bool kTurned, int kBlocks>
+__device__ inline void inner_product(const InnerPlanes& left, const InnerPlanes& right, int blocks, int across, int depth,
+                                     InnerBlock (&s)[kBlocks]) {
+  const int thread = mma::thread_here(), lane = thread & 63, wave = thread >> 6;
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) {
+    const int block = wave + b * kInnerWaves;
+    if (block >= blocks) break;
+    const int i0 = block / across * 32, j0 = block % across * 32;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s[b][i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = 0; k0 < depth; k0 += 32) {
+      u32x4 l[2][2], r[2][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          l[i][q] = inner_along(q == 0 ? left.hi : left.lo, left.ld, i0 + 16 * i, k0, lane);
+          const half* p = q == 0 ? right.hi : right.lo;
+          r[i][q] = kTurned ? inner_across(p, right.ld, j0 + 16 * i, k0, lane) : inner_along(p, right.ld, j0 + 16 * i, k0, lane);
+        }
+#pragma unroll
+      for (int o = 2; o >= 0; --o)  // low products first
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) s[b][i][j] = mma::multiply<half>(r[j][o == 2], l[i][o == 1], s[b][i][j]);
+    }
+  }
+}
+
+// f(row, column, four sums) for the wave's blocks.
+template <int kBlocks, typename F>
+__device__ inline void inner_each(const InnerBlock (&s)[kBlocks], int blocks, int across, F f) {
+  const int thread = mma::thread_here(), lane = thread & 63, wave = thread >> 6;
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) {
+    const int block = wave + b * kInnerWaves;
+    if (block >= blocks) break;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        f(block / across * 32 + i * 16 + (lane & 15), block % across * 32 + j * 16 + (lane >> 4) * 4, s[b][i][j]);
+  }
+}
+
+__device__ inline void inner_store(const InnerPlanes& p, int row, int col, f32x4 v) {
+  f16x4 h, l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    h[e] = static_cast<half>(v[e]);
+    l[e] = static_cast<half>(v[e] - static_cast<float>(h[e]));
+  }
+  *reinterpret_cast<f16x4*>(p.hi + row * p.ld + col) = h;
+  *reinterpret_cast<f16x4*>(p.lo + row * p.ld + col) = l;
+}
+__device__ inline f32x4 inner_load(const InnerPlanes& p, int row, int col) {
+  const f16x4 h = *reinterpret_cast<const f16x4*>(p.hi + row * p.ld + col);
+  const f16x4 l = *reinterpret_cast<const f16x4*>(p.lo + row * p.ld + col);
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(h[e]) + static_cast<float>(l[e]);
+  return v;
+}
+
+// The wave's blocks times alpha, and beta times a matrix.
+template <int kBlocks>
+__device__ inline void inner_add(InnerBlock (&s)[kBlocks], int blocks, int across, float alpha, const InnerPlanes& p,
+                                 float beta) {
+  const int thread = mma::thread_here(), lane = thread & 63, wave = thread >> 6;
+#pragma unroll
+  for (int b = 0; b < kBlocks; ++b) {
+    const int block = wave + b * kInnerWaves;
+    if (block >= blocks) break;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        s[b][i][j] = s[b][i][j] * alpha + inner_load(p, block / across * 32 + i * 16 + (lane & 15),
+                                                     block % across * 32 + j * 16 + (lane >> 4) * 4) * beta;
+  }
+}
+
+template <typename T, int kLds, int kBlocks>
+__global__ __launch_bounds__(kInnerThreads) void orthogonalize_inner(InnerArgs a, const T* __restrict__ update,
+                                                                     T* __restrict__ result) {
+  __shared__ __align__(16) char lds[kLds];
+  __shared__ double waves[kInnerWaves];
+  const int64_t elements = a.rows * a.cols;
+  const T* u = update + blockIdx.x * elements;
+  T* out = result + blockIdx.x * elements;
+  const int lx = a.np + 8, la = a.mp + 8;
+  half* p = reinterpret_cast<half*>(lds);
+  const InnerPlanes x{p, p + a.mp * lx, lx}, gram{p + 2 * a.mp * lx, p + 2 * a.mp * lx + a.mp * la, la};
+  const int thread = threadIdx.x;
+
+  double squares = 0.0;
+  for (int i = thread; i < elements; i += kInnerThreads) {
+    const double v = static_cast<double>(static_cast<float>(u[i]));
+    squares += v * v;
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) squares += __shfl_xor(squares, d);
+  if ((thread & 63) == 0) waves[thread >> 6] = squares;
+  for (int i = thread; i < a.mp * lx; i += kInnerThreads) x.hi[i] = x.lo[i] = static_cast<half>(0.0f);
+  __syncthreads();
+  squares = 0.0;
+#pragma unroll
+  for (int w = 0; w < kInnerWaves; ++w) squares += waves[w];
+  const double factor = a.scale / (sqrt(squares) + a.eps);
+  for (int i = thread; i < elements; i += kInnerThreads) {
+    const int r = i / static_cast<int>(a.cols), c = i % static_cast<int>(a.cols);
+    const int at = a.tall ? c * lx + r : r * lx + c;
+    to_planes(static_cast<float>(static_cast<double>(static_cast<float>(u[i])) * factor), x.hi[at], x.lo[at]);
+  }
+  __syncthreads();
+
+  const int square = a.mp / 32 * (a.mp / 32), wide = a.mp / 32 * (a.np / 32);
+  InnerBlock s[kBlocks];
+  for (int t = 0; t < a.steps; ++t) {
+    inner_product<false>(x, x, square, a.mp / 32, a.np, s);
+    inner_each(s, square, a.mp / 32, [&](int row, int col, f32x4 v) { inner_store(gram, row, col, v * a.gram[t]); });
+    __syncthreads();
+    inner_product<false>(gram, gram, square, a.mp / 32, a.mp, s);
+    inner_add(s, square, a.mp / 32, a.poly[t], gram, a.poly_a[t]);
+    __syncthreads();  // all of A has been read
+    inner_each(s, square, a.mp / 32, [&](int row, int col, f32x4 v) { inner_store(gram, row, col, v); });
+    __syncthreads();
+    inner_product<true>(gram, x, wide, a.np / 32, a.mp, s);
+    inner_add(s, wide, a.np / 32, a.update[t], x, a.update_x[t]);
+    if (t + 1 == a.steps) break;
+    __syncthreads();  // all of X has been read
+    inner_each(s, wide, a.np / 32, [&](int row, int col, f32x4 v) { inner_store(x, row, col, v); });
+    __syncthreads();
+  }
+  inner_each(s, wide, a.np / 32, [&](int row, int col, f32x4 v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = a.tall ? col + e : row, j = a.tall ? row : col + e;
+      if (i < a.rows && j < a.cols) out[i * static_cast<int>(a.cols) + j] = static_cast<T>(v[e]);
+    }
+  });
 }
 
 spmm_status check_desc(const spmm_orthogonalize_desc* d) {
@@ -326,29 +580,91 @@ struct Layout {
   }
 };
 
-template <typename T, bool kTurned, bool kPair>
+template <typename T, Kind kKind, bool kPair>
 spmm_status multiply(Product p, const Finish& f, int64_t batch, hipStream_t s) {
   if (Layout::large(batch, p.m, p.n)) {
     const unsigned tiles = static_cast<unsigned>(ceil_div(p.m, mma::kTile) * ceil_div(p.n, mma::kTile) * batch);
-    hipLaunchKernelGGL((product_large<T, kTurned, kPair ? 3 : 1>), dim3(tiles), dim3(mma::kThreads), 0, s, p, f);
+    hipLaunchKernelGGL((product_large<T, kKind, kPair>), dim3(tiles), dim3(mma::kThreads), 0, s, p, f);
     return check_launch("orthogonalize product");
   }
   p.splits = Layout::splits(batch, p.m, p.n, p.depth);
   const unsigned tiles = static_cast<unsigned>(ceil_div(p.m, 128) * ceil_div(p.n, 128) * batch * p.splits);
-  hipLaunchKernelGGL((product_small<T, kTurned, kPair>), dim3(tiles), dim3(mma::kThreads128), 0, s, p, f);
+  hipLaunchKernelGGL((product_small<T, kKind, kPair>), dim3(tiles), dim3(mma::kThreads128), 0, s, p, f);
   if (spmm_status st = check_launch("orthogonalize product")) return st;
   if (p.splits == 1) return SPMM_OK;
   const int64_t blocks = ceil_div(p.m * p.n / 4 * batch, kThreads);
-  hipLaunchKernelGGL(finish_sums<T>, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(kThreads), 0, s, p,
-                     f, batch);
+  hipLaunchKernelGGL((finish_sums<T, kKind, kPair>), dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)),
+                     dim3(kThreads), 0, s, p, f, batch);
   return check_launch("orthogonalize sums");
 }
 
-template <typename T, bool kTurned>
+// The update's type matters to the last product alone.
+template <typename T, Kind kKind>
 spmm_status multiply(const Product& p, const Finish& f, int64_t batch, bool pair, hipStream_t s) {
-  if constexpr (std::is_same_v<T, __bf16>)
-    if (!pair) return multiply<T, kTurned, false>(p, f, batch, s);
-  return multiply<T, kTurned, true>(p, f, batch, s);
+  if constexpr (kKind != kLast)
+    return pair ? multiply<half, kKind, true>(p, f, batch, s) : multiply<half, kKind, false>(p, f, batch, s);
+  else if constexpr (std::is_same_v<T, __bf16>)
+    return pair ? multiply<T, kKind, true>(p, f, batch, s) : multiply<T, kKind, false>(p, f, batch, s);
+  else
+    return multiply<T, kKind, true>(p, f, batch, s);
+}
+
+// The factors of each step's products, for planes scaled by powers of two.
+struct Scales {
+  double gram, poly, poly_a, update, update_x;
+};
+
+// Of step i, from the bound on X's largest singular value, which becomes the
+// bound after it.  The last step's result is not scaled.
+Scales scales_of(const spmm_orthogonalize_desc* d, int64_t i, double& bound) {
+  const double *c = d->coefficients + 3 * i, t = bound * bound, sx = scale_for(bound);
+  // largest |b t + c t^2| on [0, bound^2]
+  double high = std::fabs(c[1] * t + c[2] * t * t);
+  if (c[2] != 0.0 && -c[1] / (2 * c[2]) > 0.0 && -c[1] / (2 * c[2]) < t)
+    high = std::fmax(high, std::fabs(c[1] * c[1] / (4 * c[2])));
+  const double sa = scale_for(t), sp = scale_for(high);
+  bound = largest(c[0], c[1], c[2], bound);
+  const double next = i + 1 < d->steps ? scale_for(bound) : 1.0;
+  return {sa / (sx * sx), sp * c[2] / (sa * sa), sp * c[1] / sa, next / (sp * sx), next * c[0] / sx};
+}
+
+// Whether a matrix and its Gram matrix fit a work-group's LDS.
+bool inner_fits(const spmm_orthogonalize_desc* d) {
+  const int64_t m = d->rows < d->width ? d->rows : d->width, n = d->rows < d->width ? d->width : d->rows;
+  if (n > 4096 || d->steps < 1 || d->steps > kInnerSteps) return false;
+  const int64_t mp = align_up(m, 32), np = align_up(n, 32);
+  return inner_bytes(mp, np) <= kInnerLds && mp / 32 * (np / 32) <= kInnerBlocks * kInnerWaves;
+}
+
+template <typename T>
+spmm_status run_inner(const spmm_orthogonalize_desc* d, const void* update, void* out, hipStream_t s) {
+  InnerArgs a{};
+  a.rows = d->rows;
+  a.cols = d->width;
+  a.tall = d->rows > d->width;
+  a.m = static_cast<int>(a.tall ? d->width : d->rows);
+  a.n = static_cast<int>(a.tall ? d->rows : d->width);
+  a.mp = static_cast<int>(align_up(a.m, 32));
+  a.np = static_cast<int>(align_up(a.n, 32));
+  a.steps = static_cast<int>(d->steps);
+  a.eps = d->eps;
+  a.scale = scale_for(1.0);
+  double bound = 1.0;
+  for (int i = 0; i < a.steps; ++i) {
+    const Scales c = scales_of(d, i, bound);
+    a.gram[i] = static_cast<float>(c.gram);
+    a.poly[i] = static_cast<float>(c.poly);
+    a.poly_a[i] = static_cast<float>(c.poly_a);
+    a.update[i] = static_cast<float>(c.update);
+    a.update_x[i] = static_cast<float>(c.update_x);
+  }
+  const dim3 grid(static_cast<unsigned>(d->batch)), block(kInnerThreads);
+  const T* u = static_cast<const T*>(update);
+  if (inner_bytes(a.mp, a.np) <= kInnerLdsFew && a.mp / 32 * (a.np / 32) <= kInnerBlocksFew * kInnerWaves)
+    hipLaunchKernelGGL((orthogonalize_inner<T, kInnerLdsFew, kInnerBlocksFew>), grid, block, 0, s, a, u, static_cast<T*>(out));
+  else
+    hipLaunchKernelGGL((orthogonalize_inner<T, kInnerLds, kInnerBlocks>), grid, block, 0, s, a, u, static_cast<T*>(out));
+  return check_launch("orthogonalize");
 }
 
 template <typename T>
@@ -375,58 +691,49 @@ spmm_status run(const spmm_orthogonalize_desc* d, const Layout& l, const void* u
   float* sums = reinterpret_cast<float*>(ws);
   const T* u = static_cast<const T*>(update);
   const unsigned batch = static_cast<unsigned>(d->batch);
-  double bound = 1.0, sx = scale_for(bound);
   hipLaunchKernelGGL(square_sums<T>, dim3(kNormParts, batch), dim3(kThreads), 0, s, u, l.m * l.n, parts);
   hipLaunchKernelGGL(scale_update<T>, dim3(static_cast<unsigned>(l.np / 64), static_cast<unsigned>(l.mp / 64), batch),
-                     dim3(kThreads), 0, s, u, d->rows, d->width, tall, d->eps, sx, parts, l.mp, l.np, x.hi, x.lo);
+                     dim3(kThreads), 0, s, u, d->rows, d->width, tall, d->eps, scale_for(1.0), parts, l.mp, l.np, x.hi,
+                     x.lo);
   if (spmm_status st = check_launch("orthogonalize scale")) return st;
   Finish f{};
-  f.diagonal_rows = l.mp;
+  f.rest_rows = l.mp;
+  f.out = out;
   f.rows = d->rows;
   f.cols = d->width;
   f.tall = tall;
   if (d->steps == 0) {
-    f.beta = static_cast<float>(1.0 / sx);
+    f.beta = static_cast<float>(1.0 / scale_for(1.0));
     f.add = x;
-    f.out = out;
     const int64_t blocks = ceil_div(l.mp * l.np / 4 * d->batch, kThreads);
     hipLaunchKernelGGL(store_planes<T>, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(kThreads), 0, s,
                        f, l.mp, d->batch);
     return check_launch("orthogonalize result");
   }
+  double bound = 1.0;
   for (int64_t i = 0; i < d->steps; ++i) {
-    const double *c = d->coefficients + 3 * i, t = bound * bound;
-    // b t + c t^2 on [0, bound^2], as an odd polynomial's largest
-    double high = std::fabs(c[1] * t + c[2] * t * t);
-    if (c[2] != 0.0 && -c[1] / (2 * c[2]) > 0.0 && -c[1] / (2 * c[2]) < t)
-      high = std::fmax(high, std::fabs(c[1] * c[1] / (4 * c[2])));
-    const double sa = scale_for(t), sp = scale_for(high);
-    bound = largest(c[0], c[1], c[2], bound);
-    const double next = i + 1 < d->steps ? scale_for(bound) : 1.0;
-    Finish g = f;
-    g.alpha = static_cast<float>(sa / (sx * sx));
-    g.to = gram;
-    g.diagonal = gram_rest;
-    if (spmm_status st = multiply<T, false>({x, x, l.mp, l.mp, l.np, 1, sums}, g, d->batch, l.pair, s)) return st;
-    g.alpha = static_cast<float>(sp * c[2] / (sa * sa));
-    g.beta = static_cast<float>(sp * c[1] / sa);
-    g.add = gram;
-    g.left = gram_rest;
-    g.both = gram_rest != nullptr;
-    g.to = poly;
-    g.diagonal = poly_rest;
-    if (spmm_status st = multiply<T, false>({gram, gram, l.mp, l.mp, l.mp, 1, sums}, g, d->batch, l.pair, s)) return st;
-    g.alpha = static_cast<float>(next / (sp * sx));
-    g.beta = static_cast<float>(next * c[0] / sx);
-    g.add = x;
-    g.left = poly_rest;
-    g.both = false;
-    g.to = y;
-    g.diagonal = nullptr;
-    g.out = i + 1 < d->steps ? nullptr : out;
-    if (spmm_status st = multiply<T, true>({poly, x, l.mp, l.np, l.mp, 1, sums}, g, d->batch, l.pair, s)) return st;
+    const Scales c = scales_of(d, i, bound);
+    f.alpha = static_cast<float>(c.gram);
+    f.to = gram;
+    f.diagonal = gram_rest;
+    if (spmm_status st = multiply<T, kGram>({x, x, l.mp, l.mp, l.np, 1, sums}, f, d->batch, l.pair, s)) return st;
+    f.alpha = static_cast<float>(c.poly);
+    f.beta = static_cast<float>(c.poly_a);
+    f.add = gram;
+    f.rest = gram_rest;
+    f.to = poly;
+    f.diagonal = poly_rest;
+    if (spmm_status st = multiply<T, kPoly>({gram, gram, l.mp, l.mp, l.mp, 1, sums}, f, d->batch, l.pair, s)) return st;
+    f.alpha = static_cast<float>(c.update);
+    f.beta = static_cast<float>(c.update_x);
+    f.add = x;
+    f.rest = poly_rest;
+    f.to = y;
+    const Product p{poly, x, l.mp, l.np, l.mp, 1, sums};
+    if (spmm_status st = i + 1 < d->steps ? multiply<T, kUpdate>(p, f, d->batch, l.pair, s)
+                                          : multiply<T, kLast>(p, f, d->batch, l.pair, s))
+      return st;
     std::swap(x, y);
-    sx = next;
   }
   return SPMM_OK;
 }
@@ -442,7 +749,7 @@ spmm_status spmm_orthogonalize_workspace(const spmm_orthogonalize_desc* d, size_
   clear_error();
   if (bytes == nullptr) return fail(SPMM_ERR_INVALID_ARGUMENT, "null argument");
   if (spmm_status st = check_desc(d)) return st;
-  *bytes = Layout(d).total();
+  *bytes = inner_fits(d) ? 0 : Layout(d).total();
   return SPMM_OK;
 }
 
@@ -452,13 +759,18 @@ spmm_status spmm_orthogonalize_run(const spmm_orthogonalize_desc* d, const void*
   if (spmm_status st = check_desc(d)) return st;
   if (d->batch == 0 || d->rows == 0 || d->width == 0) return SPMM_OK;
   if (update == nullptr || out == nullptr) return fail(SPMM_ERR_INVALID_ARGUMENT, "orthogonalize: null device pointer");
+  hipStream_t s = as_stream(stream);
+  if (inner_fits(d)) switch (d->value_type) {
+      case SPMM_VALUE_F16: return run_inner<_Float16>(d, update, out, s);
+      case SPMM_VALUE_BF16: return run_inner<__bf16>(d, update, out, s);
+      default: return run_inner<float>(d, update, out, s);
+    }
   const Layout l(d);
   if (workspace == nullptr || workspace_bytes < l.total())
     return fail(SPMM_ERR_CONTRACT, "orthogonalize: workspace too small: need " + std::to_string(l.total()) + " bytes");
   if (ceil_div(l.mp, 128) * ceil_div(l.np, 128) * d->batch > INT32_MAX / 64 || l.np / 64 > 65535 * 64 || l.mp / 64 > 65535)
     return fail(SPMM_ERR_OVERFLOW, "orthogonalize: too many tiles for one launch");
   char* ws = static_cast<char*>(workspace);
-  hipStream_t s = as_stream(stream);
   switch (d->value_type) {
     case SPMM_VALUE_F16: return run<_Float16>(d, l, update, out, ws, s);
     case SPMM_VALUE_BF16: return run<__bf16>(d, l, update, out, ws, s);
