@@ -24,71 +24,65 @@ namespace spmm {
 namespace {
 
 struct GroupedArgs {
-  int64_t rows, groups;
-  int64_t inner, width;  // of the product at hand: depth and output columns
-  int64_t in_stride;     // rows of its left operand
+  int rows, groups;
+  int inner, width;  // of the product at hand: depth and output columns
+  int64_t in_stride; // rows of its left operand
   int64_t weight_stride;
   const void* offsets;
-  bool wide;             // offsets are int64
+  bool wide;         // offsets are int64
 };
 
-__device__ inline int64_t edge(const GroupedArgs& a, int64_t g) {
+__device__ inline int edge(const GroupedArgs& a, int g) {
   const int64_t v = a.wide ? static_cast<const int64_t*>(a.offsets)[g] : static_cast<const int32_t*>(a.offsets)[g];
-  return v < 0 ? 0 : v > a.rows ? a.rows : v;
+  return v < 0 ? 0 : v > a.rows ? a.rows : static_cast<int>(v);
 }
 
-// Finds the segment of [0, segments) that holds `at`, where segment s takes
-// size(s) places: sets `before` to the places ahead of it.  Past the last,
-// returns `segments` and their total.  Every lane of a wave calls it and gets
-// the same answer.
+// Finds the segment of [0, segments) that holds place `at`; segment s takes
+// size(s) places, and `before` is set to the places ahead of the one found.
+// Past the last, returns `segments` and their total.  Every lane of a wave
+// calls it and gets the same answer.
 template <typename F>
-__device__ inline int64_t find_segment(int64_t segments, int64_t at, F size, int64_t& before) {
+__device__ inline int find_segment(int segments, int at, F size, int& before) {
   const int lane = threadIdx.x & 63;
   before = 0;
-  for (int64_t s0 = 0; s0 < segments; s0 += 64) {
-    const int64_t mine = s0 + lane < segments ? size(s0 + lane) : 0;
-    int64_t upto = mine;
+  for (int s0 = 0; s0 < segments; s0 += 64) {
+    const int mine = s0 + lane < segments ? size(s0 + lane) : 0;
+    int upto = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int64_t o = __shfl_up(upto, d);
+      const int o = __shfl_up(upto, d);
       if (lane >= d) upto += o;
     }
     const unsigned long long past = __ballot(before + upto > at);
     if (past != 0) {
       const int found = __ffsll(past) - 1;
-      before += __shfl(upto - mine, found);
+      before += __builtin_amdgcn_readlane(upto - mine, found);
       return s0 + found;
     }
-    before += __shfl(upto, 63);
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
   return segments;
-}
-
-__device__ inline int64_t uniform(int64_t v) {
-  const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v));
-  const unsigned hi = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v >> 32));
-  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 // The `tile`-th range of at most `height` rows, none across a group's end.
 // Segment 0 is the rows before the first group, segment groups + 1 those
 // behind the last; both are `group` -1.  False past the last range.
 struct RowRange {
-  int64_t first, rows, group;
+  int first, rows, group;
 };
-__device__ inline bool find_rows(const GroupedArgs& a, int64_t height, int64_t tile, RowRange& r) {
-  auto low = [&](int64_t s) { return s == 0 ? 0 : edge(a, s - 1); };
-  auto high = [&](int64_t s) { return s == a.groups + 1 ? a.rows : edge(a, s); };
-  int64_t before;
-  const int64_t s = find_segment(a.groups + 2, tile, [&](int64_t t) {
-    const int64_t n = high(t) - low(t);
+__device__ inline bool find_rows(const GroupedArgs& a, int height, int tile, RowRange& r) {
+  auto low = [&](int s) { return s == 0 ? 0 : edge(a, s - 1); };
+  auto high = [&](int s) { return s == a.groups + 1 ? a.rows : edge(a, s); };
+  int before;
+  const int s = find_segment(a.groups + 2, tile, [&](int t) {
+    const int n = high(t) - low(t);
     return n > 0 ? (n + height - 1) / height : 0;
   }, before);
   if (s == a.groups + 2) return false;
-  r.first = uniform(low(s) + (tile - before) * height);
-  const int64_t left = uniform(high(s)) - r.first;
+  r.first = low(s) + (tile - before) * height;
+  const int left = high(s) - r.first;
   r.rows = left < height ? left : height;
-  r.group = uniform(s == 0 || s == a.groups + 1 ? -1 : s - 1);
+  r.group = s == 0 || s == a.groups + 1 ? -1 : s - 1;
   return true;
 }
 
@@ -153,10 +147,10 @@ struct Small {
 template <typename T, bool kAC, bool kBC>
 struct Middle {
   typedef T Value;
-  typedef mma::Ring<T, kAC, kBC, false> Tile;
+  typedef mma::Ring<T, kAC, kBC, false, 128, 128> Tile;
   static constexpr int kRows = 128, kCols = mma::kCols128, kThreads = mma::kThreads128, kStep = Tile::kDepth;
   static constexpr int kLds = Tile::kLdsBytes, kPerCu = 2;
-  mma::Sums128<128> s;
+  typename Tile::Sums s;
   __device__ inline void sum(const mma::Operand<T>& a, const mma::Operand<T>& b, char* lds) {
     s.clear();
     Tile::add(a, b, lds, 0, static_cast<int>((a.depth + kStep - 1) / kStep), s);
@@ -171,40 +165,41 @@ struct Middle {
 template <typename E, bool kTurned>
 __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void grouped_rows(
     GroupedArgs a, const typename E::Value* __restrict__ in, const typename E::Value* __restrict__ weight,
-    typename E::Value* __restrict__ out, int64_t down) {
+    typename E::Value* __restrict__ out, unsigned down) {
   typedef typename E::Value T;
   __shared__ __align__(1024) char lds[E::kLds];
-  const int64_t across = (a.width + E::kCols - 1) / E::kCols;
-  int64_t i, j;
+  const unsigned across = (a.width + E::kCols - 1) / E::kCols;
+  unsigned i, j;
   mma::place_tile(mma::run_of_xcd(blockIdx.x, gridDim.x), down, across, i, j);
   RowRange r;
   if (!find_rows(a, E::kRows, i, r)) return;
-  const int64_t c0 = j * E::kCols;
-  const int64_t cols = a.width - c0 < E::kCols ? a.width - c0 : E::kCols;
-  T* to = out + r.first * a.width + c0;
-  auto store = [&](int row, int col, f32x4 v) {
-    if (row < r.rows && col < cols) store_four(to + row * a.width + col, cols - col, v);
-  };
+  const int c0 = j * E::kCols, cols = a.width - c0 < E::kCols ? a.width - c0 : E::kCols;
+  T* to = out + static_cast<int64_t>(r.first) * a.width + c0;
   E e;
-  const T* w = weight + (r.group < 0 ? 0 : r.group) * a.weight_stride + (kTurned ? c0 * a.inner : c0);
+  const T* w = weight + (r.group < 0 ? 0 : r.group) * a.weight_stride + (kTurned ? static_cast<int64_t>(c0) * a.inner : c0);
   // outside the groups: an empty sum
-  e.sum({in + r.first * a.in_stride, nullptr, a.in_stride, r.rows, r.group < 0 ? 0 : a.inner},
-        {w, nullptr, kTurned ? a.inner : a.width, cols, r.group < 0 ? 0 : a.inner}, lds);
-  e.each(store);
+  const int depth = r.group < 0 ? 0 : a.inner;
+  e.sum({in + r.first * a.in_stride, nullptr, a.in_stride, r.rows, depth},
+        {w, nullptr, kTurned ? a.inner : a.width, cols, depth}, lds);
+  e.each([&](int row, int col, f32x4 v) {
+    if (row < r.rows && col < cols) store_four(to + static_cast<int64_t>(row) * a.width + col, cols - col, v);
+  });
 }
 
 // dW's sums run over the rows of all groups, counted in steps of 64 (an empty
 // group has one, which adds nothing) and cut into `parts` equal ranges.  The
 // cuts depend on sizes alone, so every engine adds in the same order.
 constexpr int kRowStep = 64;
-__device__ inline int64_t steps_of(const GroupedArgs& a, int64_t g) {
-  const int64_t n = edge(a, g + 1) - edge(a, g);
+__device__ inline int steps_of(const GroupedArgs& a, int g) {
+  const int n = edge(a, g + 1) - edge(a, g);
   return n > 0 ? (n + kRowStep - 1) / kRowStep : 1;
 }
-__device__ inline int64_t find_step(const GroupedArgs& a, int64_t at, int64_t& before) {
-  return find_segment(a.groups, at, [&](int64_t g) { return steps_of(a, g); }, before);
+__device__ inline int find_step(const GroupedArgs& a, int at, int& before) {
+  return find_segment(a.groups, at, [&](int g) { return steps_of(a, g); }, before);
 }
-__device__ inline int64_t part_start(int64_t total, int64_t part, int64_t parts) { return total * part / parts; }
+__device__ inline int part_start(int total, int part, int parts) {
+  return static_cast<int>(static_cast<int64_t>(total) * part / parts);
+}
 
 // A work-group sums one tile over one range; tiles of a range are neighbours,
 // which share its rows in their XCD's L2.  The pieces of groups that a range
@@ -214,38 +209,36 @@ template <typename E>
 __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void grouped_weights(
     GroupedArgs a, const typename E::Value* __restrict__ left, int64_t left_stride,
     const typename E::Value* __restrict__ right, int64_t right_stride, typename E::Value* __restrict__ dweight,
-    int64_t parts, float* __restrict__ pieces) {
+    int parts, float* __restrict__ pieces) {
   typedef typename E::Value T;
   __shared__ __align__(1024) char lds[E::kLds];
-  const int64_t across = (a.width + E::kCols - 1) / E::kCols, down = (a.inner + E::kRows - 1) / E::kRows;
-  int64_t total;
-  find_step(a, INT64_MAX, total);
-  total = uniform(total);
-  const int64_t block = mma::run_of_xcd(blockIdx.x, gridDim.x);
-  const int64_t part = block / (across * down);
-  int64_t i, j;
-  mma::place_tile(block % (across * down), down, across, i, j);
-  const int64_t i0 = i * E::kRows, j0 = j * E::kCols;
-  const int64_t rows = a.inner - i0 < E::kRows ? a.inner - i0 : E::kRows;
-  const int64_t cols = a.width - j0 < E::kCols ? a.width - j0 : E::kCols;
-  const int64_t u0 = part_start(total, part, parts), u1 = part_start(total, part + 1, parts);
-  for (int64_t u = u0; u < u1;) {
-    int64_t before;
-    const int64_t g = uniform(find_step(a, u, before));
-    const int64_t lo = uniform(edge(a, g)), hi = uniform(edge(a, g + 1)), n = uniform(steps_of(a, g));
-    const int64_t s0 = u - uniform(before), s1 = n - s0 < u1 - u ? n : s0 + (u1 - u);
-    const int64_t first = lo + s0 * kRowStep, last = lo + s1 * kRowStep < hi ? lo + s1 * kRowStep : hi;
-    const int64_t depth = last > first ? last - first : 0;
+  const unsigned across = (a.width + E::kCols - 1) / E::kCols, down = (a.inner + E::kRows - 1) / E::kRows;
+  int total;
+  find_step(a, INT_MAX, total);
+  const unsigned block = mma::run_of_xcd(blockIdx.x, gridDim.x), part = block / (across * down);
+  unsigned i, j;
+  mma::place_tile(block - part * (across * down), down, across, i, j);
+  const int i0 = i * E::kRows, j0 = j * E::kCols;
+  const int rows = a.inner - i0 < E::kRows ? a.inner - i0 : E::kRows;
+  const int cols = a.width - j0 < E::kCols ? a.width - j0 : E::kCols;
+  const int u0 = part_start(total, part, parts), u1 = part_start(total, part + 1, parts);
+  for (int u = u0; u < u1;) {
+    int before;
+    const int g = find_step(a, u, before);
+    const int lo = edge(a, g), hi = edge(a, g + 1), n = steps_of(a, g);
+    const int s0 = u - before, s1 = n - s0 < u1 - u ? n : s0 + (u1 - u);
+    const int first = lo + s0 * kRowStep, last = hi - lo > s1 * kRowStep ? lo + s1 * kRowStep : hi;
+    const int depth = last > first ? last - first : 0;
     E e;
     e.sum({left + first * left_stride + i0, nullptr, left_stride, rows, depth},
           {right + first * right_stride + j0, nullptr, right_stride, cols, depth}, lds);
     if (s0 == 0 && s1 == n) {
-      T* to = dweight + (g * a.inner + i0) * a.width + j0;
+      T* to = dweight + (static_cast<int64_t>(g) * a.inner + i0) * a.width + j0;
       e.each([&](int row, int col, f32x4 v) {
-        if (row < rows && col < cols) store_four(to + row * a.width + col, cols - col, v);
+        if (row < rows && col < cols) store_four(to + static_cast<int64_t>(row) * a.width + col, cols - col, v);
       });
     } else {
-      float* to = pieces + (2 * block + (u == u0 ? 0 : 1)) * E::kRows * E::kCols;
+      float* to = pieces + (2 * static_cast<int64_t>(block) + (u == u0 ? 0 : 1)) * E::kRows * E::kCols;
       e.each([&](int row, int col, f32x4 v) { *reinterpret_cast<f32x4*>(to + row * E::kCols + col) = v; });
     }
     u += s1 - s0;
@@ -254,32 +247,37 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
 
 // Adds the pieces of the groups that were cut; a work-group takes 1024 sums.
 template <typename T>
-__global__ __launch_bounds__(256) void join_pieces(GroupedArgs a, int64_t tile_rows, int64_t tile_cols, int64_t parts,
+__global__ __launch_bounds__(256) void join_pieces(GroupedArgs a, int tile_rows, int tile_cols, int parts,
                                                    const float* __restrict__ pieces, T* __restrict__ dweight) {
-  const int64_t across = (a.width + tile_cols - 1) / tile_cols, down = (a.inner + tile_rows - 1) / tile_rows;
-  const int64_t tiles = across * down, size = tile_rows * tile_cols, slices = size / 1024;
-  const int64_t g = blockIdx.x / (slices * tiles), tile = blockIdx.x / slices % tiles;
-  int64_t total, before;
-  find_step(a, INT64_MAX, total);
-  find_segment(a.groups, INT64_MAX, [&](int64_t s) { return s < g ? steps_of(a, s) : 0; }, before);
-  const int64_t u0 = before, u1 = u0 + steps_of(a, g);
+  const unsigned across = (a.width + tile_cols - 1) / tile_cols, down = (a.inner + tile_rows - 1) / tile_rows;
+  const unsigned tiles = across * down, size = tile_rows * tile_cols, slices = size / 1024;
+  const unsigned each = blockIdx.x / slices;
+  const int g = each / tiles;
+  const unsigned tile = each - g * tiles;
+  int total, before;
+  find_step(a, INT_MAX, total);
+  find_segment(a.groups, INT_MAX, [&](int s) { return s < g ? steps_of(a, s) : 0; }, before);
+  const int u0 = before, u1 = u0 + steps_of(a, g);
   // the range that holds the group's first step
-  int64_t part = u0 * parts / total;
+  int part = static_cast<int>(static_cast<int64_t>(u0) * parts / total);
   while (part > 0 && part_start(total, part, parts) > u0) --part;
   while (part_start(total, part + 1, parts) <= u0) ++part;
   if (part_start(total, part + 1, parts) >= u1) return;  // written whole
-  const int64_t e = blockIdx.x % slices * 1024 + threadIdx.x * 4;
-  const float* from = pieces + tile * 2 * size + e;
-  f32x4 s = *reinterpret_cast<const f32x4*>(from + (part * tiles * 2 + (part_start(total, part, parts) < u0)) * size);
+  const unsigned e = (blockIdx.x - each * slices) * 1024 + threadIdx.x * 4;
+  const float* from = pieces + static_cast<int64_t>(tile) * 2 * size + e;
+  const int64_t range = static_cast<int64_t>(tiles) * 2 * size;
+  f32x4 s = *reinterpret_cast<const f32x4*>(from + part * range + (part_start(total, part, parts) < u0 ? size : 0));
   // ranges that start inside the group
-  int64_t end = part + 1;
+  int end = static_cast<int>(static_cast<int64_t>(u1) * parts / total);
+  while (end > part + 1 && part_start(total, end - 1, parts) >= u1) --end;
   while (end < parts && part_start(total, end, parts) < u1) ++end;
 #pragma unroll 4
-  for (++part; part < end; ++part) s += *reinterpret_cast<const f32x4*>(from + part * tiles * 2 * size);
-  int64_t i, j;
+  for (++part; part < end; ++part) s += *reinterpret_cast<const f32x4*>(from + part * range);
+  unsigned i, j;
   mma::place_tile(tile, down, across, i, j);
-  const int64_t row = i * tile_rows + e / tile_cols, col = j * tile_cols + e % tile_cols;
-  if (row < a.inner && col < a.width) store_four(dweight + (g * a.inner + row) * a.width + col, a.width - col, s);
+  const int row = i * tile_rows + e / tile_cols, col = j * tile_cols + e % tile_cols;
+  if (row < a.inner && col < a.width)
+    store_four(dweight + (static_cast<int64_t>(g) * a.inner + row) * a.width + col, a.width - col, s);
 }
 
 constexpr int64_t kMostStride = int64_t(1) << 22;
@@ -292,6 +290,8 @@ spmm_status check_grouped_desc(const spmm_grouped_desc* d, const char* op) {
     return fail(SPMM_ERR_CONTRACT, std::string(op) + " supports only FP16, BF16 and FP32 tensors");
   if (d->rows < 0 || d->groups < 0 || d->inner < 0 || d->width < 0)
     return fail(SPMM_ERR_CONTRACT, std::string(op) + ": negative extent");
+  if (d->rows > INT32_MAX - 512 || d->groups > (1 << 24))
+    return fail(SPMM_ERR_CONTRACT, std::string(op) + ": rows must be below 2^31 and groups at most 2^24");
   // offsets inside a tile are 32-bit
   if (d->inner >= kMostStride || d->width >= kMostStride || (d->rows > 1 && d->x_stride >= kMostStride))
     return fail(SPMM_ERR_CONTRACT, std::string(op) + ": inner, width and row strides must be below 2^22");
@@ -323,19 +323,19 @@ constexpr int64_t kCus = 256;
 // with it, 413 with the small tile.
 bool large_rows(const GroupedArgs& a) {
   return a.width > mma::kCols128 && a.inner >= 2 * mma::kDepth && a.rows / mma::kTile * ceil_div(a.width, mma::kTile) >= kCus * 3 / 4 &&
-         a.rows >= a.groups * mma::kTile / 2;
+         a.rows / (mma::kTile / 2) >= a.groups;
 }
 
 // The low tile where the groups' average leaves most of a tile of 128 empty.
-bool low_rows(const GroupedArgs& a) { return a.rows <= 48 * a.groups; }
+bool low_rows(const GroupedArgs& a) { return a.rows / 48 < a.groups; }
 
 // Copies count an operand's pieces in 32 bits.
 bool small_counts(const GroupedArgs& a, int64_t stride, int64_t other) {
-  return a.rows * (stride > other ? stride : other) < (int64_t(1) << 33);
+  return static_cast<int64_t>(a.rows) * (stride > other ? stride : other) < (int64_t(1) << 33);
 }
 
 bool large_weights(const GroupedArgs& a) {
-  return a.inner > mma::kCols128 && a.width > mma::kCols128 && a.rows >= 4 * mma::kDepth * a.groups;
+  return a.inner > mma::kCols128 && a.width > mma::kCols128 && a.rows / (4 * mma::kDepth) >= a.groups;
 }
 
 // Ranges that dW's rows are cut into: the number that takes the least time by
@@ -390,7 +390,7 @@ spmm_status launch_rows(const GroupedArgs& a, const void* in, const void* weight
   const int64_t blocks = down * ceil_div(a.width, E::kCols);
   if (spmm_status st = check_grid(blocks, op)) return st;
   hipLaunchKernelGGL((grouped_rows<E, kTurned>), dim3(static_cast<unsigned>(blocks)), dim3(E::kThreads), 0, s, a,
-                     static_cast<const T*>(in), static_cast<const T*>(weight), static_cast<T*>(out), down);
+                     static_cast<const T*>(in), static_cast<const T*>(weight), static_cast<T*>(out), static_cast<unsigned>(down));
   return check_launch(op);
 }
 
@@ -401,7 +401,7 @@ spmm_status run_rows(const GroupedArgs& a, bool aligned, const void* in, const v
                      const char* op) {
   if (a.rows == 0 || a.width == 0) return SPMM_OK;
   // (copies count a matrix's pieces in 32 bits)
-  aligned = aligned && a.inner * a.width < (int64_t(1) << 33);
+  aligned = aligned && static_cast<int64_t>(a.inner) * a.width < (int64_t(1) << 33);
   if constexpr (sizeof(T) == 2)
     if (aligned && large_rows(a)) return launch_rows<Large<T, false, !kTurned>, kTurned>(a, in, weight, out, s, op);
   if (low_rows(a))
@@ -427,18 +427,18 @@ spmm_status launch_weights(const GroupedArgs& a, const void* left, int64_t left_
   if (spmm_status st = check_grid(slices > parts * tiles ? slices : parts * tiles, op)) return st;
   hipLaunchKernelGGL(grouped_weights<E>, dim3(static_cast<unsigned>(parts * tiles)), dim3(E::kThreads), 0, s, a,
                      static_cast<const T*>(left), left_stride, static_cast<const T*>(right), right_stride,
-                     static_cast<T*>(dweight), parts, static_cast<float*>(ws));
+                     static_cast<T*>(dweight), static_cast<int>(parts), static_cast<float*>(ws));
   if (spmm_status st = check_launch(op)) return st;
   if (parts == 1) return SPMM_OK;
   hipLaunchKernelGGL(join_pieces<T>, dim3(static_cast<unsigned>(slices)), dim3(256), 0, s, a,
-                     static_cast<int64_t>(E::kRows), static_cast<int64_t>(E::kCols), parts,
+                     E::kRows, E::kCols, static_cast<int>(parts),
                      static_cast<const float*>(ws), static_cast<T*>(dweight));
   return check_launch(op);
 }
 
 GroupedArgs grouped_args(const spmm_grouped_desc* d, const void* offsets) {
-  return {d->rows, d->groups, d->inner, d->width, d->x_stride, d->weight_stride, offsets,
-          d->index_type == SPMM_INDEX_I64};
+  return {static_cast<int>(d->rows), static_cast<int>(d->groups), static_cast<int>(d->inner),
+          static_cast<int>(d->width), d->x_stride, d->weight_stride, offsets, d->index_type == SPMM_INDEX_I64};
 }
 
 // dW's operands, in the order of weight's storage.

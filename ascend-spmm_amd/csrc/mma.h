@@ -38,20 +38,28 @@ __device__ inline unsigned lds_address(const void* p) {
   return static_cast<unsigned>(reinterpret_cast<uintptr_t>((lds_ptr)p));
 }
 
+// A value that is the same on all lanes, in scalar registers.
+__device__ inline int64_t uniform(int64_t v) {
+  const unsigned lo = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v));
+  const unsigned hi = __builtin_amdgcn_readfirstlane(static_cast<unsigned>(v >> 32));
+  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
 // Work-groups run on the XCDs in turn; each XCD gets one run of the tiles, so
-// that neighbours share its L2.
-__device__ inline int64_t run_of_xcd(int64_t block, int64_t blocks) {
-  const int64_t each = blocks / kXcds, rest = blocks % kXcds, x = block % kXcds;
+// that neighbours share its L2.  (32-bit: a division of 64 bits takes longer
+// than a step of the sum.)
+__device__ inline unsigned run_of_xcd(unsigned block, unsigned blocks) {
+  const unsigned each = blocks / kXcds, rest = blocks % kXcds, x = block % kXcds;
   return x * each + (x < rest ? x : rest) + block / kXcds;
 }
 
 // Tile `n` of down x across: blocks of four tile rows, down them first, so
 // that the tiles at work together share rows of both operands.
-__device__ inline void place_tile(int64_t n, int64_t down, int64_t across, int64_t& i, int64_t& j) {
-  const int64_t block = n / (4 * across), first = 4 * block, high = down - first < 4 ? down - first : 4;
-  const int64_t m = n - block * 4 * across;
-  i = first + m % high;
-  j = m / high;
+__device__ inline void place_tile(unsigned n, unsigned down, unsigned across, unsigned& i, unsigned& j) {
+  const unsigned block = n / (4 * across), first = 4 * block, high = down - first < 4 ? down - first : 4;
+  const unsigned m = n - block * 4 * across;
+  i = high == 4 ? first + (m & 3) : first + m % high;
+  j = high == 4 ? m >> 2 : m / high;
 }
 
 // The 16 x 16 x 32 matrix instruction: lane (i = lane % 16, q = lane / 16) holds

@@ -178,12 +178,10 @@ struct Reader128 {
   }
 };
 
-// The tile's sums: wave (w / kAlong, w % kAlong) holds kA x kB fragments.
-template <int kRows>
-struct Sums128 {
-  static constexpr int kAlong = kRows == 128 ? 2 : 4;  // waves along the columns
-  static constexpr int kA = kRows == 128 ? 4 : 2;
-  static constexpr int kB = kRows == 128 ? 4 : 2;
+// A tile's sums: wave (w / kAlong, w % kAlong) holds kA x kB fragments.
+template <int kRowFragments, int kColFragments, int kWavesAlong>
+struct SumsOf {
+  static constexpr int kA = kRowFragments, kB = kColFragments, kAlong = kWavesAlong;
   f32x4 c[kA][kB];
 
   __device__ inline void clear() {
@@ -205,6 +203,10 @@ struct Sums128 {
   __device__ inline int col(int k) const { return k % kB * 16 + col0; }
   __device__ inline f32x4 four(int k) const { return c[k / kB][k % kB]; }
 };
+
+// Low tiles have their waves along the columns.
+template <int kRows>
+using Sums128 = SumsOf<kRows == 128 ? 4 : 2, kRows == 128 ? 4 : 2, kRows == 128 ? 2 : 4>;
 
 template <typename T, bool kAC, bool kBC, int kRows, bool kAligned>
 struct Tile128 {

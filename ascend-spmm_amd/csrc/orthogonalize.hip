@@ -21,6 +21,7 @@
 // result is 1.05 to 1.4 times as far off as its rounding alone.
 //
 // Planes are padded with zeros to multiples of 64, which all products keep.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -34,7 +35,7 @@ namespace {
 typedef _Float16 half;
 
 constexpr int kThreads = 256;
-constexpr int kNormParts = 64;  // work-groups that add up one matrix's squares
+constexpr int kNormParts = 512;  // work-groups that add up one matrix's squares
 constexpr int64_t kCus = 256;
 
 // Partial sums of squares in fp64: no overflow, and no loss against the total.
@@ -63,7 +64,9 @@ __global__ __launch_bounds__(kThreads) void square_sums(const T* __restrict__ u,
 
 // |U|_F + eps, by the 64 lanes of a wave alike.
 __device__ inline double norm_of(const double* parts, double eps) {
-  double s = parts[threadIdx.x & 63];
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < kNormParts / 64; ++i) s += parts[i * 64 + (threadIdx.x & 63)];
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
   return sqrt(s) + eps;
@@ -133,7 +136,7 @@ struct Addend {
 };
 
 template <Kind kKind, bool kPair>
-__device__ inline Addend load_addend(const Finish& f, int64_t batch, int64_t row, int64_t col) {
+__device__ inline Addend load_addend(const Finish& f, int64_t batch, int row, int col) {
   Addend a = {};
   if constexpr (kKind != kGram) {
     const int64_t at = batch * f.add.size + row * f.add.ld + col;
@@ -150,7 +153,7 @@ __device__ inline Addend load_addend(const Finish& f, int64_t batch, int64_t row
 }
 
 template <typename T, Kind kKind, bool kPair>
-__device__ inline void finish_four(const Finish& f, const Addend& a, int64_t batch, int64_t row, int64_t col, f32x4 sum) {
+__device__ inline void finish_four(const Finish& f, const Addend& a, int64_t batch, int row, int col, f32x4 sum) {
   f32x4 v = sum * f.alpha;
   if constexpr (kKind != kGram)
 #pragma unroll
@@ -167,7 +170,7 @@ __device__ inline void finish_four(const Finish& f, const Addend& a, int64_t bat
     T* out = static_cast<T*>(f.out) + batch * f.rows * f.cols;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int64_t i = f.tall ? col + e : row, j = f.tall ? row : col + e;
+      const int i = f.tall ? col + e : row, j = f.tall ? row : col + e;
       if (i < f.rows && j < f.cols) out[i * f.cols + j] = static_cast<T>(v[e]);
     }
   } else {
@@ -188,20 +191,19 @@ __device__ inline void finish_four(const Finish& f, const Addend& a, int64_t bat
 // Finishes a tile's sums, kCount at a time: all of a batch's addends are
 // loaded before the first is used.
 template <typename T, Kind kKind, bool kPair, int kCount, typename S>
-__device__ inline void finish_tile(const Finish& f, const S& s, int64_t batch, int64_t r0, int64_t c0, int64_t m,
-                                   int64_t n) {
+__device__ inline void finish_tile(const Finish& f, const S& s, int64_t batch, int r0, int c0, int m, int n) {
 #pragma unroll
   for (int b = 0; b < S::kFours / kCount; ++b) {
     Addend a[kCount];
 #pragma unroll
     for (int k = 0; k < kCount; ++k) {
-      const int64_t row = r0 + s.row(b * kCount + k), col = c0 + s.col(b * kCount + k);
+      const int row = r0 + s.row(b * kCount + k), col = c0 + s.col(b * kCount + k);
       const bool in = row < m && col < n;
       a[k] = load_addend<kKind, kPair>(f, batch, in ? row : 0, in ? col : 0);
     }
 #pragma unroll
     for (int k = 0; k < kCount; ++k) {
-      const int64_t row = r0 + s.row(b * kCount + k), col = c0 + s.col(b * kCount + k);
+      const int row = r0 + s.row(b * kCount + k), col = c0 + s.col(b * kCount + k);
       if (row < m && col < n) finish_four<T, kKind, kPair>(f, a[k], batch, row, col, s.four(b * kCount + k));
     }
   }
@@ -211,13 +213,13 @@ __device__ inline void finish_tile(const Finish& f, const S& s, int64_t batch, i
 // where kTurned; extents are padded ones.
 struct Product {
   Planes left, right;
-  int64_t m, n, depth;
-  int64_t splits;  // parts of the depth, each a sum of its own
+  int m, n, depth;
+  int splits;      // parts of the depth, each a sum of its own
   float* sums;     // [splits][batch][m][n] where there are several
 };
 
-__device__ inline mma::Operand<half> operand(const Planes& p, int64_t batch, int64_t first, int64_t most, int64_t rows,
-                                             int64_t depth, bool turned) {
+__device__ inline mma::Operand<half> operand(const Planes& p, int64_t batch, int first, int most, int rows, int depth,
+                                             bool turned) {
   const int64_t at = batch * p.size + (turned ? first : first * p.ld);
   return {p.hi + at, p.lo == nullptr ? nullptr : p.lo + at, p.ld, rows - first < most ? rows - first : most, depth};
 }
@@ -226,11 +228,11 @@ template <typename T, Kind kKind, bool kPair>
 __global__ __launch_bounds__(mma::kThreads, 2) void product_large(Product p, Finish f) {
   constexpr bool kTurned = kKind == kUpdate || kKind == kLast;
   __shared__ __align__(1024) char lds[mma::kLdsBytes];
-  const int64_t down = (p.m + mma::kTile - 1) / mma::kTile, across = (p.n + mma::kTile - 1) / mma::kTile;
-  const int64_t block = mma::run_of_xcd(blockIdx.x, gridDim.x), batch = block / (down * across);
-  int64_t i, j;
-  mma::place_tile(block % (down * across), down, across, i, j);
-  const int64_t r0 = i * mma::kTile, c0 = j * mma::kTile;
+  const unsigned down = (p.m + mma::kTile - 1) / mma::kTile, across = (p.n + mma::kTile - 1) / mma::kTile;
+  const unsigned block = mma::run_of_xcd(blockIdx.x, gridDim.x), batch = block / (down * across);
+  unsigned i, j;
+  mma::place_tile(block - batch * (down * across), down, across, i, j);
+  const int r0 = i * mma::kTile, c0 = j * mma::kTile;
   mma::Sums s;
   mma::multiply_tile<half, false, kTurned, kPair ? 3 : 1>(
       operand(p.left, batch, r0, mma::kTile, p.m, p.depth, false),
@@ -240,43 +242,47 @@ __global__ __launch_bounds__(mma::kThreads, 2) void product_large(Product p, Fin
 }
 
 // Splits of a matrix are further apart than its tiles.
-template <typename T, Kind kKind, bool kPair>
-__global__ __launch_bounds__(mma::kThreads128, kPair ? 1 : 2) void product_small(Product p, Finish f) {
+template <typename T, Kind kKind, bool kPair, int kSide>
+__global__ __launch_bounds__(mma::kThreads128, kSide == 64 ? 2 : 1) void product_small(Product p, Finish f) {
   constexpr bool kTurned = kKind == kUpdate || kKind == kLast;
-  typedef mma::Ring<half, false, kTurned, kPair> Tile;
+  typedef mma::Ring<half, false, kTurned, kPair, kSide, kSide> Tile;
   __shared__ __align__(1024) char lds[Tile::kLdsBytes];
-  const int64_t down = (p.m + 127) / 128, across = (p.n + 127) / 128;
-  const int64_t block = mma::run_of_xcd(blockIdx.x, gridDim.x);
-  const int64_t split = block / (down * across) % p.splits, batch = block / (down * across * p.splits);
-  int64_t i, j;
-  mma::place_tile(block % (down * across), down, across, i, j);
-  const int64_t r0 = i * 128, c0 = j * 128;
-  const int64_t steps = (p.depth + Tile::kDepth - 1) / Tile::kDepth;
-  mma::Sums128<128> s;
+  const unsigned down = (p.m + kSide - 1) / kSide, across = (p.n + kSide - 1) / kSide;
+  const unsigned block = mma::run_of_xcd(blockIdx.x, gridDim.x), matrix = block / (down * across);
+  const unsigned batch = p.splits == 1 ? matrix : matrix / p.splits, split = matrix - batch * p.splits;
+  unsigned i, j;
+  mma::place_tile(block - matrix * (down * across), down, across, i, j);
+  const int r0 = i * kSide, c0 = j * kSide;
+  const unsigned steps = p.depth / Tile::kDepth;
+  typename Tile::Sums s;
   s.clear();
-  Tile::add(operand(p.left, batch, r0, 128, p.m, p.depth, false), operand(p.right, batch, c0, 128, p.n, p.depth, kTurned),
-            lds, static_cast<int>(steps * split / p.splits), static_cast<int>(steps * (split + 1) / p.splits), s);
+  Tile::add(operand(p.left, batch, r0, kSide, p.m, p.depth, false),
+            operand(p.right, batch, c0, kSide, p.n, p.depth, kTurned), lds,
+            p.splits == 1 ? 0 : static_cast<int>(steps * split / p.splits),
+            p.splits == 1 ? static_cast<int>(steps) : static_cast<int>(steps * (split + 1) / p.splits), s);
   s.place();
   if (p.splits == 1) {
-    finish_tile<T, kKind, kPair, 16>(f, s, batch, r0, c0, p.m, p.n);
+    finish_tile<T, kKind, kPair, s.kFours>(f, s, batch, r0, c0, p.m, p.n);
     return;
   }
   const int64_t batches = gridDim.x / (down * across * p.splits);
   float* to = p.sums + (split * batches + batch) * p.m * p.n;
 #pragma unroll
   for (int k = 0; k < s.kFours; ++k) {
-    const int64_t row = r0 + s.row(k), col = c0 + s.col(k);
-    if (row < p.m && col < p.n) *reinterpret_cast<f32x4*>(to + row * p.n + col) = s.four(k);
+    const int row = r0 + s.row(k), col = c0 + s.col(k);
+    if (row < p.m && col < p.n) *reinterpret_cast<f32x4*>(to + static_cast<int64_t>(row) * p.n + col) = s.four(k);
   }
 }
 
 // Adds the splits' sums in order and finishes them.
 template <typename T, Kind kKind, bool kPair>
 __global__ __launch_bounds__(kThreads) void finish_sums(Product p, Finish f, int64_t batches) {
-  const int64_t fours = p.m * p.n / 4, n = fours * batches;
+  const int64_t fours = static_cast<int64_t>(p.m) * p.n / 4, n = fours * batches;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
        i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t batch = i / fours, e = i % fours * 4, row = e / p.n, col = e % p.n;
+    // one matrix's sums are below 2^32
+    const int64_t batch = batches == 1 ? 0 : i / fours;
+    const unsigned e = static_cast<unsigned>(i - batch * fours) * 4, row = e / p.n, col = e - row * p.n;
     const Addend a = load_addend<kKind, kPair>(f, batch, row, col);
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
@@ -498,13 +504,16 @@ __global__ __launch_bounds__(kInnerThreads) void orthogonalize_inner(InnerArgs a
   });
 }
 
+// Offsets inside a tile, and pieces of an operand, are counted in 32 bits.
+constexpr int64_t kMostExtent = int64_t(1) << 22;
+
 spmm_status check_desc(const spmm_orthogonalize_desc* d) {
   if (d == nullptr) return fail(SPMM_ERR_INVALID_ARGUMENT, "null descriptor");
   if (!dense_type(d->value_type))
     return fail(SPMM_ERR_CONTRACT, "orthogonalize supports only FP16, BF16 and FP32 tensors");
   if (d->batch < 0 || d->rows < 0 || d->width < 0) return fail(SPMM_ERR_CONTRACT, "orthogonalize: negative extent");
-  if (d->batch > 65535 || d->rows > INT32_MAX || d->width > INT32_MAX)
-    return fail(SPMM_ERR_CONTRACT, "orthogonalize takes at most 65535 matrices with extents below 2^31");
+  if (d->batch > 65535 || d->rows >= kMostExtent || d->width >= kMostExtent)
+    return fail(SPMM_ERR_CONTRACT, "orthogonalize takes at most 65535 matrices with extents below 2^22");
   if (d->steps < 0) return fail(SPMM_ERR_INVALID_ARGUMENT, "orthogonalize: steps must not be negative");
   if (d->steps > 0 && d->coefficients == nullptr) return fail(SPMM_ERR_INVALID_ARGUMENT, "orthogonalize: null coefficients");
   for (int64_t i = 0; i < 3 * d->steps; ++i)
@@ -540,6 +549,39 @@ double scale_for(double most) {
   return std::exp2(std::floor(std::log2(16384.0 / most)));
 }
 
+// How a product of smaller tiles is run: the tile's side and the parts of its
+// depth.
+struct Plan {
+  int64_t side, splits;
+};
+
+// The plan that takes the least time by this count, in microseconds: a round of
+// tiles takes 3 and its steps, 0.27 each, or where work-groups share a CU what
+// each takes of it (128: 0.2, 64: 0.11; pairs 1.8 times that) if that is more;
+// sums of parts cost a launch, 5, and 8 bytes each at 4 TB/s.  Measured on 12
+// matrices of 512 x 512 x 1024: 14.8 us with 128, 17.0 with 64.
+Plan plan_for(int64_t batch, int64_t rows, int64_t cols, int64_t depth, bool pair) {
+  Plan best{64, 1};
+  double least = 1e300;
+  const int64_t steps = ceil_div(depth, 32);
+  for (const int64_t side : {64, 128}) {
+    const int64_t on_cu = side == 64 ? (pair ? 2 : 4) : (pair ? 1 : 2);
+    const int64_t tiles = batch * ceil_div(rows, side) * ceil_div(cols, side);
+    const double share = (side == 128 ? 0.2 : 0.11) * (pair ? 1.8 : 1.0);
+    for (int64_t k = 1; k == 1 || (k <= 2 * kCus / tiles && 4 * k <= steps); ++k) {
+      const int64_t each = ceil_div(steps, k), groups = tiles * k, rounds = ceil_div(groups, kCus * on_cu);
+      const double beside = static_cast<double>(std::min(on_cu, ceil_div(groups, kCus)));
+      const double time = static_cast<double>(rounds) * (3.0 + static_cast<double>(each) * std::fmax(0.27, beside * share)) +
+                          (k > 1 ? 5.0 + static_cast<double>(k * batch * rows * cols) * 8.0 / 4e6 : 0.0);
+      if (time < least) {
+        least = time;
+        best = {side, k};
+      }
+    }
+  }
+  return best;
+}
+
 // X twice (a step reads one and writes the other), A and P in planes, their
 // diagonals' rests, the sums of squares, and the sums of split products.
 // m <= n: the matrix's extents, mp and np padded.
@@ -559,7 +601,7 @@ struct Layout {
     parts = align_up(static_cast<size_t>(d->batch * kNormParts) * sizeof(double), 256);
     sums = 0;
     for (const bool wide : {false, true}) {
-      const int64_t cols = wide ? np : mp, depth = wide ? mp : np, k = splits(d->batch, mp, cols, depth);
+      const int64_t cols = wide ? np : mp, depth = wide ? mp : np, k = splits(d->batch, mp, cols, depth, pair);
       const size_t bytes = k > 1 ? static_cast<size_t>(k * d->batch * mp * cols) * sizeof(float) : 0;
       sums = sums > bytes ? sums : bytes;
     }
@@ -570,13 +612,9 @@ struct Layout {
   static bool large(int64_t batch, int64_t rows, int64_t cols) {
     return rows > 128 && cols > 128 && batch * ceil_div(rows, mma::kTile) * ceil_div(cols, mma::kTile) >= kCus * 3 / 4;
   }
-  // Parts of the depth, of four steps or more, where there are few tiles.
-  static int64_t splits(int64_t batch, int64_t rows, int64_t cols, int64_t depth) {
+  static int64_t splits(int64_t batch, int64_t rows, int64_t cols, int64_t depth, bool pair) {
     if (batch == 0 || rows == 0 || cols == 0 || large(batch, rows, cols)) return 1;
-    const int64_t tiles = batch * ceil_div(rows, 128) * ceil_div(cols, 128);
-    int64_t k = kCus / tiles, most = depth / (4 * mma::kDepth);
-    k = k < most ? k : most;
-    return k < 1 ? 1 : k;
+    return plan_for(batch, rows, cols, depth, pair).splits;
   }
 };
 
@@ -587,12 +625,17 @@ spmm_status multiply(Product p, const Finish& f, int64_t batch, hipStream_t s) {
     hipLaunchKernelGGL((product_large<T, kKind, kPair>), dim3(tiles), dim3(mma::kThreads), 0, s, p, f);
     return check_launch("orthogonalize product");
   }
-  p.splits = Layout::splits(batch, p.m, p.n, p.depth);
-  const unsigned tiles = static_cast<unsigned>(ceil_div(p.m, 128) * ceil_div(p.n, 128) * batch * p.splits);
-  hipLaunchKernelGGL((product_small<T, kKind, kPair>), dim3(tiles), dim3(mma::kThreads128), 0, s, p, f);
+  const Plan plan = plan_for(batch, p.m, p.n, p.depth, kPair);
+  p.splits = static_cast<int>(plan.splits);
+  const dim3 tiles(static_cast<unsigned>(ceil_div(p.m, plan.side) * ceil_div(p.n, plan.side) * batch * p.splits));
+  const dim3 threads(mma::kThreads128);
+  if (plan.side == 128)
+    hipLaunchKernelGGL((product_small<T, kKind, kPair, 128>), tiles, threads, 0, s, p, f);
+  else
+    hipLaunchKernelGGL((product_small<T, kKind, kPair, 64>), tiles, threads, 0, s, p, f);
   if (spmm_status st = check_launch("orthogonalize product")) return st;
   if (p.splits == 1) return SPMM_OK;
-  const int64_t blocks = ceil_div(p.m * p.n / 4 * batch, kThreads);
+  const int64_t blocks = ceil_div(static_cast<int64_t>(p.m) * p.n / 4 * batch, kThreads);
   hipLaunchKernelGGL((finish_sums<T, kKind, kPair>), dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)),
                      dim3(kThreads), 0, s, p, f, batch);
   return check_launch("orthogonalize sums");
@@ -671,6 +714,7 @@ template <typename T>
 spmm_status run(const spmm_orthogonalize_desc* d, const Layout& l, const void* update, void* out, char* ws,
                 hipStream_t s) {
   const bool tall = d->rows > d->width;
+  const int mp = static_cast<int>(l.mp), np = static_cast<int>(l.np);
   auto take = [&](size_t bytes) {
     char* p = ws;
     ws += bytes;
@@ -716,20 +760,20 @@ spmm_status run(const spmm_orthogonalize_desc* d, const Layout& l, const void* u
     f.alpha = static_cast<float>(c.gram);
     f.to = gram;
     f.diagonal = gram_rest;
-    if (spmm_status st = multiply<T, kGram>({x, x, l.mp, l.mp, l.np, 1, sums}, f, d->batch, l.pair, s)) return st;
+    if (spmm_status st = multiply<T, kGram>({x, x, mp, mp, np, 1, sums}, f, d->batch, l.pair, s)) return st;
     f.alpha = static_cast<float>(c.poly);
     f.beta = static_cast<float>(c.poly_a);
     f.add = gram;
     f.rest = gram_rest;
     f.to = poly;
     f.diagonal = poly_rest;
-    if (spmm_status st = multiply<T, kPoly>({gram, gram, l.mp, l.mp, l.mp, 1, sums}, f, d->batch, l.pair, s)) return st;
+    if (spmm_status st = multiply<T, kPoly>({gram, gram, mp, mp, mp, 1, sums}, f, d->batch, l.pair, s)) return st;
     f.alpha = static_cast<float>(c.update);
     f.beta = static_cast<float>(c.update_x);
     f.add = x;
     f.rest = poly_rest;
     f.to = y;
-    const Product p{poly, x, l.mp, l.np, l.mp, 1, sums};
+    const Product p{poly, x, mp, np, mp, 1, sums};
     if (spmm_status st = i + 1 < d->steps ? multiply<T, kUpdate>(p, f, d->batch, l.pair, s)
                                           : multiply<T, kLast>(p, f, d->batch, l.pair, s))
       return st;
@@ -768,7 +812,7 @@ spmm_status spmm_orthogonalize_run(const spmm_orthogonalize_desc* d, const void*
   const Layout l(d);
   if (workspace == nullptr || workspace_bytes < l.total())
     return fail(SPMM_ERR_CONTRACT, "orthogonalize: workspace too small: need " + std::to_string(l.total()) + " bytes");
-  if (ceil_div(l.mp, 128) * ceil_div(l.np, 128) * d->batch > INT32_MAX / 64 || l.np / 64 > 65535 * 64 || l.mp / 64 > 65535)
+  if (ceil_div(l.mp, 64) * ceil_div(l.np, 64) * d->batch > INT32_MAX / 64 || l.mp * l.np >= (int64_t(1) << 32))
     return fail(SPMM_ERR_OVERFLOW, "orthogonalize: too many tiles for one launch");
   char* ws = static_cast<char*>(workspace);
   switch (d->value_type) {

@@ -455,7 +455,7 @@ spmm_status spmm_layer_norm_grad_run(const spmm_norm_desc* desc, const void* x, 
  * offsets[0] and from offsets[groups] on become zero.  weight[g] is
  * inner x width, at weight + g * weight_stride; transposed: stored as
  * width x inner, each group's matrix contiguous either way.  inner, width and
- * the row strides are below 2^22. */
+ * the row strides are below 2^22, rows below 2^31. */
 typedef struct spmm_grouped_desc {
   int64_t rows;           /* of x, out and grad                            */
   int64_t groups;
@@ -483,7 +483,7 @@ spmm_status spmm_grouped_grad_run(const spmm_grouped_desc* desc, const void* x, 
                                   void* workspace, size_t workspace_bytes, spmm_stream stream);
 
 /* orthogonalize: `steps` Newton-Schulz steps on each of `batch` matrices of
- * rows x width (contiguous).  X = update / (|update|_F + eps), then each step
+ * rows x width (contiguous, extents below 2^22).  X = update / (|update|_F + eps), then each step
  * replaces X by a X + (b A + c A A) X with A = X X^T (for more rows than
  * columns the same polynomial from the right).  coefficients: 3 * steps host
  * values (a, b, c of each step).  out may be update itself. */
