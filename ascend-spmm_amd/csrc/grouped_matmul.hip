@@ -109,11 +109,12 @@ __device__ inline void each_four(S& s, F f) {
   for (int k = 0; k < S::kFours; ++k) f(s.row(k), s.col(k), s.four(k));
 }
 
-// The engines of one product: Large of mma_256.h, Small of mma_128.h.
+// The engines of one product: Large of mma_256.h, Middle of mma_ring.h, Small of
+// mma_staged.h.
 template <typename T, bool kAC, bool kBC>
 struct Large {
   typedef T Value;
-  static constexpr int kRows = mma::kTile, kCols = mma::kTile, kThreads = mma::kThreads, kStep = mma::kDepth;
+  static constexpr int kRows = mma::kTile, kCols = mma::kTile, kThreads = mma::kThreads;
   static constexpr int kLds = mma::kLdsBytes, kPerCu = 1;
   mma::Sums s;
   __device__ inline void sum(const mma::Operand<T>& a, const mma::Operand<T>& b, char* lds) {
@@ -128,16 +129,11 @@ struct Large {
 template <typename T, bool kAC, bool kBC, int kHeight, bool kAligned>
 struct Small {
   typedef T Value;
-  typedef mma::Tile128<T, kAC, kBC, kHeight, kAligned> Tile;
-  static constexpr int kRows = kHeight, kCols = mma::kCols128, kThreads = mma::kThreads128,
-                       kStep = mma::Step<T>::kDepth;
-  // fp32's parts take registers for 256 a thread
-  static constexpr int kLds = Tile::kLdsBytes, kPerCu = std::is_same_v<T, float> ? 2 : 3;
-  mma::Sums128<kHeight> s;
-  __device__ inline void sum(const mma::Operand<T>& a, const mma::Operand<T>& b, char* lds) {
-    s.clear();
-    Tile::add(a, b, lds, 0, (a.depth + kStep - 1) / kStep, s);
-  }
+  static constexpr int kRows = kHeight, kCols = kHeight == 32 ? 128 : 64, kThreads = mma::kThreads128;
+  typedef mma::Staged<T, kAC, kBC, kRows, kCols, kAligned> Tile;
+  static constexpr int kLds = Tile::kLdsBytes, kPerCu = 4;
+  typename Tile::Sums s;
+  __device__ inline void sum(const mma::Operand<T>& a, const mma::Operand<T>& b, char* lds) { Tile::sum(a, b, lds, s); }
   template <typename F>
   __device__ inline void each(F f) {
     each_four(s, f);
@@ -148,7 +144,7 @@ template <typename T, bool kAC, bool kBC>
 struct Middle {
   typedef T Value;
   typedef mma::Ring<T, kAC, kBC, false, 128, 128> Tile;
-  static constexpr int kRows = 128, kCols = mma::kCols128, kThreads = mma::kThreads128, kStep = Tile::kDepth;
+  static constexpr int kRows = 128, kCols = 128, kThreads = mma::kThreads128, kStep = Tile::kDepth;
   static constexpr int kLds = Tile::kLdsBytes, kPerCu = 2;
   typename Tile::Sums s;
   __device__ inline void sum(const mma::Operand<T>& a, const mma::Operand<T>& b, char* lds) {
@@ -322,7 +318,7 @@ constexpr int64_t kCus = 256;
 // average fills half of one.  65536 x 1024 x 2048 bf16 in 8 groups: 289 us
 // with it, 413 with the small tile.
 bool large_rows(const GroupedArgs& a) {
-  return a.width > mma::kCols128 && a.inner >= 2 * mma::kDepth && a.rows / mma::kTile * ceil_div(a.width, mma::kTile) >= kCus * 3 / 4 &&
+  return a.width > 128 && a.inner >= 2 * mma::kDepth && a.rows / mma::kTile * ceil_div(a.width, mma::kTile) >= kCus * 3 / 4 &&
          a.rows / (mma::kTile / 2) >= a.groups;
 }
 
@@ -335,20 +331,20 @@ bool small_counts(const GroupedArgs& a, int64_t stride, int64_t other) {
 }
 
 bool large_weights(const GroupedArgs& a) {
-  return a.inner > mma::kCols128 && a.width > mma::kCols128 && a.rows / (4 * mma::kDepth) >= a.groups;
+  return a.inner > 128 && a.width > 128 && a.rows / (4 * mma::kDepth) >= a.groups;
 }
 
 // Ranges that dW's rows are cut into: the number that takes the least time by
 // this count, in microseconds.  A round of work-groups takes its steps (1 each
-// for the large tile, 0.5 for two of the small one on a CU); a cut costs a
+// for the large tile, 0.5 for two of 128 on a CU, 2.4 for four of fp32's); a cut costs a
 // piece of each tile written and read at 4 TB/s, and joining a launch.
-int64_t weight_parts(const GroupedArgs& a) {
-  const bool large = large_weights(a);
-  const int64_t side = large ? mma::kTile : 128, at_once = kCus * (large ? 1 : 2);
+int64_t weight_parts(const GroupedArgs& a, bool fp32) {
+  const bool large = !fp32 && large_weights(a);
+  const int64_t side = large ? mma::kTile : fp32 ? 64 : 128, at_once = kCus * (large ? 1 : fp32 ? 4 : 2);
   const int64_t tiles = ceil_div(a.inner, side) * ceil_div(a.width, side);
   const int64_t steps = a.rows / kRowStep + a.groups;
   if (tiles == 0 || steps == 0) return 1;
-  const double step = large ? 1.0 : 0.5, piece = static_cast<double>(tiles * side * side) * 8.0 / 4e6;
+  const double step = large ? 1.0 : fp32 ? 2.4 : 0.5, piece = static_cast<double>(tiles * side * side) * 8.0 / 4e6;
   int64_t best = 1;
   double least = 1e300;
   auto consider = [&](int64_t parts) {
@@ -366,7 +362,7 @@ int64_t weight_parts(const GroupedArgs& a) {
 }
 template <typename E>
 size_t weight_bytes(const GroupedArgs& a) {
-  const int64_t parts = weight_parts(a), tiles = ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols);
+  const int64_t parts = weight_parts(a, std::is_same_v<typename E::Value, float>), tiles = ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols);
   return parts == 1 ? 0 : static_cast<size_t>(parts * tiles) * 2 * E::kRows * E::kCols * sizeof(float);
 }
 
@@ -410,8 +406,8 @@ spmm_status run_rows(const GroupedArgs& a, bool aligned, const void* in, const v
   if constexpr (sizeof(T) == 2)
     if (aligned) return launch_rows<Middle<T, false, !kTurned>, kTurned>(a, in, weight, out, s, op);
   if constexpr (sizeof(T) == 4)
-    if (aligned) return launch_rows<Small<T, false, !kTurned, 128, true>, kTurned>(a, in, weight, out, s, op);
-  return launch_rows<Small<T, false, !kTurned, 128, false>, kTurned>(a, in, weight, out, s, op);
+    if (aligned) return launch_rows<Small<T, false, !kTurned, 64, true>, kTurned>(a, in, weight, out, s, op);
+  return launch_rows<Small<T, false, !kTurned, 64, false>, kTurned>(a, in, weight, out, s, op);
 }
 
 template <typename E>
@@ -422,7 +418,7 @@ spmm_status launch_weights(const GroupedArgs& a, const void* left, int64_t left_
   const size_t need = weight_bytes<E>(a);
   if (need > 0 && (ws == nullptr || ws_bytes < need))
     return fail(SPMM_ERR_CONTRACT, std::string(op) + ": workspace too small: need " + std::to_string(need) + " bytes");
-  const int64_t parts = weight_parts(a), tiles = ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols);
+  const int64_t parts = weight_parts(a, std::is_same_v<typename E::Value, float>), tiles = ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols);
   const int64_t slices = a.groups * tiles * (E::kRows * E::kCols / 1024);
   if (spmm_status st = check_grid(slices > parts * tiles ? slices : parts * tiles, op)) return st;
   hipLaunchKernelGGL(grouped_weights<E>, dim3(static_cast<unsigned>(parts * tiles)), dim3(E::kThreads), 0, s, a,
@@ -463,8 +459,8 @@ spmm_status with_weight_engine(const GroupedArgs& a, bool aligned, int64_t strid
       return large_weights(a) ? f(static_cast<Large<T, true, true>*>(nullptr))
                               : f(static_cast<Middle<T, true, true>*>(nullptr));
   if constexpr (sizeof(T) == 4)
-    if (aligned) return f(static_cast<Small<T, true, true, 128, true>*>(nullptr));
-  return f(static_cast<Small<T, true, true, 128, false>*>(nullptr));
+    if (aligned) return f(static_cast<Small<T, true, true, 64, true>*>(nullptr));
+  return f(static_cast<Small<T, true, true, 64, false>*>(nullptr));
 }
 
 }  // namespace

@@ -1,4 +1,5 @@
-// Operands and matrix instructions of the product tiles (mma_256.h, mma_128.h).
+// Operands and matrix instructions of the product tiles (mma_256.h, mma_ring.h,
+// mma_staged.h).
 #pragma once
 
 #include "numeric.h"

@@ -9,7 +9,7 @@
 // read, whose place the copies started next take.
 #pragma once
 
-#include "mma_128.h"
+#include "mma_staged.h"
 #include "mma_256.h"
 
 namespace spmm {

@@ -1,15 +1,18 @@
-// kRows x 128 tiles of matrix products, four waves, for operands of any
-// alignment and for fp32.
+// Tiles of matrix products, four waves, for operands of any alignment and for
+// fp32: 64 x 64, or 32 x 128 for groups of few rows.
 //
 // Operands pass through registers into LDS, one step of the sum at a time; the
-// next step's loads are under way during the matrix instructions, and three to
-// four work-groups of a CU hide each other's barriers.
+// next step's loads are under way during the matrix instructions, and four or
+// more work-groups of a CU hide each other's barriers.
 //
 // fp32 operands are split into three bf16 parts on the way, each the leading
 // eight digits of what the ones before leave over, so their sum is the fp32
 // value; all their products but that of the last two, which is below 2^-28 of
 // the whole, are added in fp32.  That is the precision of fp32 products at 8 of
-// the 16 matrix cycles that fp32 instructions take.
+// the 16 matrix cycles that fp32 instructions take.  Parts of an infinity's
+// counterpart may be zero, and their product with it a NaN where fp32 has an
+// infinity: a tile that meets an infinity is summed again with parts that are
+// never zero (kCareful).
 #pragma once
 
 #include "mma.h"
@@ -17,7 +20,6 @@
 namespace spmm {
 namespace mma {
 
-constexpr int kCols128 = 128;
 constexpr int kThreads128 = 256;
 
 template <typename T>
@@ -26,22 +28,26 @@ struct Step {
   static constexpr int kDepth = std::is_same_v<T, float> ? 32 : 64;
 };
 
-// Three bf16 parts of fp32 values, by truncation: all parts of a value have its
-// sign, and what the last one leaves is below 2^-24 of it.  Parts that would be
-// zero are 2^-126 where the value is 2^-60 or more: nothing against the sum,
-// and the product with an infinity stays infinite.
+// Three bf16 parts of an fp32 value, by truncation: all parts of a value have
+// its sign, and what the last one leaves is below 2^-24 of it.  kCareful: parts
+// that would be zero are 2^-126 where the value is 2^-60 or more, nothing
+// against the sum, so that their product with an infinity stays infinite.
+template <bool kCareful>
 __device__ inline void split(float x, unsigned& hi, unsigned& mid, unsigned& lo) {
-  const unsigned sign = __builtin_bit_cast(unsigned, x) & 0x80000000u;
-  const unsigned least = (__builtin_bit_cast(unsigned, x) & 0x7f800000u) >= 0x21800000u ? sign | 0x00800000u : 0u;
   hi = __builtin_bit_cast(unsigned, x) & 0xffff0000u;
   const float high = __builtin_bit_cast(float, hi);
-  const float rest = x == high ? 0.0f : x - high;
+  const float rest = kCareful && x == high ? 0.0f : x - high;
   mid = __builtin_bit_cast(unsigned, rest) & 0xffff0000u;
-  const float last = rest - __builtin_bit_cast(float, mid);
-  lo = __builtin_bit_cast(unsigned, last) & 0xffff0000u;
-  mid = (mid & 0x7fffffffu) == 0u ? least : mid;
-  lo = (lo & 0x7fffffffu) == 0u ? least : lo;
+  lo = __builtin_bit_cast(unsigned, rest - __builtin_bit_cast(float, mid));
+  if constexpr (kCareful) {
+    const unsigned sign = __builtin_bit_cast(unsigned, x) & 0x80000000u;
+    const unsigned least = (__builtin_bit_cast(unsigned, x) & 0x7f800000u) >= 0x21800000u ? sign | 0x00800000u : 0u;
+    mid = (mid & 0x7fffffffu) == 0u ? least : mid;
+    lo = (lo & 0x7fff0000u) == 0u ? least : lo;
+  }
 }
+// The upper halves of a and b as two neighbouring bf16 values.
+__device__ inline unsigned upper_halves(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
 // One operand's kRows x depth of a step in LDS and its way there.  Layouts as
 // the 256 tile's halves: where k is contiguous, lines of kDepth elements whose
@@ -59,7 +65,7 @@ struct Stage {
   static constexpr int kLines = kThreads128 / kAcross;        // of a round
   static constexpr int kLineBytes = kAcross * 16;
   static constexpr int kVectors = sizeof(T) / 2;
-  static_assert(!C || kRows == 128, "low tiles are of contiguous k");
+  static_assert(!C || kRows == 128 || kRows == 64, "low tiles are of contiguous k");
   static_assert(kLines % 16 == 0, "the exchange repeats every 16 lines");
 
   u32x4 held[kEach][kVectors];
@@ -70,8 +76,10 @@ struct Stage {
 
   // The exchange: place of a 16-byte piece of a line.
   __device__ static inline int place(int line, int piece) {
-    if constexpr (C)
+    if constexpr (C && kRows == 128)
       return line * kLineBytes + (piece ^ (((line & 3) | ((line >> 3 & 1) << 2)) << 1)) * 16;
+    else if constexpr (C)
+      return line * kLineBytes + (piece ^ (((line >> 1 & 1) | ((line >> 3 & 1) << 1)) << 1)) * 16;
     else if constexpr (S::kDepth == 64)
       return line * kLineBytes + (piece ^ (line & 7)) * 16;
     else
@@ -117,7 +125,9 @@ struct Stage {
     }
   }
 
-  __device__ inline void store(char* lds) const {
+  // `most`: raised to the largest magnitude that passes (fp32).
+  template <bool kCareful>
+  __device__ inline void store(char* lds, float& most) const {
     if (!kWhole && line == 1 << 28) return;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
@@ -128,11 +138,14 @@ struct Stage {
         u32x4 parts[3];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
+          const float x = __builtin_bit_cast(float, static_cast<unsigned>(held[e][m / 2][m % 2 * 2]));
+          const float y = __builtin_bit_cast(float, static_cast<unsigned>(held[e][m / 2][m % 2 * 2 + 1]));
+          if constexpr (!kCareful) most = fmaxf(fmaxf(most, fabsf(x)), fabsf(y));
           unsigned a[3], b[3];
-          split(__builtin_bit_cast(float, static_cast<unsigned>(held[e][m / 2][m % 2 * 2])), a[0], a[1], a[2]);
-          split(__builtin_bit_cast(float, static_cast<unsigned>(held[e][m / 2][m % 2 * 2 + 1])), b[0], b[1], b[2]);
+          split<kCareful>(x, a[0], a[1], a[2]);
+          split<kCareful>(y, b[0], b[1], b[2]);
 #pragma unroll
-          for (int q = 0; q < 3; ++q) parts[q][m] = a[q] >> 16 | b[q];
+          for (int q = 0; q < 3; ++q) parts[q][m] = upper_halves(a[q], b[q]);
         }
 #pragma unroll
         for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x4*>(at + q * kBytes) = parts[q];
@@ -144,13 +157,13 @@ struct Stage {
 // Reads kCount fragments of 16 rows, from row `first`: one address for each
 // that the exchange tells apart, the rest by constant offsets.
 template <typename T, bool C, int kRows, int kCount>
-struct Reader128 {
+struct StageReader {
   typedef Stage<T, C, kRows, true> G;
   static constexpr int kDepth = G::S::kDepth;
   static constexpr int kAddresses = C ? kCount : kDepth / 32;
   int at[kAddresses];
 
-  __device__ inline Reader128(int first, int thread) {
+  __device__ inline StageReader(int first, int thread) {
     const int lane = thread & 63, q = lane >> 4;
 #pragma unroll
     for (int i = 0; i < kAddresses; ++i) {
@@ -204,42 +217,57 @@ struct SumsOf {
   __device__ inline f32x4 four(int k) const { return c[k / kB][k % kB]; }
 };
 
-// Low tiles have their waves along the columns.
-template <int kRows>
-using Sums128 = SumsOf<kRows == 128 ? 4 : 2, kRows == 128 ? 4 : 2, kRows == 128 ? 2 : 4>;
-
-template <typename T, bool kAC, bool kBC, int kRows, bool kAligned>
-struct Tile128 {
+template <typename T, bool kAC, bool kBC, int kRows, int kCols, bool kAligned>
+struct Staged {
   typedef Step<T> S;
   typedef Stage<T, kAC, kRows, kAligned> StageA;
-  typedef Stage<T, kBC, kCols128, kAligned> StageB;
+  typedef Stage<T, kBC, kCols, kAligned> StageB;
+  // A low tile has its waves along the columns.
+  static constexpr int kAlong = kRows == 32 ? 4 : 2;
+  typedef SumsOf<kRows * kAlong / 64, kCols / kAlong / 16, kAlong> Sums;
   static constexpr int kLdsBytes = S::kParts * (StageA::kBytes + StageB::kBytes);
 
-  // Adds the steps [from, to) of the sum over k of A(i, k) B(j, k).
-  __device__ static inline void add(const Operand<T>& a, const Operand<T>& b, char* lds, int64_t from, int64_t to,
-                                    Sums128<kRows>& s) {
+  // The sum over k of A(i, k) B(j, k).
+  __device__ static inline void sum(const Operand<T>& a, const Operand<T>& b, char* lds, Sums& s) {
+    float most = 0.0f;
+    s.clear();
+    add<false>(a, b, lds, s, most);
+    if constexpr (S::kParts == 3) {
+      if (__syncthreads_or(most == __builtin_inff())) {
+        s.clear();
+        add<true>(a, b, lds, s, most);
+      }
+    }
+  }
+
+  template <bool kCareful>
+  __device__ static inline void add(const Operand<T>& a, const Operand<T>& b, char* lds, Sums& s, float& most) {
     const int thread = thread_here(), wave = thread >> 6;
     char* lb = lds + S::kParts * StageA::kBytes;
-    typedef Sums128<kRows> Sums;
-    const Reader128<T, kAC, kRows, Sums::kA> ra(wave / Sums::kAlong * Sums::kA * 16, thread);
-    const Reader128<T, kBC, kCols128, Sums::kB> rb(wave % Sums::kAlong * Sums::kB * 16, thread);
+    const StageReader<T, kAC, kRows, Sums::kA> ra(wave / kAlong * Sums::kA * 16, thread);
+    const StageReader<T, kBC, kCols, Sums::kB> rb(wave % kAlong * Sums::kB * 16, thread);
     const int va = static_cast<int>(a.valid), vb = static_cast<int>(b.valid);
     StageA sa;
     StageB sb;
     sa.start(a.ld, thread);
     sb.start(b.ld, thread);
-    auto load = [&](int64_t t) {
-      const int64_t k0 = t * S::kDepth, left = a.depth - k0;
-      const int most = static_cast<int>(left < S::kDepth ? left : S::kDepth);
-      sa.load(a.p + k0 * (kAC ? a.ld : 1), va, most);
-      sb.load(b.p + k0 * (kBC ? b.ld : 1), vb, most);
+    const T *pa = a.p, *pb = b.p;
+    const int64_t step_a = S::kDepth * (kAC ? a.ld : 1), step_b = S::kDepth * (kBC ? b.ld : 1);
+    int left = static_cast<int>(a.depth);
+    auto load = [&]() {
+      const int most_k = left < S::kDepth ? left : S::kDepth;
+      sa.load(pa, va, most_k);
+      sb.load(pb, vb, most_k);
+      pa += step_a;
+      pb += step_b;
     };
-    if (from < to) load(from);
-    for (int64_t t = from; t < to; ++t) {
+    if (left > 0) load();
+    for (; left > 0;) {
       __syncthreads();  // the last step's fragments have been read
-      sa.store(lds);
-      sb.store(lb);
-      if (t + 1 < to) load(t + 1);
+      sa.template store<kCareful>(lds, most);
+      sb.template store<kCareful>(lb, most);
+      left -= S::kDepth;
+      if (left > 0) load();
       __syncthreads();
 #pragma unroll
       for (int kk = 0; kk < S::kDepth / 32; ++kk) {

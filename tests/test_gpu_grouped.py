@@ -129,6 +129,24 @@ def test_bad_values_stay_in_their_rows(spmm_npu, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("inner,width", [(40, 48), (77, 33), (256, 264)])
+def test_infinities(spmm_npu, dtype, inner, width):
+    """Infinite where the products say so, with their sign, also against
+    factors of few digits, and NaN against zeros."""
+    sizes = [40, 90]
+    x, w, dy = make(sum(sizes), 2, inner, width, dtype)
+    w[0, 3, :] = torch.randint(-2, 3, (width,), device="cuda").to(dtype)  # zeros, ones and twos
+    x[5, 3], x[17, 3], x[100, 0] = float("inf"), float("-inf"), float("inf")
+    want, _, _ = plain(x, w, edges_of(sizes), dy)
+    y, dx, dw = run_all(spmm_npu.grouped_matmul, x, w, edges_of(sizes), dy)
+    for got, ref in ((y, want[0]), (dw, want[2])):
+        got = got.double().cpu()
+        assert torch.equal(got.isnan(), ref.isnan())
+        infinite = ref.isinf()
+        assert infinite.any() and torch.equal(got[infinite], ref[infinite]) and got[ref.isfinite()].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("inner,width", [(40, 48), (129, 130), (256, 64)])
 def test_views(spmm_npu, dtype, inner, width):
     """Columns of a wider x at an odd offset, an expanded and a strided
