@@ -86,9 +86,10 @@ __device__ inline bool find_rows(const GroupedArgs& a, int height, int tile, Row
   return true;
 }
 
-// Four sums of one row, rounded; `cols`: of the row from the first of them.
+// Neighbouring sums of one row, rounded; `cols`: of the row from the first of
+// them.
 template <typename T>
-__device__ inline void store_four(T* to, int64_t cols, f32x4 v) {
+__device__ inline void store_four(T* to, int cols, f32x4 v) {
   typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
   if (cols >= 4) {
     *reinterpret_cast<four*>(to) =
@@ -99,14 +100,31 @@ __device__ inline void store_four(T* to, int64_t cols, f32x4 v) {
       if (e < cols) to[e] = static_cast<T>(v[e]);
   }
 }
+template <typename T>
+__device__ inline void store_eight(T* to, int cols, f32x4 v, f32x4 w) {
+  if constexpr (sizeof(T) == 2) {
+    if (cols >= 8) {
+      piece_t<T> p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[e] = static_cast<T>(v[e]);
+        p[e + 4] = static_cast<T>(w[e]);
+      }
+      *reinterpret_cast<piece_t<T>*>(to) = p;
+      return;
+    }
+  }
+  store_four(to, cols, v);
+  if (cols > 4) store_four(to + 4, cols - 4, w);
+}
 
-// Calls f(row, column, four sums of neighbouring columns) for the lane's part
+// Calls f(row, column, eight sums of neighbouring columns) for the lane's part
 // of a tile.
 template <typename S, typename F>
-__device__ inline void each_four(S& s, F f) {
+__device__ inline void each_eight(S& s, F f) {
   s.place();
 #pragma unroll
-  for (int k = 0; k < S::kFours; ++k) f(s.row(k), s.col(k), s.four(k));
+  for (int k = 0; k < S::kEights; ++k) f(s.row(k), s.col(k), s.four(k, 0), s.four(k, 1));
 }
 
 // The engines of one product: Large of mma_256.h, Middle of mma_ring.h, Small of
@@ -122,7 +140,7 @@ struct Large {
   }
   template <typename F>
   __device__ inline void each(F f) {
-    each_four(s, f);
+    each_eight(s, f);
   }
 };
 
@@ -136,7 +154,7 @@ struct Small {
   __device__ inline void sum(const mma::Operand<T>& a, const mma::Operand<T>& b, char* lds) { Tile::sum(a, b, lds, s); }
   template <typename F>
   __device__ inline void each(F f) {
-    each_four(s, f);
+    each_eight(s, f);
   }
 };
 
@@ -153,7 +171,7 @@ struct Middle {
   }
   template <typename F>
   __device__ inline void each(F f) {
-    each_four(s, f);
+    each_eight(s, f);
   }
 };
 
@@ -177,8 +195,8 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
   const int depth = r.group < 0 ? 0 : a.inner;
   e.sum({in + r.first * a.in_stride, nullptr, a.in_stride, r.rows, depth},
         {w, nullptr, kTurned ? a.inner : a.width, cols, depth}, lds);
-  e.each([&](int row, int col, f32x4 v) {
-    if (row < r.rows && col < cols) store_four(to + static_cast<int64_t>(row) * a.width + col, cols - col, v);
+  e.each([&](int row, int col, f32x4 v, f32x4 w) {
+    if (row < r.rows && col < cols) store_eight(to + static_cast<int64_t>(row) * a.width + col, cols - col, v, w);
   });
 }
 
@@ -230,12 +248,15 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
           {right + first * right_stride + j0, nullptr, right_stride, cols, depth}, lds);
     if (s0 == 0 && s1 == n) {
       T* to = dweight + (static_cast<int64_t>(g) * a.inner + i0) * a.width + j0;
-      e.each([&](int row, int col, f32x4 v) {
-        if (row < rows && col < cols) store_four(to + static_cast<int64_t>(row) * a.width + col, cols - col, v);
+      e.each([&](int row, int col, f32x4 v, f32x4 w) {
+        if (row < rows && col < cols) store_eight(to + static_cast<int64_t>(row) * a.width + col, cols - col, v, w);
       });
     } else {
       float* to = pieces + (2 * static_cast<int64_t>(block) + (u == u0 ? 0 : 1)) * E::kRows * E::kCols;
-      e.each([&](int row, int col, f32x4 v) { *reinterpret_cast<f32x4*>(to + row * E::kCols + col) = v; });
+      e.each([&](int row, int col, f32x4 v, f32x4 w) {
+        *reinterpret_cast<f32x4*>(to + row * E::kCols + col) = v;
+        *reinterpret_cast<f32x4*>(to + row * E::kCols + col + 4) = w;
+      });
     }
     u += s1 - s0;
   }

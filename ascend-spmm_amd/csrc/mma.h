@@ -63,6 +63,20 @@ __device__ inline void place_tile(unsigned n, unsigned down, unsigned across, un
   j = high == 4 ? m >> 2 : m / high;
 }
 
+// Two fours of neighbouring columns, of fragments 16 columns apart: lane group q
+// = lane / 16 % 4 holds columns 4 q .. 4 q + 3 of either.  Exchanged with the
+// next group, each lane holds eight neighbouring columns, from eight_column().
+__device__ inline void exchange_fours(f32x4& a, f32x4& b) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const u32x2 r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, static_cast<float>(a[e])),
+                                                     __builtin_bit_cast(unsigned, static_cast<float>(b[e])), false, false);
+    a[e] = __builtin_bit_cast(float, static_cast<unsigned>(r[0]));
+    b[e] = __builtin_bit_cast(float, static_cast<unsigned>(r[1]));
+  }
+}
+__device__ inline int eight_column(int lane) { return (lane >> 4 & 1) * 16 + (lane >> 5) * 8; }
+
 // The 16 x 16 x 32 matrix instruction: lane (i = lane % 16, q = lane / 16) holds
 // k = 8 q .. 8 q + 7 of row i of either operand, and gets the sums of b's row i
 // with a's rows 4 q .. 4 q + 3.

@@ -249,18 +249,21 @@ struct Copier {
 struct Sums {
   Quadrant c[2][2];
 
-  // The lane's sums as fours of neighbouring columns; place() comes first.
-  static constexpr int kFours = 32;
+  // The lane's sums as eights of neighbouring columns; place() comes first.
+  static constexpr int kEights = 16;
   int row0, col0;
   __device__ inline void place() {
     const int thread = thread_here(), lane = thread & 63, wave = thread >> 6;
     row0 = (wave >> 2) * 64 + (lane & 15);
-    col0 = (wave & 3) * 32 + (lane >> 4) * 4;
+    col0 = (wave & 3) * 32 + eight_column(lane);
+#pragma unroll
+    for (int k = 0; k < kEights; ++k) exchange_fours(quadrant(k)[k >> 1 & 3][0], quadrant(k)[k >> 1 & 3][1]);
   }
-  // k: row half, row, column half, column
-  __device__ inline int row(int k) const { return (k >> 4) * 128 + (k >> 2 & 3) * 16 + row0; }
-  __device__ inline int col(int k) const { return (k >> 1 & 1) * 128 + (k & 1) * 16 + col0; }
-  __device__ inline f32x4 four(int k) const { return c[k >> 4][k >> 1 & 1][k >> 2 & 3][k & 1]; }
+  // k: row half, row, column half
+  __device__ inline Quadrant& quadrant(int k) { return c[k >> 3][k & 1]; }
+  __device__ inline int row(int k) const { return (k >> 3) * 128 + (k >> 1 & 3) * 16 + row0; }
+  __device__ inline int col(int k) const { return (k & 1) * 128 + col0; }
+  __device__ inline f32x4 four(int k, int half) const { return c[k >> 3][k & 1][k >> 1 & 3][half]; }
 };
 
 // sum over k of A(i, k) B(j, k).  kPlanes 3: operands held as sums of two

@@ -204,17 +204,21 @@ struct SumsOf {
       for (int j = 0; j < kB; ++j) c[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  // The lane's sums as fours of neighbouring columns; place() comes first.
-  static constexpr int kFours = kA * kB;
+  // The lane's sums as eights of neighbouring columns; place() comes first.
+  static constexpr int kEights = kA * kB / 2;
   int row0, col0;
   __device__ inline void place() {
     const int thread = thread_here(), lane = thread & 63, wave = thread >> 6;
     row0 = wave / kAlong * kA * 16 + (lane & 15);
-    col0 = wave % kAlong * kB * 16 + (lane >> 4) * 4;
+    col0 = wave % kAlong * kB * 16 + eight_column(lane);
+#pragma unroll
+    for (int i = 0; i < kA; ++i)
+#pragma unroll
+      for (int j = 0; j < kB; j += 2) exchange_fours(c[i][j], c[i][j + 1]);
   }
-  __device__ inline int row(int k) const { return k / kB * 16 + row0; }
-  __device__ inline int col(int k) const { return k % kB * 16 + col0; }
-  __device__ inline f32x4 four(int k) const { return c[k / kB][k % kB]; }
+  __device__ inline int row(int k) const { return k / (kB / 2) * 16 + row0; }
+  __device__ inline int col(int k) const { return k % (kB / 2) * 32 + col0; }
+  __device__ inline f32x4 four(int k, int half) const { return c[k / (kB / 2)][k % (kB / 2) * 2 + half]; }
 };
 
 template <typename T, bool kAC, bool kBC, int kRows, int kCols, bool kAligned>

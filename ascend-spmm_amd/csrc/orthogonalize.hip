@@ -129,35 +129,40 @@ struct Finish {
   bool tall;
 };
 
-// Four neighbouring columns of a row of E, as they are loaded.
+// Neighbouring columns of a row of E, as they are loaded: fours or eights.
+template <int kCols>
 struct Addend {
-  f16x4 hi, lo;
-  float rest, across[4];
+  typedef half Halves __attribute__((ext_vector_type(kCols)));
+  Halves hi, lo;
+  float rest, across[kCols];
 };
 
-template <Kind kKind, bool kPair>
-__device__ inline Addend load_addend(const Finish& f, int64_t batch, int row, int col) {
-  Addend a = {};
+template <Kind kKind, bool kPair, int kCols>
+__device__ inline Addend<kCols> load_addend(const Finish& f, int64_t batch, int row, int col) {
+  typedef typename Addend<kCols>::Halves Halves;
+  Addend<kCols> a = {};
   if constexpr (kKind != kGram) {
     const int64_t at = batch * f.add.size + row * f.add.ld + col;
-    a.hi = *reinterpret_cast<const f16x4*>(f.add.hi + at);
-    if constexpr (kPair || kKind != kPoly) a.lo = *reinterpret_cast<const f16x4*>(f.add.lo + at);
+    a.hi = *reinterpret_cast<const Halves*>(f.add.hi + at);
+    if constexpr (kPair || kKind != kPoly) a.lo = *reinterpret_cast<const Halves*>(f.add.lo + at);
     if constexpr (!kPair) {
       a.rest = f.rest[batch * f.rest_rows + row];
       if constexpr (kKind == kPoly)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a.across[e] = f.rest[batch * f.rest_rows + col + e];
+        for (int e = 0; e < kCols; ++e) a.across[e] = f.rest[batch * f.rest_rows + col + e];
     }
   }
   return a;
 }
 
-template <typename T, Kind kKind, bool kPair>
-__device__ inline void finish_four(const Finish& f, const Addend& a, int64_t batch, int row, int col, f32x4 sum) {
-  f32x4 v = sum * f.alpha;
+template <typename T, Kind kKind, bool kPair, int kCols>
+__device__ inline void finish(const Finish& f, const Addend<kCols>& a, int64_t batch, int row, int col,
+                              float (&v)[kCols]) {
+#pragma unroll
+  for (int e = 0; e < kCols; ++e) v[e] *= f.alpha;
   if constexpr (kKind != kGram)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < kCols; ++e) {
       float x = static_cast<float>(a.hi[e]) + static_cast<float>(a.lo[e]);
       float w = f.beta + f.alpha * a.rest;
       if constexpr (kKind == kPoly && !kPair) {
@@ -168,43 +173,53 @@ __device__ inline void finish_four(const Finish& f, const Addend& a, int64_t bat
     }
   if constexpr (kKind == kLast) {
     T* out = static_cast<T*>(f.out) + batch * f.rows * f.cols;
+    if (!f.tall && col + kCols <= f.cols) {
+      typedef T Values __attribute__((ext_vector_type(kCols), aligned(sizeof(T))));
+      Values r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = f.tall ? col + e : row, j = f.tall ? row : col + e;
-      if (i < f.rows && j < f.cols) out[i * f.cols + j] = static_cast<T>(v[e]);
+      for (int e = 0; e < kCols; ++e) r[e] = static_cast<T>(v[e]);
+      if (row < f.rows) *reinterpret_cast<Values*>(out + row * f.cols + col) = r;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kCols; ++e) {
+        const int i = f.tall ? col + e : row, j = f.tall ? row : col + e;
+        if (i < f.rows && j < f.cols) out[i * f.cols + j] = static_cast<T>(v[e]);
+      }
     }
   } else {
-    f16x4 h, l;
+    typename Addend<kCols>::Halves h, l;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < kCols; ++e) {
       h[e] = static_cast<half>(v[e]);
       l[e] = static_cast<half>(v[e] - static_cast<float>(h[e]));
       if constexpr (!kPair && kKind != kUpdate)
         if (row == col + e) f.diagonal[batch * f.rest_rows + row] = v[e] - static_cast<float>(h[e]);
     }
     const int64_t at = batch * f.to.size + row * f.to.ld + col;
-    *reinterpret_cast<f16x4*>(f.to.hi + at) = h;
-    if constexpr (kPair || kKind == kUpdate) *reinterpret_cast<f16x4*>(f.to.lo + at) = l;
+    *reinterpret_cast<decltype(h)*>(f.to.hi + at) = h;
+    if constexpr (kPair || kKind == kUpdate) *reinterpret_cast<decltype(h)*>(f.to.lo + at) = l;
   }
 }
 
-// Finishes a tile's sums, kCount at a time: all of a batch's addends are
+// Finishes a tile's sums, kCount eights at a time: all of a batch's addends are
 // loaded before the first is used.
 template <typename T, Kind kKind, bool kPair, int kCount, typename S>
 __device__ inline void finish_tile(const Finish& f, const S& s, int64_t batch, int r0, int c0, int m, int n) {
 #pragma unroll
-  for (int b = 0; b < S::kFours / kCount; ++b) {
-    Addend a[kCount];
+  for (int b = 0; b < S::kEights / kCount; ++b) {
+    Addend<8> a[kCount];
 #pragma unroll
     for (int k = 0; k < kCount; ++k) {
       const int row = r0 + s.row(b * kCount + k), col = c0 + s.col(b * kCount + k);
       const bool in = row < m && col < n;
-      a[k] = load_addend<kKind, kPair>(f, batch, in ? row : 0, in ? col : 0);
+      a[k] = load_addend<kKind, kPair, 8>(f, batch, in ? row : 0, in ? col : 0);
     }
 #pragma unroll
     for (int k = 0; k < kCount; ++k) {
       const int row = r0 + s.row(b * kCount + k), col = c0 + s.col(b * kCount + k);
-      if (row < m && col < n) finish_four<T, kKind, kPair>(f, a[k], batch, row, col, s.four(b * kCount + k));
+      const f32x4 x = s.four(b * kCount + k, 0), y = s.four(b * kCount + k, 1);
+      float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      if (row < m && col < n) finish<T, kKind, kPair, 8>(f, a[k], batch, row, col, v);
     }
   }
 }
@@ -238,7 +253,7 @@ __global__ __launch_bounds__(mma::kThreads, 2) void product_large(Product p, Fin
       operand(p.left, batch, r0, mma::kTile, p.m, p.depth, false),
       operand(p.right, batch, c0, mma::kTile, p.n, p.depth, kTurned), lds, s);
   s.place();
-  finish_tile<T, kKind, kPair, 16>(f, s, batch, r0, c0, p.m, p.n);
+  finish_tile<T, kKind, kPair, 8>(f, s, batch, r0, c0, p.m, p.n);
 }
 
 // Splits of a matrix are further apart than its tiles.
@@ -262,15 +277,18 @@ __global__ __launch_bounds__(mma::kThreads128, kSide == 64 ? 2 : 1) void product
             p.splits == 1 ? static_cast<int>(steps) : static_cast<int>(steps * (split + 1) / p.splits), s);
   s.place();
   if (p.splits == 1) {
-    finish_tile<T, kKind, kPair, s.kFours>(f, s, batch, r0, c0, p.m, p.n);
+    finish_tile<T, kKind, kPair, s.kEights>(f, s, batch, r0, c0, p.m, p.n);
     return;
   }
   const int64_t batches = gridDim.x / (down * across * p.splits);
   float* to = p.sums + (split * batches + batch) * p.m * p.n;
 #pragma unroll
-  for (int k = 0; k < s.kFours; ++k) {
+  for (int k = 0; k < s.kEights; ++k) {
     const int row = r0 + s.row(k), col = c0 + s.col(k);
-    if (row < p.m && col < p.n) *reinterpret_cast<f32x4*>(to + static_cast<int64_t>(row) * p.n + col) = s.four(k);
+    if (row < p.m && col < p.n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<f32x4*>(to + static_cast<int64_t>(row) * p.n + col + 4 * h) = s.four(k, h);
   }
 }
 
@@ -283,11 +301,12 @@ __global__ __launch_bounds__(kThreads) void finish_sums(Product p, Finish f, int
     // one matrix's sums are below 2^32
     const int64_t batch = batches == 1 ? 0 : i / fours;
     const unsigned e = static_cast<unsigned>(i - batch * fours) * 4, row = e / p.n, col = e - row * p.n;
-    const Addend a = load_addend<kKind, kPair>(f, batch, row, col);
+    const Addend<4> a = load_addend<kKind, kPair, 4>(f, batch, row, col);
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
     for (int64_t k = 0; k < p.splits; ++k) s += *reinterpret_cast<const f32x4*>(p.sums + (k * n + i) * 4);
-    finish_four<T, kKind, kPair>(f, a, batch, row, col, s);
+    float v[4] = {s[0], s[1], s[2], s[3]};
+    finish<T, kKind, kPair, 4>(f, a, batch, row, col, v);
   }
 }
 
@@ -298,8 +317,8 @@ __global__ __launch_bounds__(kThreads) void store_planes(Finish f, int64_t mp, i
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < fours * batches;
        i += static_cast<int64_t>(gridDim.x) * kThreads) {
     const int64_t batch = i / fours, row = i % fours * 4 / f.add.ld, col = i % fours * 4 % f.add.ld;
-    finish_four<T, kLast, true>(f, load_addend<kLast, true>(f, batch, row, col), batch, row, col,
-                                f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+    float v[4] = {};
+    finish<T, kLast, true, 4>(f, load_addend<kLast, true, 4>(f, batch, row, col), batch, row, col, v);
   }
 }
 
