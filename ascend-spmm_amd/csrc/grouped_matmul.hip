@@ -200,6 +200,86 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
   });
 }
 
+// The same by 256 work-groups that stay, on large tiles: a tile's first copies
+// are started before the last one's sums are stored, so that neither the one's
+// latency nor the other's burst of stores leaves the matrix cores idle.  An
+// XCD's work-groups take neighbouring tiles of its run.
+template <typename T, bool kTurned>
+__global__ __launch_bounds__(mma::kThreads, 2) void grouped_rows_large(GroupedArgs a, const T* __restrict__ in,
+                                                                       const T* __restrict__ weight,
+                                                                       T* __restrict__ out, unsigned down) {
+  constexpr int kTile = mma::kTile, kStores = mma::Sums::kEights;
+  typedef mma::Tile256<T, false, !kTurned, 1> Tile;
+  __shared__ __align__(1024) char lds[mma::kLdsBytes];
+  const unsigned across = (a.width + kTile - 1) / kTile, tiles = down * across;
+  const unsigned x = blockIdx.x % kXcds, rest = tiles % kXcds;
+  const unsigned begin = x * (tiles / kXcds) + (x < rest ? x : rest), end = begin + tiles / kXcds + (x < rest ? 1 : 0);
+  const unsigned stride = gridDim.x / kXcds;
+
+  struct Place {
+    RowRange r;
+    int c0, cols;
+  };
+  // the first tile from `n` on that there is; false past the run
+  auto find = [&](unsigned& n, Place& p) {
+    for (; n < end; n += stride) {
+      unsigned i, j;
+      mma::place_tile(n, down, across, i, j);
+      if (find_rows(a, kTile, i, p.r)) {
+        p.c0 = j * kTile;
+        p.cols = a.width - p.c0 < kTile ? a.width - p.c0 : kTile;
+        return true;
+      }
+    }
+    return false;
+  };
+  auto tile_at = [&](const Place& p) {
+    const T* w = weight + (p.r.group < 0 ? 0 : p.r.group) * a.weight_stride +
+                 (kTurned ? static_cast<int64_t>(p.c0) * a.inner : p.c0);
+    const int depth = p.r.group < 0 ? 0 : a.inner;  // outside the groups: an empty sum
+    return Tile({in + p.r.first * a.in_stride, nullptr, a.in_stride, p.r.rows, depth},
+                {w, nullptr, kTurned ? a.inner : a.width, p.cols, depth}, lds, mma::thread_here());
+  };
+
+  unsigned n = begin + blockIdx.x / kXcds;
+  Place here, next;
+  if (!find(n, here)) return;
+  Tile t = tile_at(here);
+  t.start();
+  mma::wait_copies<0>();  // no stores are under way yet: what run() lets pass must have arrived
+  for (;;) {
+    mma::Sums s;
+    t.template run<kStores>(lds, s);
+    n += stride;
+    const bool more = find(n, next);  // nothing is under way here that its loads would wait for
+    if (more) {
+      t = tile_at(next);
+      t.start();
+    }
+    s.place();
+    // Every wave issues kStores stores; the buffer's end and the offset past it
+    // drop what lies outside.
+    T* to = out + static_cast<int64_t>(here.r.first) * a.width + here.c0;
+    const int bytes = static_cast<int>(sizeof(T)) * ((here.r.rows - 1) * a.width + here.cols);
+    const __amdgpu_buffer_rsrc_t b = __builtin_amdgcn_make_buffer_rsrc(to, static_cast<short>(0), bytes, 0x00020000);
+#pragma unroll
+    for (int k = 0; k < kStores; ++k) {
+      const f32x4 v = s.four(k, 0), w = s.four(k, 1);
+      typedef T Eight __attribute__((ext_vector_type(8)));
+      Eight p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[e] = static_cast<T>(v[e]);
+        p[e + 4] = static_cast<T>(w[e]);
+      }
+      const unsigned at = s.col(k) < here.cols ? static_cast<unsigned>(sizeof(T)) * (s.row(k) * a.width + s.col(k)) : 0x80000000u;
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, p), b, static_cast<int>(at), 0, 0);
+    }
+    if (!more) return;
+    here = next;
+  }
+}
+
 // dW's sums run over the rows of all groups, counted in steps of 64 (an empty
 // group has one, which adds nothing) and cut into `parts` equal ranges.  The
 // cuts depend on sizes alone, so every engine adds in the same order.
@@ -262,12 +342,13 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
   }
 }
 
-// Adds the pieces of the groups that were cut; a work-group takes 1024 sums.
+// Adds the pieces of the groups that were cut; a work-group takes 4096 sums.
+constexpr int kJoin = 4096;
 template <typename T>
 __global__ __launch_bounds__(256) void join_pieces(GroupedArgs a, int tile_rows, int tile_cols, int parts,
                                                    const float* __restrict__ pieces, T* __restrict__ dweight) {
   const unsigned across = (a.width + tile_cols - 1) / tile_cols, down = (a.inner + tile_rows - 1) / tile_rows;
-  const unsigned tiles = across * down, size = tile_rows * tile_cols, slices = size / 1024;
+  const unsigned tiles = across * down, size = tile_rows * tile_cols, slices = size / kJoin;
   const unsigned each = blockIdx.x / slices;
   const int g = each / tiles;
   const unsigned tile = each - g * tiles;
@@ -280,21 +361,29 @@ __global__ __launch_bounds__(256) void join_pieces(GroupedArgs a, int tile_rows,
   while (part > 0 && part_start(total, part, parts) > u0) --part;
   while (part_start(total, part + 1, parts) <= u0) ++part;
   if (part_start(total, part + 1, parts) >= u1) return;  // written whole
-  const unsigned e = (blockIdx.x - each * slices) * 1024 + threadIdx.x * 4;
-  const float* from = pieces + static_cast<int64_t>(tile) * 2 * size + e;
-  const int64_t range = static_cast<int64_t>(tiles) * 2 * size;
-  f32x4 s = *reinterpret_cast<const f32x4*>(from + part * range + (part_start(total, part, parts) < u0 ? size : 0));
   // ranges that start inside the group
   int end = static_cast<int>(static_cast<int64_t>(u1) * parts / total);
   while (end > part + 1 && part_start(total, end - 1, parts) >= u1) --end;
   while (end < parts && part_start(total, end, parts) < u1) ++end;
-#pragma unroll 4
-  for (++part; part < end; ++part) s += *reinterpret_cast<const f32x4*>(from + part * range);
+  const int64_t range = static_cast<int64_t>(tiles) * 2 * size;
+  const float* from = pieces + static_cast<int64_t>(tile) * 2 * size + (blockIdx.x - each * slices) * kJoin + threadIdx.x * 4;
+  f32x4 s[kJoin / 1024];
+#pragma unroll
+  for (int k = 0; k < kJoin / 1024; ++k)
+    s[k] = *reinterpret_cast<const f32x4*>(from + part * range + (part_start(total, part, parts) < u0 ? size : 0) + 1024 * k);
+#pragma unroll 2
+  for (++part; part < end; ++part)
+#pragma unroll
+    for (int k = 0; k < kJoin / 1024; ++k) s[k] += *reinterpret_cast<const f32x4*>(from + part * range + 1024 * k);
   unsigned i, j;
   mma::place_tile(tile, down, across, i, j);
-  const int row = i * tile_rows + e / tile_cols, col = j * tile_cols + e % tile_cols;
-  if (row < a.inner && col < a.width)
-    store_four(dweight + (static_cast<int64_t>(g) * a.inner + row) * a.width + col, a.width - col, s);
+#pragma unroll
+  for (int k = 0; k < kJoin / 1024; ++k) {
+    const unsigned e = (blockIdx.x - each * slices) * kJoin + 1024 * k + threadIdx.x * 4;
+    const int row = i * tile_rows + e / tile_cols, col = j * tile_cols + e % tile_cols;
+    if (row < a.inner && col < a.width)
+      store_four(dweight + (static_cast<int64_t>(g) * a.inner + row) * a.width + col, a.width - col, s[k]);
+  }
 }
 
 constexpr int64_t kMostStride = int64_t(1) << 22;
@@ -420,7 +509,14 @@ spmm_status run_rows(const GroupedArgs& a, bool aligned, const void* in, const v
   // (copies count a matrix's pieces in 32 bits)
   aligned = aligned && static_cast<int64_t>(a.inner) * a.width < (int64_t(1) << 33);
   if constexpr (sizeof(T) == 2)
-    if (aligned && large_rows(a)) return launch_rows<Large<T, false, !kTurned>, kTurned>(a, in, weight, out, s, op);
+    if (aligned && large_rows(a)) {
+      const int64_t down = ceil_div(a.rows, mma::kTile) + a.groups + 1;
+      if (spmm_status st = check_grid(down * ceil_div(a.width, mma::kTile), op)) return st;
+      hipLaunchKernelGGL((grouped_rows_large<T, kTurned>), dim3(kCus), dim3(mma::kThreads), 0, s, a,
+                         static_cast<const T*>(in), static_cast<const T*>(weight), static_cast<T*>(out),
+                         static_cast<unsigned>(down));
+      return check_launch(op);
+    }
   if (low_rows(a))
     return aligned ? launch_rows<Small<T, false, !kTurned, 32, true>, kTurned>(a, in, weight, out, s, op)
                    : launch_rows<Small<T, false, !kTurned, 32, false>, kTurned>(a, in, weight, out, s, op);
@@ -440,7 +536,7 @@ spmm_status launch_weights(const GroupedArgs& a, const void* left, int64_t left_
   if (need > 0 && (ws == nullptr || ws_bytes < need))
     return fail(SPMM_ERR_CONTRACT, std::string(op) + ": workspace too small: need " + std::to_string(need) + " bytes");
   const int64_t parts = weight_parts(a, std::is_same_v<typename E::Value, float>), tiles = ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols);
-  const int64_t slices = a.groups * tiles * (E::kRows * E::kCols / 1024);
+  const int64_t slices = a.groups * tiles * (E::kRows * E::kCols / kJoin);
   if (spmm_status st = check_grid(slices > parts * tiles ? slices : parts * tiles, op)) return st;
   hipLaunchKernelGGL(grouped_weights<E>, dim3(static_cast<unsigned>(parts * tiles)), dim3(E::kThreads), 0, s, a,
                      static_cast<const T*>(left), left_stride, static_cast<const T*>(right), right_stride,

@@ -266,60 +266,76 @@ struct Sums {
   __device__ inline f32x4 four(int k, int half) const { return c[k >> 3][k & 1][k >> 1 & 3][half]; }
 };
 
-// sum over k of A(i, k) B(j, k).  kPlanes 3: operands held as sums of two
-// planes, high and low; the products high high, high low and low high are
+// One tile: sum over k of A(i, k) B(j, k).  kPlanes 3: operands held as sums of
+// two planes, high and low; the products high high, high low and low high are
 // added (low low is below fp32's rounding).  `lds`: kLdsBytes.
 template <typename T, bool kAC, bool kBC, int kPlanes>
-__device__ inline void multiply_tile(const Operand<T>& a, const Operand<T>& b, char* lds, Sums& s) {
-  const int thread = thread_here(), lane = thread & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(thread >> 6);
-  const int wr = wave >> 2, wc = wave & 3;
-  Copier<T, kAC, kPlanes> ca(a, lds, wave, lane);
-  Copier<T, kBC, kPlanes> cb(b, lds + 65536, wave, lane);
-  const typename Half<kAC>::template Reader<4> ra(lds_address(lds), wr * 64, lane);
-  const typename Half<kBC>::template Reader<2> rb(lds_address(lds + 65536), wc * 32, lane);
-  const int all = kPlanes * ca.steps;
+struct Tile256 {
+  Copier<T, kAC, kPlanes> ca;
+  Copier<T, kBC, kPlanes> cb;
+
+  __device__ inline Tile256(const Operand<T>& a, const Operand<T>& b, const char* lds, int thread)
+      : ca(a, lds, __builtin_amdgcn_readfirstlane(thread >> 6), thread & 63),
+        cb(b, lds + 65536, __builtin_amdgcn_readfirstlane(thread >> 6), thread & 63) {}
+
+  // Starts the copies of the first step: B0 A0 B1 A1, two instructions each.
+  // LDS is free.
+  __device__ inline void start() {
+    cb.copy(0, 0);
+    ca.copy(0, 0);
+    cb.copy(0, 1);
+    ca.copy(0, 1);
+    cb.advance(1);
+    ca.advance(2);
+  }
+
+  // Sums the tile.  kStores: memory instructions of the wave, no more and no
+  // fewer, that may be under way since start(): another tile's stores, which
+  // the first step does not wait for.
+  template <int kStores>
+  __device__ inline void run(char* lds, Sums& s) {
+    const int thread = thread_here(), lane = thread & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(thread >> 6);
+    const int wr = wave >> 2, wc = wave & 3;
+    const typename Half<kAC>::template Reader<4> ra(lds_address(lds), wr * 64, lane);
+    const typename Half<kBC>::template Reader<2> rb(lds_address(lds + 65536), wc * 32, lane);
+    const int all = kPlanes * ca.steps;
 
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int g = 0; g < 2; ++g)
+      for (int g = 0; g < 2; ++g)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) s.c[h][g][i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          for (int j = 0; j < 2; ++j) s.c[h][g][i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  Fragments<4> fa;
-  Fragments<2> b0, b1, b2;
-  // Copies go in the order B0 A0 B1 A1, two instructions each; a phase that
-  // is about to read one waits until at most the two started after it are
-  // still under way, and the barrier makes the other waves' parts certain.
-  cb.copy(0, 0);
-  ca.copy(0, 0);
-  cb.copy(0, 1);
-  ca.copy(0, 1);
-  cb.advance(1);
-  ca.advance(2);
-  wait_copies<6>();
-  barrier();
-  rb.template read<0>(b0);
-  wait_copies<4>();
-  barrier();
-  if (wr == 1) barrier();  // half a phase behind
+    Fragments<4> fa;
+    Fragments<2> b0, b1, b2;
+    // A phase that is about to read a half tile waits until at most the two
+    // started after it are still under way, and the barrier makes the other
+    // waves' parts certain.
+    wait_copies<6 + kStores>();
+    barrier();
+    rb.template read<0>(b0);
+    wait_copies<4 + kStores>();
+    barrier();
+    if (wr == 1) barrier();  // half a phase behind
 
 // `bx`: B0 of this step, read in the last phase of the step before; `by`: of
-// the next.
-#define SPMM_MMA_STEP(buf, bx, by)                          \
+// the next.  `extra`: stores under way behind the half tiles that the first
+// two phases wait for.
+#define SPMM_MMA_STEP(buf, bx, by, extra)                      \
   {                                                            \
     ra.template read<(buf) * 32768>(fa);                       \
     cb.copy((buf) ^ 1, 0);                                     \
-    wait_copies<4>();                                          \
+    wait_copies<4 + (extra)>();                                \
     barrier();                                                 \
     multiply<T>(s.c[0][0], fa, bx);                            \
     barrier();                                                 \
     rb.template read<(buf) * 32768 + 16384>(b1);               \
     ca.copy((buf) ^ 1, 0);                                     \
-    wait_copies<4>();                                          \
+    wait_copies<4 + (extra)>();                                \
     barrier();                                                 \
     multiply<T>(s.c[0][1], fa, b1);                            \
     barrier();                                                 \
@@ -338,15 +354,30 @@ __device__ inline void multiply_tile(const Operand<T>& a, const Operand<T>& b, c
     ca.advance(2);                                             \
     barrier();                                                 \
   }
-  for (int t = 0; t < all; t += 2) {
-    SPMM_MMA_STEP(0, b0, b2)
-    SPMM_MMA_STEP(1, b2, b0)
-  }
+    int t = 0;
+    if constexpr (kStores > 0)
+      if (all > 0) {
+        SPMM_MMA_STEP(0, b0, b2, kStores)
+        SPMM_MMA_STEP(1, b2, b0, 0)
+        t = 2;
+      }
+    for (; t < all; t += 2) {
+      SPMM_MMA_STEP(0, b0, b2, 0)
+      SPMM_MMA_STEP(1, b2, b0, 0)
+    }
 #undef SPMM_MMA_STEP
-  if (wr == 0) barrier();
-  // No copy outlives the loop: LDS is free again.
-  wait_copies<0>();
-  barrier();
+    if (wr == 0) barrier();
+    // No copy outlives the loop: LDS is free again.
+    wait_copies<0>();
+    barrier();
+  }
+};
+
+template <typename T, bool kAC, bool kBC, int kPlanes>
+__device__ inline void multiply_tile(const Operand<T>& a, const Operand<T>& b, char* lds, Sums& s) {
+  Tile256<T, kAC, kBC, kPlanes> t(a, b, lds, thread_here());
+  t.start();
+  t.template run<0>(lds, s);
 }
 
 }  // namespace mma
