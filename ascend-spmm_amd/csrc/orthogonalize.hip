@@ -203,8 +203,10 @@ __device__ inline void finish(const Finish& f, const Addend<kCols>& a, int64_t b
 
 // Finishes a tile's sums, kCount eights at a time: all of a batch's addends are
 // loaded before the first is used.
-template <typename T, Kind kKind, bool kPair, int kCount, typename S>
-__device__ inline void finish_tile(const Finish& f, const S& s, int64_t batch, int r0, int c0, int m, int n) {
+// kBothWays: where `twice`, also across the diagonal.
+template <typename T, Kind kKind, bool kPair, int kCount, bool kBothWays = false, typename S>
+__device__ inline void finish_tile(const Finish& f, const S& s, int64_t batch, int r0, int c0, int m, int n,
+                                   bool twice = false) {
 #pragma unroll
   for (int b = 0; b < S::kEights / kCount; ++b) {
     Addend<8> a[kCount];
@@ -219,7 +221,17 @@ __device__ inline void finish_tile(const Finish& f, const S& s, int64_t batch, i
       const int row = r0 + s.row(b * kCount + k), col = c0 + s.col(b * kCount + k);
       const f32x4 x = s.four(b * kCount + k, 0), y = s.four(b * kCount + k, 1);
       float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-      if (row < m && col < n) finish<T, kKind, kPair, 8>(f, a[k], batch, row, col, v);
+      if (row >= m || col >= n) continue;
+      finish<T, kKind, kPair, 8>(f, a[k], batch, row, col, v);
+      if constexpr (kBothWays)
+        if (twice)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int64_t at = batch * f.to.size + (col + e) * f.to.ld + row;
+            const half h = static_cast<half>(v[e]);
+            f.to.hi[at] = h;
+            if constexpr (kPair) f.to.lo[at] = static_cast<half>(v[e] - static_cast<float>(h));
+          }
     }
   }
 }
@@ -239,21 +251,32 @@ __device__ inline mma::Operand<half> operand(const Planes& p, int64_t batch, int
   return {p.hi + at, p.lo == nullptr ? nullptr : p.lo + at, p.ld, rows - first < most ? rows - first : most, depth};
 }
 
+// A and its polynomial are symmetric: the tiles below the diagonal are summed
+// and stored both ways.
 template <typename T, Kind kKind, bool kPair>
 __global__ __launch_bounds__(mma::kThreads, 2) void product_large(Product p, Finish f) {
   constexpr bool kTurned = kKind == kUpdate || kKind == kLast;
   __shared__ __align__(1024) char lds[mma::kLdsBytes];
   const unsigned down = (p.m + mma::kTile - 1) / mma::kTile, across = (p.n + mma::kTile - 1) / mma::kTile;
-  const unsigned block = mma::run_of_xcd(blockIdx.x, gridDim.x), batch = block / (down * across);
+  const unsigned each = kTurned ? down * across : down * (down + 1) / 2;
+  const unsigned block = mma::run_of_xcd(blockIdx.x, gridDim.x), batch = block / each;
   unsigned i, j;
-  mma::place_tile(block - batch * (down * across), down, across, i, j);
+  if constexpr (kTurned) {
+    mma::place_tile(block - batch * each, down, across, i, j);
+  } else {
+    const unsigned n = block - batch * each;
+    i = static_cast<unsigned>((sqrtf(8.0f * static_cast<float>(n) + 1.0f) - 1.0f) * 0.5f);
+    while (i * (i + 1) / 2 > n) --i;
+    while ((i + 1) * (i + 2) / 2 <= n) ++i;
+    j = n - i * (i + 1) / 2;
+  }
   const int r0 = i * mma::kTile, c0 = j * mma::kTile;
   mma::Sums s;
   mma::multiply_tile<half, false, kTurned, kPair ? 3 : 1>(
       operand(p.left, batch, r0, mma::kTile, p.m, p.depth, false),
       operand(p.right, batch, c0, mma::kTile, p.n, p.depth, kTurned), lds, s);
   s.place();
-  finish_tile<T, kKind, kPair, 8>(f, s, batch, r0, c0, p.m, p.n);
+  finish_tile<T, kKind, kPair, 8, !kTurned>(f, s, batch, r0, c0, p.m, p.n, r0 != c0);
 }
 
 // Splits of a matrix are further apart than its tiles.
@@ -640,7 +663,9 @@ struct Layout {
 template <typename T, Kind kKind, bool kPair>
 spmm_status multiply(Product p, const Finish& f, int64_t batch, hipStream_t s) {
   if (Layout::large(batch, p.m, p.n)) {
-    const unsigned tiles = static_cast<unsigned>(ceil_div(p.m, mma::kTile) * ceil_div(p.n, mma::kTile) * batch);
+    const int64_t down = ceil_div(p.m, mma::kTile), across = ceil_div(p.n, mma::kTile);
+    const bool turned = kKind == kUpdate || kKind == kLast;
+    const unsigned tiles = static_cast<unsigned>((turned ? down * across : down * (down + 1) / 2) * batch);
     hipLaunchKernelGGL((product_large<T, kKind, kPair>), dim3(tiles), dim3(mma::kThreads), 0, s, p, f);
     return check_launch("orthogonalize product");
   }
