@@ -40,6 +40,17 @@ __device__ inline void load_piece(const T* p, int64_t n, float (&v)[kPiece<T>]) 
   }
 }
 
+// The same as they lie, to be converted later: a load that is converted at once
+// is waited for at once.
+template <typename T>
+__device__ inline piece_t<T> load_raw(const T* p, int64_t n) {
+  if (n >= kPiece<T>) return *reinterpret_cast<const piece_t<T>*>(p);
+  piece_t<T> x;
+#pragma unroll
+  for (int i = 0; i < kPiece<T>; ++i) x[i] = i < n ? p[i] : static_cast<T>(0.0f);
+  return x;
+}
+
 // Stores up to one piece, each value rounded once to nearest even.
 template <typename T>
 __device__ inline void store_piece(T* p, int64_t n, const float (&v)[kPiece<T>]) {
