@@ -342,9 +342,10 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
   }
 }
 
-// Adds the pieces of the groups that were cut; a work-group takes 4096 sums.
-constexpr int kJoin = 4096;
-template <typename T>
+// Adds the pieces of the groups that were cut; a work-group takes kJoin sums:
+// 4096 of large tiles, of which there are many (65536 rows, 1024 x 2048: 28 us,
+// 62 with 1024), 1024 of others (100000 rows, 128 x 128: 6.5 us, 10 with 4096).
+template <typename T, int kJoin>
 __global__ __launch_bounds__(256) void join_pieces(GroupedArgs a, int tile_rows, int tile_cols, int parts,
                                                    const float* __restrict__ pieces, T* __restrict__ dweight) {
   const unsigned across = (a.width + tile_cols - 1) / tile_cols, down = (a.inner + tile_rows - 1) / tile_rows;
@@ -536,6 +537,7 @@ spmm_status launch_weights(const GroupedArgs& a, const void* left, int64_t left_
   if (need > 0 && (ws == nullptr || ws_bytes < need))
     return fail(SPMM_ERR_CONTRACT, std::string(op) + ": workspace too small: need " + std::to_string(need) + " bytes");
   const int64_t parts = weight_parts(a, std::is_same_v<typename E::Value, float>), tiles = ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols);
+  constexpr int kJoin = E::kRows == mma::kTile ? 4096 : 1024;
   const int64_t slices = a.groups * tiles * (E::kRows * E::kCols / kJoin);
   if (spmm_status st = check_grid(slices > parts * tiles ? slices : parts * tiles, op)) return st;
   hipLaunchKernelGGL(grouped_weights<E>, dim3(static_cast<unsigned>(parts * tiles)), dim3(E::kThreads), 0, s, a,
@@ -543,7 +545,7 @@ spmm_status launch_weights(const GroupedArgs& a, const void* left, int64_t left_
                      static_cast<T*>(dweight), static_cast<int>(parts), static_cast<float*>(ws));
   if (spmm_status st = check_launch(op)) return st;
   if (parts == 1) return SPMM_OK;
-  hipLaunchKernelGGL(join_pieces<T>, dim3(static_cast<unsigned>(slices)), dim3(256), 0, s, a,
+  hipLaunchKernelGGL((join_pieces<T, kJoin>), dim3(static_cast<unsigned>(slices)), dim3(256), 0, s, a,
                      E::kRows, E::kCols, static_cast<int>(parts),
                      static_cast<const float*>(ws), static_cast<T*>(dweight));
   return check_launch(op);
