@@ -95,20 +95,20 @@ struct Stage {
     if (!kWhole && line >= (C ? S::kDepth : kRows)) line = 1 << 28;  // none
   }
 
-  // Loads the step at p, with `left` of the sum's depth, into registers; zeros
-  // outside the operand.
+  // Loads the step at p, with `left` of the sum's depth, into registers.  With
+  // aligned pieces nothing is done with the results here, so that they stay
+  // under way during the matrix instructions: outside the operand p's first
+  // piece is read instead, sums of rows that there are not hold anything, and
+  // store() clears what is past the depth.
   __device__ inline void load(const T* p, int valid, int left) {
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       const int l = line + e * kLines, c = piece * 8;
       const bool in = l < (C ? left : valid) && c < (C ? valid : left);
       const T* at = p + (in ? from + e * round : 0u);
-      if constexpr (kAligned) {  // p itself can always be read
+      if constexpr (kAligned) {
 #pragma unroll
-        for (int h = 0; h < kVectors; ++h) {
-          const u32x4 v = reinterpret_cast<const u32x4*>(at)[h];
-          held[e][h] = in ? v : u32x4{0u, 0u, 0u, 0u};
-        }
+        for (int h = 0; h < kVectors; ++h) held[e][h] = reinterpret_cast<const u32x4*>(at)[h];
       } else {
         const int count = in ? (C ? valid : left) - c : 0;
         if (count >= 8) {
@@ -125,9 +125,21 @@ struct Stage {
     }
   }
 
-  // `most`: raised to the largest magnitude that passes (fp32).
+  // Stores the step, which has `left` of the depth, to LDS.  `most`: raised to
+  // the largest magnitude that passes (fp32).
   template <bool kCareful>
-  __device__ inline void store(char* lds, float& most) const {
+  __device__ inline void store(char* lds, int left, float& most) {
+    if (kAligned && left < S::kDepth) {  // (load() has done so for others)
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int inside = C ? (line + e * kLines < left ? 8 : 0) : left - piece * 8;
+        T some[8];
+        __builtin_memcpy(some, &held[e], sizeof(some));
+#pragma unroll
+        for (int m = 0; m < 8; ++m) some[m] = m < inside ? some[m] : static_cast<T>(0.0f);
+        __builtin_memcpy(&held[e], some, sizeof(some));
+      }
+    }
     if (!kWhole && line == 1 << 28) return;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
@@ -258,20 +270,21 @@ struct Staged {
     const T *pa = a.p, *pb = b.p;
     const int64_t step_a = S::kDepth * (kAC ? a.ld : 1), step_b = S::kDepth * (kBC ? b.ld : 1);
     int left = static_cast<int>(a.depth);
+    if (left <= 0) return;
     auto load = [&]() {
       const int most_k = left < S::kDepth ? left : S::kDepth;
-      sa.load(pa, va, most_k);
-      sb.load(pb, vb, most_k);
+      sa.load(left > 0 ? pa : a.p, va, most_k);
+      sb.load(left > 0 ? pb : b.p, vb, most_k);
       pa += step_a;
       pb += step_b;
     };
-    if (left > 0) load();
-    for (; left > 0;) {
+    load();
+    do {
       __syncthreads();  // the last step's fragments have been read
-      sa.template store<kCareful>(lds, most);
-      sb.template store<kCareful>(lb, most);
+      sa.template store<kCareful>(lds, left, most);
+      sb.template store<kCareful>(lb, left, most);
       left -= S::kDepth;
-      if (left > 0) load();
+      if (kAligned || left > 0) load();  // (a last, unused one costs less than the branch)
       __syncthreads();
 #pragma unroll
       for (int kk = 0; kk < S::kDepth / 32; ++kk) {
@@ -280,23 +293,24 @@ struct Staged {
         for (int i = 0; i < Sums::kA; ++i)
 #pragma unroll
           for (int q = 0; q < S::kParts; ++q) fa[i][q] = ra.read(lds, i, kk, q);
+        u32x4 fb[Sums::kB][S::kParts];
 #pragma unroll
-        for (int j = 0; j < Sums::kB; ++j) {
-          u32x4 fb[S::kParts];
+        for (int j = 0; j < Sums::kB; ++j)
 #pragma unroll
-          for (int q = 0; q < S::kParts; ++q) fb[q] = rb.read(lb, j, kk, q);
-          // products of parts, the smallest first
-          constexpr int kProducts = S::kParts == 1 ? 1 : 8;
-          constexpr int kOrder[8][2] = {{0, 0}, {0, 1}, {1, 0}, {1, 1}, {0, 2}, {2, 0}, {1, 2}, {2, 1}};
-          typedef std::conditional_t<S::kParts == 3, __bf16, T> Part;
+          for (int q = 0; q < S::kParts; ++q) fb[j][q] = rb.read(lb, j, kk, q);
+        // products of parts, the smallest first
+        constexpr int kProducts = S::kParts == 1 ? 1 : 8;
+        constexpr int kOrder[8][2] = {{0, 0}, {0, 1}, {1, 0}, {1, 1}, {0, 2}, {2, 0}, {1, 2}, {2, 1}};
+        typedef std::conditional_t<S::kParts == 3, __bf16, T> Part;
 #pragma unroll
-          for (int o = kProducts - 1; o >= 0; --o)
+        for (int o = kProducts - 1; o >= 0; --o)
+#pragma unroll
+          for (int j = 0; j < Sums::kB; ++j)
 #pragma unroll
             for (int i = 0; i < Sums::kA; ++i)
-              s.c[i][j] = multiply<Part>(fb[kOrder[o][1]], fa[i][kOrder[o][0]], s.c[i][j]);
-        }
+              s.c[i][j] = multiply<Part>(fb[j][kOrder[o][1]], fa[i][kOrder[o][0]], s.c[i][j]);
       }
-    }
+    } while (left > 0);
     __syncthreads();
   }
 };
