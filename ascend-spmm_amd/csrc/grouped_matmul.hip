@@ -64,23 +64,28 @@ __device__ inline int find_segment(int segments, int at, F size, int& before) {
   return segments;
 }
 
-// The `tile`-th range of at most `height` rows, none across a group's end.
-// Segment 0 is the rows before the first group, segment groups + 1 those
-// behind the last; both are `group` -1.  False past the last range.
+// Ranges of at most `height` rows, none across a group's end.  Segment 0 is the
+// rows before the first group, segment groups + 1 those behind the last; both
+// are `group` -1.
+__device__ inline int first_row(const GroupedArgs& a, int s) { return s == 0 ? 0 : edge(a, s - 1); }
+__device__ inline int end_row(const GroupedArgs& a, int s) { return s == a.groups + 1 ? a.rows : edge(a, s); }
+__device__ inline int find_range(const GroupedArgs& a, int height, int at, int& before) {
+  return find_segment(a.groups + 2, at, [&](int s) {
+    const int n = end_row(a, s) - first_row(a, s);
+    return n > 0 ? (n + height - 1) / height : 0;
+  }, before);
+}
+
+// The `tile`-th range; false past the last.
 struct RowRange {
   int first, rows, group;
 };
 __device__ inline bool find_rows(const GroupedArgs& a, int height, int tile, RowRange& r) {
-  auto low = [&](int s) { return s == 0 ? 0 : edge(a, s - 1); };
-  auto high = [&](int s) { return s == a.groups + 1 ? a.rows : edge(a, s); };
   int before;
-  const int s = find_segment(a.groups + 2, tile, [&](int t) {
-    const int n = high(t) - low(t);
-    return n > 0 ? (n + height - 1) / height : 0;
-  }, before);
+  const int s = find_range(a, height, tile, before);
   if (s == a.groups + 2) return false;
-  r.first = low(s) + (tile - before) * height;
-  const int left = high(s) - r.first;
+  r.first = first_row(a, s) + (tile - before) * height;
+  const int left = end_row(a, s) - r.first;
   r.rows = left < height ? left : height;
   r.group = s == 0 || s == a.groups + 1 ? -1 : s - 1;
   return true;
@@ -203,14 +208,17 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
 // The same by 256 work-groups that stay, on large tiles: a tile's first copies
 // are started before the last one's sums are stored, so that neither the one's
 // latency nor the other's burst of stores leaves the matrix cores idle.  An
-// XCD's work-groups take neighbouring tiles of its run.
+// XCD's work-groups take neighbouring tiles of its run; runs are of the tiles
+// that there are (the host knows only how many at most).
 template <typename T, bool kTurned>
 __global__ __launch_bounds__(mma::kThreads, 2) void grouped_rows_large(GroupedArgs a, const T* __restrict__ in,
                                                                        const T* __restrict__ weight,
-                                                                       T* __restrict__ out, unsigned down) {
+                                                                       T* __restrict__ out) {
   constexpr int kTile = mma::kTile, kStores = mma::Sums::kEights;
   typedef mma::Tile256<T, false, !kTurned, 1> Tile;
   __shared__ __align__(1024) char lds[mma::kLdsBytes];
+  int down;
+  find_range(a, kTile, INT_MAX, down);
   const unsigned across = (a.width + kTile - 1) / kTile, tiles = down * across;
   const unsigned x = blockIdx.x % kXcds, rest = tiles % kXcds;
   const unsigned begin = x * (tiles / kXcds) + (x < rest ? x : rest), end = begin + tiles / kXcds + (x < rest ? 1 : 0);
@@ -220,18 +228,15 @@ __global__ __launch_bounds__(mma::kThreads, 2) void grouped_rows_large(GroupedAr
     RowRange r;
     int c0, cols;
   };
-  // the first tile from `n` on that there is; false past the run
-  auto find = [&](unsigned& n, Place& p) {
-    for (; n < end; n += stride) {
-      unsigned i, j;
-      mma::place_tile(n, down, across, i, j);
-      if (find_rows(a, kTile, i, p.r)) {
-        p.c0 = j * kTile;
-        p.cols = a.width - p.c0 < kTile ? a.width - p.c0 : kTile;
-        return true;
-      }
-    }
-    return false;
+  // tile n; false past the run
+  auto find = [&](unsigned n, Place& p) {
+    if (n >= end) return false;
+    unsigned i, j;
+    mma::place_tile(n, down, across, i, j);
+    if (!find_rows(a, kTile, i, p.r)) return false;
+    p.c0 = j * kTile;
+    p.cols = a.width - p.c0 < kTile ? a.width - p.c0 : kTile;
+    return true;
   };
   auto tile_at = [&](const Place& p) {
     const T* w = weight + (p.r.group < 0 ? 0 : p.r.group) * a.weight_stride +
@@ -514,8 +519,7 @@ spmm_status run_rows(const GroupedArgs& a, bool aligned, const void* in, const v
       const int64_t down = ceil_div(a.rows, mma::kTile) + a.groups + 1;
       if (spmm_status st = check_grid(down * ceil_div(a.width, mma::kTile), op)) return st;
       hipLaunchKernelGGL((grouped_rows_large<T, kTurned>), dim3(kCus), dim3(mma::kThreads), 0, s, a,
-                         static_cast<const T*>(in), static_cast<const T*>(weight), static_cast<T*>(out),
-                         static_cast<unsigned>(down));
+                         static_cast<const T*>(in), static_cast<const T*>(weight), static_cast<T*>(out));
       return check_launch(op);
     }
   if (low_rows(a))
