@@ -317,6 +317,8 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
   const unsigned block = mma::run_of_xcd(blockIdx.x, gridDim.x), part = block / (across * down);
   unsigned i, j;
   mma::place_tile(block - part * (across * down), down, across, i, j);
+  if (parts > total) parts = total;  // of which the host knows only how many at most
+  if (part >= static_cast<unsigned>(parts)) return;
   const int i0 = i * E::kRows, j0 = j * E::kCols;
   const int rows = a.inner - i0 < E::kRows ? a.inner - i0 : E::kRows;
   const int cols = a.width - j0 < E::kCols ? a.width - j0 : E::kCols;
@@ -347,25 +349,33 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
   }
 }
 
-// Adds the pieces of the groups that were cut; a work-group takes kJoin sums:
-// 4096 of large tiles, of which there are many (65536 rows, 1024 x 2048: 28 us,
-// 62 with 1024), 1024 of others (100000 rows, 128 x 128: 6.5 us, 10 with 4096).
+// Adds the pieces of the groups that were cut; a work-group takes kJoin sums of
+// a group's tile.  by_cut: of the group that holds the cut before range n + 1,
+// where that is the group's first cut; else of group n.
 template <typename T, int kJoin>
-__global__ __launch_bounds__(256) void join_pieces(GroupedArgs a, int tile_rows, int tile_cols, int parts,
+__global__ __launch_bounds__(256) void join_pieces(GroupedArgs a, int tile_rows, int tile_cols, int parts, bool by_cut,
                                                    const float* __restrict__ pieces, T* __restrict__ dweight) {
   const unsigned across = (a.width + tile_cols - 1) / tile_cols, down = (a.inner + tile_rows - 1) / tile_rows;
   const unsigned tiles = across * down, size = tile_rows * tile_cols, slices = size / kJoin;
-  const unsigned each = blockIdx.x / slices;
-  const int g = each / tiles;
-  const unsigned tile = each - g * tiles;
-  int total, before;
+  const unsigned each = blockIdx.x / slices, n = each / tiles, tile = each - n * tiles;
+  int total;
   find_step(a, INT_MAX, total);
-  find_segment(a.groups, INT_MAX, [&](int s) { return s < g ? steps_of(a, s) : 0; }, before);
-  const int u0 = before, u1 = u0 + steps_of(a, g);
-  // the range that holds the group's first step
-  int part = static_cast<int>(static_cast<int64_t>(u0) * parts / total);
-  while (part > 0 && part_start(total, part, parts) > u0) --part;
-  while (part_start(total, part + 1, parts) <= u0) ++part;
+  if (parts > total) parts = total;
+  int g, u0, part;  // the group, its first step, and the range that holds it
+  if (by_cut) {
+    if (n + 1 >= static_cast<unsigned>(parts)) return;
+    const int cut = part_start(total, n + 1, parts);
+    g = find_step(a, cut, u0);
+    if (cut == u0 || part_start(total, n, parts) > u0) return;
+    part = n;
+  } else {
+    g = n;
+    find_segment(a.groups, INT_MAX, [&](int s) { return s < g ? steps_of(a, s) : 0; }, u0);
+    part = static_cast<int>(static_cast<int64_t>(u0) * parts / total);
+    while (part > 0 && part_start(total, part, parts) > u0) --part;
+    while (part_start(total, part + 1, parts) <= u0) ++part;
+  }
+  const int u1 = u0 + steps_of(a, g);
   if (part_start(total, part + 1, parts) >= u1) return;  // written whole
   // ranges that start inside the group
   int end = static_cast<int>(static_cast<int64_t>(u1) * parts / total);
@@ -377,7 +387,7 @@ __global__ __launch_bounds__(256) void join_pieces(GroupedArgs a, int tile_rows,
 #pragma unroll
   for (int k = 0; k < kJoin / 1024; ++k)
     s[k] = *reinterpret_cast<const f32x4*>(from + part * range + (part_start(total, part, parts) < u0 ? size : 0) + 1024 * k);
-#pragma unroll 2
+#pragma unroll 8192 / kJoin
   for (++part; part < end; ++part)
 #pragma unroll
     for (int k = 0; k < kJoin / 1024; ++k) s[k] += *reinterpret_cast<const f32x4*>(from + part * range + 1024 * k);
@@ -478,7 +488,8 @@ int64_t weight_parts(const GroupedArgs& a, bool fp32) {
 }
 template <typename E>
 size_t weight_bytes(const GroupedArgs& a) {
-  const int64_t parts = weight_parts(a, std::is_same_v<typename E::Value, float>), tiles = ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols);
+  const int64_t parts = weight_parts(a, std::is_same_v<typename E::Value, float>);
+  const int64_t tiles = ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols);
   return parts == 1 ? 0 : static_cast<size_t>(parts * tiles) * 2 * E::kRows * E::kCols * sizeof(float);
 }
 
@@ -540,18 +551,29 @@ spmm_status launch_weights(const GroupedArgs& a, const void* left, int64_t left_
   const size_t need = weight_bytes<E>(a);
   if (need > 0 && (ws == nullptr || ws_bytes < need))
     return fail(SPMM_ERR_CONTRACT, std::string(op) + ": workspace too small: need " + std::to_string(need) + " bytes");
-  const int64_t parts = weight_parts(a, std::is_same_v<typename E::Value, float>), tiles = ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols);
-  constexpr int kJoin = E::kRows == mma::kTile ? 4096 : 1024;
-  const int64_t slices = a.groups * tiles * (E::kRows * E::kCols / kJoin);
-  if (spmm_status st = check_grid(slices > parts * tiles ? slices : parts * tiles, op)) return st;
+  const int64_t parts = weight_parts(a, std::is_same_v<typename E::Value, float>);
+  const int64_t tiles = ceil_div(a.inner, E::kRows) * ceil_div(a.width, E::kCols);
+  // Joined by groups or by cuts, whichever are fewer.
+  const bool by_cut = parts - 1 < a.groups;
+  const int64_t sums = (by_cut ? parts - 1 : a.groups) * tiles * (E::kRows * E::kCols);
+  if (spmm_status st = check_grid(sums / 1024 > parts * tiles ? sums / 1024 : parts * tiles, op)) return st;
   hipLaunchKernelGGL(grouped_weights<E>, dim3(static_cast<unsigned>(parts * tiles)), dim3(E::kThreads), 0, s, a,
                      static_cast<const T*>(left), left_stride, static_cast<const T*>(right), right_stride,
                      static_cast<T*>(dweight), static_cast<int>(parts), static_cast<float*>(ws));
   if (spmm_status st = check_launch(op)) return st;
   if (parts == 1) return SPMM_OK;
-  hipLaunchKernelGGL((join_pieces<T, kJoin>), dim3(static_cast<unsigned>(slices)), dim3(256), 0, s, a,
-                     E::kRows, E::kCols, static_cast<int>(parts),
-                     static_cast<const float*>(ws), static_cast<T*>(dweight));
+  // A work-group takes 4096 sums where that leaves eight for each CU (24 groups
+  // of 1024 x 2048: 28 us, 62 with 1024), else 1024 (12 of 512 x 512: 6.5, 10).
+  auto join = [&](auto size) {
+    constexpr int kJoin = decltype(size)::value;
+    hipLaunchKernelGGL((join_pieces<T, kJoin>), dim3(static_cast<unsigned>(sums / kJoin)), dim3(256), 0, s, a, E::kRows,
+                       E::kCols, static_cast<int>(parts), by_cut, static_cast<const float*>(ws),
+                       static_cast<T*>(dweight));
+  };
+  if (sums >= 8 * kCus * 4096)
+    join(std::integral_constant<int, 4096>());
+  else
+    join(std::integral_constant<int, 1024>());
   return check_launch(op);
 }
 

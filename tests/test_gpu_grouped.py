@@ -207,6 +207,31 @@ def test_large_tiles(spmm_npu, sizes, inner, width, turned, dtype):
         assert not t[:before].any() and not t[before + sum(sizes):].any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("edges,inner,width", [([100, 230], 128, 128), ([0, 64, 130, 131], 72, 40), ([19000, 19000, 19500], 256, 512),
+                                               ([0, 0], 200, 136), ([5, 390], 33, 65)])
+def test_few_of_many_rows_in_groups(spmm_npu, edges, inner, width, dtype):
+    """Far fewer rows in the groups than the tensor has.  Memory that held NaN
+    before is handed out again as the gradient's workspace."""
+    x, w, dy = make(20000, len(edges) - 1, inner, width, dtype)
+    want, mag, terms = plain(x, w, edges, dy)
+    for size in (24, 26, 27):
+        torch.full((1 << size,), float("nan"), device="cuda")
+    for got, ref, m, n, what in zip(run_all(spmm_npu.grouped_matmul, x, w, edges, dy), want, mag, terms, ("y", "dx", "dw")):
+        check(got, ref, m, n, dtype, what)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("groups,most,inner,width", [(150, 200, 512, 512), (40, 900, 256, 264), (300, 5, 128, 128), (90, 130, 640, 321)])
+def test_many_groups(spmm_npu, groups, most, inner, width, dtype):
+    sizes = [int(v) for v in np.random.default_rng(groups).integers(0, most, groups)]
+    x, w, dy = make(sum(sizes), groups, inner, width, dtype)
+    edges = edges_of(sizes)
+    want, mag, terms = plain(x, w, edges, dy)
+    for got, ref, m, n, what in zip(run_all(spmm_npu.grouped_matmul, x, w, edges, dy), want, mag, terms, ("y", "dx", "dw")):
+        check(got, ref, m, n, dtype, what)
+
+
 def test_offsets_past_32_bits(spmm_npu):
     """x of more than 2^31 elements: its last rows are where they should be."""
     rows, inner, width = 270_000, 8192, 16
