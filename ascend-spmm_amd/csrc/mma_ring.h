@@ -161,17 +161,19 @@ struct Ring {
   // The matrix instructions of a step in rows of the wave's sums, and between
   // them the step's copies.
   template <int i>
-  __device__ static inline void multiply_some(const Fragments& f, Sums& s, const Copier<kAC, kRows>& a,
+  __device__ static inline void multiply_some(const Fragments& f, Sums& s, Sums& low, const Copier<kAC, kRows>& a,
                                               const Copier<kBC, kCols>& b, unsigned lds) {
     if constexpr (i < kA) {
 #pragma unroll
       for (int q = 2 * kPlanes - 2; q >= 0; --q)  // planes (0, 1), (1, 0), then (0, 0)
 #pragma unroll
-        for (int j = 0; j < kB; ++j)
-          s.c[i][j] = multiply<T>(f.b[q == 2 ? 1 : 0][j], f.a[q == 1 ? 1 : 0][i], s.c[i][j]);
+        for (int j = 0; j < kB; ++j) {
+          f32x4& c = q == 0 ? s.c[i][j] : low.c[i][j];
+          c = multiply<T>(f.b[q == 2 ? 1 : 0][j], f.a[q == 1 ? 1 : 0][i], c);
+        }
       __builtin_amdgcn_sched_barrier(0);
       copy_some<i * kCopies / kA, (i + 1) * kCopies / kA>(a, b, lds);
-      multiply_some<i + 1>(f, s, a, b, lds);
+      multiply_some<i + 1>(f, s, low, a, b, lds);
     }
   }
 
@@ -216,6 +218,10 @@ struct Ring {
     for (int t = 0; t < kStages - 1; ++t) copy_all();
     int stage = 0;  // of the step at hand
     Fragments f0, f1;
+    // Products with a low plane, apart: an instruction's sum is cut to fp32, not
+    // rounded, and the large sums are cut by a third as many.
+    Sums low;
+    if constexpr (kPair) low.clear();
     wait_copies<(kStages - 2) * kCopies>();
     barrier();
     read_all(f0, stage);
@@ -226,7 +232,7 @@ struct Ring {
       begin_copies();
       stage = next(stage);
       read_all(g, stage);
-      multiply_some<0>(f, s, ca, cb, base + fill);
+      multiply_some<0>(f, s, low, ca, cb, base + fill);
       end_copies();
     };
     for (int t = from; t < to; t += 2) {
@@ -236,6 +242,12 @@ struct Ring {
     // No copy outlives the loop: LDS is free again.
     wait_copies<0>();
     barrier();
+    if constexpr (kPair) {
+#pragma unroll
+      for (int i = 0; i < kA; ++i)
+#pragma unroll
+        for (int j = 0; j < kB; ++j) s.c[i][j] += low.c[i][j];
+    }
   }
 };
 

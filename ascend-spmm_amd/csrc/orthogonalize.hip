@@ -12,13 +12,15 @@
 // plane has 22 bits or more, and three products of planes (high high, high
 // low, low high) added in fp32 give what fp32 products give.
 //
-// A bf16 update is rounded to 8 bits at the end, so its factors need fewer:
-// one product of high planes, of 11 bits.  X keeps its low plane for a X, so
-// that weak directions, which the steps raise most, are not lost beside strong
-// ones; and the diagonals of A and P, where most of these matrices lies, are
-// carried in fp32: with D what the high plane leaves of the diagonal, A A is
-// taken as Ah Ah + D Ah + Ah D, and P X as Ph X + D X.  Against 64 bits the
-// result is 1.05 to 1.4 times as far off as its rounding alone.
+// The diagonals of A and P, where most of these matrices lies, are carried in
+// fp32 and are zeros in the planes: with D the diagonal, A A is taken as A' A' +
+// D A' + A' D + D D, and P X as P' X + D X.  Matrix instructions cut their sums
+// to fp32 (they do not round), always to the same side; without the large
+// terms, and with products of low planes summed apart, little is lost.
+//
+// A bf16 update is rounded to 8 bits at the end, so its factors need fewer: one
+// product of high planes, of 11 bits.  X keeps its low plane for a X, so that
+// weak directions, which the steps raise most, are not lost beside strong ones.
 //
 // Planes are padded with zeros to multiples of 64, which all products keep.
 #include <algorithm>
@@ -111,19 +113,18 @@ struct Planes {
 };
 
 // What is done with the sums of a product: v = alpha * sum + (beta + alpha *
-// rest[i]) * E(i, j), E the planes `add`; stored as planes or as the result.
-// rest, on one plane's products, is what the high planes leave of the left
-// factor's diagonal: of the polynomial for the update of X; of A for the
-// polynomial, where it counts on both sides and E lacks it on the diagonal.
+// d[i]) * E(i, j), E the planes `add`; stored as planes or as the result.  d is
+// the left factor's diagonal, which its planes hold as zeros: the polynomial's
+// for the update of X; A's for the polynomial, where it counts on both sides.
 enum Kind { kGram, kPoly, kUpdate, kLast };
 
 struct Finish {
   float alpha, beta;
   Planes add;           // not for kGram
-  const float* rest;    // [batch][rest_rows]
+  const float* left;    // [batch][diagonals]: d; not for kGram
   Planes to;            // not for kLast
-  float* diagonal;      // [batch][rest_rows]: what to.hi leaves of the diagonal (one plane's products)
-  int64_t rest_rows;
+  float* diagonal;      // [batch][diagonals]: of the result of kGram and kPoly
+  int64_t diagonals;
   void* out;            // kLast: the result, [rows][cols] of the update's type and shape
   int64_t rows, cols;
   bool tall;
@@ -134,7 +135,7 @@ template <int kCols>
 struct Addend {
   typedef half Halves __attribute__((ext_vector_type(kCols)));
   Halves hi, lo;
-  float rest, across[kCols];
+  float left, across[kCols];
 };
 
 template <Kind kKind, bool kPair, int kCols>
@@ -145,12 +146,10 @@ __device__ inline Addend<kCols> load_addend(const Finish& f, int64_t batch, int 
     const int64_t at = batch * f.add.size + row * f.add.ld + col;
     a.hi = *reinterpret_cast<const Halves*>(f.add.hi + at);
     if constexpr (kPair || kKind != kPoly) a.lo = *reinterpret_cast<const Halves*>(f.add.lo + at);
-    if constexpr (!kPair) {
-      a.rest = f.rest[batch * f.rest_rows + row];
-      if constexpr (kKind == kPoly)
+    a.left = f.left[batch * f.diagonals + row];
+    if constexpr (kKind == kPoly)
 #pragma unroll
-        for (int e = 0; e < kCols; ++e) a.across[e] = f.rest[batch * f.rest_rows + col + e];
-    }
+      for (int e = 0; e < kCols; ++e) a.across[e] = f.left[batch * f.diagonals + col + e];
   }
   return a;
 }
@@ -164,10 +163,10 @@ __device__ inline void finish(const Finish& f, const Addend<kCols>& a, int64_t b
 #pragma unroll
     for (int e = 0; e < kCols; ++e) {
       float x = static_cast<float>(a.hi[e]) + static_cast<float>(a.lo[e]);
-      float w = f.beta + f.alpha * a.rest;
-      if constexpr (kKind == kPoly && !kPair) {
-        w += f.alpha * a.across[e];
-        if (row == col + e) x += a.rest;
+      float w = f.beta + f.alpha * a.left;
+      if constexpr (kKind == kPoly) {
+        if (row == col + e) x = a.left;
+        else w += f.alpha * a.across[e];
       }
       v[e] += w * x;
     }
@@ -190,10 +189,13 @@ __device__ inline void finish(const Finish& f, const Addend<kCols>& a, int64_t b
     typename Addend<kCols>::Halves h, l;
 #pragma unroll
     for (int e = 0; e < kCols; ++e) {
+      if constexpr (kKind != kUpdate)
+        if (row == col + e) {
+          f.diagonal[batch * f.diagonals + row] = v[e];
+          v[e] = 0.0f;
+        }
       h[e] = static_cast<half>(v[e]);
       l[e] = static_cast<half>(v[e] - static_cast<float>(h[e]));
-      if constexpr (!kPair && kKind != kUpdate)
-        if (row == col + e) f.diagonal[batch * f.rest_rows + row] = v[e] - static_cast<float>(h[e]);
     }
     const int64_t at = batch * f.to.size + row * f.to.ld + col;
     *reinterpret_cast<decltype(h)*>(f.to.hi + at) = h;
@@ -341,7 +343,10 @@ __global__ __launch_bounds__(kThreads) void store_planes(Finish f, int64_t mp, i
        i += static_cast<int64_t>(gridDim.x) * kThreads) {
     const int64_t batch = i / fours, row = i % fours * 4 / f.add.ld, col = i % fours * 4 % f.add.ld;
     float v[4] = {};
-    finish<T, kLast, true, 4>(f, load_addend<kLast, true, 4>(f, batch, row, col), batch, row, col, v);
+    Addend<4> a = {};  // without a left factor
+    a.hi = *reinterpret_cast<const f16x4*>(f.add.hi + batch * f.add.size + row * f.add.ld + col);
+    a.lo = *reinterpret_cast<const f16x4*>(f.add.lo + batch * f.add.size + row * f.add.ld + col);
+    finish<T, kLast, true, 4>(f, a, batch, row, col, v);
   }
 }
 
@@ -357,7 +362,8 @@ constexpr int kInnerSteps = 16;   // most steps
 // Most blocks of a wave: 40 of 1024 sums, and 16 where little LDS leaves room
 // for a second work-group on a CU.
 constexpr int kInnerBlocks = 5, kInnerBlocksFew = 2;
-constexpr int kInnerLds = 160 * 1024 - 512, kInnerLdsFew = 40 * 1024;
+constexpr int kInnerLds = 160 * 1024 - 1024, kInnerLdsFew = 40 * 1024;
+constexpr int kInnerMost = 128;  // most padded rows: two square matrices in kInnerLds
 
 struct InnerArgs {
   int64_t rows, cols;
@@ -398,7 +404,8 @@ __device__ inline u32x4 inner_across(const half* p, int ld, int first, int k0, i
 
 typedef f32x4 InnerBlock[2][2];
 
-// The wave's blocks of left times right (turned: k across right's lines).
+// The wave's blocks of left times right (turned: k across right's lines).  Each
+// instruction's large products are added in fp32, rounded.
 template <bool kTurned, int kBlocks>
 __device__ inline void inner_product(const InnerPlanes& left, const InnerPlanes& right, int blocks, int across, int depth,
                                      InnerBlock (&s)[kBlocks]) {
@@ -412,6 +419,7 @@ __device__ inline void inner_product(const InnerPlanes& left, const InnerPlanes&
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) s[b][i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    InnerBlock low = {};
     for (int k0 = 0; k0 < depth; k0 += 32) {
       u32x4 l[2][2], r[2][2];
 #pragma unroll
@@ -423,14 +431,21 @@ __device__ inline void inner_product(const InnerPlanes& left, const InnerPlanes&
           r[i][q] = kTurned ? inner_across(p, right.ld, j0 + 16 * i, k0, lane) : inner_along(p, right.ld, j0 + 16 * i, k0, lane);
         }
 #pragma unroll
-      for (int o = 2; o >= 0; --o)  // low products first
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) s[b][i][j] = mma::multiply<half>(r[j][o == 2], l[i][o == 1], s[b][i][j]);
+        for (int j = 0; j < 2; ++j) {
+          low[i][j] = mma::multiply<half>(r[j][1], l[i][0], low[i][j]);
+          s[b][i][j] += mma::multiply<half>(r[j][0], l[i][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+          low[i][j] = mma::multiply<half>(r[j][0], l[i][1], low[i][j]);
+        }
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s[b][i][j] += low[i][j];
   }
 }
+
 
 // f(row, column, four sums) for the wave's blocks.
 template <int kBlocks, typename F>
@@ -467,10 +482,12 @@ __device__ inline f32x4 inner_load(const InnerPlanes& p, int row, int col) {
   return v;
 }
 
-// The wave's blocks times alpha, and beta times a matrix.
-template <int kBlocks>
+// The wave's blocks as finish() takes them: times alpha, and a matrix times
+// beta + alpha d, d the left factor's diagonal; kPoly: on both sides, of a
+// matrix whose own diagonal it is.
+template <bool kPoly, int kBlocks>
 __device__ inline void inner_add(InnerBlock (&s)[kBlocks], int blocks, int across, float alpha, const InnerPlanes& p,
-                                 float beta) {
+                                 float beta, const float* d) {
   const int thread = mma::thread_here(), lane = thread & 63, wave = thread >> 6;
 #pragma unroll
   for (int b = 0; b < kBlocks; ++b) {
@@ -479,9 +496,20 @@ __device__ inline void inner_add(InnerBlock (&s)[kBlocks], int blocks, int acros
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        s[b][i][j] = s[b][i][j] * alpha + inner_load(p, block / across * 32 + i * 16 + (lane & 15),
-                                                     block % across * 32 + j * 16 + (lane >> 4) * 4) * beta;
+      for (int j = 0; j < 2; ++j) {
+        const int row = block / across * 32 + i * 16 + (lane & 15), col = block % across * 32 + j * 16 + (lane >> 4) * 4;
+        const f32x4 x = inner_load(p, row, col);
+        const float left = d[row];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float w = beta + alpha * left, v = x[e];
+          if constexpr (kPoly) {
+            if (row == col + e) v = left;
+            else w += alpha * d[col + e];
+          }
+          s[b][i][j][e] = s[b][i][j][e] * alpha + w * v;
+        }
+      }
   }
 }
 
@@ -490,6 +518,7 @@ __global__ __launch_bounds__(kInnerThreads) void orthogonalize_inner(InnerArgs a
                                                                      T* __restrict__ result) {
   __shared__ __align__(16) char lds[kLds];
   __shared__ double waves[kInnerWaves];
+  __shared__ float diagonal[kInnerMost];  // of A, then of its polynomial, whose planes hold zeros there
   const int64_t elements = a.rows * a.cols;
   const T* u = update + blockIdx.x * elements;
   T* out = result + blockIdx.x * elements;
@@ -521,17 +550,26 @@ __global__ __launch_bounds__(kInnerThreads) void orthogonalize_inner(InnerArgs a
 
   const int square = a.mp / 32 * (a.mp / 32), wide = a.mp / 32 * (a.np / 32);
   InnerBlock s[kBlocks];
+  auto store_square = [&](int row, int col, f32x4 v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (row == col + e) {
+        diagonal[row] = v[e];
+        v[e] = 0.0f;
+      }
+    inner_store(gram, row, col, v);
+  };
   for (int t = 0; t < a.steps; ++t) {
     inner_product<false>(x, x, square, a.mp / 32, a.np, s);
-    inner_each(s, square, a.mp / 32, [&](int row, int col, f32x4 v) { inner_store(gram, row, col, v * a.gram[t]); });
+    inner_each(s, square, a.mp / 32, [&](int row, int col, f32x4 v) { store_square(row, col, v * a.gram[t]); });
     __syncthreads();
     inner_product<false>(gram, gram, square, a.mp / 32, a.mp, s);
-    inner_add(s, square, a.mp / 32, a.poly[t], gram, a.poly_a[t]);
+    inner_add<true>(s, square, a.mp / 32, a.poly[t], gram, a.poly_a[t], diagonal);
     __syncthreads();  // all of A has been read
-    inner_each(s, square, a.mp / 32, [&](int row, int col, f32x4 v) { inner_store(gram, row, col, v); });
+    inner_each(s, square, a.mp / 32, store_square);
     __syncthreads();
     inner_product<true>(gram, x, wide, a.np / 32, a.mp, s);
-    inner_add(s, wide, a.np / 32, a.update[t], x, a.update_x[t]);
+    inner_add<false>(s, wide, a.np / 32, a.update[t], x, a.update_x[t], diagonal);
     if (t + 1 == a.steps) break;
     __syncthreads();  // all of X has been read
     inner_each(s, wide, a.np / 32, [&](int row, int col, f32x4 v) { inner_store(x, row, col, v); });
@@ -625,7 +663,7 @@ Plan plan_for(int64_t batch, int64_t rows, int64_t cols, int64_t depth, bool pai
 }
 
 // X twice (a step reads one and writes the other), A and P in planes, their
-// diagonals' rests, the sums of squares, and the sums of split products.
+// diagonals, the sums of squares, and the sums of split products.
 // m <= n: the matrix's extents, mp and np padded.
 struct Layout {
   int64_t m, n, mp, np;
@@ -771,10 +809,8 @@ spmm_status run(const spmm_orthogonalize_desc* d, const Layout& l, const void* u
   };
   Planes x = planes(l.x, l.np, true), y = planes(l.x, l.np, true);
   const Planes gram = planes(l.gram, l.mp, l.pair), poly = planes(l.gram, l.mp, l.pair);
-  float* gram_rest = l.pair ? nullptr : reinterpret_cast<float*>(ws);
-  take(l.diagonal);
-  float* poly_rest = l.pair ? nullptr : reinterpret_cast<float*>(ws);
-  take(l.diagonal);
+  float* gram_diagonal = reinterpret_cast<float*>(take(l.diagonal));
+  float* poly_diagonal = reinterpret_cast<float*>(take(l.diagonal));
   double* parts = reinterpret_cast<double*>(take(l.parts));
   float* sums = reinterpret_cast<float*>(ws);
   const T* u = static_cast<const T*>(update);
@@ -785,7 +821,7 @@ spmm_status run(const spmm_orthogonalize_desc* d, const Layout& l, const void* u
                      x.lo);
   if (spmm_status st = check_launch("orthogonalize scale")) return st;
   Finish f{};
-  f.rest_rows = l.mp;
+  f.diagonals = l.mp;
   f.out = out;
   f.rows = d->rows;
   f.cols = d->width;
@@ -803,19 +839,19 @@ spmm_status run(const spmm_orthogonalize_desc* d, const Layout& l, const void* u
     const Scales c = scales_of(d, i, bound);
     f.alpha = static_cast<float>(c.gram);
     f.to = gram;
-    f.diagonal = gram_rest;
+    f.diagonal = gram_diagonal;
     if (spmm_status st = multiply<T, kGram>({x, x, mp, mp, np, 1, sums}, f, d->batch, l.pair, s)) return st;
     f.alpha = static_cast<float>(c.poly);
     f.beta = static_cast<float>(c.poly_a);
     f.add = gram;
-    f.rest = gram_rest;
+    f.left = gram_diagonal;
     f.to = poly;
-    f.diagonal = poly_rest;
+    f.diagonal = poly_diagonal;
     if (spmm_status st = multiply<T, kPoly>({gram, gram, mp, mp, mp, 1, sums}, f, d->batch, l.pair, s)) return st;
     f.alpha = static_cast<float>(c.update);
     f.beta = static_cast<float>(c.update_x);
     f.add = x;
-    f.rest = poly_rest;
+    f.left = poly_diagonal;
     f.to = y;
     const Product p{poly, x, mp, np, mp, 1, sums};
     if (spmm_status st = i + 1 < d->steps ? multiply<T, kUpdate>(p, f, d->batch, l.pair, s)
