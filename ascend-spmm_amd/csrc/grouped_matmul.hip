@@ -3,8 +3,9 @@
 //
 // All three are products of operands as they lie in memory: x and grad are
 // read along their rows for out and dx and across them for dW, W either way,
-// so nothing is turned first.  Tiles are those of mma_256.h (fp16 and bf16,
-// 16-byte aligned, large) and mma_128.h (the rest).
+// so nothing is turned first.  Tiles are those of mma_256.h and mma_ring.h
+// (fp16 and bf16 whose pieces of 16 bytes are aligned) and mma_staged.h (fp32,
+// any alignment, and groups of few rows).
 //
 // out and dx: one work-group per tile, none across a group's end; which group
 // a tile belongs to is found on the device by one wave-wide scan of offsets.
@@ -440,15 +441,19 @@ bool pieces_aligned(const spmm_grouped_desc* d, const void* x, const void* weigh
 
 constexpr int64_t kCus = 256;
 
-// The large tile for out and dx: at least three quarters of the CUs get a tile, and the groups'
-// average fills half of one.  65536 x 1024 x 2048 bf16 in 8 groups: 289 us
-// with it, 413 with the small tile.
+// The large tile for out and dx, where three quarters of the CUs get one and the
+// groups' average fills half of it: 65536 rows in 24 groups, 1024 x 2048 bf16,
+// 300 and 310 us against 444 and 459 with tiles of 128; at the rule's edges,
+// 49152 rows of 256 x 256, 17 against 20, and 192 groups of 128 rows, 1024 x
+// 1024, 138 against 179.
 bool large_rows(const GroupedArgs& a) {
   return a.width > 128 && a.inner >= 2 * mma::kDepth && a.rows / mma::kTile * ceil_div(a.width, mma::kTile) >= kCus * 3 / 4 &&
          a.rows / (mma::kTile / 2) >= a.groups;
 }
 
-// The low tile where the groups' average leaves most of a tile of 128 empty.
+// The low tile where the groups' average leaves most of a tile of 128 empty: 13
+// rows in 7 groups, 512 x 512 bf16, 6.8 us against 9.4; at the edge, 42 groups
+// of 48 rows, 10.1 against 10.9.
 bool low_rows(const GroupedArgs& a) { return a.rows / 48 < a.groups; }
 
 // Copies count an operand's pieces in 32 bits.
@@ -456,21 +461,25 @@ bool small_counts(const GroupedArgs& a, int64_t stride, int64_t other) {
   return static_cast<int64_t>(a.rows) * (stride > other ? stride : other) < (int64_t(1) << 33);
 }
 
+// The large tile for dW, where the groups' average keeps it busy for 8 steps:
+// 24 groups of 2731 rows, 1024 x 2048 bf16, 262 us against 342 with tiles of
+// 128; 60 groups of 273 rows, 1024 x 1024, 105 against 100.
 bool large_weights(const GroupedArgs& a) {
-  return a.inner > 128 && a.width > 128 && a.rows / (4 * mma::kDepth) >= a.groups;
+  return a.inner > 128 && a.width > 128 && a.rows / (8 * mma::kDepth) >= a.groups;
 }
 
 // Ranges that dW's rows are cut into: the number that takes the least time by
-// this count, in microseconds.  A round of work-groups takes its steps (1 each
-// for the large tile, 0.5 for two of 128 on a CU, 2.4 for four of fp32's); a cut costs a
-// piece of each tile written and read at 4 TB/s, and joining a launch.
+// this count, in microseconds.  A round of work-groups takes 1.6 a step for the
+// large tile (4096 x 4096 x 4096: 108 us), 0.8 for two of 128 on a CU, and 4.6
+// for four of fp32's (the same product: 1150 us); a cut costs a piece of each
+// tile written and read at 4 TB/s, and joining a launch.
 int64_t weight_parts(const GroupedArgs& a, bool fp32) {
   const bool large = !fp32 && large_weights(a);
   const int64_t side = large ? mma::kTile : fp32 ? 64 : 128, at_once = kCus * (large ? 1 : fp32 ? 4 : 2);
   const int64_t tiles = ceil_div(a.inner, side) * ceil_div(a.width, side);
   const int64_t steps = a.rows / kRowStep + a.groups;
   if (tiles == 0 || steps == 0) return 1;
-  const double step = large ? 1.0 : fp32 ? 2.4 : 0.5, piece = static_cast<double>(tiles * side * side) * 8.0 / 4e6;
+  const double step = large ? 1.6 : fp32 ? 4.6 : 0.8, piece = static_cast<double>(tiles * side * side) * 8.0 / 4e6;
   int64_t best = 1;
   double least = 1e300;
   auto consider = [&](int64_t parts) {

@@ -19,7 +19,7 @@ constexpr int kThreads = 256;
 // Most work-groups.  Each of the backward kernel leaves one row of partial sums
 // of the parameters' gradients: 65536 x 1024 bf16 takes 77 + 11 us (with adding
 // them) with 512 and 78 + 16 with 768; the forward pass 50 us with 2048, 46 with
-// 3072 or 4096.  Both move 5.2 TB/s and more.
+// 4096.  Both move 5.2 TB/s and more.
 constexpr int64_t kBackwardGroups = 512, kForwardGroups = 4096;
 
 struct NormArgs {
