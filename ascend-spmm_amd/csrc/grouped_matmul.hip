@@ -442,7 +442,7 @@ bool pieces_aligned(const spmm_grouped_desc* d, const void* x, const void* weigh
 constexpr int64_t kCus = 256;
 
 // The large tile for out and dx, where three quarters of the CUs get one and the
-// groups' average fills half of it: 65536 rows in 24 groups, 1024 x 2048 bf16,
+// groups' average fills half of it: 65536 rows in 8 groups, 1024 x 2048 bf16,
 // 300 and 310 us against 444 and 459 with tiles of 128; at the rule's edges,
 // 49152 rows of 256 x 256, 17 against 20, and 192 groups of 128 rows, 1024 x
 // 1024, 138 against 179.
@@ -452,7 +452,7 @@ bool large_rows(const GroupedArgs& a) {
 }
 
 // The low tile where the groups' average leaves most of a tile of 128 empty: 13
-// rows in 7 groups, 512 x 512 bf16, 6.8 us against 9.4; at the edge, 42 groups
+// rows in 8 groups, 512 x 512 bf16, 6.8 us against 9.4; at the edge, 42 groups
 // of 48 rows, 10.1 against 10.9.
 bool low_rows(const GroupedArgs& a) { return a.rows / 48 < a.groups; }
 
@@ -462,7 +462,7 @@ bool small_counts(const GroupedArgs& a, int64_t stride, int64_t other) {
 }
 
 // The large tile for dW, where the groups' average keeps it busy for 8 steps:
-// 24 groups of 2731 rows, 1024 x 2048 bf16, 262 us against 342 with tiles of
+// 8 groups of 8192 rows, 1024 x 2048 bf16, 262 us against 342 with tiles of
 // 128; 60 groups of 273 rows, 1024 x 1024, 105 against 100.
 bool large_weights(const GroupedArgs& a) {
   return a.inner > 128 && a.width > 128 && a.rows / (8 * mma::kDepth) >= a.groups;
@@ -571,8 +571,8 @@ spmm_status launch_weights(const GroupedArgs& a, const void* left, int64_t left_
                      static_cast<T*>(dweight), static_cast<int>(parts), static_cast<float*>(ws));
   if (spmm_status st = check_launch(op)) return st;
   if (parts == 1) return SPMM_OK;
-  // A work-group takes 4096 sums where that leaves eight for each CU (24 groups
-  // of 1024 x 2048: 28 us, 62 with 1024), else 1024 (12 of 512 x 512: 6.5, 10).
+  // A work-group takes 4096 sums where that leaves eight for each CU (8 groups
+  // of 1024 x 2048: 28 us, 62 with 1024), else 1024 (12 of 128 x 128: 6.5, 10).
   auto join = [&](auto size) {
     constexpr int kJoin = decltype(size)::value;
     hipLaunchKernelGGL((join_pieces<T, kJoin>), dim3(static_cast<unsigned>(sums / kJoin)), dim3(256), 0, s, a, E::kRows,
