@@ -586,9 +586,18 @@ spmm_status launch_weights(const GroupedArgs& a, const void* left, int64_t left_
   return check_launch(op);
 }
 
+// The stride of an operand's rows.  A single row's is not looked at by the
+// checks and may be anything, but where rows are a product's depth, lines past
+// the last one are kept out by lying past the operand's end: at least as far
+// apart as they are wide, and in whole pieces as every stride there.
+int64_t stride_of(const spmm_grouped_desc* d, int64_t stride, int64_t columns) {
+  return d->rows > 1 ? stride : static_cast<int64_t>(align_up(static_cast<size_t>(columns), 8));
+}
+
 GroupedArgs grouped_args(const spmm_grouped_desc* d, const void* offsets) {
   return {static_cast<int>(d->rows), static_cast<int>(d->groups), static_cast<int>(d->inner),
-          static_cast<int>(d->width), d->x_stride, d->weight_stride, offsets, d->index_type == SPMM_INDEX_I64};
+          static_cast<int>(d->width), stride_of(d, d->x_stride, d->inner), d->weight_stride, offsets,
+          d->index_type == SPMM_INDEX_I64};
 }
 
 // dW's operands, in the order of weight's storage.
@@ -597,7 +606,11 @@ struct WeightSides {
   const void *left, *right;
   int64_t left_stride, right_stride;
   WeightSides(const spmm_grouped_desc* d, const void* offsets, const void* x, const void* grad)
-      : a(grouped_args(d, offsets)), left(x), right(grad), left_stride(d->x_stride), right_stride(d->grad_stride) {
+      : a(grouped_args(d, offsets)),
+        left(x),
+        right(grad),
+        left_stride(stride_of(d, d->x_stride, d->inner)),
+        right_stride(stride_of(d, d->grad_stride, d->width)) {
     if (d->weight_transposed) {
       std::swap(a.inner, a.width);
       std::swap(left, right);
@@ -692,7 +705,7 @@ spmm_status spmm_grouped_grad_run(const spmm_grouped_desc* d, const void* x, con
     if (dx != nullptr) {
       GroupedArgs a = grouped_args(d, offsets);
       std::swap(a.inner, a.width);
-      a.in_stride = d->grad_stride;
+      a.in_stride = stride_of(d, d->grad_stride, d->width);
       // W^T: its depth is W's columns, contiguous unless W is transposed
       if (spmm_status st = d->weight_transposed ? run_rows<T, false>(a, aligned, grad, weight, dx, s, op)
                                                 : run_rows<T, true>(a, aligned, grad, weight, dx, s, op))
