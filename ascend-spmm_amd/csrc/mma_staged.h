@@ -12,8 +12,9 @@
 // the 16 matrix cycles that fp32 instructions take: 4096^3 runs at 119 TFLOP/s,
 // bound by the bf16 rate that the card's power allows.  Parts of an infinity's
 // counterpart may be zero, and their product with it a NaN where fp32 has an
-// infinity: a tile that meets an infinity is summed again with parts that are
-// never zero (kCareful).
+// infinity: a tile that meets an infinity is summed once more with each finite
+// value's sign in its place (kSigns).  That sum is infinite or NaN exactly where
+// fp32's is for its factors' sake, and takes the first one's place there.
 #pragma once
 
 #include "mma.h"
@@ -30,22 +31,18 @@ struct Step {
 };
 
 // Three bf16 parts of an fp32 value, by truncation: all parts of a value have
-// its sign, and what the last one leaves is below 2^-24 of it.  kCareful: parts
-// that would be zero are 2^-126 where the value is 2^-60 or more, nothing
-// against the sum, so that their product with an infinity stays infinite.
-template <bool kCareful>
+// its sign, and what the last one leaves is below 2^-24 of it.
 __device__ inline void split(float x, unsigned& hi, unsigned& mid, unsigned& lo) {
   hi = __builtin_bit_cast(unsigned, x) & 0xffff0000u;
-  const float high = __builtin_bit_cast(float, hi);
-  const float rest = kCareful && x == high ? 0.0f : x - high;
+  const float rest = x - __builtin_bit_cast(float, hi);
   mid = __builtin_bit_cast(unsigned, rest) & 0xffff0000u;
   lo = __builtin_bit_cast(unsigned, rest - __builtin_bit_cast(float, mid));
-  if constexpr (kCareful) {
-    const unsigned sign = __builtin_bit_cast(unsigned, x) & 0x80000000u;
-    const unsigned least = (__builtin_bit_cast(unsigned, x) & 0x7f800000u) >= 0x21800000u ? sign | 0x00800000u : 0u;
-    mid = (mid & 0x7fffffffu) == 0u ? least : mid;
-    lo = (lo & 0x7fff0000u) == 0u ? least : lo;
-  }
+}
+// In the upper half: an infinity, a NaN or a zero as it is, else 1 with x's
+// sign.
+__device__ inline unsigned sign_part(float x) {
+  const unsigned u = __builtin_bit_cast(unsigned, x), size = u & 0x7fffffffu;
+  return size > 0x7f800000u ? 0x7fc00000u : size == 0x7f800000u || size == 0u ? u : (u & 0x80000000u) | 0x3f800000u;
 }
 // The upper halves of a and b as two neighbouring bf16 values.
 __device__ inline unsigned upper_halves(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
@@ -127,8 +124,8 @@ struct Stage {
   }
 
   // Stores the step, which has `left` of the depth, to LDS.  `most`: raised to
-  // the largest magnitude that passes (fp32).
-  template <bool kCareful>
+  // the largest magnitude that passes (fp32).  kSigns: the first part alone.
+  template <bool kSigns>
   __device__ inline void store(char* lds, int left, float& most) {
     if (kAligned && left < S::kDepth) {  // (load() has done so for others)
 #pragma unroll
@@ -153,15 +150,19 @@ struct Stage {
         for (int m = 0; m < 4; ++m) {
           const float x = __builtin_bit_cast(float, static_cast<unsigned>(held[e][m / 2][m % 2 * 2]));
           const float y = __builtin_bit_cast(float, static_cast<unsigned>(held[e][m / 2][m % 2 * 2 + 1]));
-          if constexpr (!kCareful) most = fmaxf(fmaxf(most, fabsf(x)), fabsf(y));
-          unsigned a[3], b[3];
-          split<kCareful>(x, a[0], a[1], a[2]);
-          split<kCareful>(y, b[0], b[1], b[2]);
+          if constexpr (kSigns) {
+            parts[0][m] = upper_halves(sign_part(x), sign_part(y));
+          } else {
+            most = fmaxf(fmaxf(most, fabsf(x)), fabsf(y));
+            unsigned a[3], b[3];
+            split(x, a[0], a[1], a[2]);
+            split(y, b[0], b[1], b[2]);
 #pragma unroll
-          for (int q = 0; q < 3; ++q) parts[q][m] = upper_halves(a[q], b[q]);
+            for (int q = 0; q < 3; ++q) parts[q][m] = upper_halves(a[q], b[q]);
+          }
         }
 #pragma unroll
-        for (int q = 0; q < 3; ++q) *reinterpret_cast<u32x4*>(at + q * kBytes) = parts[q];
+        for (int q = 0; q < (kSigns ? 1 : 3); ++q) *reinterpret_cast<u32x4*>(at + q * kBytes) = parts[q];
       }
     }
   }
@@ -251,13 +252,21 @@ struct Staged {
     add<false>(a, b, lds, s, most);
     if constexpr (S::kParts == 3) {
       if (__syncthreads_or(most == __builtin_inff())) {
-        s.clear();
-        add<true>(a, b, lds, s, most);
+        Sums t;
+        t.clear();
+        add<true>(a, b, lds, t, most);
+#pragma unroll
+        for (int i = 0; i < Sums::kA; ++i)
+#pragma unroll
+          for (int j = 0; j < Sums::kB; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!__builtin_isfinite(t.c[i][j][e])) s.c[i][j][e] = t.c[i][j][e];
       }
     }
   }
 
-  template <bool kCareful>
+  template <bool kSigns>
   __device__ static inline void add(const Operand<T>& a, const Operand<T>& b, char* lds, Sums& s, float& most) {
     const int thread = thread_here(), wave = thread >> 6;
     char* lb = lds + S::kParts * StageA::kBytes;
@@ -282,25 +291,26 @@ struct Staged {
     load();
     do {
       __syncthreads();  // the last step's fragments have been read
-      sa.template store<kCareful>(lds, left, most);
-      sb.template store<kCareful>(lb, left, most);
+      sa.template store<kSigns>(lds, left, most);
+      sb.template store<kSigns>(lb, left, most);
       left -= S::kDepth;
       if (kAligned || left > 0) load();  // (a last, unused one costs less than the branch)
       __syncthreads();
 #pragma unroll
       for (int kk = 0; kk < S::kDepth / 32; ++kk) {
-        u32x4 fa[Sums::kA][S::kParts];
+        constexpr int kParts = kSigns ? 1 : S::kParts;
+        u32x4 fa[Sums::kA][kParts];
 #pragma unroll
         for (int i = 0; i < Sums::kA; ++i)
 #pragma unroll
-          for (int q = 0; q < S::kParts; ++q) fa[i][q] = ra.read(lds, i, kk, q);
-        u32x4 fb[Sums::kB][S::kParts];
+          for (int q = 0; q < kParts; ++q) fa[i][q] = ra.read(lds, i, kk, q);
+        u32x4 fb[Sums::kB][kParts];
 #pragma unroll
         for (int j = 0; j < Sums::kB; ++j)
 #pragma unroll
-          for (int q = 0; q < S::kParts; ++q) fb[j][q] = rb.read(lb, j, kk, q);
+          for (int q = 0; q < kParts; ++q) fb[j][q] = rb.read(lb, j, kk, q);
         // products of parts, the smallest first
-        constexpr int kProducts = S::kParts == 1 ? 1 : 8;
+        constexpr int kProducts = kParts == 1 ? 1 : 8;
         constexpr int kOrder[8][2] = {{0, 0}, {0, 1}, {1, 0}, {1, 1}, {0, 2}, {2, 0}, {1, 2}, {2, 1}};
         typedef std::conditional_t<S::kParts == 3, __bf16, T> Part;
 #pragma unroll
