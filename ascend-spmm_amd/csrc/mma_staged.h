@@ -313,13 +313,28 @@ struct Staged {
         constexpr int kProducts = kParts == 1 ? 1 : 8;
         constexpr int kOrder[8][2] = {{0, 0}, {0, 1}, {1, 0}, {1, 1}, {0, 2}, {2, 0}, {1, 2}, {2, 1}};
         typedef std::conditional_t<S::kParts == 3, __bf16, T> Part;
-#pragma unroll
-        for (int o = kProducts - 1; o >= 0; --o)
+        if constexpr (kProducts == 1) {
 #pragma unroll
           for (int j = 0; j < Sums::kB; ++j)
 #pragma unroll
-            for (int i = 0; i < Sums::kA; ++i)
-              s.c[i][j] = multiply<Part>(fb[j][kOrder[o][1]], fa[i][kOrder[o][0]], s.c[i][j]);
+            for (int i = 0; i < Sums::kA; ++i) s.c[i][j] = multiply<Part>(fb[j][0], fa[i][0], s.c[i][j]);
+        } else {
+          // Matrix instructions cut their sums to fp32, always to the same side:
+          // the parts' products of 32 k are summed apart, from zero, and their
+          // sum is added with fp32's rounding.
+          f32x4 c[Sums::kA][Sums::kB] = {};
+#pragma unroll
+          for (int o = kProducts - 1; o >= 0; --o)
+#pragma unroll
+            for (int j = 0; j < Sums::kB; ++j)
+#pragma unroll
+              for (int i = 0; i < Sums::kA; ++i)
+                c[i][j] = multiply<Part>(fb[j][kOrder[o][1]], fa[i][kOrder[o][0]], c[i][j]);
+#pragma unroll
+          for (int j = 0; j < Sums::kB; ++j)
+#pragma unroll
+            for (int i = 0; i < Sums::kA; ++i) s.c[i][j] += c[i][j];
+        }
       }
     } while (left > 0);
     __syncthreads();
