@@ -8,7 +8,7 @@
 // any alignment, and groups of few rows).
 //
 // out and dx: one work-group per tile, none across a group's end; which group
-// a tile belongs to is found on the device by one wave-wide scan of offsets.
+// a tile belongs to is found on the device by a wave-wide search of offsets.
 //
 // dW: groups differ in length and there may be few tiles, so the rows of all
 // groups are counted through and cut into equal ranges, and a work-group sums
@@ -38,59 +38,110 @@ __device__ inline int edge(const GroupedArgs& a, int g) {
   return v < 0 ? 0 : v > a.rows ? a.rows : static_cast<int>(v);
 }
 
-// Finds the segment of [0, segments) that holds place `at`; segment s takes
-// size(s) places, and `before` is set to the places ahead of the one found.
-// Past the last, returns `segments` and their total.  Every lane of a wave
-// calls it and gets the same answer.
+// The last s of [0, top) with start(s) <= at, where start(0) <= at < start(top)
+// and start ascends: 64 starts a round, three rounds for 262144.  Every lane of
+// a wave calls it and gets the same answer.
 template <typename F>
-__device__ inline int find_segment(int segments, int at, F size, int& before) {
+__device__ inline int find_start(int top, int at, F start) {
   const int lane = threadIdx.x & 63;
-  before = 0;
-  for (int s0 = 0; s0 < segments; s0 += 64) {
-    const int mine = s0 + lane < segments ? size(s0 + lane) : 0;
-    int upto = mine;
+  int lo = 0, hi = top;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) >> 6, probe = lo + (lane + 1) * step;
+    const int f = __ffsll(__ballot(probe >= hi || start(probe) > at)) - 1;  // the last lane's probe is past hi
+    const int next = lo + (f + 1) * step;
+    hi = next < hi ? next : hi;
+    lo += f * step;
+  }
+  return lo;
+}
+
+// The rows as segments: 0 is the rows before the first group, groups + 1 those
+// behind the last; both are `group` -1.  Segment s is [bound(s), bound(s + 1)).
+__device__ inline int bound(const GroupedArgs& a, int s) {
+  return s == 0 ? 0 : s == a.groups + 2 ? a.rows : edge(a, s - 1);
+}
+
+struct RowRange {
+  int first, rows, group;
+};
+
+// Tile `tile` of tiles of kHeight rows, none across a group's end; false where
+// it has no rows.  Segment s has the tiles from bound(s) / kHeight + s on, at
+// least as many as it needs, so that its first is known without a sum over the
+// segments before it.
+template <int kHeight>
+__device__ inline bool find_rows(const GroupedArgs& a, int tile, RowRange& r) {
+  auto start = [&](int s) { return static_cast<int>(static_cast<unsigned>(bound(a, s)) / kHeight) + s; };
+  if (tile >= a.rows / kHeight + a.groups + 2) return false;
+  const int s = find_start(a.groups + 2, tile, start);
+  r.first = bound(a, s) + (tile - start(s)) * kHeight;
+  const int left = bound(a, s + 1) - r.first;
+  r.rows = left < kHeight ? left : kHeight;
+  r.group = s == 0 || s == a.groups + 1 ? -1 : s - 1;
+  return left > 0;
+}
+
+// The same of the tiles that have rows, counted through: what work-groups that
+// stay share out evenly.  `marks` (LDS, kMarks) takes the tiles ahead of every
+// 64th segment.
+constexpr int kMarks = 256;
+template <int kHeight>
+struct CountedRows {
+  const GroupedArgs& a;
+  int* marks;
+  int tiles;  // in all
+
+  __device__ inline int size(int s) const {
+    const int n = s < a.groups + 2 ? bound(a, s + 1) - bound(a, s) : 0;
+    return n > 0 ? (n + kHeight - 1) / kHeight : 0;
+  }
+  // `upto`: the tiles of the window's segments up to the lane's own.
+  __device__ inline int window(int w, int& upto) const {
+    const int lane = threadIdx.x & 63, mine = size(w * 64 + lane);
+    upto = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int o = __shfl_up(upto, d);
       if (lane >= d) upto += o;
     }
-    const unsigned long long past = __ballot(before + upto > at);
-    if (past != 0) {
-      const int found = __ffsll(past) - 1;
-      before += __builtin_amdgcn_readlane(upto - mine, found);
-      return s0 + found;
-    }
-    before += __builtin_amdgcn_readlane(upto, 63);
+    return mine;
   }
-  return segments;
-}
 
-// Ranges of at most `height` rows, none across a group's end.  Segment 0 is the
-// rows before the first group, segment groups + 1 those behind the last; both
-// are `group` -1.
-__device__ inline int first_row(const GroupedArgs& a, int s) { return s == 0 ? 0 : edge(a, s - 1); }
-__device__ inline int end_row(const GroupedArgs& a, int s) { return s == a.groups + 1 ? a.rows : edge(a, s); }
-__device__ inline int find_range(const GroupedArgs& a, int height, int at, int& before) {
-  return find_segment(a.groups + 2, at, [&](int s) {
-    const int n = end_row(a, s) - first_row(a, s);
-    return n > 0 ? (n + height - 1) / height : 0;
-  }, before);
-}
+  __device__ inline CountedRows(const GroupedArgs& a, int* marks) : a(a), marks(marks) {
+    const int most = a.rows / kHeight + a.groups + 2;  // more only where offsets do not ascend
+    int before = 0;
+    for (int w = 0; w * 64 < a.groups + 2; ++w) {
+      if (threadIdx.x == 0) marks[w] = before;
+      int upto;
+      window(w, upto);
+      before += __builtin_amdgcn_readlane(upto, 63);
+      before = before < most ? before : most;
+    }
+    tiles = before;
+    __syncthreads();
+  }
 
-// The `tile`-th range; false past the last.
-struct RowRange {
-  int first, rows, group;
+  // 0 <= tile < tiles.  (False only where offsets do not ascend.)
+  __device__ inline bool find(int tile, RowRange& r) const {
+    const int lane = threadIdx.x & 63, windows = (a.groups + 2 + 63) >> 6;
+    int w = 0;
+    for (int w0 = 0; w0 < windows; w0 += 64) {
+      const unsigned long long ahead = __ballot(w0 + lane < windows && marks[w0 + lane] <= tile);
+      if (ahead == 0) break;
+      w = w0 + 63 - __clzll(ahead);
+    }
+    int upto;
+    const int mine = window(w, upto), before = __builtin_amdgcn_readfirstlane(marks[w]);
+    const unsigned long long past = __ballot(before + upto > tile);
+    if (past == 0) return false;
+    const int found = __ffsll(past) - 1, s = w * 64 + found;
+    r.first = bound(a, s) + (tile - before - __builtin_amdgcn_readlane(upto - mine, found)) * kHeight;
+    const int left = bound(a, s + 1) - r.first;
+    r.rows = left < kHeight ? left : kHeight;
+    r.group = s == 0 || s == a.groups + 1 ? -1 : s - 1;
+    return left > 0;
+  }
 };
-__device__ inline bool find_rows(const GroupedArgs& a, int height, int tile, RowRange& r) {
-  int before;
-  const int s = find_range(a, height, tile, before);
-  if (s == a.groups + 2) return false;
-  r.first = first_row(a, s) + (tile - before) * height;
-  const int left = end_row(a, s) - r.first;
-  r.rows = left < height ? left : height;
-  r.group = s == 0 || s == a.groups + 1 ? -1 : s - 1;
-  return true;
-}
 
 // Neighbouring sums of one row, rounded; `cols`: of the row from the first of
 // them.
@@ -192,7 +243,7 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
   unsigned i, j;
   mma::place_tile(mma::run_of_xcd(blockIdx.x, gridDim.x), down, across, i, j);
   RowRange r;
-  if (!find_rows(a, E::kRows, i, r)) return;
+  if (!find_rows<E::kRows>(a, i, r)) return;
   const int c0 = j * E::kCols, cols = a.width - c0 < E::kCols ? a.width - c0 : E::kCols;
   T* to = out + static_cast<int64_t>(r.first) * a.width + c0;
   E e;
@@ -218,9 +269,9 @@ __global__ __launch_bounds__(mma::kThreads, 2) void grouped_rows_large(GroupedAr
   constexpr int kTile = mma::kTile, kStores = mma::Sums::kEights;
   typedef mma::Tile256<T, false, !kTurned, 1> Tile;
   __shared__ __align__(1024) char lds[mma::kLdsBytes];
-  int down;
-  find_range(a, kTile, INT_MAX, down);
-  const unsigned across = (a.width + kTile - 1) / kTile, tiles = down * across;
+  __shared__ int marks[kMarks];
+  const CountedRows<kTile> counted(a, marks);
+  const unsigned down = counted.tiles, across = (a.width + kTile - 1) / kTile, tiles = down * across;
   const unsigned x = blockIdx.x % kXcds, rest = tiles % kXcds;
   const unsigned begin = x * (tiles / kXcds) + (x < rest ? x : rest), end = begin + tiles / kXcds + (x < rest ? 1 : 0);
   const unsigned stride = gridDim.x / kXcds;
@@ -234,7 +285,7 @@ __global__ __launch_bounds__(mma::kThreads, 2) void grouped_rows_large(GroupedAr
     if (n >= end) return false;
     unsigned i, j;
     mma::place_tile(n, down, across, i, j);
-    if (!find_rows(a, kTile, i, p.r)) return false;
+    if (!counted.find(i, p.r)) return false;
     p.c0 = j * kTile;
     p.cols = a.width - p.c0 < kTile ? a.width - p.c0 : kTile;
     return true;
@@ -286,17 +337,21 @@ __global__ __launch_bounds__(mma::kThreads, 2) void grouped_rows_large(GroupedAr
   }
 }
 
-// dW's sums run over the rows of all groups, counted in steps of 64 (an empty
-// group has one, which adds nothing) and cut into `parts` equal ranges.  The
-// cuts depend on sizes alone, so every engine adds in the same order.
+// dW's sums run over the rows of all groups, counted in steps of 64 (every
+// group has one at least, and may have one that adds nothing) and cut into
+// `parts` equal ranges.  The cuts depend on sizes alone, so every engine adds
+// in the same order.  Group g's steps are [steps.start(g), steps.start(g + 1)).
 constexpr int kRowStep = 64;
-__device__ inline int steps_of(const GroupedArgs& a, int g) {
-  const int n = edge(a, g + 1) - edge(a, g);
-  return n > 0 ? (n + kRowStep - 1) / kRowStep : 1;
-}
-__device__ inline int find_step(const GroupedArgs& a, int at, int& before) {
-  return find_segment(a.groups, at, [&](int g) { return steps_of(a, g); }, before);
-}
+struct Steps {
+  const GroupedArgs& a;
+  int origin, total;
+  __device__ inline explicit Steps(const GroupedArgs& a) : a(a), origin(edge(a, 0) / kRowStep) { total = start(a.groups); }
+  __device__ inline int start(int g) const { return static_cast<int>(static_cast<unsigned>(edge(a, g)) / kRowStep) + g - origin; }
+  // 0 <= at < total
+  __device__ inline int find(int at) const {
+    return find_start(a.groups, at, [&](int g) { return start(g); });
+  }
+};
 __device__ inline int part_start(int total, int part, int parts) {
   return static_cast<int>(static_cast<int64_t>(total) * part / parts);
 }
@@ -313,21 +368,20 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
   typedef typename E::Value T;
   __shared__ __align__(1024) char lds[E::kLds];
   const unsigned across = (a.width + E::kCols - 1) / E::kCols, down = (a.inner + E::kRows - 1) / E::kRows;
-  int total;
-  find_step(a, INT_MAX, total);
-  const unsigned block = mma::run_of_xcd(blockIdx.x, gridDim.x), part = block / (across * down);
+  const Steps steps(a);
+  const unsigned block = mma::run_of_xcd(blockIdx.x, gridDim.x);
+  const int part = block / (across * down);
   unsigned i, j;
   mma::place_tile(block - part * (across * down), down, across, i, j);
-  if (parts > total) parts = total;  // of which the host knows only how many at most
-  if (part >= static_cast<unsigned>(parts)) return;
+  if (parts > steps.total) parts = steps.total;  // of which the host knows only how many at most
+  if (part >= parts) return;
   const int i0 = i * E::kRows, j0 = j * E::kCols;
   const int rows = a.inner - i0 < E::kRows ? a.inner - i0 : E::kRows;
   const int cols = a.width - j0 < E::kCols ? a.width - j0 : E::kCols;
-  const int u0 = part_start(total, part, parts), u1 = part_start(total, part + 1, parts);
-  for (int u = u0; u < u1;) {
-    int before;
-    const int g = find_step(a, u, before);
-    const int lo = edge(a, g), hi = edge(a, g + 1), n = steps_of(a, g);
+  const int u0 = part_start(steps.total, part, parts), u1 = part_start(steps.total, part + 1, parts);
+  int g = steps.find(u0), before = steps.start(g);
+  for (int u = u0; u < u1 && g < a.groups; ++g) {
+    const int lo = edge(a, g), hi = edge(a, g + 1), n = steps.start(g + 1) - before;
     const int s0 = u - before, s1 = n - s0 < u1 - u ? n : s0 + (u1 - u);
     const int first = lo + s0 * kRowStep, last = hi - lo > s1 * kRowStep ? lo + s1 * kRowStep : hi;
     const int depth = last > first ? last - first : 0;
@@ -346,7 +400,8 @@ __global__ __launch_bounds__(E::kThreads, E::kPerCu* E::kThreads / 256) void gro
         *reinterpret_cast<f32x4*>(to + row * E::kCols + col + 4) = w;
       });
     }
-    u += s1 - s0;
+    u += s1 > s0 ? s1 - s0 : 1;
+    before += n;
   }
 }
 
@@ -359,25 +414,28 @@ __global__ __launch_bounds__(256) void join_pieces(GroupedArgs a, int tile_rows,
   const unsigned across = (a.width + tile_cols - 1) / tile_cols, down = (a.inner + tile_rows - 1) / tile_rows;
   const unsigned tiles = across * down, size = tile_rows * tile_cols, slices = size / kJoin;
   const unsigned each = blockIdx.x / slices, n = each / tiles, tile = each - n * tiles;
-  int total;
-  find_step(a, INT_MAX, total);
+  const Steps steps(a);
+  const int total = steps.total;
   if (parts > total) parts = total;
+  if (parts <= 0) return;
   int g, u0, part;  // the group, its first step, and the range that holds it
   if (by_cut) {
     if (n + 1 >= static_cast<unsigned>(parts)) return;
     const int cut = part_start(total, n + 1, parts);
-    g = find_step(a, cut, u0);
+    g = steps.find(cut);
+    u0 = steps.start(g);
     if (cut == u0 || part_start(total, n, parts) > u0) return;
     part = n;
   } else {
     g = n;
-    find_segment(a.groups, INT_MAX, [&](int s) { return s < g ? steps_of(a, s) : 0; }, u0);
+    u0 = steps.start(g);
+    if (u0 < 0 || u0 >= total) return;  // (offsets that do not ascend)
     part = static_cast<int>(static_cast<int64_t>(u0) * parts / total);
     while (part > 0 && part_start(total, part, parts) > u0) --part;
-    while (part_start(total, part + 1, parts) <= u0) ++part;
+    while (part + 1 < parts && part_start(total, part + 1, parts) <= u0) ++part;
   }
-  const int u1 = u0 + steps_of(a, g);
-  if (part_start(total, part + 1, parts) >= u1) return;  // written whole
+  const int u_end = steps.start(g + 1), u1 = u_end < total ? u_end : total;
+  if (u1 <= u0 || part_start(total, part + 1, parts) >= u1) return;  // written whole
   // ranges that start inside the group
   int end = static_cast<int>(static_cast<int64_t>(u1) * parts / total);
   while (end > part + 1 && part_start(total, end - 1, parts) >= u1) --end;
@@ -424,9 +482,10 @@ spmm_status check_grouped_desc(const spmm_grouped_desc* d, const char* op) {
   return SPMM_OK;
 }
 
-// Work-groups of a launch: a grid's limit is an error, not a wrapped count.
-spmm_status check_grid(int64_t blocks, const char* op) {
-  if (blocks > INT32_MAX) return fail(SPMM_ERR_OVERFLOW, std::string(op) + ": too many tiles for one launch");
+// Work-groups of a launch: a grid's limit, 2^32 work-items, is an error, not a
+// wrapped count.
+spmm_status check_grid(int64_t blocks, int64_t threads, const char* op) {
+  if (blocks * threads > UINT32_MAX) return fail(SPMM_ERR_OVERFLOW, std::string(op) + ": too many tiles for one launch");
   return SPMM_OK;
 }
 
@@ -445,10 +504,10 @@ constexpr int64_t kCus = 256;
 // groups' average fills half of it: 65536 rows in 8 groups, 1024 x 2048 bf16,
 // 300 and 310 us against 444 and 459 with tiles of 128; at the rule's edges,
 // 49152 rows of 256 x 256, 17 against 20, and 192 groups of 128 rows, 1024 x
-// 1024, 138 against 179.
+// 1024, 138 against 179.  More groups than its marks hold go to tiles of 128.
 bool large_rows(const GroupedArgs& a) {
   return a.width > 128 && a.inner >= 2 * mma::kDepth && a.rows / mma::kTile * ceil_div(a.width, mma::kTile) >= kCus * 3 / 4 &&
-         a.rows / (mma::kTile / 2) >= a.groups;
+         a.rows / (mma::kTile / 2) >= a.groups && a.groups + 2 <= 64 * kMarks;
 }
 
 // The low tile where the groups' average leaves most of a tile of 128 empty: 13
@@ -520,7 +579,7 @@ spmm_status launch_rows(const GroupedArgs& a, const void* in, const void* weight
   typedef typename E::Value T;
   const int64_t down = ceil_div(a.rows, E::kRows) + a.groups + 1;
   const int64_t blocks = down * ceil_div(a.width, E::kCols);
-  if (spmm_status st = check_grid(blocks, op)) return st;
+  if (spmm_status st = check_grid(blocks, E::kThreads, op)) return st;
   hipLaunchKernelGGL((grouped_rows<E, kTurned>), dim3(static_cast<unsigned>(blocks)), dim3(E::kThreads), 0, s, a,
                      static_cast<const T*>(in), static_cast<const T*>(weight), static_cast<T*>(out), static_cast<unsigned>(down));
   return check_launch(op);
@@ -536,8 +595,9 @@ spmm_status run_rows(const GroupedArgs& a, bool aligned, const void* in, const v
   aligned = aligned && static_cast<int64_t>(a.inner) * a.width < (int64_t(1) << 33);
   if constexpr (sizeof(T) == 2)
     if (aligned && large_rows(a)) {
+      // (the kernel counts its tiles in 32 bits)
       const int64_t down = ceil_div(a.rows, mma::kTile) + a.groups + 1;
-      if (spmm_status st = check_grid(down * ceil_div(a.width, mma::kTile), op)) return st;
+      if (spmm_status st = check_grid(down * ceil_div(a.width, mma::kTile), 1, op)) return st;
       hipLaunchKernelGGL((grouped_rows_large<T, kTurned>), dim3(kCus), dim3(mma::kThreads), 0, s, a,
                          static_cast<const T*>(in), static_cast<const T*>(weight), static_cast<T*>(out));
       return check_launch(op);
@@ -565,7 +625,8 @@ spmm_status launch_weights(const GroupedArgs& a, const void* left, int64_t left_
   // Joined by groups or by cuts, whichever are fewer.
   const bool by_cut = parts - 1 < a.groups;
   const int64_t sums = (by_cut ? parts - 1 : a.groups) * tiles * (E::kRows * E::kCols);
-  if (spmm_status st = check_grid(sums / 1024 > parts * tiles ? sums / 1024 : parts * tiles, op)) return st;
+  if (spmm_status st = check_grid(parts * tiles, E::kThreads, op)) return st;
+  if (spmm_status st = check_grid(sums / 1024, 256, op)) return st;
   hipLaunchKernelGGL(grouped_weights<E>, dim3(static_cast<unsigned>(parts * tiles)), dim3(E::kThreads), 0, s, a,
                      static_cast<const T*>(left), left_stride, static_cast<const T*>(right), right_stride,
                      static_cast<T*>(dweight), static_cast<int>(parts), static_cast<float*>(ws));
