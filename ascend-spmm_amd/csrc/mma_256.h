@@ -185,9 +185,10 @@ struct Copier {
   unsigned lds;             // the wave's part of the first buffer's first half tile
   __amdgpu_buffer_rsrc_t b;
 
-  __device__ inline Copier(const Operand<T>& o, const char* base, int wave, int lane) {
-    p = reinterpret_cast<const char*>(o.p);
-    second = reinterpret_cast<const char*>(o.lo);
+  // `low_first`: the first of the three rounds is the low plane's.
+  __device__ inline Copier(const Operand<T>& o, bool low_first, const char* base, int wave, int lane) {
+    p = reinterpret_cast<const char*>(kPlanes > 1 && low_first ? o.lo : o.p);
+    second = reinterpret_cast<const char*>(kPlanes > 1 && low_first ? o.p : o.lo);
     step_bytes = C ? 2 * kDepth * o.ld : 2 * kDepth;
     step_pieces = static_cast<int>(step_bytes / 16);
     const int64_t elements = C ? (o.depth - 1) * o.ld + (o.valid + 7) / 8 * 8 : (o.valid - 1) * o.ld + o.depth;
@@ -216,20 +217,20 @@ struct Copier {
         for (int h = 0; h < 2; ++h) offset[h][0] = offset[h][1] = 0x80000000u;
   }
 
-  // To the next step.  Of three rounds over the depth, `plane` is the one with
-  // the second plane.  Past all of them, zeros.
-  __device__ inline void advance(int plane) {
+  // To the next step.  Of three rounds over the depth, the plane changes before
+  // round `first` and, where they differ, round `then`.  Past all of them, zeros.
+  __device__ inline void advance(int first, int then) {
     ++at;
     p += step_bytes;
     left -= step_pieces;
     if constexpr (kPlanes == 1) {
       if (at >= steps) left = 0;
     } else if (at == steps || at == 2 * steps || at == 3 * steps) {
-      // back to the origin, of the other plane before and after its turn
+      // back to the origin, of the other plane where it is its turn
       const int64_t back = static_cast<int64_t>(steps) * step_bytes;
       p -= back;
       left = at < 3 * steps ? total : 0;
-      if (at == plane * steps || at == (plane + 1) * steps) {
+      if (at == first * steps || at == then * steps) {
         const char* other = p;
         p = second;
         second = other;
@@ -269,16 +270,21 @@ struct Sums {
 };
 
 // One tile: sum over k of A(i, k) B(j, k).  kPlanes 3: operands held as sums of
-// two planes, high and low; the products high high, high low and low high are
-// added (low low is below fp32's rounding).  `lds`: kLdsBytes.
+// two planes, high and low; the products low high, high low and high high are
+// added, in this order (low low is below fp32's rounding): matrix instructions
+// cut their sums to fp32, always to the same side, and the large sums of high
+// high are cut by their own steps alone.  `lds`: kLdsBytes.
 template <typename T, bool kAC, bool kBC, int kPlanes>
 struct Tile256 {
   Copier<T, kAC, kPlanes> ca;
   Copier<T, kBC, kPlanes> cb;
 
   __device__ inline Tile256(const Operand<T>& a, const Operand<T>& b, const char* lds, int thread)
-      : ca(a, lds, __builtin_amdgcn_readfirstlane(thread >> 6), thread & 63),
-        cb(b, lds + 65536, __builtin_amdgcn_readfirstlane(thread >> 6), thread & 63) {}
+      : ca(a, true, lds, __builtin_amdgcn_readfirstlane(thread >> 6), thread & 63),
+        cb(b, false, lds + 65536, __builtin_amdgcn_readfirstlane(thread >> 6), thread & 63) {}
+  // Planes: A low, high, high; B high, low, high.
+  __device__ inline void advance_a() { ca.advance(1, 1); }
+  __device__ inline void advance_b() { cb.advance(1, 2); }
 
   // Starts the copies of the first step: B0 A0 B1 A1, two instructions each.
   // LDS is free.
@@ -287,8 +293,8 @@ struct Tile256 {
     ca.copy(0, 0);
     cb.copy(0, 1);
     ca.copy(0, 1);
-    cb.advance(1);
-    ca.advance(2);
+    advance_b();
+    advance_a();
   }
 
   // Sums the tile.  kStores: memory instructions of the wave, no more and no
@@ -346,14 +352,14 @@ struct Tile256 {
     wait_copies<4>();                                          \
     barrier();                                                 \
     multiply<T>(s.c[1][1], fa, b1);                            \
-    cb.advance(1);                                             \
+    advance_b();                                               \
     barrier();                                                 \
     rb.template read<((buf) ^ 1) * 32768>(by);                 \
     ca.copy((buf) ^ 1, 1);                                     \
     wait_copies<4>();                                          \
     barrier();                                                 \
     multiply<T>(s.c[1][0], fa, bx);                            \
-    ca.advance(2);                                             \
+    advance_a();                                               \
     barrier();                                                 \
   }
     int t = 0;
