@@ -262,6 +262,10 @@ struct Sums {
 #pragma unroll
     for (int k = 0; k < kEights; ++k) exchange_fours(quadrant(k)[k >> 1 & 3][0], quadrant(k)[k >> 1 & 3][1]);
   }
+  // Columns that eights share: group(k) of kGroups, from group_col().
+  static constexpr int kGroups = 2;
+  __device__ static inline constexpr int group(int k) { return k & 1; }
+  __device__ inline int group_col(int g) const { return g * 128 + col0; }
   // k: row half, row, column half
   __device__ inline Quadrant& quadrant(int k) { return c[k >> 3][k & 1]; }
   __device__ inline int row(int k) const { return (k >> 3) * 128 + (k >> 1 & 3) * 16 + row0; }

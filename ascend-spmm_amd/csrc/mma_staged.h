@@ -230,6 +230,10 @@ struct SumsOf {
 #pragma unroll
       for (int j = 0; j < kB; j += 2) exchange_fours(c[i][j], c[i][j + 1]);
   }
+  // Columns that eights share: group(k) of kGroups, from group_col().
+  static constexpr int kGroups = kB / 2;
+  __device__ static inline constexpr int group(int k) { return k % kGroups; }
+  __device__ inline int group_col(int g) const { return g * 32 + col0; }
   __device__ inline int row(int k) const { return k / (kB / 2) * 16 + row0; }
   __device__ inline int col(int k) const { return k % (kB / 2) * 32 + col0; }
   __device__ inline f32x4 four(int k, int half) const { return c[k / (kB / 2)][k % (kB / 2) * 2 + half]; }
