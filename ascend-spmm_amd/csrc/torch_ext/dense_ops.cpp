@@ -241,7 +241,7 @@ at::Tensor grouped_matmul(const at::Tensor& x, const at::Tensor& weight, const a
 // ----------------------------------------------------------- orthogonalize
 
 // coefficients: a, b, c of every step.
-at::Tensor orthogonalize(const at::Tensor& update, const std::vector<double>& coefficients, double eps) {
+at::Tensor orthogonalize(const at::Tensor& update, const std::vector<double>& coefficients, double eps, bool precise) {
   TORCH_CHECK_GPU(update);
   TORCH_CHECK(update.dim() >= 2, "orthogonalize: update must have at least two dimensions, but got: ", update.dim());
   TORCH_CHECK(coefficients.size() % 3 == 0, "orthogonalize: coefficients must hold three values for each step");
@@ -252,7 +252,7 @@ at::Tensor orthogonalize(const at::Tensor& update, const std::vector<double>& co
   int64_t batch = 1;
   for (int64_t i = 0; i + 2 < u.dim(); ++i) batch *= u.size(i);
   const spmm_orthogonalize_desc d{batch, rows, width, static_cast<int64_t>(coefficients.size() / 3),
-                                  coefficients.data(), eps, dense_type_of(u, "orthogonalize")};
+                                  coefficients.data(), eps, dense_type_of(u, "orthogonalize"), precise ? 1 : 0};
   at::Tensor out = at::empty(u.sizes(), u.options());
   size_t bytes = 0;
   raise_status(spmm_orthogonalize_workspace(&d, &bytes), "orthogonalize");
@@ -290,5 +290,5 @@ void bind_dense_ops(pybind11::module_& m) {
     )doc",
         pybind11::arg("x"), pybind11::arg("weight"), pybind11::arg("offsets"));
   m.def("orthogonalize", &orthogonalize, "Newton-Schulz steps on matrix updates (GPU)", pybind11::arg("update"),
-        pybind11::arg("coefficients"), pybind11::arg("eps"));
+        pybind11::arg("coefficients"), pybind11::arg("eps"), pybind11::arg("precise") = false);
 }

@@ -486,7 +486,9 @@ spmm_status spmm_grouped_grad_run(const spmm_grouped_desc* desc, const void* x, 
  * rows x width (contiguous, extents below 2^22).  X = update / (|update|_F + eps), then each step
  * replaces X by a X + (b A + c A A) X with A = X X^T (for more rows than
  * columns the same polynomial from the right).  coefficients: 3 * steps host
- * values (a, b, c of each step).  out may be update itself. */
+ * values (a, b, c of each step).  out may be update itself.  X is held in fp32;
+ * the products' factors have 22 bits or more, a BF16 update's 11 where
+ * min(rows, width) >= 128, unless `precise` is set. */
 typedef struct spmm_orthogonalize_desc {
   int64_t batch;
   int64_t rows;
@@ -495,6 +497,7 @@ typedef struct spmm_orthogonalize_desc {
   const double* coefficients;
   double eps;
   int32_t value_type;
+  int32_t precise;  /* not 0: factors of 22 bits for BF16 too                */
 } spmm_orthogonalize_desc;
 
 spmm_status spmm_orthogonalize_workspace(const spmm_orthogonalize_desc* desc, size_t* bytes);
