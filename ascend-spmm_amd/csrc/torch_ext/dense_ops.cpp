@@ -4,6 +4,7 @@
 // current stream.  Gradients are not differentiable themselves.
 #include "ext_common.h"
 
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -38,6 +39,12 @@ int64_t row_stride(const at::Tensor& rows) {
 bool wants_grad(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 bool wants_grad(const c10::optional<at::Tensor>& t) { return t.has_value() && wants_grad(*t); }
 
+// Forward-mode derivatives are refused: the kernels would drop them.
+void check_no_tangent(const at::Tensor& t, const char* op) {
+  TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), op,
+              ": forward-mode derivatives are not supported");
+}
+
 // ------------------------------------------------------------- layer_norm
 
 void check_layer_norm(const at::Tensor& x, const c10::optional<at::Tensor>& weight,
@@ -46,8 +53,10 @@ void check_layer_norm(const at::Tensor& x, const c10::optional<at::Tensor>& weig
   TORCH_CHECK(x.dim() >= 1, "layer_norm: x must have at least one dimension");
   TORCH_CHECK(x.size(-1) >= 1, "layer_norm requires a last dimension of at least one element");
   dense_type_of(x, "layer_norm");
+  check_no_tangent(x, "layer_norm");
   for (const auto* p : {&weight, &bias}) {
     if (!p->has_value()) continue;
+    check_no_tangent(**p, "layer_norm");
     const char* name = p == &weight ? "weight" : "bias";
     const at::Tensor& t = **p;
     TORCH_CHECK(t.device() == x.device(), "layer_norm: ", name, " must be on the same device as x");
@@ -166,6 +175,8 @@ void check_grouped(const at::Tensor& x, const at::Tensor& weight, const at::Tens
   TORCH_CHECK(weight.dim() == 3, "grouped_matmul: weight must be a 3D Tensor, but got: ", weight.dim());
   TORCH_CHECK(offsets.dim() == 1, "grouped_matmul: offsets must be a 1D Tensor, but got: ", offsets.dim());
   dense_type_of(x, "grouped_matmul");
+  check_no_tangent(x, "grouped_matmul");
+  check_no_tangent(weight, "grouped_matmul");
   TORCH_CHECK(weight.scalar_type() == x.scalar_type(), "grouped_matmul: weight must have the dtype of x");
   TORCH_CHECK(weight.size(1) == x.size(1), "grouped_matmul: x has ", x.size(1), " columns, but weight takes ",
               weight.size(1));
@@ -246,6 +257,7 @@ at::Tensor orthogonalize(const at::Tensor& update, const std::vector<double>& co
   TORCH_CHECK(update.dim() >= 2, "orthogonalize: update must have at least two dimensions, but got: ", update.dim());
   TORCH_CHECK(coefficients.size() % 3 == 0, "orthogonalize: coefficients must hold three values for each step");
   TORCH_CHECK(!wants_grad(update), "orthogonalize is not differentiable: call it under torch.no_grad()");
+  check_no_tangent(update, "orthogonalize");
   c10::DeviceGuard guard(update.device());
   const at::Tensor u = update.contiguous();
   const int64_t rows = u.size(-2), width = u.size(-1);
