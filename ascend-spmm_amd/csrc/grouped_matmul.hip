@@ -594,7 +594,9 @@ spmm_status run_rows(const GroupedArgs& a, bool aligned, const void* in, const v
   // (copies count a matrix's pieces in 32 bits)
   aligned = aligned && static_cast<int64_t>(a.inner) * a.width < (int64_t(1) << 33);
   if constexpr (sizeof(T) == 2)
-    if (aligned && large_rows(a)) {
+    // Its buffer stores are of whole, aligned pieces; the other tiles store at any
+    // element.
+    if (aligned && reinterpret_cast<uintptr_t>(out) % 16 == 0 && large_rows(a)) {
       // (the kernel counts its tiles in 32 bits)
       const int64_t down = ceil_div(a.rows, mma::kTile) + a.groups + 1;
       if (spmm_status st = check_grid(down * ceil_div(a.width, mma::kTile), 1, op)) return st;
