@@ -86,18 +86,21 @@ struct Ring {
 
     // Instruction n of the step's copies, to `lds` (the wave's part).  Written
     // as assembly, which keeps the compiler from waiting for it before every
-    // read of LDS: the barriers order them.  (m0 holds nothing else in these
-    // kernels: no other instruction of theirs takes it.)
+    // read of LDS: the barriers order them.  m0, which holds the place in LDS, is
+    // the compiler's own, and is left as it was.
     static constexpr int kInstructions = kPlanes * kRounds;
     template <int n>
     __device__ inline void copy(unsigned lds) const {
       const uint64_t from = reinterpret_cast<uint64_t>(n / kRounds == 0 ? p : lo);
       const u32x4 b = {static_cast<unsigned>(from), static_cast<unsigned>(from >> 32) & 0xffffu,
                        static_cast<unsigned>(bytes), 0x00020000u};
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
-                       lds + n / kRounds * kSize * kDepth * 2 + n % kRounds * 4096),
-                   "v"(offset[n % kRounds]), "s"(b)
-                   : "memory");
+      unsigned m0;
+      asm volatile(
+          "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
+          "s_mov_b32 m0, %0"
+          : "=&s"(m0)
+          : "s"(lds + n / kRounds * kSize * kDepth * 2 + n % kRounds * 4096), "v"(offset[n % kRounds]), "s"(b)
+          : "memory");
     }
 
     __device__ inline void advance() {
