@@ -455,7 +455,8 @@ spmm_status spmm_layer_norm_grad_run(const spmm_norm_desc* desc, const void* x, 
  * offsets[0] and from offsets[groups] on become zero.  weight[g] is
  * inner x width, at weight + g * weight_stride; transposed: stored as
  * width x inner, each group's matrix contiguous either way.  inner, width and
- * the row strides are below 2^22, rows below 2^31. */
+ * the row strides are below 2^22, rows below 2^31, groups at most 2^24.  A single
+ * row's strides are not used.  The forward call's workspace is 0 bytes. */
 typedef struct spmm_grouped_desc {
   int64_t rows;           /* of x, out and grad                            */
   int64_t groups;
