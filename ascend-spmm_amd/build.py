@@ -37,8 +37,13 @@ HIP_SOURCES = [
     "layer_norm.hip",
     "grouped_matmul.hip",
     "orthogonalize.hip",
+    "sort_ids.hip",
+    "embedding.hip",
+    "route.hip",
+    "experts.hip",
+    "log_probs.hip",
 ]
-EXT_SOURCES = ["custom_op.cpp", "dense_ops.cpp"]
+EXT_SOURCES = ["custom_op.cpp", "dense_ops.cpp", "expert_ops.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # Packed-FP32 instructions (v_pk_*_f32) are disabled for all device code:

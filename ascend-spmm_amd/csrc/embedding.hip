@@ -1,0 +1,387 @@
+// Rows of a table by ids, scaled, and the gradient of the table.
+//
+//   out[i] = scale * weight[ids[i]],   dweight[v] = scale * sum of grad[i] over ids[i] = v
+//
+// An id outside the table gives a row of zeros and adds to none.  The gradient's
+// sums are fp32, in the order of the positions, so that they repeat exactly: the
+// ids are sorted (stably) and each run of equal ones is summed.
+#include "lane_reduce.h"
+#include "numeric.h"
+#include "sort_ids.h"
+
+namespace spmm {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct TableArgs {
+  int64_t count, table, width, weight_stride, grad_stride;
+  float scale;
+  bool index64;
+};
+
+__device__ inline int64_t id_at(const void* ids, bool index64, int64_t i) {
+  return index64 ? static_cast<const int64_t*>(ids)[i] : static_cast<const int32_t*>(ids)[i];
+}
+
+// A group of L lanes takes one row of the output after another, kRows at a time
+// so that their loads are under way together.
+constexpr int kRows = 4;
+template <typename T, int L>
+__global__ __launch_bounds__(kThreads) void gather_table(TableArgs a, const T* __restrict__ weight,
+                                                         const void* __restrict__ ids, T* __restrict__ out) {
+  constexpr int V = kPiece<T>, kGroups = kThreads / L;
+  const int64_t pieces = (a.width + V - 1) / V, step = static_cast<int64_t>(gridDim.x) * kGroups * kRows;
+  const int lane = threadIdx.x % L;
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L) * kRows; i < a.count; i += step) {
+    int64_t id[kRows];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) id[u] = i + u < a.count ? id_at(ids, a.index64, i + u) : -1;
+    for (int64_t p = lane; p < pieces; p += L) {
+      piece_t<T> raw[kRows];
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        raw[u] = {};
+        if (static_cast<uint64_t>(id[u]) < static_cast<uint64_t>(a.table))
+          raw[u] = load_raw(weight + id[u] * a.weight_stride + p * V, a.width - p * V);
+      }
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        if (i + u >= a.count) break;
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          v[j] = static_cast<uint64_t>(id[u]) < static_cast<uint64_t>(a.table) ? static_cast<float>(raw[u][j]) * a.scale
+                                                                               : 0.0f;
+        store_piece(out + (i + u) * a.width + p * V, a.width - p * V, v);
+      }
+    }
+  }
+}
+
+// The keys of the sort: an id, or the table's rows for one outside of it.
+struct IdKeys {
+  const void* ids;
+  bool index64;
+  int64_t table;
+  __device__ inline uint32_t operator()(int64_t i) const {
+    const int64_t id = id_at(ids, index64, i);
+    return static_cast<uint32_t>(static_cast<uint64_t>(id) < static_cast<uint64_t>(table) ? id : table);
+  }
+};
+struct SortedKeys {
+  const uint32_t* keys;
+  __device__ inline uint32_t operator()(int64_t i) const { return keys[i]; }
+};
+// Keys and positions at their places; `from` holds the positions so far (null: i itself).
+struct PutPairs {
+  const uint32_t* from;
+  uint32_t *keys, *order;
+  __device__ inline void operator()(int64_t i, uint32_t key, uint32_t place) const {
+    keys[place] = key;
+    order[place] = from == nullptr ? static_cast<uint32_t>(i) : from[i];
+  }
+};
+struct NoBases {
+  __device__ inline void operator()(int, uint32_t) const {}
+};
+
+// Sorted positions that a group of lanes sums, and those whose rows it loads at
+// a time.  A run of one id that lies in one range is stored at once; each part
+// of a longer run goes to a slot: [2 * range] for a run that began before the
+// range, [2 * range + 1] for one that begins in it.
+constexpr int kRange = 32, kBatch = 8;
+
+struct SumArgs {
+  TableArgs a;
+  const uint32_t *keys, *order;
+  float* slots;
+  uint32_t* runs;  // [0]: runs over several ranges so far; then the range in which each begins
+  int64_t ranges, sum_blocks, pieces;
+};
+
+template <typename T, int L>
+__global__ __launch_bounds__(kThreads) void sum_runs(SumArgs s, const T* __restrict__ grad, T* __restrict__ dweight) {
+  constexpr int V = kPiece<T>, kGroups = kThreads / L;
+  const TableArgs& a = s.a;
+  const int64_t n = a.count;
+  if (static_cast<int64_t>(blockIdx.x) >= s.sum_blocks) {
+    // Rows of the table that no id names become zero: a wave looks 64 of them up.
+    if (blockIdx.y != 0) return;
+    const int lane = threadIdx.x & 63;
+    const int64_t first = ((static_cast<int64_t>(blockIdx.x) - s.sum_blocks) * (kThreads / 64) + (threadIdx.x >> 6)) * 64;
+    const int64_t v = first + lane;
+    int64_t lo = 0, hi = n;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (s.keys[mid] < v) lo = mid + 1;
+      else hi = mid;
+    }
+    uint64_t absent = __ballot(v < a.table && (lo >= n || s.keys[lo] != v));
+    const float zero[V] = {};
+    while (absent != 0) {
+      const int64_t row = first + __builtin_ctzll(absent);
+      absent &= absent - 1;
+      for (int64_t c = lane * V; c < a.width; c += 64 * V) store_piece(dweight + row * a.width + c, a.width - c, zero);
+    }
+    return;
+  }
+  const int64_t range = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L;
+  const int64_t p = static_cast<int64_t>(blockIdx.y) * L + threadIdx.x % L, c = p * V;
+  if (range >= s.ranges || p >= s.pieces) return;
+  const int64_t begin = range * kRange, end = begin + kRange < n ? begin + kRange : n;
+  const uint32_t before = begin > 0 ? s.keys[begin - 1] : ~0u, after = end < n ? s.keys[end] : ~0u;
+  float sum[V] = {};
+  uint32_t key = s.keys[begin];
+  bool head = key == before;
+  auto flush = [&](bool tail) {
+    if (key >= a.table) return;
+    if (head || tail) {
+      float* slot = s.slots + ((2 * range + (head ? 0 : 1)) * s.pieces + p) * V;
+#pragma unroll
+      for (int j = 0; j < V; j += 4) *reinterpret_cast<f32x4*>(slot + j) = f32x4{sum[j], sum[j + 1], sum[j + 2], sum[j + 3]};
+      if (!head && p == 0) s.runs[1 + atomicAdd(s.runs, 1u)] = static_cast<uint32_t>(range);
+    } else {
+      float v[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = sum[j] * a.scale;
+      store_piece(dweight + static_cast<int64_t>(key) * a.width + c, a.width - c, v);
+    }
+  };
+  for (int64_t i = begin; i < end; i += kBatch) {
+    uint32_t k[kBatch];
+    piece_t<T> raw[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      k[u] = i + u < end ? s.keys[i + u] : static_cast<uint32_t>(a.table);
+      raw[u] = {};
+      if (k[u] < a.table) raw[u] = load_raw(grad + static_cast<int64_t>(s.order[i + u]) * a.grad_stride + c, a.width - c);
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (i + u >= end) break;
+      if (k[u] != key) {
+        flush(false);
+        key = k[u];
+        head = false;
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[j] += static_cast<float>(raw[u][j]);
+    }
+  }
+  flush(key == after);
+}
+
+// Adds the slots of the runs over several ranges, a work-group a run and 64
+// pieces of its columns; each wave adds consecutive ranges, the waves are added
+// in order.
+constexpr int kJoinWaves = 8;
+template <typename T>
+__global__ __launch_bounds__(64 * kJoinWaves) void join_runs(SumArgs s, T* __restrict__ dweight) {
+  constexpr int V = kPiece<T>;
+  __shared__ float part[kJoinWaves][64 * V];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t p = static_cast<int64_t>(blockIdx.y) * 64 + lane, c = p * V;
+  const uint32_t runs = s.runs[0];
+  for (uint32_t q = blockIdx.x; q < runs; q += gridDim.x) {
+    const int64_t first = s.runs[1 + q];
+    const uint32_t key = s.keys[(first + 1) * kRange];
+    // The last range that the run reaches: the last whose first key is it.
+    int64_t lo = first + 1, hi = s.ranges;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (s.keys[mid * kRange] <= key) lo = mid + 1;
+      else hi = mid;
+    }
+    const int64_t parts = lo - first, w0 = parts * wave / kJoinWaves, w1 = parts * (wave + 1) / kJoinWaves;
+    float sum[V] = {};
+    if (p < s.pieces) {
+#pragma unroll 4
+      for (int64_t k = w0; k < w1; ++k) {
+        const float* slot = s.slots + ((2 * (first + k) + (k == 0 ? 1 : 0)) * s.pieces + p) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] += slot[j];
+      }
+    }
+    __syncthreads();  // readers of the last run's parts are done
+#pragma unroll
+    for (int j = 0; j < V; ++j) part[wave][lane * V + j] = sum[j];
+    __syncthreads();
+    if (wave == 0 && p < s.pieces) {
+      float v[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        v[j] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kJoinWaves; ++w) v[j] += part[w][lane * V + j];
+        v[j] *= s.a.scale;
+      }
+      store_piece(dweight + static_cast<int64_t>(key) * s.a.width + c, s.a.width - c, v);
+    }
+  }
+}
+
+__global__ void clear_word(uint32_t* p) { *p = 0; }
+
+spmm_status check_embedding_desc(const spmm_embedding_desc* d) {
+  if (d == nullptr) return fail(SPMM_ERR_INVALID_ARGUMENT, "null descriptor");
+  if (!dense_type(d->value_type)) return fail(SPMM_ERR_CONTRACT, "embedding supports only FP16, BF16 and FP32 tensors");
+  if (d->index_type != SPMM_INDEX_I32 && d->index_type != SPMM_INDEX_I64)
+    return fail(SPMM_ERR_CONTRACT, "embedding: ids must be int32 or int64");
+  if (d->count < 0 || d->table_rows < 0 || d->width < 0) return fail(SPMM_ERR_CONTRACT, "embedding: negative extent");
+  if (d->count >= (1 << 30) || d->table_rows >= (1 << 30) || d->width >= (1 << 22))
+    return fail(SPMM_ERR_CONTRACT, "embedding: ids and rows of the table must be below 2^30, the width below 2^22");
+  if (d->table_rows > 1 && d->weight_stride < d->width)
+    return fail(SPMM_ERR_CONTRACT, "embedding: rows of weight overlap");
+  if (!(d->scale - d->scale == 0.0)) return fail(SPMM_ERR_INVALID_ARGUMENT, "embedding: scale must be finite");
+  return SPMM_OK;
+}
+
+TableArgs table_args(const spmm_embedding_desc* d) {
+  return {d->count,       d->table_rows, d->width, d->weight_stride, d->grad_stride, static_cast<float>(d->scale),
+          d->index_type == SPMM_INDEX_I64};
+}
+
+// Lanes of a row: one piece of 16 bytes each.
+template <typename F>
+void with_row_lanes(int64_t pieces, F f) {
+  if (pieces <= 4) f(std::integral_constant<int, 4>());
+  else if (pieces <= 8) f(std::integral_constant<int, 8>());
+  else if (pieces <= 16) f(std::integral_constant<int, 16>());
+  else if (pieces <= 32) f(std::integral_constant<int, 32>());
+  else f(std::integral_constant<int, 64>());
+}
+
+template <typename T>
+spmm_status run_gather(const spmm_embedding_desc* d, const void* weight, const void* ids, void* out, hipStream_t s) {
+  with_row_lanes(ceil_div(d->width, kPiece<T>), [&](auto L) {
+    constexpr int kGroups = kThreads / decltype(L)::value;
+    const int64_t blocks = ceil_div(d->count, kGroups * kRows);
+    hipLaunchKernelGGL((gather_table<T, decltype(L)::value>), dim3(static_cast<unsigned>(blocks < 16384 ? blocks : 16384)),
+                       dim3(kThreads), 0, s, table_args(d), static_cast<const T*>(weight), ids, static_cast<T*>(out));
+  });
+  return check_launch("embedding");
+}
+
+// How the ids are sorted, and where in the workspace what lies.
+struct SortLayout {
+  int passes, bits;
+  int64_t ranges, pieces;
+  size_t counts, keys[2], order[2], runs, slots, bytes;
+};
+
+SortLayout sort_layout(const spmm_embedding_desc* d) {
+  SortLayout l;
+  const int all = bits_of(d->table_rows);
+  l.passes = (all + kSortBits - 1) / kSortBits;
+  l.bits = (all + l.passes - 1) / l.passes;
+  l.ranges = ceil_div(d->count, kRange);
+  const int64_t piece = 16 / dense_type_bytes(d->value_type);
+  l.pieces = ceil_div(d->width, piece);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += align_up(bytes, 256);
+    return here;
+  };
+  l.counts = take(static_cast<size_t>(sort_words(d->count, 1 << l.bits)) * 4);
+  for (int k = 0; k < 2; ++k) {
+    l.keys[k] = take(static_cast<size_t>(d->count) * 4);
+    l.order[k] = take(static_cast<size_t>(d->count) * 4);
+  }
+  l.runs = take(static_cast<size_t>(l.ranges + 1) * 4);
+  l.slots = take(static_cast<size_t>(l.ranges) * 2 * l.pieces * piece * 4);
+  l.bytes = at;
+  return l;
+}
+
+template <typename T>
+spmm_status run_gradient(const spmm_embedding_desc* d, const void* ids, const void* grad, void* dweight,
+                         void* workspace, hipStream_t s) {
+  const SortLayout l = sort_layout(d);
+  char* ws = static_cast<char*>(workspace);
+  uint32_t* counts = reinterpret_cast<uint32_t*>(ws + l.counts);
+  uint32_t* runs = reinterpret_cast<uint32_t*>(ws + l.runs);
+  uint32_t *keys = nullptr, *order = nullptr;
+  hipLaunchKernelGGL(clear_word, dim3(1), dim3(1), 0, s, runs);
+  if (spmm_status st = check_launch("embedding_grad clear")) return st;
+  for (int pass = 0; pass < l.passes && d->count > 0; ++pass) {
+    const Digit digit = {pass * l.bits, l.bits, 1 << l.bits};
+    const PutPairs put = {order, reinterpret_cast<uint32_t*>(ws + l.keys[pass & 1]),
+                          reinterpret_cast<uint32_t*>(ws + l.order[pass & 1])};
+    spmm_status st = pass == 0 ? sort_digit(digit, d->count, IdKeys{ids, d->index_type == SPMM_INDEX_I64, d->table_rows},
+                                            counts, put, NoBases(), s)
+                               : sort_digit(digit, d->count, SortedKeys{keys}, counts, put, NoBases(), s);
+    if (st) return st;
+    keys = put.keys;
+    order = put.order;
+  }
+  SumArgs a = {table_args(d), keys, order, reinterpret_cast<float*>(ws + l.slots), runs, l.ranges, 0, l.pieces};
+  const int64_t zero_blocks = ceil_div(d->table_rows, kThreads);
+  with_row_lanes(l.pieces, [&](auto L) {
+    a.sum_blocks = ceil_div(l.ranges, kThreads / decltype(L)::value);
+    hipLaunchKernelGGL((sum_runs<T, decltype(L)::value>),
+                       dim3(static_cast<unsigned>(a.sum_blocks + zero_blocks),
+                            static_cast<unsigned>(ceil_div(l.pieces, decltype(L)::value))),
+                       dim3(kThreads), 0, s, a, static_cast<const T*>(grad), static_cast<T*>(dweight));
+  });
+  if (spmm_status st = check_launch("embedding_grad")) return st;
+  if (l.ranges < 2) return SPMM_OK;
+  const int64_t groups = l.ranges < 512 ? l.ranges : 512;
+  hipLaunchKernelGGL(join_runs<T>, dim3(static_cast<unsigned>(groups), static_cast<unsigned>(ceil_div(l.pieces, 64))),
+                     dim3(64 * kJoinWaves), 0, s, a, static_cast<T*>(dweight));
+  return check_launch("embedding_grad join");
+}
+
+}  // namespace
+}  // namespace spmm
+
+using namespace spmm;
+
+extern "C" {
+
+spmm_status spmm_embedding_run(const spmm_embedding_desc* d, const void* weight, const void* ids, void* out,
+                               spmm_stream stream) {
+  clear_error();
+  if (spmm_status st = check_embedding_desc(d)) return st;
+  if (d->count == 0 || d->width == 0) return SPMM_OK;
+  if ((d->table_rows > 0 && weight == nullptr) || ids == nullptr || out == nullptr)
+    return fail(SPMM_ERR_INVALID_ARGUMENT, "embedding: null device pointer");
+  hipStream_t s = as_stream(stream);
+  switch (d->value_type) {
+    case SPMM_VALUE_F16: return run_gather<_Float16>(d, weight, ids, out, s);
+    case SPMM_VALUE_BF16: return run_gather<__bf16>(d, weight, ids, out, s);
+    default: return run_gather<float>(d, weight, ids, out, s);
+  }
+}
+
+spmm_status spmm_embedding_grad_workspace(const spmm_embedding_desc* d, size_t* bytes) {
+  clear_error();
+  if (bytes == nullptr) return fail(SPMM_ERR_INVALID_ARGUMENT, "null argument");
+  if (spmm_status st = check_embedding_desc(d)) return st;
+  *bytes = sort_layout(d).bytes;
+  return SPMM_OK;
+}
+
+spmm_status spmm_embedding_grad_run(const spmm_embedding_desc* d, const void* ids, const void* grad, void* dweight,
+                                    void* workspace, size_t workspace_bytes, spmm_stream stream) {
+  clear_error();
+  if (spmm_status st = check_embedding_desc(d)) return st;
+  if (d->count > 1 && d->grad_stride < d->width) return fail(SPMM_ERR_CONTRACT, "embedding: rows of grad overlap");
+  if (d->table_rows == 0 || d->width == 0) return SPMM_OK;
+  if (dweight == nullptr || (d->count > 0 && (ids == nullptr || grad == nullptr)))
+    return fail(SPMM_ERR_INVALID_ARGUMENT, "embedding: null device pointer");
+  const size_t need = sort_layout(d).bytes;
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(SPMM_ERR_CONTRACT, "embedding: workspace too small: need " + std::to_string(need) + " bytes");
+  hipStream_t s = as_stream(stream);
+  switch (d->value_type) {
+    case SPMM_VALUE_F16: return run_gradient<_Float16>(d, ids, grad, dweight, workspace, s);
+    case SPMM_VALUE_BF16: return run_gradient<__bf16>(d, ids, grad, dweight, workspace, s);
+    default: return run_gradient<float>(d, ids, grad, dweight, workspace, s);
+  }
+}
+
+}  // extern "C"

@@ -1,0 +1,601 @@
+// Log probabilities of given classes under a softmax over each row of logits,
+// the entropy, and the best classes; and the gradient of the first two.
+//
+// With m the row's maximum, z = x - m, s = sum e^z and ls = log s:
+//   logp = z_t - ls,   H = ls - sum e^z z / s,
+//   dx_i = a ([i = t] - p_i) - h p_i (log p_i + H),   p_i = e^(z_i - ls),
+// for incoming gradients a of logp and h of H.  H is a sum of two terms of one
+// sign, so it keeps its digits where it is small.  All of it is fp32; a row
+// keeps m and ls apart, as their sum would round |m| / 2^24 off every log p.
+#include <cfloat>
+#include <cmath>
+
+#include "lane_reduce.h"
+#include "numeric.h"
+
+namespace spmm {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWideThreads = 512;
+constexpr int kMaxTop = 64;
+constexpr int kMaxParts = 64;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2eLow = 1.925963033500011e-08f;  // log2(e) - kLog2e
+constexpr float kLn2 = 0.693147180559945309417f;
+
+// e^z.  The product with log2(e) rounds, which puts z 2^-24 on the result: 32-bit
+// logits take the rounded part back, those of 16 bits leave it (their results
+// round to 8 or 11 bits, and in s the largest terms have the smallest z).
+template <typename T>
+__device__ inline float exp_of(float z) {
+  const float t = z * kLog2e;
+  const float e = __builtin_amdgcn_exp2f(t);
+  if constexpr (sizeof(T) == 4) {
+    const float low = __builtin_fmaf(z, kLog2eLow, __builtin_fmaf(z, kLog2e, -t));
+    // Where z is infinite or far below, low is no number: e is 0 or infinite by itself.
+    return z > -128.0f && z < 128.0f ? __builtin_fmaf(e, low * kLn2, e) : e;
+  }
+  return e;
+}
+
+struct LogArgs {
+  int64_t rows, classes, stride;
+  int32_t top;
+  bool index64;
+};
+
+__device__ inline int64_t target_of(const void* targets, bool index64, int64_t r) {
+  return index64 ? static_cast<const int64_t*>(targets)[r] : static_cast<const int32_t*>(targets)[r];
+}
+
+struct RowOut {
+  float* logp;
+  float* entropy;
+  float* top_values;
+  int32_t* top_ids;
+  float* stats;  // [rows][2]: m and ls, or null
+};
+
+// What a row's m, s and t = sum e^z z say, by one thread.  A row whose logits
+// are all -inf has s = 0: logp -inf, no entropy, and ls = inf, which makes every
+// p of the gradient zero.
+__device__ inline float finish_row(const LogArgs& a, const RowOut& out, int64_t r, int64_t target, float xt, float m,
+                                   float s, float t) {
+  const float ls = s == 0.0f ? INFINITY : logf(s);
+  const bool named = static_cast<uint64_t>(target) < static_cast<uint64_t>(a.classes);
+  out.logp[r] = named ? (s == 0.0f ? -INFINITY : (xt - m) - ls) : 0.0f;
+  out.entropy[r] = s == 0.0f ? 0.0f : ls - t / s;
+  if (out.stats != nullptr) {
+    out.stats[2 * r] = m;
+    out.stats[2 * r + 1] = ls;
+  }
+  return ls;
+}
+
+__device__ inline float best_value(uint32_t key, float m, float ls) {
+  return key > kKeyOfMinusInf ? (key_value(key) - m) - ls : -INFINITY;
+}
+
+// A logit's key among the best classes: NaN is none of them.
+__device__ inline uint32_t class_key(float v) { return v != v ? 0u : order_key(v); }
+
+// The rows that fit the registers of L lanes, I pieces of 16 bytes each.
+template <typename T, int L, int I>
+__global__ __launch_bounds__(kThreads) void log_probs_rows(LogArgs a, const T* __restrict__ x,
+                                                           const void* __restrict__ targets, RowOut out) {
+  constexpr int V = kPiece<T>, kGroups = kThreads / L;
+  const int lane = threadIdx.x % L;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L; r < a.rows; r += step) {
+    const T* row = x + r * a.stride;
+    float v[I][V];
+    piece_t<T> raw[I];
+    auto column = [&](int i) { return static_cast<int64_t>(i * L + lane) * V; };
+#pragma unroll
+    for (int i = 0; i < I; ++i) raw[i] = load_raw(row + column(i), a.classes - column(i));
+    const int64_t target = target_of(targets, a.index64, r);
+    const float xt =
+        static_cast<uint64_t>(target) < static_cast<uint64_t>(a.classes) ? static_cast<float>(row[target]) : 0.0f;
+    float m = -FLT_MAX, s = 0.0f, t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        v[i][j] = column(i) + j < a.classes ? static_cast<float>(raw[i][j]) : -INFINITY;
+        m = fmaxf(m, v[i][j]);
+      }
+    m = lane_max<L>(m);
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float z = v[i][j] - m, e = exp_of<T>(z);
+        s += e;
+        t += e * fmaxf(z, -200.0f);  // e is 0 from -104 on
+      }
+    s = lane_sum<L>(s);
+    t = lane_sum<L>(t);
+    float ls = 0.0f;
+    if (lane == 0) ls = finish_row(a, out, r, target, xt, m, s, t);
+    if (a.top == 0) continue;
+    uint32_t key[I][V];
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) key[i][j] = class_key(v[i][j]);
+    for (int q = 0; q < a.top; ++q) {
+      uint32_t best = 0, at = 0;
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (key[i][j] > best) {
+            best = key[i][j];
+            at = static_cast<uint32_t>(column(i)) + j;
+          }
+      // The greatest key, then the lowest index that has it.
+      const uint32_t top = lane_max<L>(best);
+      const uint32_t win = lane_min<L>(best == top ? at : 0xFFFFFFFFu);
+      if (lane == 0) {
+        out.top_values[r * a.top + q] = best_value(top, m, ls);
+        out.top_ids[r * a.top + q] = top > kKeyOfMinusInf ? static_cast<int32_t>(win) : -1;
+      }
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (static_cast<uint32_t>(column(i)) + j == win) key[i][j] = 0;
+    }
+  }
+}
+
+// Best classes as (key, ~index): the greatest is the likeliest, ties by the
+// lowest index.
+__device__ inline uint64_t pair_of(uint32_t key, uint32_t index) {
+  return (static_cast<uint64_t>(key) << 32) | (0xFFFFFFFFu - index);
+}
+
+template <int L>
+__device__ inline uint64_t lane_max_pair(uint64_t p) {
+  const uint32_t high = lane_max<L>(static_cast<uint32_t>(p >> 32));
+  const uint32_t low = lane_max<L>(static_cast<uint32_t>(p >> 32) == high ? static_cast<uint32_t>(p) : 0u);
+  return (static_cast<uint64_t>(high) << 32) | low;
+}
+
+struct Part {
+  float m, s, t;
+};
+
+// Wider rows: a work-group streams one part of a row, each thread with a
+// running maximum and sums relative to it, and joins them at the end.
+//
+// The best classes cost the stream nothing: each thread's maximum is there
+// anyway.  The top-th greatest of them is a bound that at least `top` logits
+// reach, and only the threads whose maximum reaches it have such logits: their
+// elements are read again (cache), some top * classes / threads of them, and
+// those that reach the bound are ranked against each other.  Where more do than
+// the buffer holds (many equal logits), the row is gone through once for each
+// best class instead.
+constexpr int kCandidates = 1024;
+
+template <typename T>
+__global__ __launch_bounds__(kWideThreads) void log_probs_wide(LogArgs a, const T* __restrict__ x,
+                                                               const void* __restrict__ targets, RowOut out, int parts,
+                                                               Part* part_sums, uint64_t* part_best) {
+  constexpr int V = kPiece<T>, W = kWideThreads / 64, U = 4;
+  __shared__ float red[3][W];
+  __shared__ uint32_t keys[kWideThreads];
+  __shared__ uint64_t cand[kCandidates];
+  __shared__ uint64_t best[kMaxTop];
+  __shared__ uint32_t bound, reached, found;
+  const int64_t r = blockIdx.x / static_cast<unsigned>(parts);
+  const int part = blockIdx.x % static_cast<unsigned>(parts);
+  const T* row = x + r * a.stride;
+  const int64_t pieces = (a.classes + V - 1) / V;
+  const int64_t p0 = pieces * part / parts, p1 = pieces * (part + 1) / parts;
+  const int tid = threadIdx.x;
+
+  float m = -FLT_MAX, s = 0.0f, t = 0.0f;
+  auto add = [&](const piece_t<T>& raw, int64_t p) {
+    float v[V], top = m;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      v[j] = p * V + j < a.classes ? static_cast<float>(raw[j]) : -INFINITY;
+      top = fmaxf(top, v[j]);
+    }
+    const float shift = m - top, f = exp_of<T>(shift);
+    t = f * (t + s * fmaxf(shift, -200.0f));
+    s *= f;
+    m = top;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float z = v[j] - m, e = exp_of<T>(z);
+      s += e;
+      t += e * fmaxf(z, -200.0f);
+    }
+  };
+  int64_t p = p0 + tid;
+  for (; p + (U - 1) * kWideThreads < p1; p += U * kWideThreads) {
+    piece_t<T> raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t c = (p + u * kWideThreads) * V;
+      raw[u] = load_raw(row + c, a.classes - c);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) add(raw[u], p + u * kWideThreads);
+  }
+  for (; p < p1; p += kWideThreads) add(load_raw(row + p * V, a.classes - p * V), p);
+
+  const float all = block_max<W>(m, red[0]);
+  const float shift = m - all, f = exp_of<T>(shift);
+  t = lane_sum<64>(f * (t + s * fmaxf(shift, -200.0f)));
+  s = lane_sum<64>(s * f);
+  if ((tid & 63) == 0) {
+    red[1][tid >> 6] = s;
+    red[2][tid >> 6] = t;
+  }
+  const uint32_t own_key = order_key(m);
+  keys[tid] = own_key;
+  if (tid == 0) reached = found = 0;
+  __syncthreads();
+  s = t = 0.0f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    s += red[1][w];
+    t += red[2][w];
+  }
+  float ls = 0.0f;
+  if (tid == 0) {
+    if (parts > 1) {
+      part_sums[blockIdx.x] = {all, s, t};
+    } else {
+      const int64_t target = target_of(targets, a.index64, r);
+      const bool named = static_cast<uint64_t>(target) < static_cast<uint64_t>(a.classes);
+      ls = finish_row(a, out, r, target, named ? static_cast<float>(row[target]) : 0.0f, all, s, t);
+    }
+  }
+  if (a.top == 0) return;
+
+  if (tid < 64) {  // the top-th greatest of the threads' maxima
+    uint32_t mine[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) mine[w] = keys[w * 64 + tid];
+    uint32_t limit = 0;
+    for (int q = 0; q < a.top; ++q) {
+      uint32_t own = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) own = mine[w] > own ? mine[w] : own;
+      limit = lane_max<64>(own);
+      const uint64_t has = __ballot(own == limit);
+      if (tid == __builtin_ctzll(has)) {
+        bool gone = false;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+          if (!gone && mine[w] == limit) {
+            mine[w] = 0;
+            gone = true;
+          }
+      }
+    }
+    if (tid == 0) bound = limit > kKeyOfMinusInf ? limit : kKeyOfMinusInf + 1;
+  }
+  __syncthreads();
+  const uint32_t limit = bound;
+  // A thread without a finite logit has its starting maximum for a key, which no logit is below:
+  // at worst the bound is that, and all are candidates.
+  uint32_t* list = keys;  // the maxima are read
+  if (own_key >= limit) list[atomicAdd(&reached, 1u)] = tid;
+  __syncthreads();
+  const uint32_t lists = reached;
+  for (uint32_t e = tid >> 6; e < lists; e += W) {
+    const int64_t first = p0 + list[e];
+    const int lane = tid & 63;
+    for (int64_t q = first + static_cast<int64_t>(lane / V) * kWideThreads; q < p1; q += (64 / V) * kWideThreads) {
+      const int64_t c = q * V + lane % V;
+      if (c < a.classes) {
+        const uint32_t key = class_key(static_cast<float>(row[c]));
+        if (key >= limit) {
+          const uint32_t at = atomicAdd(&found, 1u);
+          if (at < kCandidates) cand[at] = pair_of(key, static_cast<uint32_t>(c));
+        }
+      }
+    }
+  }
+  if (tid < kMaxTop) best[tid] = 0;
+  __syncthreads();
+  const uint32_t count = found;
+  if (count <= kCandidates) {
+    for (uint32_t c = tid; c < count; c += kWideThreads) {
+      const uint64_t mine = cand[c];
+      uint32_t rank = 0;
+      for (uint32_t o = 0; o < count; ++o) rank += cand[o] > mine;
+      if (rank < static_cast<uint32_t>(a.top)) best[rank] = mine;
+    }
+  } else {
+    uint64_t last = ~uint64_t(0);
+    for (int q = 0; q < a.top; ++q) {
+      uint64_t mine = 0;
+      for (int64_t c = p0 * V + tid; c < p1 * V && c < a.classes; c += kWideThreads) {
+        const uint32_t key = class_key(static_cast<float>(row[c]));
+        const uint64_t pair = pair_of(key, static_cast<uint32_t>(c));
+        if (key > kKeyOfMinusInf && pair < last && pair > mine) mine = pair;
+      }
+      mine = lane_max_pair<64>(mine);
+      __syncthreads();  // cand is free: readers of the last round are done
+      if ((tid & 63) == 0) cand[tid >> 6] = mine;
+      __syncthreads();
+      mine = cand[0];
+      for (int w = 1; w < W; ++w) mine = cand[w] > mine ? cand[w] : mine;
+      if (tid == 0) best[q] = mine;
+      if (mine == 0) break;
+      last = mine;
+    }
+  }
+  __syncthreads();
+  if (tid >= 64) return;
+  ls = as_float(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(as_bits(ls)))));
+  if (tid < a.top) {
+    const uint64_t pair = best[tid];
+    if (parts > 1) {
+      part_best[static_cast<int64_t>(blockIdx.x) * a.top + tid] = pair;
+    } else {
+      const uint32_t key = static_cast<uint32_t>(pair >> 32);
+      out.top_values[r * a.top + tid] = best_value(key, all, ls);
+      out.top_ids[r * a.top + tid] =
+          key > kKeyOfMinusInf ? static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(pair)) : -1;
+    }
+  }
+}
+
+// Joins a row's parts: one wave a row, a lane a part.  Each part's best classes
+// are in order, so the row's are taken from the heads of the lists.
+template <typename T>
+__global__ __launch_bounds__(64) void log_probs_join(LogArgs a, const T* __restrict__ x,
+                                                     const void* __restrict__ targets, RowOut out, int parts,
+                                                     const Part* __restrict__ part_sums,
+                                                     const uint64_t* __restrict__ part_best) {
+  const int64_t r = blockIdx.x;
+  const int lane = threadIdx.x;
+  const int64_t target = target_of(targets, a.index64, r);
+  const bool named = static_cast<uint64_t>(target) < static_cast<uint64_t>(a.classes);
+  const float xt = named ? static_cast<float>(x[r * a.stride + target]) : 0.0f;
+  Part mine = {-FLT_MAX, 0.0f, 0.0f};
+  if (lane < parts) mine = part_sums[r * parts + lane];
+  const uint64_t* heads = part_best + (r * parts + lane) * a.top;
+  int taken = 0;
+  uint64_t head = lane < parts && a.top > 0 ? heads[0] : 0;
+  const float m = lane_max<64>(mine.m), shift = mine.m - m, f = exp_of<float>(shift);
+  const float t = lane_sum<64>(f * (mine.t + mine.s * fmaxf(shift, -200.0f))), s = lane_sum<64>(mine.s * f);
+  float ls = 0.0f;
+  if (lane == 0) ls = finish_row(a, out, r, target, xt, m, s, t);
+  for (int q = 0; q < a.top; ++q) {
+    const uint64_t pair = lane_max_pair<64>(head);
+    if (lane == 0) {
+      const uint32_t key = static_cast<uint32_t>(pair >> 32);
+      out.top_values[r * a.top + q] = best_value(key, m, ls);
+      out.top_ids[r * a.top + q] =
+          key > kKeyOfMinusInf ? static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(pair)) : -1;
+    }
+    // Pairs differ by their index: one lane at most has this one, but for the empty pair.
+    if (head == pair && pair != 0) head = ++taken < a.top ? heads[taken] : 0;
+  }
+}
+
+// dlogits, each group of L lanes (256: the work-group) walking the pieces
+// [p0, p1) of a row; rows over blockIdx.x, parts of a row over blockIdx.y.
+template <typename T, int L>
+__global__ __launch_bounds__(kThreads) void log_probs_grad(LogArgs a, const T* __restrict__ x,
+                                                           const void* __restrict__ targets,
+                                                           const float* __restrict__ stats,
+                                                           const float* __restrict__ entropy,
+                                                           const float* __restrict__ grad_logp,
+                                                           const float* __restrict__ grad_entropy,
+                                                           T* __restrict__ dx) {
+  constexpr int V = kPiece<T>, kGroups = kThreads / L;
+  const int lane = threadIdx.x % L;
+  const int64_t pieces = (a.classes + V - 1) / V, step = static_cast<int64_t>(gridDim.x) * kGroups;
+  const int64_t p0 = pieces * blockIdx.y / gridDim.y, p1 = pieces * (blockIdx.y + 1) / gridDim.y;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L; r < a.rows; r += step) {
+    const int64_t target = target_of(targets, a.index64, r);
+    const float m = stats[2 * r], ls = stats[2 * r + 1], H = entropy[r];
+    const bool named = static_cast<uint64_t>(target) < static_cast<uint64_t>(a.classes) && ls != INFINITY;
+    const float ga = named && grad_logp != nullptr ? grad_logp[r] : 0.0f;
+    const float gh = grad_entropy != nullptr ? grad_entropy[r] : 0.0f;
+    const T* row = x + r * a.stride;
+    T* out = dx + r * a.classes;
+    for (int64_t p = p0 + lane; p < p1; p += L) {
+      const piece_t<T> raw = load_raw(row + p * V, a.classes - p * V);
+      float v[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float lp = (static_cast<float>(raw[j]) - m) - ls;
+        v[j] = -exp_of<T>(lp) * (ga + gh * (fmaxf(lp, -200.0f) + H));
+        if (p * V + j == target) v[j] += ga;
+      }
+      store_piece(out + p * V, a.classes - p * V, v);
+    }
+  }
+}
+
+spmm_status check_log_desc(const spmm_log_probs_desc* d) {
+  if (d == nullptr) return fail(SPMM_ERR_INVALID_ARGUMENT, "null descriptor");
+  if (!dense_type(d->value_type)) return fail(SPMM_ERR_CONTRACT, "log_probs supports only FP16, BF16 and FP32 tensors");
+  if (d->index_type != SPMM_INDEX_I32 && d->index_type != SPMM_INDEX_I64)
+    return fail(SPMM_ERR_CONTRACT, "log_probs: targets must be int32 or int64");
+  if (d->rows < 0 || d->rows > INT32_MAX)
+    return fail(SPMM_ERR_CONTRACT, "log_probs: rows must be at least 0 and below 2^31, but got " + std::to_string(d->rows));
+  if (d->classes < 1 || d->classes > INT32_MAX)
+    return fail(SPMM_ERR_CONTRACT, "log_probs requires 1 <= classes < 2^31, but got " + std::to_string(d->classes));
+  if (d->rows > 1 && d->logits_stride < d->classes)
+    return fail(SPMM_ERR_CONTRACT, "log_probs: rows of logits overlap");
+  if (d->top < 0 || d->top > kMaxTop || d->top > d->classes)
+    return fail(SPMM_ERR_INVALID_ARGUMENT, "log_probs: top must be at least 0, at most 64 and at most the classes, but got " +
+                                               std::to_string(d->top));
+  return SPMM_OK;
+}
+
+LogArgs log_args(const spmm_log_probs_desc* d) {
+  return {d->rows, d->classes, d->logits_stride, static_cast<int32_t>(d->top), d->index_type == SPMM_INDEX_I64};
+}
+
+// Rows that a wave's registers hold, with L and I to match; false where they
+// are wider.
+template <typename T, typename F>
+bool with_lanes(int64_t classes, F f) {
+  const int64_t pieces = ceil_div(classes, kPiece<T>);
+#define SPMM_TILE(L, I) \
+  if (pieces <= (L) * (I)) return f(std::integral_constant<int, L>(), std::integral_constant<int, I>()), true
+  SPMM_TILE(2, 1);
+  SPMM_TILE(4, 1);
+  SPMM_TILE(8, 1);
+  SPMM_TILE(16, 1);
+  SPMM_TILE(32, 1);
+  SPMM_TILE(64, 1);
+  SPMM_TILE(64, 2);
+  SPMM_TILE(64, 4);
+#undef SPMM_TILE
+  return false;
+}
+
+bool in_registers(const spmm_log_probs_desc* d) {
+  return ceil_div(d->classes, 16 / dense_type_bytes(d->value_type)) <= 256;
+}
+
+// Parts of a row: as many as give the chip four work-groups a CU, each with a
+// piece for every thread at least.
+int row_parts(const spmm_log_probs_desc* d) {
+  const int64_t pieces = ceil_div(d->classes, 16 / dense_type_bytes(d->value_type));
+  int64_t parts = d->rows > 0 ? 1024 / d->rows : 1;
+  if (parts > pieces / kWideThreads) parts = pieces / kWideThreads;
+  if (parts > kMaxParts) parts = kMaxParts;
+  return static_cast<int>(parts < 1 ? 1 : parts);
+}
+
+size_t part_sums_bytes(const spmm_log_probs_desc* d, int parts) {
+  return align_up(static_cast<size_t>(d->rows) * parts * sizeof(Part), 256);
+}
+
+size_t log_workspace(const spmm_log_probs_desc* d) {
+  if (in_registers(d) || d->rows == 0) return 0;
+  const int parts = row_parts(d);
+  if (parts == 1) return 0;
+  return part_sums_bytes(d, parts) + static_cast<size_t>(d->rows) * parts * d->top * sizeof(uint64_t);
+}
+
+// A launch has fewer than 2^32 work-items: so many wide rows go into one.
+constexpr int64_t kWideRows = int64_t(1) << 22;
+
+template <typename T>
+spmm_status run_forward(const spmm_log_probs_desc* d, const void* logits, const void* targets, const RowOut& out,
+                        void* workspace, hipStream_t s) {
+  LogArgs a = log_args(d);
+  const T* x = static_cast<const T*>(logits);
+  const bool held = with_lanes<T>(d->classes, [&](auto L, auto I) {
+    const int64_t blocks = ceil_div(d->rows, kThreads / decltype(L)::value);
+    hipLaunchKernelGGL((log_probs_rows<T, decltype(L)::value, decltype(I)::value>),
+                       dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(kThreads), 0, s, a, x, targets,
+                       out);
+  });
+  if (held) return check_launch("log_probs");
+  const int parts = row_parts(d);
+  Part* sums = static_cast<Part*>(workspace);
+  uint64_t* best = parts > 1 ? reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + part_sums_bytes(d, parts))
+                             : nullptr;
+  for (int64_t r = 0; r < d->rows; r += kWideRows) {
+    a.rows = d->rows - r < kWideRows ? d->rows - r : kWideRows;
+    const RowOut part = {out.logp + r, out.entropy + r, out.top_values + r * a.top, out.top_ids + r * a.top,
+                         out.stats == nullptr ? nullptr : out.stats + 2 * r};
+    hipLaunchKernelGGL(log_probs_wide<T>, dim3(static_cast<unsigned>(a.rows * parts)), dim3(kWideThreads), 0, s, a,
+                       x + r * a.stride, static_cast<const char*>(targets) + r * (a.index64 ? 8 : 4), part, parts,
+                       sums, best);
+    if (spmm_status st = check_launch("log_probs")) return st;
+  }
+  if (parts == 1) return SPMM_OK;
+  hipLaunchKernelGGL(log_probs_join<T>, dim3(static_cast<unsigned>(d->rows)), dim3(64), 0, s, a, x, targets, out, parts,
+                     sums, best);
+  return check_launch("log_probs join");
+}
+
+template <typename T>
+spmm_status run_backward(const spmm_log_probs_desc* d, const void* logits, const void* targets, const float* stats,
+                         const float* entropy, const float* grad_logp, const float* grad_entropy, void* dlogits,
+                         hipStream_t s) {
+  const LogArgs a = log_args(d);
+  const int64_t pieces = ceil_div(d->classes, kPiece<T>);
+  auto launch = [&](auto L) {
+    constexpr int kGroups = kThreads / decltype(L)::value;
+    int64_t blocks = ceil_div(d->rows, kGroups);
+    // Few rows: in parts of four pieces a lane or more.
+    int64_t parts = blocks < 2048 ? ceil_div(2048, blocks) : 1;
+    const int64_t most = ceil_div(pieces, 4 * decltype(L)::value);
+    if (parts > most) parts = most;
+    if (blocks > 65536) blocks = 65536;
+    hipLaunchKernelGGL((log_probs_grad<T, decltype(L)::value>),
+                       dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(parts)), dim3(kThreads), 0, s, a,
+                       static_cast<const T*>(logits), targets, stats, entropy, grad_logp, grad_entropy,
+                       static_cast<T*>(dlogits));
+  };
+  if (pieces <= 4) launch(std::integral_constant<int, 4>());
+  else if (pieces <= 16) launch(std::integral_constant<int, 16>());
+  else if (pieces <= 256) launch(std::integral_constant<int, 64>());
+  else launch(std::integral_constant<int, 256>());
+  return check_launch("log_probs_grad");
+}
+
+}  // namespace
+}  // namespace spmm
+
+using namespace spmm;
+
+extern "C" {
+
+spmm_status spmm_log_probs_workspace(const spmm_log_probs_desc* d, size_t* bytes) {
+  clear_error();
+  if (bytes == nullptr) return fail(SPMM_ERR_INVALID_ARGUMENT, "null argument");
+  if (spmm_status st = check_log_desc(d)) return st;
+  *bytes = log_workspace(d);
+  return SPMM_OK;
+}
+
+spmm_status spmm_log_probs_run(const spmm_log_probs_desc* d, const void* logits, const void* targets, float* logp,
+                               float* entropy, float* top_values, int32_t* top_ids, float* stats, void* workspace,
+                               size_t workspace_bytes, spmm_stream stream) {
+  clear_error();
+  if (spmm_status st = check_log_desc(d)) return st;
+  if (d->rows == 0) return SPMM_OK;
+  if (logits == nullptr || targets == nullptr || logp == nullptr || entropy == nullptr ||
+      (d->top > 0 && (top_values == nullptr || top_ids == nullptr)))
+    return fail(SPMM_ERR_INVALID_ARGUMENT, "log_probs: null device pointer");
+  const size_t need = log_workspace(d);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(SPMM_ERR_CONTRACT, "log_probs: workspace too small: need " + std::to_string(need) + " bytes");
+  const RowOut out = {logp, entropy, top_values, top_ids, stats};
+  hipStream_t s = as_stream(stream);
+  switch (d->value_type) {
+    case SPMM_VALUE_F16: return run_forward<_Float16>(d, logits, targets, out, workspace, s);
+    case SPMM_VALUE_BF16: return run_forward<__bf16>(d, logits, targets, out, workspace, s);
+    default: return run_forward<float>(d, logits, targets, out, workspace, s);
+  }
+}
+
+spmm_status spmm_log_probs_grad_run(const spmm_log_probs_desc* d, const void* logits, const void* targets,
+                                    const float* stats, const float* entropy, const float* grad_logp,
+                                    const float* grad_entropy, void* dlogits, spmm_stream stream) {
+  clear_error();
+  if (spmm_status st = check_log_desc(d)) return st;
+  if (d->rows == 0) return SPMM_OK;
+  if (logits == nullptr || targets == nullptr || stats == nullptr || entropy == nullptr || dlogits == nullptr)
+    return fail(SPMM_ERR_INVALID_ARGUMENT, "log_probs: null device pointer");
+  hipStream_t s = as_stream(stream);
+  switch (d->value_type) {
+    case SPMM_VALUE_F16:
+      return run_backward<_Float16>(d, logits, targets, stats, entropy, grad_logp, grad_entropy, dlogits, s);
+    case SPMM_VALUE_BF16:
+      return run_backward<__bf16>(d, logits, targets, stats, entropy, grad_logp, grad_entropy, dlogits, s);
+    default: return run_backward<float>(d, logits, targets, stats, entropy, grad_logp, grad_entropy, dlogits, s);
+  }
+}
+
+}  // extern "C"

@@ -1,0 +1,161 @@
+// A stable counting sort by ids: what brings equal ids together in the order
+// of their positions, so that sums over them repeat exactly.
+//
+// Three launches a digit: count_digits counts the digits of each tile of
+// kSortTile keys, add_digits adds each digit's counts up over the tiles, and
+// place_digits finds each key's place.  Within a tile a wave takes 64
+// consecutive keys at a time, in order, and ranks each among the equal ones by
+// ballots over the digit's bits: no atomic decides an order.
+#pragma once
+
+#include "common.h"
+
+namespace spmm {
+
+constexpr int kSortThreads = 256;
+constexpr int kSortWaves = kSortThreads / 64;
+constexpr int kSortRounds = 16;
+constexpr int kSortTile = kSortThreads * kSortRounds;  // keys
+constexpr int kSortBits = 11;                          // most bits of one digit of several
+constexpr int kSortBins = (1 << kSortBits) + 1;        // most values of a single digit
+
+inline int64_t sort_tiles(int64_t n) { return ceil_div(n, kSortTile); }
+
+// Bits of the values 0 to `most`.
+inline int bits_of(int64_t most) {
+  int bits = 1;
+  while ((most >> bits) != 0) ++bits;
+  return bits;
+}
+
+// One digit of the keys: (key >> shift) & mask, below `bins`.
+struct Digit {
+  int shift, bits, bins;
+  __device__ inline uint32_t of(uint32_t key) const { return (key >> shift) & ((1u << bits) - 1); }
+};
+
+// Counts by wave of the tile's digits in LDS: hist[wave][bins].
+template <typename Keys>
+__device__ inline void count_tile(uint32_t* hist, Digit d, int64_t n, Keys keys) {
+  for (int k = threadIdx.x; k < kSortWaves * d.bins; k += kSortThreads) hist[k] = 0;
+  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kSortTile + wave * kSortRounds * 64 + lane;
+#pragma unroll 8
+  for (int q = 0; q < kSortRounds; ++q)
+    if (first + q * 64 < n) atomicAdd(&hist[wave * d.bins + d.of(keys(first + q * 64))], 1u);
+  __syncthreads();
+}
+
+// counts: [tiles][bins].  keys(i) gives key i.
+template <typename Keys>
+__global__ __launch_bounds__(kSortThreads) void count_digits(Digit d, int64_t n, Keys keys, uint32_t* counts) {
+  __shared__ uint32_t hist[kSortWaves * kSortBins];
+  count_tile(hist, d, n, keys);
+  for (int b = threadIdx.x; b < d.bins; b += kSortThreads) {
+    uint32_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) sum += hist[w * d.bins + b];
+    counts[static_cast<int64_t>(blockIdx.x) * d.bins + b] = sum;
+  }
+}
+
+// Exclusive sums of values[0..bins) in LDS over the work-group, in place.
+__device__ inline void scan_bins(uint32_t* values, int bins, uint32_t* sums) {
+  const int per = (bins + kSortThreads - 1) / kSortThreads, tid = threadIdx.x;
+  uint32_t own = 0;
+  for (int k = 0; k < per; ++k)
+    if (tid * per + k < bins) own += values[tid * per + k];
+  uint32_t run = own;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t up = __shfl_up(run, d);
+    if ((tid & 63) >= d) run += up;
+  }
+  if ((tid & 63) == 63) sums[tid >> 6] = run;
+  __syncthreads();
+  uint32_t at = run - own;
+  for (int w = 0; w < (tid >> 6); ++w) at += sums[w];
+  for (int k = 0; k < per; ++k) {
+    const int b = tid * per + k;
+    if (b < bins) {
+      const uint32_t v = values[b];
+      values[b] = at;
+      at += v;
+    }
+  }
+  __syncthreads();
+}
+
+// Lanes of the wave with this lane's digit, among those with `valid`.
+__device__ inline uint64_t same_digit(uint32_t digit, int bits, bool valid) {
+  uint64_t peers = __ballot(valid);
+  for (int b = 0; b < bits; ++b) {
+    const bool set = (digit >> b) & 1u;
+    const uint64_t has = __ballot(set);
+    peers &= set ? has : ~has;
+  }
+  return peers;
+}
+
+// put(i, key, place) for each key; base_of(bin, start) for each digit, with the
+// place of its first key, by the first work-group.
+template <typename Keys, typename Put, typename Bases>
+__global__ __launch_bounds__(kSortThreads) void place_digits(Digit d, int64_t n, Keys keys, const uint32_t* counts,
+                                                             const uint32_t* totals, Put put, Bases base_of) {
+  __shared__ uint32_t hist[kSortWaves * kSortBins], base[kSortBins], sums[kSortWaves];
+  for (int b = threadIdx.x; b < d.bins; b += kSortThreads) base[b] = totals[b];
+  count_tile(hist, d, n, keys);  // with barriers
+  scan_bins(base, d.bins, sums);
+  for (int b = threadIdx.x; b < d.bins; b += kSortThreads) {
+    uint32_t at = base[b];
+    if (blockIdx.x == 0) base_of(b, at);
+    at += counts[static_cast<int64_t>(blockIdx.x) * d.bins + b];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t c = hist[w * d.bins + b];
+      hist[w * d.bins + b] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  volatile uint32_t* next = hist + wave * d.bins;  // the place of the wave's next key of each digit
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kSortTile + wave * kSortRounds * 64 + lane;
+  for (int q = 0; q < kSortRounds; ++q) {
+    const int64_t i = first + q * 64;
+    const bool valid = i < n;
+    const uint32_t key = valid ? keys(i) : 0, digit = d.of(key);
+    const uint64_t peers = same_digit(digit, d.bits, valid);
+    if (valid) {
+      // A wave's LDS accesses are performed in order: all peers read before the first of them writes.
+      const uint64_t before = peers & ((uint64_t(1) << lane) - 1);
+      const uint32_t start = next[digit];
+      if (before == 0) next[digit] = start + static_cast<uint32_t>(__popcll(peers));
+      put(i, key, start + static_cast<uint32_t>(__popcll(before)));
+    }
+  }
+}
+
+// Words of the counts and totals of n keys.
+inline int64_t sort_words(int64_t n, int bins) { return ((n > 0 ? sort_tiles(n) : 1) + 1) * bins; }
+
+// Turns each digit's counts into those of the tiles before, and totals[bins]
+// into the counts of all.
+spmm_status launch_add_digits(int bins, int64_t tiles, uint32_t* counts, uint32_t* totals, hipStream_t s);
+
+// One digit's three launches.  `counts` holds sort_words(n, d.bins) words.
+template <typename Keys, typename Put, typename Bases>
+spmm_status sort_digit(Digit d, int64_t n, Keys keys, uint32_t* counts, Put put, Bases base_of, hipStream_t s) {
+  const int64_t tiles = sort_tiles(n);
+  uint32_t* totals = counts + tiles * d.bins;
+  const dim3 grid(static_cast<unsigned>(tiles > 0 ? tiles : 1));
+  hipLaunchKernelGGL(count_digits<Keys>, grid, dim3(kSortThreads), 0, s, d, n, keys, counts);
+  if (spmm_status st = check_launch("count_digits")) return st;
+  if (spmm_status st = launch_add_digits(d.bins, tiles > 0 ? tiles : 1, counts, totals, s)) return st;
+  hipLaunchKernelGGL((place_digits<Keys, Put, Bases>), grid, dim3(kSortThreads), 0, s, d, n, keys, counts, totals, put,
+                     base_of);
+  return check_launch("place_digits");
+}
+
+}  // namespace spmm

@@ -618,5 +618,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("pack_rows", &pack_rows, "packed[inv[i]] = tensor[i]; other rows zero (GPU)");
   m.def("restore_rows", &restore_rows, "out[i] = packed[inv[i]] (GPU)");
   bind_dense_ops(m);
+  bind_expert_ops(m);
   m.def("library_version", []() { return std::string(spmm_version()); });
 }

@@ -47,3 +47,5 @@ inline at::Tensor workspace(const at::Tensor& like, size_t bytes) {
 
 // Registers the dense operators (dense_ops.cpp) with the Python module.
 void bind_dense_ops(pybind11::module_& m);
+// And the operators around a layer of experts (expert_ops.cpp).
+void bind_expert_ops(pybind11::module_& m);

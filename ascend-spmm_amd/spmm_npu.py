@@ -23,12 +23,18 @@ from custom_ops_lib import (  # noqa: E402
     block_level_split,
     csr_to_ascend_cube,
     csr_to_bcsr,
+    embedding,
+    expert_pack as _expert_pack,
+    expert_plan as _expert_plan,
+    expert_restore as _expert_restore,
     grouped_matmul,
     layer_norm,
+    log_probs,
     orthogonalize as _orthogonalize,
     pack_rows as _pack_rows,
     preprocess,
     restore_rows as _restore_rows,
+    route as _route,
     spmm_ascend_cube,
     spmm_ascend_cube_aic_without_pipeline,
     spmm_ascend_cube_aiv_mb,
@@ -228,18 +234,82 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
     return _orthogonalize(update, flat, eps, bool(precise))
 
 
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def route(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, renormalize=True, scale=1.0):
+    """The ``top_k`` experts of each row of ``logits`` ([..., experts], FP16,
+    BF16 or FP32 on the GPU) and their weights: ``(weights, experts)``, FP32 and
+    int32 of shape [..., top_k], best first.
+
+    The experts with the greatest ``score + bias`` are chosen, ties to the lowest
+    index.  ``score`` is the softmax over the row or the sigmoid of each logit;
+    ``bias`` (FP32, one value an expert) balances the experts and has no part in
+    the weights, which are ``scale`` times the scores, divided by their sum over
+    the chosen if ``renormalize`` is set.  With ``groups`` > 1 the experts are
+    that many equal consecutive groups, and only those of the ``top_groups``
+    groups with the greatest sums of their two best values are chosen from.
+
+    An expert whose logit or bias is -inf is never chosen: where fewer than
+    ``top_k`` are left, the rest are -1 with weight 0, which ``ExpertPlan`` leaves
+    out.  A NaN counts as greatest, so that it is seen in the weights.  Values are
+    compared in 64 bits.  The weights are differentiable with respect to
+    ``logits``; ``bias`` has no gradient.
+    """
+    if score not in _SCORES:
+        raise ValueError("score must be one of " + ", ".join(sorted(_SCORES)))
+    groups = int(groups)
+    return _route(logits, int(top_k), _SCORES[score], bias, groups, groups if top_groups is None else int(top_groups),
+                  bool(renormalize), float(scale))
+
+
+class ExpertPlan:
+    """Where the rows of a layer of experts go, from each row's choices.
+
+    ``experts`` ([rows, top_k] or [rows], int32 or int64 on the GPU, as ``route``
+    returns them) holds ids of ``count`` experts (1 to 2048), and any other id for
+    no expert.  The choices are sorted by expert, in the order of the rows: expert
+    e has the packed rows ``offsets[e]`` to ``offsets[e + 1]``, as
+    ``grouped_matmul`` takes them, and choice j of row r is packed row
+    ``place[r, j]``.  Choices of no expert come behind all others.  Nothing is
+    read back to the host::
+
+        weights, experts = route(logits, 2)
+        plan = ExpertPlan(experts, count)
+        y = plan.restore(grouped_matmul(plan.pack(x), w, plan.offsets), weights)
+    """
+
+    def __init__(self, experts, count):
+        self.offsets, self.place = _expert_plan(experts, int(count))
+
+    def pack(self, x):
+        """Each row of ``x`` at the places of its choices: [rows * top_k, width],
+        zero where a choice is of no expert.  Differentiable."""
+        return _expert_pack(x, self.place, self.offsets)
+
+    def restore(self, results, weights):
+        """The weighted sum of each row's choices from the packed ``results``,
+        those of no expert left out; ``weights`` [rows, top_k] FP32.
+        Differentiable with respect to both."""
+        return _expert_restore(results, weights, self.place, self.offsets)
+
+
 __all__ = [
+    "ExpertPlan",
     "PackedGraph",
     "block_level_split",
     "csr_to_ascend_cube",
     "csr_to_bcsr",
+    "embedding",
     "grouped_matmul",
     "layer_norm",
+    "log_probs",
     "make_start",
     "orthogonalize",
     "pack_node_tensor",
     "preprocess",
     "restore_node_tensor",
+    "route",
     "spmm_ascend_cube",
     "spmm_ascend_cube_aic_without_pipeline",
     "spmm_ascend_cube_aiv_mb",

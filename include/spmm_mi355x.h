@@ -49,7 +49,7 @@ typedef enum spmm_status {
 } spmm_status;
 
 typedef enum spmm_index_type { SPMM_INDEX_I32 = 0, SPMM_INDEX_I64 = 1 } spmm_index_type;
-/* BF16: the dense operators only (layer norm, grouped products, orthogonalised updates). */
+/* BF16: the dense operators and those around experts only. */
 typedef enum spmm_value_type {
   SPMM_VALUE_F16 = 0,
   SPMM_VALUE_F32 = 1,
@@ -505,6 +505,137 @@ spmm_status spmm_orthogonalize_workspace(const spmm_orthogonalize_desc* desc, si
 spmm_status spmm_orthogonalize_run(const spmm_orthogonalize_desc* desc, const void* update,
                                    void* out, void* workspace, size_t workspace_bytes,
                                    spmm_stream stream);
+
+/* ------------------------------------------------------------------------
+ * Operators around a layer of experts: rows of a table by ids, the experts of
+ * each row from a router's logits, rows brought to their experts (whose ranges
+ * spmm_grouped_run takes) and back, and log probabilities of labels.  Types,
+ * sums and strides as above.  Launches only: all of them may be captured.
+ * ---------------------------------------------------------------------- */
+
+/* embedding: out[i] = scale * weight[ids[i]], a row of zeros for an id outside
+ * [0, table_rows).  ids and table rows below 2^30, the width below 2^22. */
+typedef struct spmm_embedding_desc {
+  int64_t count;          /* ids, and rows of out and grad                 */
+  int64_t table_rows;
+  int64_t width;
+  int64_t weight_stride;  /* elements between rows of weight               */
+  int64_t grad_stride;    /* elements between rows of grad (gradient only) */
+  double scale;           /* finite                                        */
+  int32_t index_type;
+  int32_t value_type;
+} spmm_embedding_desc;
+
+spmm_status spmm_embedding_run(const spmm_embedding_desc* desc, const void* weight, const void* ids,
+                               void* out, spmm_stream stream);
+
+/* Its gradient: dweight[v] = scale * the sum of grad[i] over ids[i] = v in the
+ * order of i, every row of the contiguous table_rows x width written. */
+spmm_status spmm_embedding_grad_workspace(const spmm_embedding_desc* desc, size_t* bytes);
+spmm_status spmm_embedding_grad_run(const spmm_embedding_desc* desc, const void* ids, const void* grad,
+                                    void* dweight, void* workspace, size_t workspace_bytes,
+                                    spmm_stream stream);
+
+typedef enum spmm_score { SPMM_SCORE_SOFTMAX = 0, SPMM_SCORE_SIGMOID = 1 } spmm_score;
+
+/* route: the top_k experts of each row by score + bias, best first, ties to the
+ * lowest index, and their weights: scale * score, divided by the sum of the
+ * chosen scores where `renormalize` is set.  bias (fp32, one an expert, NULL
+ * for none) has no part in the weights.  With groups > 1 the experts are that
+ * many equal consecutive groups, and only those of the top_groups groups with
+ * the greatest sums of their two best values are chosen from.  An expert whose
+ * logit or bias is -inf is never chosen; where fewer than top_k are left, the
+ * rest of `chosen` is -1 and their weights 0.  NaN counts as greatest.
+ * Values are compared in 64 bits (the logits themselves without bias and
+ * groups).  stats (fp32, 2 a row, or NULL) is what the gradient of a softmax
+ * that is not renormalised takes. */
+typedef struct spmm_route_desc {
+  int64_t rows;
+  int64_t experts;        /* 1 to 1024                                     */
+  int64_t logits_stride;  /* elements between rows of logits               */
+  int64_t top_k;          /* 1 to 64                                       */
+  int64_t groups;         /* 1 to 64, divides the experts                  */
+  int64_t top_groups;
+  double scale;           /* finite and positive                           */
+  int32_t score;          /* spmm_score                                    */
+  int32_t renormalize;
+  int32_t value_type;     /* logits and dlogits                            */
+} spmm_route_desc;
+
+spmm_status spmm_route_run(const spmm_route_desc* desc, const void* logits, const float* bias,
+                           float* weights, int32_t* chosen, float* stats, spmm_stream stream);
+
+/* Gradient with respect to the logits (contiguous), from that of the weights. */
+spmm_status spmm_route_grad_run(const spmm_route_desc* desc, const void* logits, const int32_t* chosen,
+                                const float* weights, const float* stats, const float* grad,
+                                void* dlogits, spmm_stream stream);
+
+/* Plan of rows for experts: the `choices` expert ids sorted by expert, equal
+ * ones in their order, those outside [0, experts) behind all.  place[i] is the
+ * packed row of choice i, offsets[e] to offsets[e + 1] are expert e's packed
+ * rows.  choices below 2^31, experts 1 to 2048. */
+spmm_status spmm_expert_plan_workspace(int64_t choices, int64_t experts, size_t* bytes);
+spmm_status spmm_expert_plan_run(int32_t index_type, const void* ids, int64_t choices, int64_t experts,
+                                 int32_t* offsets, int32_t* place, void* workspace,
+                                 size_t workspace_bytes, spmm_stream stream);
+
+/* With the plan of `rows` x top_k choices: packed[place[r][j]] = x[r], zero for
+ * a choice of no expert, and its gradient dx[r] = sum over j of
+ * grad[place[r][j]].  Packed tensors have rows * top_k rows. */
+typedef struct spmm_experts_desc {
+  int64_t rows;
+  int64_t top_k;          /* choices a row, 1 to 64                        */
+  int64_t experts;        /* of the plan                                   */
+  int64_t width;
+  int64_t stride;         /* elements between rows of the first tensor     */
+  int64_t grad_stride;    /* of grad (spmm_expert_restore_grad_run only)   */
+  int32_t value_type;
+} spmm_experts_desc;
+
+spmm_status spmm_expert_pack_run(const spmm_experts_desc* desc, const void* x, const int32_t* place,
+                                 const int32_t* offsets, void* packed, spmm_stream stream);
+spmm_status spmm_expert_pack_grad_run(const spmm_experts_desc* desc, const void* grad,
+                                      const int32_t* place, const int32_t* offsets, void* dx,
+                                      spmm_stream stream);
+
+/* out[r] = sum over j of weights[r][j] * y[place[r][j]] (fp32 weights; nothing
+ * for a choice of no expert), and its gradients: dy (rows of no expert zero)
+ * and dweights, either may be NULL. */
+spmm_status spmm_expert_restore_run(const spmm_experts_desc* desc, const void* y, const float* weights,
+                                    const int32_t* place, const int32_t* offsets, void* out,
+                                    spmm_stream stream);
+spmm_status spmm_expert_restore_grad_run(const spmm_experts_desc* desc, const void* y,
+                                         const float* weights, const int32_t* place,
+                                         const int32_t* offsets, const void* grad, void* dy,
+                                         float* dweights, spmm_stream stream);
+
+/* log_probs: of each row's softmax, the log probability of class targets[r]
+ * (0 for a target outside the classes), the entropy, and the `top` likeliest
+ * classes with their log probabilities, best first, ties to the lowest index;
+ * a logit of -inf or NaN is none of them (id -1, -inf).  A row whose logits are
+ * all -inf has the log probability -inf, no entropy and no gradient.  stats
+ * (fp32, 2 a row, or NULL) is for the gradient. */
+typedef struct spmm_log_probs_desc {
+  int64_t rows;
+  int64_t classes;        /* below 2^31                                    */
+  int64_t logits_stride;  /* elements between rows of logits               */
+  int64_t top;            /* 0 to 64, at most the classes                  */
+  int32_t index_type;     /* targets                                       */
+  int32_t value_type;     /* logits and dlogits                            */
+} spmm_log_probs_desc;
+
+spmm_status spmm_log_probs_workspace(const spmm_log_probs_desc* desc, size_t* bytes);
+spmm_status spmm_log_probs_run(const spmm_log_probs_desc* desc, const void* logits, const void* targets,
+                               float* logp, float* entropy, float* top_values, int32_t* top_ids,
+                               float* stats, void* workspace, size_t workspace_bytes,
+                               spmm_stream stream);
+
+/* Gradient with respect to the logits (contiguous) from those of logp and the
+ * entropy, either of which may be NULL. */
+spmm_status spmm_log_probs_grad_run(const spmm_log_probs_desc* desc, const void* logits,
+                                    const void* targets, const float* stats, const float* entropy,
+                                    const float* grad_logp, const float* grad_entropy, void* dlogits,
+                                    spmm_stream stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */
