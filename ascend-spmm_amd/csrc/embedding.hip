@@ -82,22 +82,35 @@ struct PutPairs {
     order[place] = from == nullptr ? static_cast<uint32_t>(i) : from[i];
   }
 };
-struct NoBases {
-  __device__ inline void operator()(int, uint32_t) const {}
+// The count of the runs over several ranges starts at zero: cleared by the sort, as it runs before the sums.
+struct ClearRuns {
+  uint32_t* runs;
+  __device__ inline void operator()(int b, uint32_t) const {
+    if (b == 0) *runs = 0;
+  }
 };
 
-// Sorted positions that a group of lanes sums, and those whose rows it loads at
-// a time.  A run of one id that lies in one range is stored at once; each part
-// of a longer run goes to a slot: [2 * range] for a run that began before the
-// range, [2 * range + 1] for one that begins in it.
-constexpr int kRange = 32, kBatch = 8;
+// A group of lanes sums the rows of `range` sorted positions, loading kBatch of
+// them at a time.  A run of one id that lies in one range is stored at once; each
+// part of a longer run goes to a slot: [2 * range] for a run that began before
+// the range, [2 * range + 1] for one that begins in it.
+constexpr int kBatch = 8;
+
+// Positions of a range: 32, so that the slots of long runs stay few against
+// their rows, down to 8 where that leaves less than 8192 waves.
+inline int range_of(int64_t count, int64_t pieces) {
+  int range = 32;
+  const int64_t lanes = pieces < 64 ? (pieces < 4 ? 4 : pieces) : ceil_div(pieces, 64) * 64;
+  while (range > kBatch && count / range * lanes < int64_t(8192) * 64) range /= 2;
+  return range;
+}
 
 struct SumArgs {
   TableArgs a;
   const uint32_t *keys, *order;
   float* slots;
   uint32_t* runs;  // [0]: runs over several ranges so far; then the range in which each begins
-  int64_t ranges, sum_blocks, pieces;
+  int64_t range, ranges, sum_blocks, pieces;
 };
 
 template <typename T, int L>
@@ -129,7 +142,7 @@ __global__ __launch_bounds__(kThreads) void sum_runs(SumArgs s, const T* __restr
   const int64_t range = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L;
   const int64_t p = static_cast<int64_t>(blockIdx.y) * L + threadIdx.x % L, c = p * V;
   if (range >= s.ranges || p >= s.pieces) return;
-  const int64_t begin = range * kRange, end = begin + kRange < n ? begin + kRange : n;
+  const int64_t begin = range * s.range, end = begin + s.range < n ? begin + s.range : n;
   const uint32_t before = begin > 0 ? s.keys[begin - 1] : ~0u, after = end < n ? s.keys[end] : ~0u;
   float sum[V] = {};
   uint32_t key = s.keys[begin];
@@ -148,21 +161,32 @@ __global__ __launch_bounds__(kThreads) void sum_runs(SumArgs s, const T* __restr
       store_piece(dweight + static_cast<int64_t>(key) * a.width + c, a.width - c, v);
     }
   };
-  for (int64_t i = begin; i < end; i += kBatch) {
-    uint32_t k[kBatch];
-    piece_t<T> raw[kBatch];
+  // Keys and positions are read one batch ahead of the rows.
+  uint32_t k[kBatch], at[kBatch];
+  auto fetch = [&](int64_t i) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       k[u] = i + u < end ? s.keys[i + u] : static_cast<uint32_t>(a.table);
-      raw[u] = {};
-      if (k[u] < a.table) raw[u] = load_raw(grad + static_cast<int64_t>(s.order[i + u]) * a.grad_stride + c, a.width - c);
+      at[u] = i + u < end ? s.order[i + u] : 0;
     }
+  };
+  fetch(begin);
+  for (int64_t i = begin; i < end; i += kBatch) {
+    uint32_t now[kBatch];
+    piece_t<T> raw[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      raw[u] = {};
+      now[u] = k[u];
+      if (k[u] < a.table) raw[u] = load_raw(grad + static_cast<int64_t>(at[u]) * a.grad_stride + c, a.width - c);
+    }
+    if (i + kBatch < end) fetch(i + kBatch);
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       if (i + u >= end) break;
-      if (k[u] != key) {
+      if (now[u] != key) {
         flush(false);
-        key = k[u];
+        key = now[u];
         head = false;
 #pragma unroll
         for (int j = 0; j < V; ++j) sum[j] = 0.0f;
@@ -177,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void sum_runs(SumArgs s, const T* __restr
 // Adds the slots of the runs over several ranges, a work-group a run and 64
 // pieces of its columns; each wave adds consecutive ranges, the waves are added
 // in order.
-constexpr int kJoinWaves = 8;
+constexpr int kJoinWaves = 16;
 template <typename T>
 __global__ __launch_bounds__(64 * kJoinWaves) void join_runs(SumArgs s, T* __restrict__ dweight) {
   constexpr int V = kPiece<T>;
@@ -187,18 +211,24 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_runs(SumArgs s, T* __res
   const uint32_t runs = s.runs[0];
   for (uint32_t q = blockIdx.x; q < runs; q += gridDim.x) {
     const int64_t first = s.runs[1 + q];
-    const uint32_t key = s.keys[(first + 1) * kRange];
-    // The last range that the run reaches: the last whose first key is it.
-    int64_t lo = first + 1, hi = s.ranges;
+    const uint32_t key = s.keys[(first + 1) * s.range];
+    // One past the last range whose first key is the run's: 64 probes at a time.
+    int64_t lo = first + 2, hi = s.ranges;
     while (lo < hi) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (s.keys[mid * kRange] <= key) lo = mid + 1;
-      else hi = mid;
+      const int64_t step = (hi - lo + 63) / 64, probe = lo + lane * step;
+      const uint64_t more = __ballot(probe < hi && s.keys[probe * s.range] != key);
+      if (more == 0) {
+        lo += (hi - 1 - lo) / step * step + 1;  // past the last probe
+      } else {
+        const int at = __builtin_ctzll(more);
+        hi = lo + at * step;
+        lo = at == 0 ? hi : lo + (at - 1) * step + 1;
+      }
     }
     const int64_t parts = lo - first, w0 = parts * wave / kJoinWaves, w1 = parts * (wave + 1) / kJoinWaves;
     float sum[V] = {};
     if (p < s.pieces) {
-#pragma unroll 4
+#pragma unroll 8
       for (int64_t k = w0; k < w1; ++k) {
         const float* slot = s.slots + ((2 * (first + k) + (k == 0 ? 1 : 0)) * s.pieces + p) * V;
 #pragma unroll
@@ -222,8 +252,6 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_runs(SumArgs s, T* __res
     }
   }
 }
-
-__global__ void clear_word(uint32_t* p) { *p = 0; }
 
 spmm_status check_embedding_desc(const spmm_embedding_desc* d) {
   if (d == nullptr) return fail(SPMM_ERR_INVALID_ARGUMENT, "null descriptor");
@@ -268,7 +296,7 @@ spmm_status run_gather(const spmm_embedding_desc* d, const void* weight, const v
 // How the ids are sorted, and where in the workspace what lies.
 struct SortLayout {
   int passes, bits;
-  int64_t ranges, pieces;
+  int64_t range, ranges, pieces;
   size_t counts, keys[2], order[2], runs, slots, bytes;
 };
 
@@ -277,9 +305,10 @@ SortLayout sort_layout(const spmm_embedding_desc* d) {
   const int all = bits_of(d->table_rows);
   l.passes = (all + kSortBits - 1) / kSortBits;
   l.bits = (all + l.passes - 1) / l.passes;
-  l.ranges = ceil_div(d->count, kRange);
   const int64_t piece = 16 / dense_type_bytes(d->value_type);
   l.pieces = ceil_div(d->width, piece);
+  l.range = range_of(d->count, l.pieces);
+  l.ranges = ceil_div(d->count, l.range);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -305,20 +334,21 @@ spmm_status run_gradient(const spmm_embedding_desc* d, const void* ids, const vo
   uint32_t* counts = reinterpret_cast<uint32_t*>(ws + l.counts);
   uint32_t* runs = reinterpret_cast<uint32_t*>(ws + l.runs);
   uint32_t *keys = nullptr, *order = nullptr;
-  hipLaunchKernelGGL(clear_word, dim3(1), dim3(1), 0, s, runs);
-  if (spmm_status st = check_launch("embedding_grad clear")) return st;
-  for (int pass = 0; pass < l.passes && d->count > 0; ++pass) {
+  const IdKeys from_ids = {ids, d->index_type == SPMM_INDEX_I64, d->table_rows};
+  const ClearRuns clear = {runs};
+  const bool ranked = d->count <= kRankMost;
+  for (int pass = 0; pass < (ranked ? 1 : l.passes) && d->count > 0; ++pass) {
     const Digit digit = {pass * l.bits, l.bits, 1 << l.bits};
     const PutPairs put = {order, reinterpret_cast<uint32_t*>(ws + l.keys[pass & 1]),
                           reinterpret_cast<uint32_t*>(ws + l.order[pass & 1])};
-    spmm_status st = pass == 0 ? sort_digit(digit, d->count, IdKeys{ids, d->index_type == SPMM_INDEX_I64, d->table_rows},
-                                            counts, put, NoBases(), s)
-                               : sort_digit(digit, d->count, SortedKeys{keys}, counts, put, NoBases(), s);
+    spmm_status st = ranked      ? sort_by_rank(d->count, 1, from_ids, put, clear, s)
+                     : pass == 0 ? sort_digit(digit, d->count, from_ids, counts, put, clear, s)
+                                 : sort_digit(digit, d->count, SortedKeys{keys}, counts, put, clear, s);
     if (st) return st;
     keys = put.keys;
     order = put.order;
   }
-  SumArgs a = {table_args(d), keys, order, reinterpret_cast<float*>(ws + l.slots), runs, l.ranges, 0, l.pieces};
+  SumArgs a = {table_args(d), keys, order, reinterpret_cast<float*>(ws + l.slots), runs, l.range, l.ranges, 0, l.pieces};
   const int64_t zero_blocks = ceil_div(d->table_rows, kThreads);
   with_row_lanes(l.pieces, [&](auto L) {
     a.sum_blocks = ceil_div(l.ranges, kThreads / decltype(L)::value);

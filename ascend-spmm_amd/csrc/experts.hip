@@ -64,98 +64,160 @@ __device__ inline void store_raw(T* p, int64_t n, const piece_t<T>& v) {
   }
 }
 
-// packed = x's rows: L lanes a row, which read it once and write it k times.
-template <typename T, int L>
+// The kernels' common walk: L lanes a row, which take L * I pieces of 16 bytes of
+// it at a time, and kTogether choices, whose rows' loads are all under way
+// together.  A whole wave's row is a scalar, and so are the loads of its places
+// and weights.
+constexpr int kTogether = 8;
+
+template <typename T, int L, int I>
+struct ChoiceTile {
+  static constexpr int V = kPiece<T>, kGroups = kThreads / L, kChunk = L * I * V;
+
+  __device__ static inline int64_t first_row() {
+    int64_t group = static_cast<int64_t>(blockIdx.x) * kGroups;
+    if constexpr (L == 64) group += __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    else group += threadIdx.x / L;
+    return group;
+  }
+  __device__ static inline int64_t row_step() { return static_cast<int64_t>(gridDim.x) * kGroups; }
+  // The first column of the lane's piece i in the chunk from c0 on.
+  __device__ static inline int64_t column(int64_t c0, int i) {
+    return c0 + static_cast<int64_t>(i * L + threadIdx.x % L) * V;
+  }
+  __device__ static inline void load(const T* row, int64_t c0, int64_t width, piece_t<T> (&v)[I]) {
+#pragma unroll
+    for (int i = 0; i < I; ++i) v[i] = load_raw(row + column(c0, i), width - column(c0, i));
+  }
+};
+
+// packed = x's rows, read once and written k times.
+template <typename T, int L, int I>
 __global__ __launch_bounds__(kThreads) void pack_choices(RowsArgs a, const T* __restrict__ x,
                                                          const int32_t* __restrict__ place,
                                                          const int32_t* __restrict__ offsets, T* __restrict__ packed) {
-  constexpr int V = kPiece<T>, kGroups = kThreads / L;
-  const int lane = threadIdx.x % L;
+  using Tile = ChoiceTile<T, L, I>;
   const uint32_t end = kept_rows(a, offsets);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L; r < a.rows; r += step)
-    for (int64_t c = lane * V; c < a.width; c += L * V) {
-      const piece_t<T> raw = load_raw(x + r * a.stride + c, a.width - c), none = {};
+  for (int64_t r = Tile::first_row(); r < a.rows; r += Tile::row_step())
+    for (int64_t c0 = 0; c0 < a.width; c0 += Tile::kChunk) {
+      piece_t<T> raw[I];
+      const piece_t<T> none = {};
+      Tile::load(x + r * a.stride, c0, a.width, raw);
       for (int j = 0; j < a.k; ++j) {
         const uint32_t p = place[r * a.k + j];
-        if (p < a.choices) store_raw(packed + p * a.width + c, a.width - c, p < end ? raw : none);
+        if (p >= a.choices) continue;
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+          const int64_t c = Tile::column(c0, i);
+          store_raw(packed + p * a.width + c, a.width - c, p < end ? raw[i] : none);
+        }
       }
     }
 }
 
 // out[r] = sum over its choices of (w or 1) * y[place]: restore, and pack's gradient.
-constexpr int kTogether = 4;  // rows loaded at a time
-template <typename T, int L, bool Weighted>
+template <typename T, int L, int I, bool Weighted>
 __global__ __launch_bounds__(kThreads) void add_choices(RowsArgs a, const T* __restrict__ y,
                                                         const float* __restrict__ weights,
                                                         const int32_t* __restrict__ place,
                                                         const int32_t* __restrict__ offsets, T* __restrict__ out) {
-  constexpr int V = kPiece<T>, kGroups = kThreads / L;
-  const int lane = threadIdx.x % L;
+  using Tile = ChoiceTile<T, L, I>;
+  constexpr int V = Tile::V;
   const uint32_t end = kept_rows(a, offsets);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L; r < a.rows; r += step)
-    for (int64_t c = lane * V; c < a.width; c += L * V) {
-      float sum[V] = {};
+  for (int64_t r = Tile::first_row(); r < a.rows; r += Tile::row_step())
+    for (int64_t c0 = 0; c0 < a.width; c0 += Tile::kChunk) {
+      float sum[I][V] = {};
       for (int j = 0; j < a.k; j += kTogether) {
-        piece_t<T> raw[kTogether];
+        piece_t<T> raw[kTogether][I];
         float w[kTogether];
 #pragma unroll
         for (int u = 0; u < kTogether; ++u) {
-          raw[u] = {};
-          w[u] = 0.0f;
-          if (j + u >= a.k) continue;
-          const uint32_t p = place[r * a.k + j + u];
-          if (p >= end) continue;
-          raw[u] = load_raw(y + p * a.stride + c, a.width - c);
-          w[u] = Weighted ? weights[r * a.k + j + u] : 1.0f;
+          const uint32_t p = j + u < a.k ? static_cast<uint32_t>(place[r * a.k + j + u]) : ~0u;
+          w[u] = p < end ? (Weighted ? weights[r * a.k + j + u] : 1.0f) : 0.0f;
+          if (p < end) {
+            Tile::load(y + p * a.stride, c0, a.width, raw[u]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < I; ++i) raw[u][i] = {};
+          }
         }
 #pragma unroll
         for (int u = 0; u < kTogether; ++u)
 #pragma unroll
-          for (int i = 0; i < V; ++i) sum[i] = __builtin_fmaf(w[u], static_cast<float>(raw[u][i]), sum[i]);
+          for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int q = 0; q < V; ++q) sum[i][q] = __builtin_fmaf(w[u], static_cast<float>(raw[u][i][q]), sum[i][q]);
       }
-      store_piece(out + r * a.width + c, a.width - c, sum);
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        const int64_t c = Tile::column(c0, i);
+        store_piece(out + r * a.width + c, a.width - c, sum[i]);
+      }
     }
 }
 
-// dy and dw of restore.  L lanes a row; each choice's product of two rows is
-// summed over them.
-template <typename T, int L>
+// dy and dw of restore.  The products of grad's row with its choices' rows are
+// summed over the row's lanes.
+template <typename T, int L, int I>
 __global__ __launch_bounds__(kThreads) void restore_grad(RowsArgs a, const T* __restrict__ y,
                                                          const float* __restrict__ weights,
                                                          const int32_t* __restrict__ place,
                                                          const int32_t* __restrict__ offsets,
                                                          const T* __restrict__ grad, T* __restrict__ dy,
                                                          float* __restrict__ dw) {
-  constexpr int V = kPiece<T>, kGroups = kThreads / L;
-  const int lane = threadIdx.x % L;
+  using Tile = ChoiceTile<T, L, I>;
+  constexpr int V = Tile::V, kBatch = kTogether / 2;
   const uint32_t end = kept_rows(a, offsets);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L; r < a.rows; r += step)
-    for (int j = 0; j < a.k; ++j) {
-      const int64_t at = r * a.k + j;
-      const uint32_t p = place[at];
-      const bool kept = p < end;
-      const float w = kept ? weights[at] : 0.0f;
-      float dot = 0.0f;
-      for (int64_t c = lane * V; c < a.width; c += L * V) {
-        float g[V], v[V];
-        load_piece(grad + r * a.other_stride + c, a.width - c, g);
-        if (dw != nullptr && kept) {
-          load_piece(y + p * a.stride + c, a.width - c, v);
+  for (int64_t r = Tile::first_row(); r < a.rows; r += Tile::row_step())
+    for (int j = 0; j < a.k; j += kBatch) {
+      uint32_t p[kBatch];
+      float w[kBatch], dot[kBatch];
 #pragma unroll
-          for (int i = 0; i < V; ++i) dot = __builtin_fmaf(g[i], v[i], dot);
-        }
-        if (dy != nullptr && p < a.choices) {
+      for (int u = 0; u < kBatch; ++u) {
+        p[u] = j + u < a.k ? static_cast<uint32_t>(place[r * a.k + j + u]) : ~0u;
+        w[u] = p[u] < end ? weights[r * a.k + j + u] : 0.0f;
+        dot[u] = 0.0f;
+      }
+      for (int64_t c0 = 0; c0 < a.width; c0 += Tile::kChunk) {
+        piece_t<T> g[I], raw[kBatch][I];
+        Tile::load(grad + r * a.other_stride, c0, a.width, g);
 #pragma unroll
-          for (int i = 0; i < V; ++i) v[i] = kept ? w * g[i] : 0.0f;
-          store_piece(dy + p * a.width + c, a.width - c, v);
+        for (int u = 0; u < kBatch; ++u) {
+          if (dw != nullptr && p[u] < end) {
+            Tile::load(y + p[u] * a.stride, c0, a.width, raw[u]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < I; ++i) raw[u][i] = {};
+          }
         }
+        if (dy != nullptr) {
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u)
+            if (p[u] < a.choices)
+#pragma unroll
+              for (int i = 0; i < I; ++i) {
+                const int64_t c = Tile::column(c0, i);
+                float v[V];
+#pragma unroll
+                for (int q = 0; q < V; ++q) v[q] = p[u] < end ? w[u] * static_cast<float>(g[i][q]) : 0.0f;
+                store_piece(dy + p[u] * a.width + c, a.width - c, v);
+              }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+          for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int q = 0; q < V; ++q)
+              dot[u] = p[u] < end ? __builtin_fmaf(static_cast<float>(g[i][q]), static_cast<float>(raw[u][i][q]), dot[u])
+                                  : 0.0f;
       }
       if (dw == nullptr) continue;
-      dot = lane_sum<L>(dot);
-      if (lane == 0) dw[at] = dot;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const float sum = lane_sum<L>(dot[u]);
+        if (threadIdx.x % L == 0 && j + u < a.k) dw[r * a.k + j + u] = sum;
+      }
     }
 }
 
@@ -181,11 +243,13 @@ RowsArgs rows_args(const spmm_experts_desc* d) {
 
 template <typename T, typename F>
 void with_row(int64_t width, F f) {
+  using std::integral_constant;
   const int64_t pieces = ceil_div(width, kPiece<T>);
-  if (pieces <= 8) f(std::integral_constant<int, 8>());
-  else if (pieces <= 16) f(std::integral_constant<int, 16>());
-  else if (pieces <= 32) f(std::integral_constant<int, 32>());
-  else f(std::integral_constant<int, 64>());
+  if (pieces <= 8) f(integral_constant<int, 8>(), integral_constant<int, 1>());
+  else if (pieces <= 16) f(integral_constant<int, 16>(), integral_constant<int, 1>());
+  else if (pieces <= 32) f(integral_constant<int, 32>(), integral_constant<int, 1>());
+  else if (pieces <= 64) f(integral_constant<int, 64>(), integral_constant<int, 1>());
+  else f(integral_constant<int, 64>(), integral_constant<int, 2>());
 }
 
 template <int L>
@@ -208,8 +272,8 @@ spmm_status run_add(const spmm_experts_desc* d, const void* y, const float* weig
                     const int32_t* offsets, void* out, hipStream_t s) {
   return with_type(d->value_type, [&](auto zero) {
     using T = decltype(zero);
-    with_row<T>(d->width, [&](auto L) {
-      hipLaunchKernelGGL((add_choices<T, decltype(L)::value, Weighted>), row_grid<decltype(L)::value>(d->rows),
+    with_row<T>(d->width, [&](auto L, auto I) {
+      hipLaunchKernelGGL((add_choices<T, decltype(L)::value, decltype(I)::value, Weighted>), row_grid<decltype(L)::value>(d->rows),
                          dim3(kThreads), 0, s, rows_args(d), static_cast<const T*>(y), weights, place, offsets,
                          static_cast<T*>(out));
     });
@@ -244,11 +308,14 @@ spmm_status spmm_expert_plan_run(int32_t index_type, const void* ids, int64_t ch
     return fail(SPMM_ERR_CONTRACT, "ExpertPlan: experts must be int32 or int64");
   if (offsets == nullptr || (choices > 0 && (ids == nullptr || place == nullptr)))
     return fail(SPMM_ERR_INVALID_ARGUMENT, "ExpertPlan: null device pointer");
-  if (workspace == nullptr || workspace_bytes < need)
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(SPMM_ERR_CONTRACT, "ExpertPlan: workspace too small: need " + std::to_string(need) + " bytes");
   const int bins = static_cast<int>(experts) + 1;
-  return sort_digit(Digit{0, bits_of(experts), bins}, choices, ChoiceKeys{ids, index_type == SPMM_INDEX_I64, experts},
-                    static_cast<uint32_t*>(workspace), PutPlace{place}, PutOffsets{offsets}, as_stream(stream));
+  const ChoiceKeys keys = {ids, index_type == SPMM_INDEX_I64, experts};
+  if (choices <= kRankMost)
+    return sort_by_rank(choices, bins, keys, PutPlace{place}, PutOffsets{offsets}, as_stream(stream));
+  return sort_digit(Digit{0, bits_of(experts), bins}, choices, keys, static_cast<uint32_t*>(workspace),
+                    PutPlace{place}, PutOffsets{offsets}, as_stream(stream));
 }
 
 spmm_status spmm_expert_pack_run(const spmm_experts_desc* d, const void* x, const int32_t* place,
@@ -260,8 +327,8 @@ spmm_status spmm_expert_pack_run(const spmm_experts_desc* d, const void* x, cons
     return fail(SPMM_ERR_INVALID_ARGUMENT, "ExpertPlan: null device pointer");
   return with_type(d->value_type, [&](auto zero) {
     using T = decltype(zero);
-    with_row<T>(d->width, [&](auto L) {
-      hipLaunchKernelGGL((pack_choices<T, decltype(L)::value>), row_grid<decltype(L)::value>(d->rows), dim3(kThreads), 0,
+    with_row<T>(d->width, [&](auto L, auto I) {
+      hipLaunchKernelGGL((pack_choices<T, decltype(L)::value, decltype(I)::value>), row_grid<decltype(L)::value>(d->rows), dim3(kThreads), 0,
                          as_stream(stream), rows_args(d), static_cast<const T*>(x), place, offsets,
                          static_cast<T*>(packed));
     });
@@ -301,8 +368,8 @@ spmm_status spmm_expert_restore_grad_run(const spmm_experts_desc* d, const void*
     return fail(SPMM_ERR_INVALID_ARGUMENT, "ExpertPlan: null device pointer");
   return with_type(d->value_type, [&](auto zero) {
     using T = decltype(zero);
-    with_row<T>(d->width, [&](auto L) {
-      hipLaunchKernelGGL((restore_grad<T, decltype(L)::value>), row_grid<decltype(L)::value>(d->rows), dim3(kThreads), 0,
+    with_row<T>(d->width, [&](auto L, auto I) {
+      hipLaunchKernelGGL((restore_grad<T, decltype(L)::value, decltype(I)::value>), row_grid<decltype(L)::value>(d->rows), dim3(kThreads), 0,
                          as_stream(stream), rows_args(d), static_cast<const T*>(y), weights, place, offsets,
                          static_cast<const T*>(grad), static_cast<T*>(dy), dweights);
     });

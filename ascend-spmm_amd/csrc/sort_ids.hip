@@ -1,33 +1,50 @@
-// The part of the counting sort that does not depend on what is sorted.
+// The part of the sort that does not depend on what is sorted.
 #include "sort_ids.h"
 
 namespace spmm {
 namespace {
 
-// One thread a digit: counts of the tiles before, and the sum of all.
-__global__ __launch_bounds__(64) void add_digits(int bins, int64_t tiles, uint32_t* counts, uint32_t* totals) {
-  const int b = blockIdx.x * 64 + threadIdx.x;
-  if (b >= bins) return;
-  uint32_t sum = 0;
-  for (int64_t t = 0; t < tiles; t += 8) {
-    uint32_t c[8];
+// Counts of the tiles before, and the sum of all, for kBins digits a work-group:
+// 16 threads a digit take kTiles tiles each at a time, and hand their sums on.
+constexpr int kBins = 16, kShares = 16, kTiles = 8;
+__global__ __launch_bounds__(kBins * kShares) void add_digits(int bins, int64_t tiles, uint32_t* counts,
+                                                              uint32_t* totals) {
+  __shared__ uint32_t sums[kShares][kBins];
+  const int bin = threadIdx.x % kBins, share = threadIdx.x / kBins, b = blockIdx.x * kBins + bin;
+  uint32_t carry = 0;
+  for (int64_t t0 = 0; t0 < tiles; t0 += kShares * kTiles) {
+    const int64_t t = t0 + share * kTiles;
+    uint32_t c[kTiles], sum = 0;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) c[u] = t + u < tiles ? counts[(t + u) * bins + b] : 0;
+    for (int u = 0; u < kTiles; ++u) {
+      c[u] = b < bins && t + u < tiles ? counts[(t + u) * bins + b] : 0;
+      sum += c[u];
+    }
+    __syncthreads();  // readers of the last sums are done
+    sums[share][bin] = sum;
+    __syncthreads();
+    uint32_t at = carry;
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
-      if (t + u < tiles) {
-        counts[(t + u) * bins + b] = sum;
-        sum += c[u];
+    for (int s = 0; s < kShares; ++s) {
+      const uint32_t v = sums[s][bin];
+      at += s < share ? v : 0;
+      carry += v;
+    }
+#pragma unroll
+    for (int u = 0; u < kTiles; ++u)
+      if (b < bins && t + u < tiles) {
+        counts[(t + u) * bins + b] = at;
+        at += c[u];
       }
   }
-  totals[b] = sum;
+  if (share == 0 && b < bins) totals[b] = carry;
 }
 
 }  // namespace
 
 spmm_status launch_add_digits(int bins, int64_t tiles, uint32_t* counts, uint32_t* totals, hipStream_t s) {
-  hipLaunchKernelGGL(add_digits, dim3(static_cast<unsigned>(ceil_div(bins, 64))), dim3(64), 0, s, bins, tiles, counts,
-                     totals);
+  hipLaunchKernelGGL(add_digits, dim3(static_cast<unsigned>(ceil_div(bins, kBins))), dim3(kBins * kShares), 0, s, bins,
+                     tiles, counts, totals);
   return check_launch("add_digits");
 }
 

@@ -125,7 +125,7 @@ def test_experts_refusals(lib):
         assert text in lib.spmm_last_error()
     for choices, experts in ((0, 1), (1, 2048), (100000, 64)):
         assert lib.spmm_expert_plan_workspace(I64(choices), I64(experts), ctypes.byref(size)) == 0
-        assert 0 < size.value <= 4 * (choices // 4096 + 3) * (experts + 1)
+        assert size.value <= 4 * (choices // 256 + 3) * (experts + 1)
 
     def plan(index=0, ids=FAKE, choices=8, ws=FAKE, size=1 << 20, offsets=FAKE):
         return lib.spmm_expert_plan_run(I32(index), ids, I64(choices), I64(8), offsets, FAKE, ws, ctypes.c_size_t(size),
