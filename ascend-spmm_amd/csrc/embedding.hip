@@ -6,7 +6,7 @@
 // sums are fp32, in the order of the positions, so that they repeat exactly: the
 // ids are sorted (stably) and each run of equal ones is summed.
 #include "lane_reduce.h"
-#include "numeric.h"
+#include "row_pieces.h"
 #include "sort_ids.h"
 
 namespace spmm {
@@ -24,39 +24,51 @@ __device__ inline int64_t id_at(const void* ids, bool index64, int64_t i) {
   return index64 ? static_cast<const int64_t*>(ids)[i] : static_cast<const int32_t*>(ids)[i];
 }
 
-// A group of L lanes takes one row of the output after another, kRows at a time
-// so that their loads are under way together.
+// A group of L lanes takes kRows rows of the output at a time, whose loads are
+// under way together.  Ids outside the table read a row of it all the same (the
+// table has one) and keep nothing of it.
 constexpr int kRows = 4;
-template <typename T, int L>
+template <typename T, int L, bool Narrow>
 __global__ __launch_bounds__(kThreads) void gather_table(TableArgs a, const T* __restrict__ weight,
                                                          const void* __restrict__ ids, T* __restrict__ out) {
+  using Piece = RowPiece<T, Narrow>;
   constexpr int V = kPiece<T>, kGroups = kThreads / L;
-  const int64_t pieces = (a.width + V - 1) / V, step = static_cast<int64_t>(gridDim.x) * kGroups * kRows;
   const int lane = threadIdx.x % L;
-  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L) * kRows; i < a.count; i += step) {
+  int64_t group = static_cast<int64_t>(blockIdx.x) * kGroups;
+  if constexpr (L == 64) group += __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  else group += threadIdx.x / L;
+  for (int64_t i = group * kRows; i < a.count; i += static_cast<int64_t>(gridDim.x) * kGroups * kRows) {
     int64_t id[kRows];
+    bool present[kRows];
 #pragma unroll
-    for (int u = 0; u < kRows; ++u) id[u] = i + u < a.count ? id_at(ids, a.index64, i + u) : -1;
-    for (int64_t p = lane; p < pieces; p += L) {
+    for (int u = 0; u < kRows; ++u) id[u] = id_at(ids, a.index64, i + u < a.count ? i + u : a.count - 1);
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      present[u] = static_cast<uint64_t>(id[u]) < static_cast<uint64_t>(a.table);
+      if (!present[u]) id[u] = 0;
+    }
+    for (int64_t c = lane * V; c < a.width; c += L * V) {
       piece_t<T> raw[kRows];
 #pragma unroll
-      for (int u = 0; u < kRows; ++u) {
-        raw[u] = {};
-        if (static_cast<uint64_t>(id[u]) < static_cast<uint64_t>(a.table))
-          raw[u] = load_raw(weight + id[u] * a.weight_stride + p * V, a.width - p * V);
-      }
+      for (int u = 0; u < kRows; ++u) raw[u] = Piece::load(weight + id[u] * a.weight_stride, c, a.width);
 #pragma unroll
       for (int u = 0; u < kRows; ++u) {
         if (i + u >= a.count) break;
         float v[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          v[j] = static_cast<uint64_t>(id[u]) < static_cast<uint64_t>(a.table) ? static_cast<float>(raw[u][j]) * a.scale
-                                                                               : 0.0f;
-        store_piece(out + (i + u) * a.width + p * V, a.width - p * V, v);
+        for (int j = 0; j < V; ++j) v[j] = present[u] ? static_cast<float>(raw[u][j]) * a.scale : 0.0f;
+        Piece::template store<true>(out + (i + u) * a.width, c, a.width, v);
       }
     }
   }
+}
+
+// An empty table: zeros.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void zero_rows(int64_t n, T* out) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
+       i += static_cast<int64_t>(gridDim.x) * kThreads)
+    out[i] = static_cast<T>(0.0f);
 }
 
 // The keys of the sort: an id, or the table's rows for one outside of it.
@@ -110,19 +122,20 @@ struct SumArgs {
   const uint32_t *keys, *order;
   float* slots;
   uint32_t* runs;  // [0]: runs over several ranges so far; then the range in which each begins
-  int64_t range, ranges, sum_blocks, pieces;
+  int64_t range, ranges, zero_blocks, pieces;
 };
 
-template <typename T, int L>
+template <typename T, int L, bool Narrow>
 __global__ __launch_bounds__(kThreads) void sum_runs(SumArgs s, const T* __restrict__ grad, T* __restrict__ dweight) {
+  using Piece = RowPiece<T, Narrow>;
   constexpr int V = kPiece<T>, kGroups = kThreads / L;
   const TableArgs& a = s.a;
   const int64_t n = a.count;
-  if (static_cast<int64_t>(blockIdx.x) >= s.sum_blocks) {
+  if (static_cast<int64_t>(blockIdx.x) < s.zero_blocks) {
     // Rows of the table that no id names become zero: a wave looks 64 of them up.
     if (blockIdx.y != 0) return;
     const int lane = threadIdx.x & 63;
-    const int64_t first = ((static_cast<int64_t>(blockIdx.x) - s.sum_blocks) * (kThreads / 64) + (threadIdx.x >> 6)) * 64;
+    const int64_t first = (static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6)) * 64;
     const int64_t v = first + lane;
     int64_t lo = 0, hi = n;
     while (lo < hi) {
@@ -131,15 +144,19 @@ __global__ __launch_bounds__(kThreads) void sum_runs(SumArgs s, const T* __restr
       else hi = mid;
     }
     uint64_t absent = __ballot(v < a.table && (lo >= n || s.keys[lo] != v));
-    const float zero[V] = {};
+    const piece_t<T> zero = {};
     while (absent != 0) {
       const int64_t row = first + __builtin_ctzll(absent);
       absent &= absent - 1;
-      for (int64_t c = lane * V; c < a.width; c += 64 * V) store_piece(dweight + row * a.width + c, a.width - c, zero);
+      for (int64_t c = lane * V; c < a.width; c += 64 * V)
+        Piece::template store<true>(dweight + row * a.width, c, a.width, zero);
     }
     return;
   }
-  const int64_t range = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L;
+  const int64_t block = static_cast<int64_t>(blockIdx.x) - s.zero_blocks;
+  int64_t range = block * kGroups;
+  if constexpr (L == 64) range += __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  else range += threadIdx.x / L;
   const int64_t p = static_cast<int64_t>(blockIdx.y) * L + threadIdx.x % L, c = p * V;
   if (range >= s.ranges || p >= s.pieces) return;
   const int64_t begin = range * s.range, end = begin + s.range < n ? begin + s.range : n;
@@ -158,7 +175,7 @@ __global__ __launch_bounds__(kThreads) void sum_runs(SumArgs s, const T* __restr
       float v[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) v[j] = sum[j] * a.scale;
-      store_piece(dweight + static_cast<int64_t>(key) * a.width + c, a.width - c, v);
+      Piece::template store<true>(dweight + static_cast<int64_t>(key) * a.width, c, a.width, v);
     }
   };
   // Keys and positions are read one batch ahead of the rows.
@@ -166,8 +183,8 @@ __global__ __launch_bounds__(kThreads) void sum_runs(SumArgs s, const T* __restr
   auto fetch = [&](int64_t i) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      k[u] = i + u < end ? s.keys[i + u] : static_cast<uint32_t>(a.table);
-      at[u] = i + u < end ? s.order[i + u] : 0;
+      k[u] = s.keys[i + u < end ? i + u : end - 1];
+      at[u] = s.order[i + u < end ? i + u : end - 1];
     }
   };
   fetch(begin);
@@ -176,9 +193,8 @@ __global__ __launch_bounds__(kThreads) void sum_runs(SumArgs s, const T* __restr
     piece_t<T> raw[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      raw[u] = {};
       now[u] = k[u];
-      if (k[u] < a.table) raw[u] = load_raw(grad + static_cast<int64_t>(at[u]) * a.grad_stride + c, a.width - c);
+      raw[u] = Piece::template load<true>(grad + static_cast<int64_t>(at[u]) * a.grad_stride, c, a.width);
     }
     if (i + kBatch < end) fetch(i + kBatch);
 #pragma unroll
@@ -202,7 +218,7 @@ __global__ __launch_bounds__(kThreads) void sum_runs(SumArgs s, const T* __restr
 // pieces of its columns; each wave adds consecutive ranges, the waves are added
 // in order.
 constexpr int kJoinWaves = 16;
-template <typename T>
+template <typename T, bool Narrow>
 __global__ __launch_bounds__(64 * kJoinWaves) void join_runs(SumArgs s, T* __restrict__ dweight) {
   constexpr int V = kPiece<T>;
   __shared__ float part[kJoinWaves][64 * V];
@@ -248,7 +264,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_runs(SumArgs s, T* __res
         for (int w = 0; w < kJoinWaves; ++w) v[j] += part[w][lane * V + j];
         v[j] *= s.a.scale;
       }
-      store_piece(dweight + static_cast<int64_t>(key) * s.a.width + c, s.a.width - c, v);
+      RowPiece<T, Narrow>::store(dweight + static_cast<int64_t>(key) * s.a.width, c, s.a.width, v);
     }
   }
 }
@@ -272,23 +288,33 @@ TableArgs table_args(const spmm_embedding_desc* d) {
           d->index_type == SPMM_INDEX_I64};
 }
 
-// Lanes of a row: one piece of 16 bytes each.
-template <typename F>
-void with_row_lanes(int64_t pieces, F f) {
-  if (pieces <= 4) f(std::integral_constant<int, 4>());
-  else if (pieces <= 8) f(std::integral_constant<int, 8>());
-  else if (pieces <= 16) f(std::integral_constant<int, 16>());
-  else if (pieces <= 32) f(std::integral_constant<int, 32>());
-  else f(std::integral_constant<int, 64>());
+// f(L, Narrow): lanes of a row, one piece of 16 bytes each.
+template <typename T, typename F>
+void with_row_lanes(int64_t width, F f) {
+  using std::integral_constant;
+  const int64_t pieces = ceil_div(width, kPiece<T>);
+  if (width < kPiece<T>) f(integral_constant<int, 4>(), std::true_type());
+  else if (pieces <= 4) f(integral_constant<int, 4>(), std::false_type());
+  else if (pieces <= 8) f(integral_constant<int, 8>(), std::false_type());
+  else if (pieces <= 16) f(integral_constant<int, 16>(), std::false_type());
+  else if (pieces <= 32) f(integral_constant<int, 32>(), std::false_type());
+  else f(integral_constant<int, 64>(), std::false_type());
 }
 
 template <typename T>
 spmm_status run_gather(const spmm_embedding_desc* d, const void* weight, const void* ids, void* out, hipStream_t s) {
-  with_row_lanes(ceil_div(d->width, kPiece<T>), [&](auto L) {
+  if (d->table_rows == 0) {
+    const int64_t n = d->count * d->width, blocks = ceil_div(n, kThreads);
+    hipLaunchKernelGGL(zero_rows<T>, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(kThreads), 0, s, n,
+                       static_cast<T*>(out));
+    return check_launch("embedding");
+  }
+  with_row_lanes<T>(d->width, [&](auto L, auto Narrow) {
     constexpr int kGroups = kThreads / decltype(L)::value;
     const int64_t blocks = ceil_div(d->count, kGroups * kRows);
-    hipLaunchKernelGGL((gather_table<T, decltype(L)::value>), dim3(static_cast<unsigned>(blocks < 16384 ? blocks : 16384)),
-                       dim3(kThreads), 0, s, table_args(d), static_cast<const T*>(weight), ids, static_cast<T*>(out));
+    hipLaunchKernelGGL((gather_table<T, decltype(L)::value, decltype(Narrow)::value>),
+                       dim3(static_cast<unsigned>(blocks < 16384 ? blocks : 16384)), dim3(kThreads), 0, s, table_args(d),
+                       static_cast<const T*>(weight), ids, static_cast<T*>(out));
   });
   return check_launch("embedding");
 }
@@ -349,19 +375,21 @@ spmm_status run_gradient(const spmm_embedding_desc* d, const void* ids, const vo
     order = put.order;
   }
   SumArgs a = {table_args(d), keys, order, reinterpret_cast<float*>(ws + l.slots), runs, l.range, l.ranges, 0, l.pieces};
-  const int64_t zero_blocks = ceil_div(d->table_rows, kThreads);
-  with_row_lanes(l.pieces, [&](auto L) {
-    a.sum_blocks = ceil_div(l.ranges, kThreads / decltype(L)::value);
-    hipLaunchKernelGGL((sum_runs<T, decltype(L)::value>),
-                       dim3(static_cast<unsigned>(a.sum_blocks + zero_blocks),
+  a.zero_blocks = ceil_div(d->table_rows, kThreads);
+  with_row_lanes<T>(d->width, [&](auto L, auto Narrow) {
+    const int64_t sum_blocks = ceil_div(l.ranges, kThreads / decltype(L)::value);
+    hipLaunchKernelGGL((sum_runs<T, decltype(L)::value, decltype(Narrow)::value>),
+                       dim3(static_cast<unsigned>(a.zero_blocks + sum_blocks),
                             static_cast<unsigned>(ceil_div(l.pieces, decltype(L)::value))),
                        dim3(kThreads), 0, s, a, static_cast<const T*>(grad), static_cast<T*>(dweight));
   });
   if (spmm_status st = check_launch("embedding_grad")) return st;
   if (l.ranges < 2) return SPMM_OK;
-  const int64_t groups = l.ranges < 512 ? l.ranges : 512;
-  hipLaunchKernelGGL(join_runs<T>, dim3(static_cast<unsigned>(groups), static_cast<unsigned>(ceil_div(l.pieces, 64))),
-                     dim3(64 * kJoinWaves), 0, s, a, static_cast<T*>(dweight));
+  const dim3 grid(static_cast<unsigned>(l.ranges < 512 ? l.ranges : 512), static_cast<unsigned>(ceil_div(l.pieces, 64)));
+  if (d->width < kPiece<T>)
+    hipLaunchKernelGGL((join_runs<T, true>), grid, dim3(64 * kJoinWaves), 0, s, a, static_cast<T*>(dweight));
+  else
+    hipLaunchKernelGGL((join_runs<T, false>), grid, dim3(64 * kJoinWaves), 0, s, a, static_cast<T*>(dweight));
   return check_launch("embedding_grad join");
 }
 

@@ -11,7 +11,7 @@
 // All four are bound by memory.  They go row by row of the unpacked side, so
 // that x and dout are read once for all k choices and the sums need no atomics.
 #include "lane_reduce.h"
-#include "numeric.h"
+#include "row_pieces.h"
 #include "sort_ids.h"
 
 namespace spmm {
@@ -53,93 +53,99 @@ __device__ inline uint32_t kept_rows(const RowsArgs& a, const int32_t* offsets) 
   return end < 0 ? 0u : end < a.choices ? static_cast<uint32_t>(end) : static_cast<uint32_t>(a.choices);
 }
 
-template <typename T>
-__device__ inline void store_raw(T* p, int64_t n, const piece_t<T>& v) {
-  if (n >= kPiece<T>) {
-    *reinterpret_cast<piece_t<T>*>(p) = v;
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPiece<T>; ++i)
-      if (i < n) p[i] = v[i];
-  }
-}
-
 // The kernels' common walk: L lanes a row, which take L * I pieces of 16 bytes of
 // it at a time, and kTogether choices, whose rows' loads are all under way
-// together.  A whole wave's row is a scalar, and so are the loads of its places
-// and weights.
+// together.  Each group of lanes has consecutive rows.  A whole wave's row is a
+// scalar, and so are the loads of its places and weights.
 constexpr int kTogether = 8;
 
-template <typename T, int L, int I>
+template <typename T, int L, int I, bool Narrow>
 struct ChoiceTile {
+  using Piece = RowPiece<T, Narrow>;
   static constexpr int V = kPiece<T>, kGroups = kThreads / L, kChunk = L * I * V;
 
-  __device__ static inline int64_t first_row() {
+  // Rows [first, last) of the group.
+  __device__ static inline void rows(int64_t all, int64_t& first, int64_t& last) {
     int64_t group = static_cast<int64_t>(blockIdx.x) * kGroups;
     if constexpr (L == 64) group += __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     else group += threadIdx.x / L;
-    return group;
+    const int64_t groups = static_cast<int64_t>(gridDim.x) * kGroups, each = (all + groups - 1) / groups;
+    first = group * each;
+    last = first + each < all ? first + each : all;
   }
-  __device__ static inline int64_t row_step() { return static_cast<int64_t>(gridDim.x) * kGroups; }
   // The first column of the lane's piece i in the chunk from c0 on.
   __device__ static inline int64_t column(int64_t c0, int i) {
     return c0 + static_cast<int64_t>(i * L + threadIdx.x % L) * V;
   }
+  template <bool Once>
   __device__ static inline void load(const T* row, int64_t c0, int64_t width, piece_t<T> (&v)[I]) {
 #pragma unroll
-    for (int i = 0; i < I; ++i) v[i] = load_raw(row + column(c0, i), width - column(c0, i));
+    for (int i = 0; i < I; ++i) v[i] = Piece::template load<Once>(row, column(c0, i), width);
+  }
+  // The packed rows of N choices from j on, ~0 beyond the last.
+  template <int N>
+  __device__ static inline void places(const RowsArgs& a, const int32_t* place, int64_t r, int j, uint32_t (&p)[N]) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) p[u] = static_cast<uint32_t>(place[r * a.k + (j + u < a.k ? j + u : a.k - 1)]);
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      if (j + u >= a.k) p[u] = ~0u;
   }
 };
 
 // packed = x's rows, read once and written k times.
-template <typename T, int L, int I>
+template <typename T, int L, int I, bool Narrow>
 __global__ __launch_bounds__(kThreads) void pack_choices(RowsArgs a, const T* __restrict__ x,
                                                          const int32_t* __restrict__ place,
                                                          const int32_t* __restrict__ offsets, T* __restrict__ packed) {
-  using Tile = ChoiceTile<T, L, I>;
+  using Tile = ChoiceTile<T, L, I, Narrow>;
   const uint32_t end = kept_rows(a, offsets);
-  for (int64_t r = Tile::first_row(); r < a.rows; r += Tile::row_step())
+  int64_t r, last;
+  for (Tile::rows(a.rows, r, last); r < last; ++r)
     for (int64_t c0 = 0; c0 < a.width; c0 += Tile::kChunk) {
       piece_t<T> raw[I];
       const piece_t<T> none = {};
-      Tile::load(x + r * a.stride, c0, a.width, raw);
-      for (int j = 0; j < a.k; ++j) {
-        const uint32_t p = place[r * a.k + j];
-        if (p >= a.choices) continue;
+      Tile::template load<true>(x + r * a.stride, c0, a.width, raw);
+      for (int j = 0; j < a.k; j += kTogether) {
+        uint32_t p[kTogether];
+        Tile::places(a, place, r, j, p);
 #pragma unroll
-        for (int i = 0; i < I; ++i) {
-          const int64_t c = Tile::column(c0, i);
-          store_raw(packed + p * a.width + c, a.width - c, p < end ? raw[i] : none);
+        for (int u = 0; u < kTogether; ++u) {
+          if (p[u] >= a.choices) continue;
+#pragma unroll
+          for (int i = 0; i < I; ++i)
+            Tile::Piece::store(packed + p[u] * a.width, Tile::column(c0, i), a.width, p[u] < end ? raw[i] : none);
         }
       }
     }
 }
 
 // out[r] = sum over its choices of (w or 1) * y[place]: restore, and pack's gradient.
-template <typename T, int L, int I, bool Weighted>
+template <typename T, int L, int I, bool Narrow, bool Weighted>
 __global__ __launch_bounds__(kThreads) void add_choices(RowsArgs a, const T* __restrict__ y,
                                                         const float* __restrict__ weights,
                                                         const int32_t* __restrict__ place,
                                                         const int32_t* __restrict__ offsets, T* __restrict__ out) {
-  using Tile = ChoiceTile<T, L, I>;
+  using Tile = ChoiceTile<T, L, I, Narrow>;
   constexpr int V = Tile::V;
   const uint32_t end = kept_rows(a, offsets);
-  for (int64_t r = Tile::first_row(); r < a.rows; r += Tile::row_step())
+  int64_t r, last;
+  for (Tile::rows(a.rows, r, last); r < last; ++r)
     for (int64_t c0 = 0; c0 < a.width; c0 += Tile::kChunk) {
       float sum[I][V] = {};
       for (int j = 0; j < a.k; j += kTogether) {
         piece_t<T> raw[kTogether][I];
+        uint32_t p[kTogether];
         float w[kTogether];
+        Tile::places(a, place, r, j, p);
+#pragma unroll
+        for (int u = 0; u < kTogether; ++u) w[u] = Weighted ? weights[r * a.k + (j + u < a.k ? j + u : a.k - 1)] : 1.0f;
 #pragma unroll
         for (int u = 0; u < kTogether; ++u) {
-          const uint32_t p = j + u < a.k ? static_cast<uint32_t>(place[r * a.k + j + u]) : ~0u;
-          w[u] = p < end ? (Weighted ? weights[r * a.k + j + u] : 1.0f) : 0.0f;
-          if (p < end) {
-            Tile::load(y + p * a.stride, c0, a.width, raw[u]);
-          } else {
 #pragma unroll
-            for (int i = 0; i < I; ++i) raw[u][i] = {};
-          }
+          for (int i = 0; i < I; ++i) raw[u][i] = {};
+          if (p[u] < end) Tile::template load<true>(y + p[u] * a.stride, c0, a.width, raw[u]);
+          else w[u] = 0.0f;
         }
 #pragma unroll
         for (int u = 0; u < kTogether; ++u)
@@ -149,73 +155,69 @@ __global__ __launch_bounds__(kThreads) void add_choices(RowsArgs a, const T* __r
             for (int q = 0; q < V; ++q) sum[i][q] = __builtin_fmaf(w[u], static_cast<float>(raw[u][i][q]), sum[i][q]);
       }
 #pragma unroll
-      for (int i = 0; i < I; ++i) {
-        const int64_t c = Tile::column(c0, i);
-        store_piece(out + r * a.width + c, a.width - c, sum[i]);
-      }
+      for (int i = 0; i < I; ++i) Tile::Piece::store(out + r * a.width, Tile::column(c0, i), a.width, sum[i]);
     }
 }
 
 // dy and dw of restore.  The products of grad's row with its choices' rows are
 // summed over the row's lanes.
-template <typename T, int L, int I>
+template <typename T, int L, int I, bool Narrow>
 __global__ __launch_bounds__(kThreads) void restore_grad(RowsArgs a, const T* __restrict__ y,
                                                          const float* __restrict__ weights,
                                                          const int32_t* __restrict__ place,
                                                          const int32_t* __restrict__ offsets,
                                                          const T* __restrict__ grad, T* __restrict__ dy,
                                                          float* __restrict__ dw) {
-  using Tile = ChoiceTile<T, L, I>;
+  using Tile = ChoiceTile<T, L, I, Narrow>;
   constexpr int V = Tile::V, kBatch = kTogether / 2;
   const uint32_t end = kept_rows(a, offsets);
-  for (int64_t r = Tile::first_row(); r < a.rows; r += Tile::row_step())
+  int64_t r, last;
+  for (Tile::rows(a.rows, r, last); r < last; ++r)
     for (int j = 0; j < a.k; j += kBatch) {
       uint32_t p[kBatch];
-      float w[kBatch], dot[kBatch];
+      float w[kBatch], dot[kBatch] = {};
+      Tile::places(a, place, r, j, p);
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        p[u] = j + u < a.k ? static_cast<uint32_t>(place[r * a.k + j + u]) : ~0u;
-        w[u] = p[u] < end ? weights[r * a.k + j + u] : 0.0f;
-        dot[u] = 0.0f;
-      }
+      for (int u = 0; u < kBatch; ++u) w[u] = weights[r * a.k + (j + u < a.k ? j + u : a.k - 1)];
       for (int64_t c0 = 0; c0 < a.width; c0 += Tile::kChunk) {
         piece_t<T> g[I], raw[kBatch][I];
-        Tile::load(grad + r * a.other_stride, c0, a.width, g);
+        Tile::template load<false>(grad + r * a.other_stride, c0, a.width, g);
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-          if (dw != nullptr && p[u] < end) {
-            Tile::load(y + p[u] * a.stride, c0, a.width, raw[u]);
-          } else {
 #pragma unroll
-            for (int i = 0; i < I; ++i) raw[u][i] = {};
-          }
+          for (int i = 0; i < I; ++i) raw[u][i] = {};
+          if (dw != nullptr && p[u] < end) Tile::template load<true>(y + p[u] * a.stride, c0, a.width, raw[u]);
         }
         if (dy != nullptr) {
 #pragma unroll
-          for (int u = 0; u < kBatch; ++u)
-            if (p[u] < a.choices)
+          for (int u = 0; u < kBatch; ++u) {
+            if (p[u] >= a.choices) continue;
 #pragma unroll
-              for (int i = 0; i < I; ++i) {
-                const int64_t c = Tile::column(c0, i);
-                float v[V];
+            for (int i = 0; i < I; ++i) {
+              float v[V];
 #pragma unroll
-                for (int q = 0; q < V; ++q) v[q] = p[u] < end ? w[u] * static_cast<float>(g[i][q]) : 0.0f;
-                store_piece(dy + p[u] * a.width + c, a.width - c, v);
-              }
+              for (int q = 0; q < V; ++q) v[q] = p[u] < end ? w[u] * static_cast<float>(g[i][q]) : 0.0f;
+              Tile::Piece::store(dy + p[u] * a.width, Tile::column(c0, i), a.width, v);
+            }
+          }
         }
+        if (dw == nullptr) continue;
+        // A product of a piece that was moved back counts its own elements alone.
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u)
+        for (int i = 0; i < I; ++i) {
+          const int shift = Tile::Piece::shift(Tile::column(c0, i), a.width);
 #pragma unroll
-          for (int i = 0; i < I; ++i)
+          for (int q = 0; q < V; ++q)
 #pragma unroll
-            for (int q = 0; q < V; ++q)
-              dot[u] = p[u] < end ? __builtin_fmaf(static_cast<float>(g[i][q]), static_cast<float>(raw[u][i][q]), dot[u])
-                                  : 0.0f;
+            for (int u = 0; u < kBatch; ++u)
+              dot[u] = q >= shift ? __builtin_fmaf(static_cast<float>(g[i][q]), static_cast<float>(raw[u][i][q]), dot[u])
+                                  : dot[u];
+        }
       }
       if (dw == nullptr) continue;
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        const float sum = lane_sum<L>(dot[u]);
+        const float sum = lane_sum<L>(p[u] < end ? dot[u] : 0.0f);
         if (threadIdx.x % L == 0 && j + u < a.k) dw[r * a.k + j + u] = sum;
       }
     }
@@ -241,21 +243,23 @@ RowsArgs rows_args(const spmm_experts_desc* d) {
           d->rows * d->top_k};
 }
 
+// f(L, I, Narrow) for rows of `width`.
 template <typename T, typename F>
 void with_row(int64_t width, F f) {
   using std::integral_constant;
   const int64_t pieces = ceil_div(width, kPiece<T>);
-  if (pieces <= 8) f(integral_constant<int, 8>(), integral_constant<int, 1>());
-  else if (pieces <= 16) f(integral_constant<int, 16>(), integral_constant<int, 1>());
-  else if (pieces <= 32) f(integral_constant<int, 32>(), integral_constant<int, 1>());
-  else if (pieces <= 64) f(integral_constant<int, 64>(), integral_constant<int, 1>());
-  else f(integral_constant<int, 64>(), integral_constant<int, 2>());
+  if (width < kPiece<T>) f(integral_constant<int, 8>(), integral_constant<int, 1>(), std::true_type());
+  else if (pieces <= 8) f(integral_constant<int, 8>(), integral_constant<int, 1>(), std::false_type());
+  else if (pieces <= 16) f(integral_constant<int, 16>(), integral_constant<int, 1>(), std::false_type());
+  else if (pieces <= 32) f(integral_constant<int, 32>(), integral_constant<int, 1>(), std::false_type());
+  else if (pieces <= 64) f(integral_constant<int, 64>(), integral_constant<int, 1>(), std::false_type());
+  else f(integral_constant<int, 64>(), integral_constant<int, 2>(), std::false_type());
 }
 
 template <int L>
 dim3 row_grid(int64_t rows) {
   const int64_t blocks = ceil_div(rows, kThreads / L);
-  return dim3(static_cast<unsigned>(blocks < 65536 ? blocks : 65536));
+  return dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096));
 }
 
 template <typename F>
@@ -272,8 +276,8 @@ spmm_status run_add(const spmm_experts_desc* d, const void* y, const float* weig
                     const int32_t* offsets, void* out, hipStream_t s) {
   return with_type(d->value_type, [&](auto zero) {
     using T = decltype(zero);
-    with_row<T>(d->width, [&](auto L, auto I) {
-      hipLaunchKernelGGL((add_choices<T, decltype(L)::value, decltype(I)::value, Weighted>), row_grid<decltype(L)::value>(d->rows),
+    with_row<T>(d->width, [&](auto L, auto I, auto Narrow) {
+      hipLaunchKernelGGL((add_choices<T, decltype(L)::value, decltype(I)::value, decltype(Narrow)::value, Weighted>), row_grid<decltype(L)::value>(d->rows),
                          dim3(kThreads), 0, s, rows_args(d), static_cast<const T*>(y), weights, place, offsets,
                          static_cast<T*>(out));
     });
@@ -327,8 +331,8 @@ spmm_status spmm_expert_pack_run(const spmm_experts_desc* d, const void* x, cons
     return fail(SPMM_ERR_INVALID_ARGUMENT, "ExpertPlan: null device pointer");
   return with_type(d->value_type, [&](auto zero) {
     using T = decltype(zero);
-    with_row<T>(d->width, [&](auto L, auto I) {
-      hipLaunchKernelGGL((pack_choices<T, decltype(L)::value, decltype(I)::value>), row_grid<decltype(L)::value>(d->rows), dim3(kThreads), 0,
+    with_row<T>(d->width, [&](auto L, auto I, auto Narrow) {
+      hipLaunchKernelGGL((pack_choices<T, decltype(L)::value, decltype(I)::value, decltype(Narrow)::value>), row_grid<decltype(L)::value>(d->rows), dim3(kThreads), 0,
                          as_stream(stream), rows_args(d), static_cast<const T*>(x), place, offsets,
                          static_cast<T*>(packed));
     });
@@ -368,8 +372,8 @@ spmm_status spmm_expert_restore_grad_run(const spmm_experts_desc* d, const void*
     return fail(SPMM_ERR_INVALID_ARGUMENT, "ExpertPlan: null device pointer");
   return with_type(d->value_type, [&](auto zero) {
     using T = decltype(zero);
-    with_row<T>(d->width, [&](auto L, auto I) {
-      hipLaunchKernelGGL((restore_grad<T, decltype(L)::value, decltype(I)::value>), row_grid<decltype(L)::value>(d->rows), dim3(kThreads), 0,
+    with_row<T>(d->width, [&](auto L, auto I, auto Narrow) {
+      hipLaunchKernelGGL((restore_grad<T, decltype(L)::value, decltype(I)::value, decltype(Narrow)::value>), row_grid<decltype(L)::value>(d->rows), dim3(kThreads), 0,
                          as_stream(stream), rows_args(d), static_cast<const T*>(y), weights, place, offsets,
                          static_cast<const T*>(grad), static_cast<T*>(dy), dweights);
     });

@@ -5,13 +5,17 @@
 //   logp = z_t - ls,   H = ls - sum e^z z / s,
 //   dx_i = a ([i = t] - p_i) - h p_i (log p_i + H),   p_i = e^(z_i - ls),
 // for incoming gradients a of logp and h of H.  H is a sum of two terms of one
-// sign, so it keeps its digits where it is small.  All of it is fp32; a row
-// keeps m and ls apart, as their sum would round |m| / 2^24 off every log p.
+// sign, so it keeps its digits where it is small.
+//
+// All of it is fp32 and in powers of two: y = fma(x, log2(e), -c), c = m log2(e)
+// rounded, rounds once for each logit.  c need not be exact, as every y has the
+// same c: it is taken out again as a whole.  Where c would overflow (|m| above
+// 1e37, so rows of a type's lowest value), y = (x - m) log2(e).
 #include <cfloat>
 #include <cmath>
 
 #include "lane_reduce.h"
-#include "numeric.h"
+#include "row_pieces.h"
 
 namespace spmm {
 namespace {
@@ -21,23 +25,33 @@ constexpr int kWideThreads = 512;
 constexpr int kMaxTop = 64;
 constexpr int kMaxParts = 64;
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kLog2eLow = 1.925963033500011e-08f;  // log2(e) - kLog2e
 constexpr float kLn2 = 0.693147180559945309417f;
+constexpr float kFar = 1e37f;     // of a maximum whose c would not do
+constexpr float kFloor = -300.0f;  // below it 2^y is zero; a finite stand-in for an infinite y
 
-// e^z.  The product with log2(e) rounds, which puts z 2^-24 on the result: 32-bit
-// logits take the rounded part back, those of 16 bits leave it (their results
-// round to 8 or 11 bits, and in s the largest terms have the smallest z).
-template <typename T>
-__device__ inline float exp_of(float z) {
-  const float t = z * kLog2e;
-  const float e = __builtin_amdgcn_exp2f(t);
-  if constexpr (sizeof(T) == 4) {
-    const float low = __builtin_fmaf(z, kLog2eLow, __builtin_fmaf(z, kLog2e, -t));
-    // Where z is infinite or far below, low is no number: e is 0 or infinite by itself.
-    return z > -128.0f && z < 128.0f ? __builtin_fmaf(e, low * kLn2, e) : e;
-  }
-  return e;
+// The product by itself: contracted with a difference of two of them it would
+// leave their rounding, and equal origins would not be equal.
+__device__ inline float origin_of(float m) {
+#pragma clang fp contract(off)
+  return fmaxf(m, -kFar) * kLog2e;
 }
+
+// What the logits of a row are measured from.
+struct Origin {
+  float m, c;
+  bool far;
+  __device__ inline explicit Origin(float max)
+      : m(max), c(origin_of(max)), far(!(fabsf(max) <= kFar)) {}
+  __device__ inline float near(float x) const { return __builtin_fmaf(x, kLog2e, -c); }
+  __device__ inline float operator()(float x) const { return far ? (x - m) * kLog2e : near(x); }
+  // log p of a logit, given log2 s.  So far below the maximum that its y may overflow where its
+  // distance does not (a type's lowest value), it is the distance: log s is nothing against it,
+  // unless it is NaN.
+  __device__ inline float log_p(float x, float ls) const {
+    const float y = (*this)(x);
+    return y < -1e30f ? (x - m) - ls : (y - ls) * kLn2;
+  }
+};
 
 struct LogArgs {
   int64_t rows, classes, stride;
@@ -54,70 +68,89 @@ struct RowOut {
   float* entropy;
   float* top_values;
   int32_t* top_ids;
-  float* stats;  // [rows][2]: m and ls, or null
+  float* stats;  // [rows][2]: m and log2 s, or null
 };
 
-// What a row's m, s and t = sum e^z z say, by one thread.  A row whose logits
-// are all -inf has s = 0: logp -inf, no entropy, and ls = inf, which makes every
-// p of the gradient zero.
-__device__ inline float finish_row(const LogArgs& a, const RowOut& out, int64_t r, int64_t target, float xt, float m,
-                                   float s, float t) {
-  const float ls = s == 0.0f ? INFINITY : logf(s);
+// What a row's maximum, s = sum 2^y and t = sum 2^y y say, by one thread: returns
+// log2 s.  A row whose logits are all -inf has s = 0: logp -inf, no entropy, and
+// an infinite log2 s, which makes every p of the gradient zero.
+__device__ inline float finish_row(const LogArgs& a, const RowOut& out, int64_t r, int64_t target, float xt,
+                                   const Origin& o, float s, float t) {
+  const float ls = s == 0.0f ? INFINITY : log2f(s);
   const bool named = static_cast<uint64_t>(target) < static_cast<uint64_t>(a.classes);
-  out.logp[r] = named ? (s == 0.0f ? -INFINITY : (xt - m) - ls) : 0.0f;
-  out.entropy[r] = s == 0.0f ? 0.0f : ls - t / s;
+  out.logp[r] = named ? (s == 0.0f ? -INFINITY : o.log_p(xt, ls)) : 0.0f;
+  out.entropy[r] = s == 0.0f ? 0.0f : (ls - t / s) * kLn2;
   if (out.stats != nullptr) {
-    out.stats[2 * r] = m;
+    out.stats[2 * r] = o.m;
     out.stats[2 * r + 1] = ls;
   }
   return ls;
 }
 
-__device__ inline float best_value(uint32_t key, float m, float ls) {
-  return key > kKeyOfMinusInf ? (key_value(key) - m) - ls : -INFINITY;
+__device__ inline float best_value(uint32_t key, const Origin& o, float ls) {
+  return key > kKeyOfMinusInf ? o.log_p(key_value(key), ls) : -INFINITY;
 }
 
 // A logit's key among the best classes: NaN is none of them.
 __device__ inline uint32_t class_key(float v) { return v != v ? 0u : order_key(v); }
 
-// The rows that fit the registers of L lanes, I pieces of 16 bytes each.
-template <typename T, int L, int I>
+// The rows that fit the registers of L lanes, I pieces of 16 bytes each.  The
+// next row's loads are under way while a row is summed.
+template <typename T, int L, int I, bool Narrow>
 __global__ __launch_bounds__(kThreads) void log_probs_rows(LogArgs a, const T* __restrict__ x,
                                                            const void* __restrict__ targets, RowOut out) {
+  using Piece = RowPiece<T, Narrow>;
   constexpr int V = kPiece<T>, kGroups = kThreads / L;
   const int lane = threadIdx.x % L;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L; r < a.rows; r += step) {
-    const T* row = x + r * a.stride;
-    float v[I][V];
-    piece_t<T> raw[I];
-    auto column = [&](int i) { return static_cast<int64_t>(i * L + lane) * V; };
+  int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L;
+  if (r >= a.rows) return;
+  piece_t<T> raw[I];
+  int64_t target;
+  float xt;
+  auto column = [&](int i) { return static_cast<int64_t>(i * L + lane) * V; };
+  auto fetch = [&](int64_t row) {
 #pragma unroll
-    for (int i = 0; i < I; ++i) raw[i] = load_raw(row + column(i), a.classes - column(i));
-    const int64_t target = target_of(targets, a.index64, r);
-    const float xt =
-        static_cast<uint64_t>(target) < static_cast<uint64_t>(a.classes) ? static_cast<float>(row[target]) : 0.0f;
-    float m = -FLT_MAX, s = 0.0f, t = 0.0f;
+    for (int i = 0; i < I; ++i) raw[i] = Piece::load(x + row * a.stride, column(i), a.classes);
+    target = target_of(targets, a.index64, row);
+    xt = static_cast<float>(x[row * a.stride + (static_cast<uint64_t>(target) < static_cast<uint64_t>(a.classes) ? target : 0)]);
+  };
+  fetch(r);
+  for (; r < a.rows; r += step) {
+    float v[I][V], m = -INFINITY, s = 0.0f, t = 0.0f;
+    const int64_t mine = target;
+    const float xm = xt;
 #pragma unroll
-    for (int i = 0; i < I; ++i)
+    for (int i = 0; i < I; ++i) {
+      const int64_t first = Narrow ? 0 : Piece::shift(column(i), a.classes), count = Narrow ? a.classes - column(i) : V;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        v[i][j] = column(i) + j < a.classes ? static_cast<float>(raw[i][j]) : -INFINITY;
+        v[i][j] = j >= first && j < count ? static_cast<float>(raw[i][j]) : -INFINITY;
         m = fmaxf(m, v[i][j]);
       }
-    m = lane_max<L>(m);
+    }
+    if (r + step < a.rows) fetch(r + step);
+    const Origin o(fmaxf(lane_max<L>(m), -FLT_MAX));
+    auto add = [&](float y) {
+      const float e = __builtin_amdgcn_exp2f(y);
+      s += e;
+      t = __builtin_fmaf(e, fmaxf(y, kFloor), t);
+    };
+    if (o.far) {
 #pragma unroll
-    for (int i = 0; i < I; ++i)
+      for (int i = 0; i < I; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float z = v[i][j] - m, e = exp_of<T>(z);
-        s += e;
-        t += e * fmaxf(z, -200.0f);  // e is 0 from -104 on
-      }
+        for (int j = 0; j < V; ++j) add((v[i][j] - o.m) * kLog2e);
+    } else {
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) add(o.near(v[i][j]));
+    }
     s = lane_sum<L>(s);
     t = lane_sum<L>(t);
     float ls = 0.0f;
-    if (lane == 0) ls = finish_row(a, out, r, target, xt, m, s, t);
+    if (lane == 0) ls = finish_row(a, out, r, mine, xm, o, s, t);
     if (a.top == 0) continue;
     uint32_t key[I][V];
 #pragma unroll
@@ -132,20 +165,20 @@ __global__ __launch_bounds__(kThreads) void log_probs_rows(LogArgs a, const T* _
         for (int j = 0; j < V; ++j)
           if (key[i][j] > best) {
             best = key[i][j];
-            at = static_cast<uint32_t>(column(i)) + j;
+            at = static_cast<uint32_t>(Piece::begin(column(i), a.classes)) + j;
           }
       // The greatest key, then the lowest index that has it.
       const uint32_t top = lane_max<L>(best);
       const uint32_t win = lane_min<L>(best == top ? at : 0xFFFFFFFFu);
       if (lane == 0) {
-        out.top_values[r * a.top + q] = best_value(top, m, ls);
+        out.top_values[r * a.top + q] = best_value(top, o, ls);
         out.top_ids[r * a.top + q] = top > kKeyOfMinusInf ? static_cast<int32_t>(win) : -1;
       }
 #pragma unroll
       for (int i = 0; i < I; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          if (static_cast<uint32_t>(column(i)) + j == win) key[i][j] = 0;
+          if (static_cast<uint32_t>(Piece::begin(column(i), a.classes)) + j == win) key[i][j] = 0;
     }
   }
 }
@@ -167,6 +200,12 @@ struct Part {
   float m, s, t;
 };
 
+// 2^(y of one origin - y of another): the factor that takes sums from `from` to
+// `to`, and the shift that t takes besides.  Sums from far below vanish.
+__device__ inline float origin_shift(const Origin& from, const Origin& to) {
+  return to.far ? (from.m - to.m) * kLog2e : from.c - to.c;
+}
+
 // Wider rows: a work-group streams one part of a row, each thread with a
 // running maximum and sums relative to it, and joins them at the end.
 //
@@ -183,6 +222,7 @@ template <typename T>
 __global__ __launch_bounds__(kWideThreads) void log_probs_wide(LogArgs a, const T* __restrict__ x,
                                                                const void* __restrict__ targets, RowOut out, int parts,
                                                                Part* part_sums, uint64_t* part_best) {
+  using Piece = RowPiece<T, false>;
   constexpr int V = kPiece<T>, W = kWideThreads / 64, U = 4;
   __shared__ float red[3][W];
   __shared__ uint32_t keys[kWideThreads];
@@ -192,51 +232,74 @@ __global__ __launch_bounds__(kWideThreads) void log_probs_wide(LogArgs a, const 
   const int64_t r = blockIdx.x / static_cast<unsigned>(parts);
   const int part = blockIdx.x % static_cast<unsigned>(parts);
   const T* row = x + r * a.stride;
-  const int64_t pieces = (a.classes + V - 1) / V;
+  const int64_t pieces = (a.classes + V - 1) / V, whole = a.classes / V;
   const int64_t p0 = pieces * part / parts, p1 = pieces * (part + 1) / parts;
   const int tid = threadIdx.x;
 
-  float m = -FLT_MAX, s = 0.0f, t = 0.0f;
-  auto add = [&](const piece_t<T>& raw, int64_t p) {
-    float v[V], top = m;
+  // Sums relative to a maximum no lower than -kFar, so that lower logits alone leave s zero.
+  float m = -INFINITY, s = 0.0f, t = 0.0f;
+  auto add = [&](auto N, const float (&v)[decltype(N)::value]) {
+    float top = m;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      v[j] = p * V + j < a.classes ? static_cast<float>(raw[j]) : -INFINITY;
-      top = fmaxf(top, v[j]);
-    }
-    const float shift = m - top, f = exp_of<T>(shift);
-    t = f * (t + s * fmaxf(shift, -200.0f));
+    for (int j = 0; j < decltype(N)::value; ++j) top = fmaxf(top, v[j]);
+    const float c = origin_of(top), shift = origin_of(m) - c;
+    const float f = __builtin_amdgcn_exp2f(shift);
+    t = f * __builtin_fmaf(s, fmaxf(shift, kFloor), t);
     s *= f;
     m = top;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float z = v[j] - m, e = exp_of<T>(z);
+    for (int j = 0; j < decltype(N)::value; ++j) {
+      const float y = __builtin_fmaf(v[j], kLog2e, -c), e = __builtin_amdgcn_exp2f(y);
       s += e;
-      t += e * fmaxf(z, -200.0f);
+      t = __builtin_fmaf(e, fmaxf(y, kFloor), t);
     }
   };
   int64_t p = p0 + tid;
-  for (; p + (U - 1) * kWideThreads < p1; p += U * kWideThreads) {
+  const int64_t end = p1 < whole ? p1 : whole;
+  for (; p + (U - 1) * kWideThreads < end; p += U * kWideThreads) {
     piece_t<T> raw[U];
+    float v[U * V];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t c = (p + u * kWideThreads) * V;
-      raw[u] = load_raw(row + c, a.classes - c);
-    }
+    for (int u = 0; u < U; ++u) raw[u] = Piece::template load<true>(row, (p + u * kWideThreads) * V, a.classes);
 #pragma unroll
-    for (int u = 0; u < U; ++u) add(raw[u], p + u * kWideThreads);
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[u * V + j] = static_cast<float>(raw[u][j]);
+    add(std::integral_constant<int, U * V>(), v);
   }
-  for (; p < p1; p += kWideThreads) add(load_raw(row + p * V, a.classes - p * V), p);
+  for (; p < p1; p += kWideThreads) {
+    const piece_t<T> raw = Piece::template load<true>(row, p * V, a.classes);
+    const int first = Piece::shift(p * V, a.classes);
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = j >= first ? static_cast<float>(raw[j]) : -INFINITY;
+    add(std::integral_constant<int, V>(), v);
+  }
 
-  const float all = block_max<W>(m, red[0]);
-  const float shift = m - all, f = exp_of<T>(shift);
-  t = lane_sum<64>(f * (t + s * fmaxf(shift, -200.0f)));
-  s = lane_sum<64>(s * f);
+  const Origin o(fmaxf(block_max<W>(m, red[0]), -FLT_MAX));
+  if (o.far) {
+    s = t = 0.0f;
+    for (p = p0 + tid; p < p1; p += kWideThreads) {
+      const piece_t<T> raw = Piece::load(row, p * V, a.classes);
+      const int first = Piece::shift(p * V, a.classes);
+      for (int j = first; j < V; ++j) {
+        const float y = o(static_cast<float>(raw[j])), e = __builtin_amdgcn_exp2f(y);
+        s += e;
+        t = __builtin_fmaf(e, fmaxf(y, kFloor), t);
+      }
+    }
+  } else {
+    const float shift = origin_of(m) - o.c, f = __builtin_amdgcn_exp2f(shift);
+    t = f * __builtin_fmaf(s, fmaxf(shift, kFloor), t);
+    s *= f;
+  }
+  s = lane_sum<64>(s);
+  t = lane_sum<64>(t);
   if ((tid & 63) == 0) {
     red[1][tid >> 6] = s;
     red[2][tid >> 6] = t;
   }
-  const uint32_t own_key = order_key(m);
+  const uint32_t own_key = order_key(fmaxf(m, -FLT_MAX));
   keys[tid] = own_key;
   if (tid == 0) reached = found = 0;
   __syncthreads();
@@ -249,11 +312,11 @@ __global__ __launch_bounds__(kWideThreads) void log_probs_wide(LogArgs a, const 
   float ls = 0.0f;
   if (tid == 0) {
     if (parts > 1) {
-      part_sums[blockIdx.x] = {all, s, t};
+      part_sums[blockIdx.x] = {o.m, s, t};
     } else {
       const int64_t target = target_of(targets, a.index64, r);
       const bool named = static_cast<uint64_t>(target) < static_cast<uint64_t>(a.classes);
-      ls = finish_row(a, out, r, target, named ? static_cast<float>(row[target]) : 0.0f, all, s, t);
+      ls = finish_row(a, out, r, target, named ? static_cast<float>(row[target]) : 0.0f, o, s, t);
     }
   }
   if (a.top == 0) return;
@@ -342,7 +405,7 @@ __global__ __launch_bounds__(kWideThreads) void log_probs_wide(LogArgs a, const 
       part_best[static_cast<int64_t>(blockIdx.x) * a.top + tid] = pair;
     } else {
       const uint32_t key = static_cast<uint32_t>(pair >> 32);
-      out.top_values[r * a.top + tid] = best_value(key, all, ls);
+      out.top_values[r * a.top + tid] = best_value(key, o, ls);
       out.top_ids[r * a.top + tid] =
           key > kKeyOfMinusInf ? static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(pair)) : -1;
     }
@@ -366,15 +429,16 @@ __global__ __launch_bounds__(64) void log_probs_join(LogArgs a, const T* __restr
   const uint64_t* heads = part_best + (r * parts + lane) * a.top;
   int taken = 0;
   uint64_t head = lane < parts && a.top > 0 ? heads[0] : 0;
-  const float m = lane_max<64>(mine.m), shift = mine.m - m, f = exp_of<float>(shift);
-  const float t = lane_sum<64>(f * (mine.t + mine.s * fmaxf(shift, -200.0f))), s = lane_sum<64>(mine.s * f);
+  const Origin o(lane_max<64>(mine.m));
+  const float shift = origin_shift(Origin(mine.m), o), f = __builtin_amdgcn_exp2f(shift);
+  const float t = lane_sum<64>(f * __builtin_fmaf(mine.s, fmaxf(shift, kFloor), mine.t)), s = lane_sum<64>(mine.s * f);
   float ls = 0.0f;
-  if (lane == 0) ls = finish_row(a, out, r, target, xt, m, s, t);
+  if (lane == 0) ls = finish_row(a, out, r, target, xt, o, s, t);
   for (int q = 0; q < a.top; ++q) {
     const uint64_t pair = lane_max_pair<64>(head);
     if (lane == 0) {
       const uint32_t key = static_cast<uint32_t>(pair >> 32);
-      out.top_values[r * a.top + q] = best_value(key, m, ls);
+      out.top_values[r * a.top + q] = best_value(key, o, ls);
       out.top_ids[r * a.top + q] =
           key > kKeyOfMinusInf ? static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(pair)) : -1;
     }
@@ -385,7 +449,7 @@ __global__ __launch_bounds__(64) void log_probs_join(LogArgs a, const T* __restr
 
 // dlogits, each group of L lanes (256: the work-group) walking the pieces
 // [p0, p1) of a row; rows over blockIdx.x, parts of a row over blockIdx.y.
-template <typename T, int L>
+template <typename T, int L, bool Narrow>
 __global__ __launch_bounds__(kThreads) void log_probs_grad(LogArgs a, const T* __restrict__ x,
                                                            const void* __restrict__ targets,
                                                            const float* __restrict__ stats,
@@ -393,29 +457,48 @@ __global__ __launch_bounds__(kThreads) void log_probs_grad(LogArgs a, const T* _
                                                            const float* __restrict__ grad_logp,
                                                            const float* __restrict__ grad_entropy,
                                                            T* __restrict__ dx) {
-  constexpr int V = kPiece<T>, kGroups = kThreads / L;
+  using Piece = RowPiece<T, Narrow>;
+  constexpr int V = kPiece<T>, kGroups = kThreads / L, U = L == 256 ? 4 : 1;
   const int lane = threadIdx.x % L;
   const int64_t pieces = (a.classes + V - 1) / V, step = static_cast<int64_t>(gridDim.x) * kGroups;
   const int64_t p0 = pieces * blockIdx.y / gridDim.y, p1 = pieces * (blockIdx.y + 1) / gridDim.y;
   for (int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L; r < a.rows; r += step) {
     const int64_t target = target_of(targets, a.index64, r);
-    const float m = stats[2 * r], ls = stats[2 * r + 1], H = entropy[r];
+    const Origin o(stats[2 * r]);
+    const float ls = stats[2 * r + 1];
     const bool named = static_cast<uint64_t>(target) < static_cast<uint64_t>(a.classes) && ls != INFINITY;
     const float ga = named && grad_logp != nullptr ? grad_logp[r] : 0.0f;
     const float gh = grad_entropy != nullptr ? grad_entropy[r] : 0.0f;
+    // -(a + h (log p + H)), with log p in powers of two.
+    const float factor = -gh * kLn2, rest = -__builtin_fmaf(gh, entropy[r], ga);
     const T* row = x + r * a.stride;
     T* out = dx + r * a.classes;
-    for (int64_t p = p0 + lane; p < p1; p += L) {
-      const piece_t<T> raw = load_raw(row + p * V, a.classes - p * V);
-      float v[V];
+    auto walk = [&](auto y) {
+      auto piece = [&](int64_t p, const piece_t<T>& raw) {
+        const int64_t c = Piece::begin(p * V, a.classes);
+        float v[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float lp = (static_cast<float>(raw[j]) - m) - ls;
-        v[j] = -exp_of<T>(lp) * (ga + gh * (fmaxf(lp, -200.0f) + H));
-        if (p * V + j == target) v[j] += ga;
+        for (int j = 0; j < V; ++j) {
+          const float lp = y(static_cast<float>(raw[j])) - ls;
+          v[j] = __builtin_amdgcn_exp2f(lp) * __builtin_fmaf(factor, fmaxf(lp, kFloor), rest);
+        }
+        if (static_cast<uint64_t>(target - c) < V)
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] += c + j == target ? ga : 0.0f;
+        Piece::template store<(L == 256)>(out, p * V, a.classes, v);
+      };
+      int64_t p = p0 + lane;
+      for (; p + (U - 1) * L < p1; p += U * L) {
+        piece_t<T> raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = Piece::template load<(L == 256)>(row, (p + u * L) * V, a.classes);
+#pragma unroll
+        for (int u = 0; u < U; ++u) piece(p + u * L, raw[u]);
       }
-      store_piece(out + p * V, a.classes - p * V, v);
-    }
+      for (; p < p1; p += L) piece(p, Piece::load(row, p * V, a.classes));
+    };
+    if (o.far) walk([&](float v) { return (v - o.m) * kLog2e; });
+    else walk([&](float v) { return o.near(v); });
   }
 }
 
@@ -440,13 +523,16 @@ LogArgs log_args(const spmm_log_probs_desc* d) {
   return {d->rows, d->classes, d->logits_stride, static_cast<int32_t>(d->top), d->index_type == SPMM_INDEX_I64};
 }
 
-// Rows that a wave's registers hold, with L and I to match; false where they
-// are wider.
+// f(L, I, Narrow) for rows that a wave's registers hold; false where they are
+// wider.
 template <typename T, typename F>
 bool with_lanes(int64_t classes, F f) {
   const int64_t pieces = ceil_div(classes, kPiece<T>);
+  if (classes < kPiece<T>)
+    return f(std::integral_constant<int, 2>(), std::integral_constant<int, 1>(), std::true_type()), true;
 #define SPMM_TILE(L, I) \
-  if (pieces <= (L) * (I)) return f(std::integral_constant<int, L>(), std::integral_constant<int, I>()), true
+  if (pieces <= (L) * (I)) \
+  return f(std::integral_constant<int, L>(), std::integral_constant<int, I>(), std::false_type()), true
   SPMM_TILE(2, 1);
   SPMM_TILE(4, 1);
   SPMM_TILE(8, 1);
@@ -492,10 +578,10 @@ spmm_status run_forward(const spmm_log_probs_desc* d, const void* logits, const 
                         void* workspace, hipStream_t s) {
   LogArgs a = log_args(d);
   const T* x = static_cast<const T*>(logits);
-  const bool held = with_lanes<T>(d->classes, [&](auto L, auto I) {
+  const bool held = with_lanes<T>(d->classes, [&](auto L, auto I, auto Narrow) {
     const int64_t blocks = ceil_div(d->rows, kThreads / decltype(L)::value);
-    hipLaunchKernelGGL((log_probs_rows<T, decltype(L)::value, decltype(I)::value>),
-                       dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(kThreads), 0, s, a, x, targets,
+    hipLaunchKernelGGL((log_probs_rows<T, decltype(L)::value, decltype(I)::value, decltype(Narrow)::value>),
+                       dim3(static_cast<unsigned>(blocks < 2048 ? blocks : 2048)), dim3(kThreads), 0, s, a, x, targets,
                        out);
   });
   if (held) return check_launch("log_probs");
@@ -524,7 +610,7 @@ spmm_status run_backward(const spmm_log_probs_desc* d, const void* logits, const
                          hipStream_t s) {
   const LogArgs a = log_args(d);
   const int64_t pieces = ceil_div(d->classes, kPiece<T>);
-  auto launch = [&](auto L) {
+  auto launch = [&](auto L, auto Narrow) {
     constexpr int kGroups = kThreads / decltype(L)::value;
     int64_t blocks = ceil_div(d->rows, kGroups);
     // Few rows: in parts of four pieces a lane or more.
@@ -532,15 +618,16 @@ spmm_status run_backward(const spmm_log_probs_desc* d, const void* logits, const
     const int64_t most = ceil_div(pieces, 4 * decltype(L)::value);
     if (parts > most) parts = most;
     if (blocks > 65536) blocks = 65536;
-    hipLaunchKernelGGL((log_probs_grad<T, decltype(L)::value>),
+    hipLaunchKernelGGL((log_probs_grad<T, decltype(L)::value, decltype(Narrow)::value>),
                        dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(parts)), dim3(kThreads), 0, s, a,
                        static_cast<const T*>(logits), targets, stats, entropy, grad_logp, grad_entropy,
                        static_cast<T*>(dlogits));
   };
-  if (pieces <= 4) launch(std::integral_constant<int, 4>());
-  else if (pieces <= 16) launch(std::integral_constant<int, 16>());
-  else if (pieces <= 256) launch(std::integral_constant<int, 64>());
-  else launch(std::integral_constant<int, 256>());
+  if (d->classes < kPiece<T>) launch(std::integral_constant<int, 4>(), std::true_type());
+  else if (pieces <= 4) launch(std::integral_constant<int, 4>(), std::false_type());
+  else if (pieces <= 16) launch(std::integral_constant<int, 16>(), std::false_type());
+  else if (pieces <= 256) launch(std::integral_constant<int, 64>(), std::false_type());
+  else launch(std::integral_constant<int, 256>(), std::false_type());
   return check_launch("log_probs_grad");
 }
 

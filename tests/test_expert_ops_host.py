@@ -127,7 +127,7 @@ def test_experts_refusals(lib):
         assert lib.spmm_expert_plan_workspace(I64(choices), I64(experts), ctypes.byref(size)) == 0
         assert size.value <= 4 * (choices // 256 + 3) * (experts + 1)
 
-    def plan(index=0, ids=FAKE, choices=8, ws=FAKE, size=1 << 20, offsets=FAKE):
+    def plan(index=0, ids=FAKE, choices=5000, ws=FAKE, size=1 << 20, offsets=FAKE):
         return lib.spmm_expert_plan_run(I32(index), ids, I64(choices), I64(8), offsets, FAKE, ws, ctypes.c_size_t(size),
                                         None)
 
