@@ -155,7 +155,7 @@ __global__ __launch_bounds__(kThreads) void add_choices(RowsArgs a, const T* __r
             for (int q = 0; q < V; ++q) sum[i][q] = __builtin_fmaf(w[u], static_cast<float>(raw[u][i][q]), sum[i][q]);
       }
 #pragma unroll
-      for (int i = 0; i < I; ++i) Tile::Piece::store(out + r * a.width, Tile::column(c0, i), a.width, sum[i]);
+      for (int i = 0; i < I; ++i) Tile::Piece::template store<true>(out + r * a.width, Tile::column(c0, i), a.width, sum[i]);
     }
 }
 
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(kThreads) void restore_grad(RowsArgs a, const T* __
               float v[V];
 #pragma unroll
               for (int q = 0; q < V; ++q) v[q] = p[u] < end ? w[u] * static_cast<float>(g[i][q]) : 0.0f;
-              Tile::Piece::store(dy + p[u] * a.width, Tile::column(c0, i), a.width, v);
+              Tile::Piece::template store<true>(dy + p[u] * a.width, Tile::column(c0, i), a.width, v);
             }
           }
         }
@@ -259,7 +259,7 @@ void with_row(int64_t width, F f) {
 template <int L>
 dim3 row_grid(int64_t rows) {
   const int64_t blocks = ceil_div(rows, kThreads / L);
-  return dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096));
+  return dim3(static_cast<unsigned>(blocks < 16384 ? blocks : 16384));
 }
 
 template <typename F>

@@ -17,7 +17,7 @@
 #include <cmath>
 
 #include "lane_reduce.h"
-#include "numeric.h"
+#include "row_pieces.h"
 
 namespace spmm {
 namespace {
@@ -34,177 +34,335 @@ struct RouteArgs {
 
 __device__ inline float log_sigmoid(float x) { return fminf(x, 0.0f) - log1pf(expf(-fabsf(x))); }
 
-// Order of doubles as whole numbers; NaN above all, so that it is chosen and seen.
-__device__ inline uint64_t wide_key(double v) {
+// Order of doubles and floats as whole numbers; NaN above all, so that it is
+// chosen and seen, and zero below all, for what is taken.
+__device__ inline uint64_t key_of(double v) {
   if (v != v) return ~uint64_t(0);
   const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);
   return u ^ (static_cast<uint64_t>(static_cast<int64_t>(u) >> 63) | 0x8000000000000000ull);
 }
+__device__ inline uint32_t key_of(float v) { return v != v ? 0xFFFFFFFFu : order_key(v); }
 constexpr uint64_t kWideMinusInf = 0x000FFFFFFFFFFFFFull;
-__device__ inline uint64_t narrow_key(float v) { return v != v ? 0xFFFFFFFFull : order_key(v); }
+constexpr double kInf64 = __builtin_huge_val();
+constexpr float kLog2e = 1.44269504088896340736f;
 
+// Greatest key over L lanes and the lowest index that has it.  (Names of their
+// own: one more lane_max here would hide those for 32 bits.)
 template <int L>
-__device__ inline double lane_sum64(double v) {
-#pragma unroll
-  for (int d = 1; d < L; d <<= 1) v += __shfl_xor(v, d, L);
-  return v;
+__device__ inline uint32_t best_index(uint32_t own, uint32_t at, uint32_t& best) {
+  best = lane_max<L>(own);
+  return lane_min<L>(own == best ? at : 0xFFFFFFFFu);
+}
+template <int L>
+__device__ inline uint32_t best_index(uint64_t own, uint32_t at, uint64_t& best) {
+  const uint32_t high = lane_max<L>(static_cast<uint32_t>(own >> 32));
+  const uint32_t low = lane_max<L>(static_cast<uint32_t>(own >> 32) == high ? static_cast<uint32_t>(own) : 0u);
+  best = (static_cast<uint64_t>(high) << 32) | low;
+  return lane_min<L>(own == best ? at : 0xFFFFFFFFu);
 }
 
-// Greatest key over L lanes and the lowest index that has it.
+// The two greatest values.
+template <typename F>
+struct BestTwo {
+  F first, second;
+  bool nan;
+  __device__ inline void add(F a, F b) {  // a >= b
+    second = fmax(fmin(first, a), fmax(second, b));
+    first = fmax(first, a);
+  }
+};
+
+// What the lanes of a row share when they look for its open groups: evenly many
+// lanes a group, each of which looks through a part of it.
 template <int L>
-__device__ inline void lane_best(uint64_t& key, uint32_t& at) {
-  const uint32_t own_high = static_cast<uint32_t>(key >> 32), own_low = static_cast<uint32_t>(key);
-  const uint32_t high = lane_max<L>(own_high);
-  const uint32_t low = lane_max<L>(own_high == high ? own_low : 0u);
-  at = lane_min<L>(own_high == high && own_low == low ? at : 0xFFFFFFFFu);
-  key = (static_cast<uint64_t>(high) << 32) | low;
+struct GroupLanes {
+  int each, group, size;
+  __device__ inline explicit GroupLanes(const RouteArgs& a) : each(1), size(a.experts / a.groups) {
+    while (2 * each * a.groups <= L) each *= 2;
+    group = threadIdx.x % L / each;
+  }
+  template <typename F>
+  __device__ inline BestTwo<F> best(const RouteArgs& a, const F* values) const {
+    const F none = -static_cast<F>(INFINITY);
+    BestTwo<F> b = {none, none, false};
+    if (group < a.groups)
+      for (int e = threadIdx.x % each; e < size; e += each) {
+        const F v = values[group * size + e];
+        b.nan |= v != v;
+        b.add(v, none);
+      }
+    for (int d = 1; d < each; d <<= 1) {
+      const F first = __shfl_xor(b.first, d, L), second = __shfl_xor(b.second, d, L);
+      b.nan |= __shfl_xor(static_cast<int>(b.nan), d, L) != 0;
+      b.add(first, second);
+    }
+    return b;
+  }
+  // A bit for each group, from its lanes' answer.
+  __device__ inline uint64_t bits(const RouteArgs& a, bool open) const {
+    const uint64_t all = __ballot(group < a.groups && open) >> (threadIdx.x & 63 & ~(L - 1));
+    if (each == 1) return all;
+    uint64_t found = 0;
+    for (int o = 0; o < a.groups; ++o) found |= ((all >> (o * each)) & 1u) << o;
+    return found;
+  }
+};
+
+// Exact choice of the rows of a wave, in 64 bits: for rows whose choice 32 bits
+// do not decide.  It takes a row's logits and leaves ids[0..k) (-1 where no
+// expert is left); values: `experts` doubles of LDS for each row.  Compact rather
+// than fast: about one row in 2000 of random logits comes here.  Returns whether
+// a softmax's values are no numbers, as a NaN or an infinity is among its logits.
+template <typename T, int L>
+__device__ inline bool choose_exactly(const RouteArgs& a, const T* row, const float* bias, double* values,
+                                            int32_t* ids) {
+  const int lane = threadIdx.x % L;
+  double m = -kInf64, total = 0.0;
+  if (!a.sigmoid) {
+#pragma unroll 1
+    for (int e = lane; e < a.experts; e += L) m = fmax(m, static_cast<double>(static_cast<float>(row[e])));
+    for (int d = 1; d < L; d <<= 1) m = fmax(m, __shfl_xor(m, d, L));
+#pragma unroll 1
+    for (int e = lane; e < a.experts; e += L) {
+      const float x = static_cast<float>(row[e]);
+      if (x != -INFINITY) total += exp(static_cast<double>(x) - m);
+    }
+    for (int d = 1; d < L; d <<= 1) total += __shfl_xor(total, d, L);
+  }
+#pragma unroll 1
+  for (int e = lane; e < a.experts; e += L) {
+    const float x = static_cast<float>(row[e]), b = bias != nullptr ? bias[e] : 0.0f;
+    const double score = a.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x)))
+                                   : exp(static_cast<double>(x) - m) / total;
+    values[e] = x == -INFINITY || b == -INFINITY ? -kInf64 : score + b;
+  }
+  // A wave's LDS accesses are performed in order, and a row's lanes are of one wave.
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  if (a.groups > 1) {
+    const GroupLanes<L> lanes(a);
+    const BestTwo<double> best = lanes.best(a, values);
+    const uint64_t key = best.nan ? ~uint64_t(0) : key_of(best.second == -kInf64 ? best.first : best.first + best.second);
+    int rank = 0;
+    for (int o = 0; o < a.groups; ++o) {
+      const uint64_t other = __shfl(key, o * lanes.each, L);
+      rank += other > key || (other == key && o < lanes.group);
+    }
+    const uint64_t open = lanes.bits(a, rank < a.top_groups);
+#pragma unroll 1
+    for (int e = lane; e < a.experts; e += L)
+      if (!((open >> (e / lanes.size)) & 1u)) values[e] = -kInf64;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+#pragma unroll 1
+  for (int q = 0; q < a.k; ++q) {
+    uint64_t own = 0, best;
+    uint32_t at = 0xFFFFFFFFu;
+#pragma unroll 1
+    for (int e = lane; e < a.experts; e += L) {
+      const uint64_t key = key_of(values[e]);
+      if (key > own) {
+        own = key;
+        at = e;
+      }
+    }
+    const uint32_t win = best_index<L>(own, at, best);
+    if (lane == 0) ids[q] = best > kWideMinusInf ? static_cast<int32_t>(win) : -1;
+    if (best > kWideMinusInf && win % L == static_cast<uint32_t>(lane)) values[win] = -kInf64;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  return total != total;
 }
 
-// L lanes a row, N logits a lane: expert lane + i * L.  Wide: selection values
-// in 64 bits (a bias or groups).
-template <typename T, int L, int N, bool Wide>
-__global__ __launch_bounds__(kThreads) void route_rows(RouteArgs a, const T* __restrict__ logits,
+// How far apart two selection values in 32 bits have to be for their order to be
+// the exact one: a score is off by less than 2^-20 (of sums of up to 1024 terms),
+// a value by its own rounding more; four times that for a pair of group sums.
+__device__ inline float margin_of(float v) { return 0x1p-19f * fmaxf(1.0f, fabsf(v)); }
+
+// L lanes a row, which hold I pieces of 16 bytes of it each.  The k best are taken
+// one after another, each the greatest key of the row's lanes and the lowest index
+// that has it.  Without a bias the logits are the keys, and exact.  With one
+// (Biased) the keys are selection values in 32 bits, and two more than k are
+// taken: where neighbours among them are closer than margin_of, and not of the
+// same logit and bias, or groups are as close, the row's choice is made again in
+// 64 bits.  (All in 64 bits: 132 us for 65536 rows of 256 experts in 8 groups,
+// k = 8; one wave a row 233.)
+template <typename T, int L, int I, bool Narrow, bool Biased, bool Grouped>
+__global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* __restrict__ logits,
                                                        const float* __restrict__ bias, float* __restrict__ weights,
                                                        int32_t* __restrict__ chosen, float* stats) {
-  constexpr int kGroups = kThreads / L;
-  __shared__ double values[Wide ? kGroups * L * N : 1];
+  using Piece = RowPiece<T, Narrow>;
+  constexpr int V = kPiece<T>, kGroups = kThreads / L;
+  constexpr bool kChecked = Biased || Grouped;
+  extern __shared__ double lds[];
+  // The row's values, and its choices' ids and scores.
+  double* exact = lds + (threadIdx.x / L) * a.experts;
+  float* values = reinterpret_cast<float*>(exact);
+  int32_t* ids = reinterpret_cast<int32_t*>(lds + (kChecked ? kGroups * a.experts : 0)) + (threadIdx.x / L) * (2 * a.k + 2);
+  float* scores = reinterpret_cast<float*>(ids + a.k + 2);
   const int lane = threadIdx.x % L;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
-  // All lanes of the work-group take part in every round (barriers).
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * kGroups; r0 < a.rows; r0 += step) {
-    const int64_t r = r0 + threadIdx.x / L;
-    const bool live = r < a.rows;
-    const T* row = logits + (live ? r : 0) * a.stride;
-    float x[N], m = -FLT_MAX;
+  int begin[I], first[I];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      x[i] = lane + i * L < a.experts ? static_cast<float>(row[lane + i * L]) : -INFINITY;
-      m = fmaxf(m, x[i]);
+  for (int i = 0; i < I; ++i) {
+    begin[i] = static_cast<int>(Piece::begin((i * L + lane) * V, a.experts));
+    // Elements before it are another piece's.
+    first[i] = Narrow ? 0 : Piece::shift((i * L + lane) * V, a.experts);
+  }
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L; r < a.rows; r += step) {
+    const T* row = logits + r * a.stride;
+    float x[I][V], m = -FLT_MAX, ls = 0.0f, c = 0.0f, l2s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const piece_t<T> raw = Piece::load(row, (i * L + lane) * V, a.experts);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const bool in = j >= first[i] && (!Narrow || begin[i] + j < a.experts);
+        x[i][j] = in ? static_cast<float>(raw[j]) : -INFINITY;
+        m = fmaxf(m, x[i][j]);
+      }
     }
-    float ls = 0.0f;
-    m = lane_max<L>(m);
-    if (!a.sigmoid) {
+    if (!a.sigmoid && (kChecked || !a.renormalize)) m = lane_max<L>(m);
+    if (!a.sigmoid && !a.renormalize) {
       float s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) s += expf(x[i] - m);
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) s += expf(x[i][j] - m);
       ls = logf(lane_sum<L>(s));
     }
-    uint64_t key[N];
-    if constexpr (Wide) {
-      double v[N], total = 0.0;
+    if (kChecked && !a.sigmoid) {
+      float s = 0.0f;
+      c = m * kLog2e;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const double d = x[i];
-        v[i] = a.sigmoid ? 1.0 / (1.0 + exp(-d)) : exp(d - static_cast<double>(m));
-        total += v[i];
-      }
-      if (!a.sigmoid) {
-        total = lane_sum64<L>(total);
+      for (int i = 0; i < I; ++i)
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] /= total;
-      }
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float b = bias != nullptr && lane + i * L < a.experts ? bias[lane + i * L] : 0.0f;
-        v[i] = x[i] == -INFINITY || b == -INFINITY ? -static_cast<double>(INFINITY) : v[i] + b;
-        key[i] = wide_key(v[i]);
-      }
-      if (a.groups > 1) {
-        // A group's value is the sum of its two greatest: lane g looks through group g.
-        double* mine = values + (threadIdx.x / L) * L * N;
-        const int size = a.experts / a.groups;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (lane + i * L < a.experts) mine[lane + i * L] = v[i];
-        __syncthreads();
-        uint64_t group_key = 0;
-        bool open = false;
-        if (lane < a.groups) {
-          double first = -static_cast<double>(INFINITY), second = first;
-          bool nan = false;
-          for (int e = 0; e < size; ++e) {
-            const double d = mine[lane * size + e];
-            nan |= d != d;
-            if (d > first) {
-              second = first;
-              first = d;
-            } else if (d > second) {
-              second = d;
-            }
-          }
-          group_key = nan ? ~uint64_t(0) : wide_key(first + (second == -static_cast<double>(INFINITY) ? 0.0 : second));
-          if (!nan && first == -static_cast<double>(INFINITY)) group_key = kWideMinusInf;
-        }
-        int rank = 0;
-        for (int g = 0; g < a.groups; ++g) {
-          const uint64_t other = __shfl(group_key, g, L);
-          rank += other > group_key || (other == group_key && g < lane);
-        }
-        open = lane < a.groups && rank < a.top_groups;
-        const uint64_t opened = __ballot(open) >> (threadIdx.x & 63 & ~(L - 1));
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (lane + i * L < a.experts && !((opened >> ((lane + i * L) / size)) & 1u)) key[i] = kWideMinusInf;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) key[i] = narrow_key(x[i]);
+        for (int j = 0; j < V; ++j) s += __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], kLog2e, -c));
+      l2s = __builtin_amdgcn_logf(lane_sum<L>(s));
     }
-    const uint64_t none = Wide ? kWideMinusInf : static_cast<uint64_t>(kKeyOfMinusInf);
-    // Lane j keeps choice j (and j + L, ...): its expert and log score.
-    constexpr int K = (kMaxTopK + L - 1) / L;
-    int32_t ids[K];
-    float score[K], most = -INFINITY;
+    // A score in 32 bits: of the choice alone, not of the weights.
+    auto score = [&](float v) {
+      return a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v * kLog2e))
+                       : __builtin_amdgcn_exp2f(__builtin_fmaf(v, kLog2e, -c) - l2s);
+    };
+    auto selection = [&](float v, float b) { return v == -INFINITY || b == -INFINITY ? -INFINITY : score(v) + b; };
+    float v[I][V];
 #pragma unroll
-    for (int c = 0; c < K; ++c) {
-      ids[c] = -1;
-      score[c] = -INFINITY;
-    }
-    for (int q = 0; q < a.k; ++q) {
-      uint64_t best = 0;
-      uint32_t at = 0;
-      float value = 0.0f;
+    for (int i = 0; i < I; ++i)
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (key[i] > best) {
-          best = key[i];
-          at = lane + i * L;
-          value = x[i];
+      for (int j = 0; j < V; ++j)
+        v[i][j] = Biased ? selection(x[i][j], bias[Narrow && begin[i] + j >= a.experts ? 0 : begin[i] + j]) : x[i][j];
+    uint32_t key[I][V];
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) key[i][j] = key_of(v[i][j]);
+    bool close = false;
+    float seen = 0.0f;
+    if constexpr (Grouped) {
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j >= first[i] && begin[i] + j < a.experts) values[begin[i] + j] = v[i][j];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const GroupLanes<L> lanes(a);
+      const BestTwo<float> best = lanes.best(a, values);
+      // Without a bias the two best logits have the two best scores.
+      const float one = Biased || best.first == -INFINITY ? best.first : score(best.first);
+      const float two = best.second == -INFINITY ? 0.0f : Biased ? best.second : score(best.second);
+      const float sum = best.nan ? NAN : one == -INFINITY ? -INFINITY : one + two;
+      int rank = 0;
+      for (int o = 0; o < a.groups; ++o) {
+        const float other = __shfl(sum, o * lanes.each, L);
+        const bool same = !Biased && __shfl(best.first, o * lanes.each, L) == best.first &&
+                          __shfl(best.second, o * lanes.each, L) == best.second;
+        const bool none = other == -INFINITY && sum == -INFINITY;
+        rank += other > sum || ((same || none) && o < lanes.group);
+        close |= o != lanes.group && lanes.group < a.groups && !same && !none &&
+                 !(fabsf(other - sum) > 4.0f * margin_of(sum));
+      }
+      const uint64_t open = lanes.bits(a, rank < a.top_groups);
+      const float inverse = static_cast<float>(a.groups) / static_cast<float>(a.experts);
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          // The group of an expert: half a step from a border at least, so the product decides it.
+          const int g = static_cast<int>((static_cast<float>(begin[i] + j) + 0.5f) * inverse);
+          if (!((open >> (g & 63)) & 1u)) key[i][j] = 0;
         }
-      const uint32_t own = at;
-      lane_best<L>(best, at);
-      if (best <= none) break;  // no expert is left; the same on all lanes of the row
-      const bool winner = own == at && own % L == static_cast<uint32_t>(lane);
-      // The winner's logit, for all lanes of the row: its order and bits by a maximum.
-      const uint32_t bits = lane_max<L>(winner ? as_bits(value) : 0u);
-      const float xj = as_float(bits);
-      const float l = a.sigmoid ? log_sigmoid(xj) : (xj - m) - ls;
-      most = fmaxf(most, l);
-#pragma unroll
-      for (int c = 0; c < K; ++c)
-        if (q == lane + c * L) {
-          ids[c] = static_cast<int32_t>(at);
-          score[c] = l;
-        }
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (lane + i * L == static_cast<int>(at)) key[i] = 0;
     }
-    float sum = 0.0f;
+    const int rounds = Biased ? (a.k + 2 < a.experts ? a.k + 2 : a.experts) : a.k;
+#pragma unroll 1
+    for (int q = 0; q < rounds; ++q) {
+      uint32_t own = 0, at = 0xFFFFFFFFu, best;
 #pragma unroll
-    for (int c = 0; c < K; ++c) {
-      score[c] = ids[c] < 0 ? 0.0f : expf(a.renormalize ? score[c] - most : score[c]);
-      sum += score[c];
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) own = key[i][j] > own ? key[i][j] : own;
+#pragma unroll
+      for (int i = I - 1; i >= 0; --i)
+#pragma unroll
+        for (int j = V - 1; j >= 0; --j) at = key[i][j] == own ? begin[i] + j : at;
+      const uint32_t win = best_index<L>(own, at, best);
+      if (lane == 0) ids[q] = best > kKeyOfMinusInf ? static_cast<int32_t>(win) : -1;
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        const uint32_t j0 = win - begin[i];
+#pragma unroll
+        for (int j = 0; j < V; ++j) key[i][j] = j0 == static_cast<uint32_t>(j) ? 0 : key[i][j];
+      }
+    }
+    // A wave's LDS accesses are performed in order, and a row's lanes are of one wave.
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if constexpr (Biased) {
+      // Neighbours among the k and the next one have to be clear of each other, or the same.
+      for (int q = lane; q < a.k && q + 1 < rounds; q += L) {
+        const int32_t i = ids[q], j = ids[q + 1];
+        if (j < 0) continue;  // none is left
+        const float vi = selection(static_cast<float>(row[i]), bias[i]);
+        const float vj = selection(static_cast<float>(row[j]), bias[j]);
+        close |= !(vi - vj > margin_of(vi)) && !(row[i] == row[j] && bias[i] == bias[j]);
+      }
+      // Where the last chosen and the next one are the same, one behind them could yet be greater.
+      if (rounds == a.k + 2 && ids[a.k + 1] >= 0) {
+        const int32_t i = ids[a.k - 1], j = ids[a.k], n = ids[a.k + 1];
+        const float vj = selection(static_cast<float>(row[j]), bias[j]);
+        const float vn = selection(static_cast<float>(row[n]), bias[n]);
+        close |= row[i] == row[j] && bias[i] == bias[j] && !(vj - vn > margin_of(vj));
+      }
+    } else if constexpr (Grouped) {
+      // Where logits differ and their scores in 64 bits do not (1, or 0), the scores decide.
+      for (int q = lane; q < a.k; q += L) {
+        const float xq = ids[q] < 0 ? 0.0f : static_cast<float>(row[ids[q]]);
+        close |= ids[q] >= 0 && (a.sigmoid ? !(xq < 30.0f && xq > -700.0f) : !(xq - m > -700.0f));
+      }
+    }
+    if constexpr (kChecked) {
+      // Any row of the wave: all do it, those that were decided with the same result.
+      // With values that are no numbers, the chosen may be others than the NaN: it is to be seen all the same.
+      if (__ballot(close) != 0 && choose_exactly<T, L>(a, row, bias, exact, ids)) seen = NAN;
+    }
+    float most = -INFINITY, sum = 0.0f;
+#pragma unroll 1
+    for (int q = lane; q < a.k; q += L) {
+      const int32_t id = ids[q];
+      const float xj = id < 0 ? 0.0f : static_cast<float>(row[id]);
+      scores[q] = a.sigmoid ? log_sigmoid(xj) : a.renormalize ? xj : (xj - m) - ls;
+      if (id >= 0) most = fmaxf(most, scores[q]);
+    }
+    most = lane_max<L>(most);
+#pragma unroll 1
+    for (int q = lane; q < a.k; q += L) {
+      scores[q] = ids[q] < 0 ? 0.0f : expf(a.renormalize ? scores[q] - most : scores[q]) + seen;
+      sum += scores[q];
     }
     const float over = a.renormalize ? lane_sum<L>(sum) : 1.0f;
-    if (!live) continue;
-#pragma unroll
-    for (int c = 0; c < K; ++c)
-      if (lane + c * L < a.k) {
-        weights[r * a.k + lane + c * L] = ids[c] < 0 ? 0.0f : a.scale * (score[c] / over);
-        chosen[r * a.k + lane + c * L] = ids[c];
-      }
+#pragma unroll 1
+    for (int q = lane; q < a.k; q += L) {
+      weights[r * a.k + q] = ids[q] < 0 ? 0.0f : a.scale * (scores[q] / over);
+      chosen[r * a.k + q] = ids[q];
+    }
     if (stats != nullptr && lane == 0) {
       stats[2 * r] = m;
       stats[2 * r + 1] = ls;
@@ -212,43 +370,55 @@ __global__ __launch_bounds__(kThreads) void route_rows(RouteArgs a, const T* __r
   }
 }
 
-// dlogits of kRowsLds / experts rows a work-group, put together in LDS: what
-// every expert has of it (softmax that is not renormalised), then the chosen.
-constexpr int kRowsLds = 4096;
-template <typename T>
+// dlogits of kTile / experts rows a work-group, put together in LDS: what every
+// expert has of it (softmax that is not renormalised), then the chosen.
+constexpr int kTile = 2048;
+template <typename T, bool Narrow>
 __global__ __launch_bounds__(kThreads) void route_grad(RouteArgs a, const T* __restrict__ logits,
                                                        const int32_t* __restrict__ chosen,
                                                        const float* __restrict__ weights,
                                                        const float* __restrict__ stats, const float* __restrict__ grad,
                                                        T* __restrict__ dlogits) {
-  __shared__ float out[kRowsLds];
-  __shared__ float sums[kRowsLds];  // by row
-  const int tile = kRowsLds / a.experts;
+  using Piece = RowPiece<T, Narrow>;
+  constexpr int V = kPiece<T>;
+  __shared__ float out[kTile + V];
+  __shared__ float parts[kTile], sums[kTile];  // by choice, by row
+  const int tile = kTile / a.experts;
   const bool dense = !a.sigmoid && !a.renormalize;
   for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * tile; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * tile) {
     const int rows = static_cast<int>(a.rows - r0 < tile ? a.rows - r0 : tile);
+    const int choices = rows * a.k, all = rows * a.experts;
+    for (int q = threadIdx.x; q < choices; q += kThreads) {
+      const int64_t at = r0 * a.k + q;
+      const float w = a.renormalize ? weights[at] / a.scale : weights[at], g = grad[at];
+      parts[q] = static_cast<uint32_t>(chosen[at]) < static_cast<uint32_t>(a.experts) ? w * g : 0.0f;
+    }
+    __syncthreads();
     for (int q = threadIdx.x; q < rows; q += kThreads) {
       float sum = 0.0f;
-      for (int j = 0; j < a.k; ++j) {
-        const int64_t at = (r0 + q) * a.k + j;
-        if (static_cast<uint32_t>(chosen[at]) < static_cast<uint32_t>(a.experts))
-          sum += (a.renormalize ? weights[at] / a.scale : weights[at]) * grad[at];
-      }
+      for (int j = 0; j < a.k; ++j) sum += parts[q * a.k + j];
       sums[q] = sum;
     }
+    if (!dense)
+      for (int q = threadIdx.x * 4; q < all; q += kThreads * 4) *reinterpret_cast<f32x4*>(out + q) = f32x4{};
     __syncthreads();
-    for (int q = threadIdx.x; q < rows * a.experts; q += kThreads) {
-      float v = 0.0f;
-      if (dense) {
-        const int row = q / a.experts;
-        const float x = static_cast<float>(logits[(r0 + row) * a.stride + (q - row * a.experts)]);
-        const float p = expf((x - stats[2 * (r0 + row)]) - stats[2 * (r0 + row) + 1]);
-        v = x == -INFINITY ? 0.0f : -p * sums[row];
+    if (dense) {
+      const int pieces = (a.experts + V - 1) / V;
+      for (int q = threadIdx.x; q < rows * pieces; q += kThreads) {
+        const int row = q / pieces, column = (q - row * pieces) * V;
+        const piece_t<T> raw = Piece::load(logits + (r0 + row) * a.stride, column, a.experts);
+        const int begin = static_cast<int>(Piece::begin(column, a.experts));
+        const float m = stats[2 * (r0 + row)], ls = stats[2 * (r0 + row) + 1], sum = sums[row];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (Narrow && column + j >= a.experts) break;
+          const float x = static_cast<float>(raw[j]);
+          out[row * a.experts + begin + j] = x == -INFINITY ? 0.0f : -expf((x - m) - ls) * sum;
+        }
       }
-      out[q] = v;
+      __syncthreads();
     }
-    __syncthreads();
-    for (int q = threadIdx.x; q < rows * a.k; q += kThreads) {
+    for (int q = threadIdx.x; q < choices; q += kThreads) {
       const int64_t at = r0 * a.k + q;
       const int32_t e = chosen[at];
       if (static_cast<uint32_t>(e) >= static_cast<uint32_t>(a.experts)) continue;
@@ -260,7 +430,12 @@ __global__ __launch_bounds__(kThreads) void route_grad(RouteArgs a, const T* __r
       out[row * a.experts + e] += v;
     }
     __syncthreads();
-    for (int q = threadIdx.x; q < rows * a.experts; q += kThreads) dlogits[r0 * a.experts + q] = static_cast<T>(out[q]);
+    for (int q = threadIdx.x * V; q < all; q += kThreads * V) {
+      float v[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = out[q + j];
+      store_piece(dlogits + r0 * a.experts + q, all - q, v);
+    }
     __syncthreads();
   }
 }
@@ -305,24 +480,48 @@ template <typename T>
 spmm_status run_route(const spmm_route_desc* d, const void* logits, const float* bias, float* weights, int32_t* chosen,
                       float* stats, hipStream_t s) {
   const RouteArgs a = route_args(d);
-  auto launch = [&](auto L, auto N) {
+  auto launch = [&](auto L, auto I, auto Narrow) {
     constexpr int kGroups = kThreads / decltype(L)::value;
     const int64_t blocks = ceil_div(d->rows, kGroups);
     const dim3 grid(static_cast<unsigned>(blocks < 16384 ? blocks : 16384));
-    if (bias != nullptr || d->groups > 1)
-      hipLaunchKernelGGL((route_rows<T, decltype(L)::value, decltype(N)::value, true>), grid, dim3(kThreads), 0, s, a,
-                         static_cast<const T*>(logits), bias, weights, chosen, stats);
+    const size_t values = bias != nullptr || a.groups > 1 ? static_cast<size_t>(a.experts) * 8 : 0;
+    const size_t lds = kGroups * (values + (2 * static_cast<size_t>(a.k) + 2) * 4);
+    const T* x = static_cast<const T*>(logits);
+    constexpr int kL = decltype(L)::value, kI = decltype(I)::value;
+    constexpr bool kNarrow = decltype(Narrow)::value;
+    if (bias != nullptr && a.groups > 1)
+      hipLaunchKernelGGL((route_rows<T, kL, kI, kNarrow, true, true>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
+                         chosen, stats);
+    else if (bias != nullptr)
+      hipLaunchKernelGGL((route_rows<T, kL, kI, kNarrow, true, false>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
+                         chosen, stats);
+    else if (a.groups > 1)
+      hipLaunchKernelGGL((route_rows<T, kL, kI, kNarrow, false, true>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
+                         chosen, stats);
     else
-      hipLaunchKernelGGL((route_rows<T, decltype(L)::value, decltype(N)::value, false>), grid, dim3(kThreads), 0, s, a,
-                         static_cast<const T*>(logits), bias, weights, chosen, stats);
+      hipLaunchKernelGGL((route_rows<T, kL, kI, kNarrow, false, false>), grid, dim3(kThreads), lds, s, a, x, bias,
+                         weights, chosen, stats);
   };
   using std::integral_constant;
-  // Groups are looked through by a lane each, 64 at most.
-  if (d->experts <= 16 && d->groups <= 16) launch(integral_constant<int, 16>(), integral_constant<int, 1>());
-  else if (d->experts <= 64 && d->groups <= 16) launch(integral_constant<int, 16>(), integral_constant<int, 4>());
-  else if (d->experts <= 64) launch(integral_constant<int, 64>(), integral_constant<int, 1>());
-  else if (d->experts <= 256) launch(integral_constant<int, 64>(), integral_constant<int, 4>());
-  else launch(integral_constant<int, 64>(), integral_constant<int, 16>());
+  constexpr int V = kPiece<T>;
+  const int64_t pieces = ceil_div(d->experts, V);
+  // A lane a group at least.
+  if (d->experts < V && d->groups <= 4)
+    launch(integral_constant<int, 4>(), integral_constant<int, 1>(), std::true_type());
+  else if (d->experts < V)
+    launch(integral_constant<int, 8>(), integral_constant<int, 1>(), std::true_type());
+  else if (pieces <= 4 && d->groups <= 4)
+    launch(integral_constant<int, 4>(), integral_constant<int, 1>(), std::false_type());
+  else if (pieces <= 8 && d->groups <= 8)
+    launch(integral_constant<int, 8>(), integral_constant<int, 1>(), std::false_type());
+  else if (pieces <= 16 && d->groups <= 16)
+    launch(integral_constant<int, 16>(), integral_constant<int, 1>(), std::false_type());
+  else if (pieces <= 16 * (16 / V) && d->groups <= 16)
+    launch(integral_constant<int, 16>(), integral_constant<int, 16 / V>(), std::false_type());
+  else if (pieces <= 64)
+    launch(integral_constant<int, 64>(), integral_constant<int, 1>(), std::false_type());
+  else
+    launch(integral_constant<int, 64>(), integral_constant<int, 16 / V>(), std::false_type());
   return check_launch("route");
 }
 
@@ -330,9 +529,14 @@ template <typename T>
 spmm_status run_route_grad(const spmm_route_desc* d, const void* logits, const int32_t* chosen, const float* weights,
                            const float* stats, const float* grad, void* dlogits, hipStream_t s) {
   const RouteArgs a = route_args(d);
-  const int64_t blocks = ceil_div(d->rows, kRowsLds / d->experts);
-  hipLaunchKernelGGL(route_grad<T>, dim3(static_cast<unsigned>(blocks < 65536 ? blocks : 65536)), dim3(kThreads), 0, s,
-                     a, static_cast<const T*>(logits), chosen, weights, stats, grad, static_cast<T*>(dlogits));
+  const int64_t blocks = ceil_div(d->rows, kTile / d->experts);
+  const dim3 grid(static_cast<unsigned>(blocks < 16384 ? blocks : 16384));
+  if (d->experts < kPiece<T>)
+    hipLaunchKernelGGL((route_grad<T, true>), grid, dim3(kThreads), 0, s, a, static_cast<const T*>(logits), chosen,
+                       weights, stats, grad, static_cast<T*>(dlogits));
+  else
+    hipLaunchKernelGGL((route_grad<T, false>), grid, dim3(kThreads), 0, s, a, static_cast<const T*>(logits), chosen,
+                       weights, stats, grad, static_cast<T*>(dlogits));
   return check_launch("route_grad");
 }
 

@@ -54,7 +54,9 @@ __device__ inline void count_tile(uint32_t* hist, Digit d, int64_t n, int rounds
   __syncthreads();
 }
 
-// counts: [tiles][bins].  keys(i) gives key i.
+// counts: [tiles][bins].  keys(i) gives key i.  (Counting the next digit in
+// place_digits, by atomics, costs more than this launch: 10.4 and 22.9 us for
+// 6.6 + 2.7 and 9.2 + 4.8.)
 template <typename Keys>
 __global__ __launch_bounds__(kSortThreads) void count_digits(Digit d, int64_t n, int rounds, Keys keys,
                                                              uint32_t* counts) {

@@ -4,9 +4,9 @@
 namespace spmm {
 namespace {
 
-// Counts of the tiles before, and the sum of all, for kBins digits a work-group:
-// 16 threads a digit take kTiles tiles each at a time, and hand their sums on.
-constexpr int kBins = 16, kShares = 16, kTiles = 8;
+// Counts of the tiles before, and the sum of all, for kBins digits (a cache line)
+// a work-group: kShares threads a digit take kTiles tiles each at a time.
+constexpr int kBins = 32, kShares = 32, kTiles = 8;
 __global__ __launch_bounds__(kBins * kShares) void add_digits(int bins, int64_t tiles, uint32_t* counts,
                                                               uint32_t* totals) {
   __shared__ uint32_t sums[kShares][kBins];
@@ -14,14 +14,13 @@ __global__ __launch_bounds__(kBins * kShares) void add_digits(int bins, int64_t 
   uint32_t carry = 0;
   for (int64_t t0 = 0; t0 < tiles; t0 += kShares * kTiles) {
     const int64_t t = t0 + share * kTiles;
-    uint32_t c[kTiles], sum = 0;
+    uint32_t c[kTiles], own = 0;
 #pragma unroll
-    for (int u = 0; u < kTiles; ++u) {
-      c[u] = b < bins && t + u < tiles ? counts[(t + u) * bins + b] : 0;
-      sum += c[u];
-    }
+    for (int u = 0; u < kTiles; ++u) c[u] = b < bins && t + u < tiles ? counts[(t + u) * bins + b] : 0;
+#pragma unroll
+    for (int u = 0; u < kTiles; ++u) own += c[u];
     __syncthreads();  // readers of the last sums are done
-    sums[share][bin] = sum;
+    sums[share][bin] = own;
     __syncthreads();
     uint32_t at = carry;
 #pragma unroll

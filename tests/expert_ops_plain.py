@@ -147,6 +147,28 @@ def choose(x, top_k, score, bias, groups, top_groups):
     return torch.from_numpy(out)
 
 
+def undecided(x, score, bias, groups, top_groups):
+    """Rows in which two groups at the border of the choice have sums within
+    2^-50 of each other.  Such a sum is of four numbers, s_i + b_i and s_j + b_j:
+    where another group has the same scores with the biases exchanged, the two
+    are equal, and each is off by up to four roundings of 2^-53 of at most its
+    size (two additions, their sum, the scores' own): 64 bits leave either
+    first."""
+    if groups == 1:
+        return torch.zeros(x.size(0), dtype=torch.bool)
+    v = x.double().cpu()
+    v = torch.softmax(v, 1) if score == "softmax" else torch.sigmoid(v)
+    v = v if bias is None else v + bias.double().cpu()
+    v = torch.where(x.cpu() == -INF, torch.full_like(v, -INF), v)
+    two = v.view(x.size(0), groups, -1).sort(2, descending=True).values[:, :, :2]
+    total = torch.where(two == -INF, torch.zeros_like(two), two).sum(2)
+    total = total.sort(1, descending=True).values
+    if top_groups == groups:
+        return torch.zeros(x.size(0), dtype=torch.bool)
+    gap = total[:, top_groups - 1] - total[:, top_groups]
+    return gap <= 2.0 ** -50 * total[:, 0].abs().clamp_min(1.0)
+
+
 def route(x, chosen, score, renormalize, scale, g=None):
     """Weights of the chosen experts, their bound, and (with the incoming
     gradient g) dx and its bound, in 64 bits."""
