@@ -56,6 +56,11 @@ __device__ inline float lane_max(float v) {
       lane_reduce<L>(as_bits(v), [](uint32_t a, uint32_t b) { return as_bits(fmaxf(as_float(a), as_float(b))); }));
 }
 template <int L>
+__device__ inline float lane_min_value(float v) {
+  return as_float(
+      lane_reduce<L>(as_bits(v), [](uint32_t a, uint32_t b) { return as_bits(fminf(as_float(a), as_float(b))); }));
+}
+template <int L>
 __device__ inline uint32_t lane_max(uint32_t v) {
   return lane_reduce<L>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }

@@ -46,13 +46,6 @@ constexpr uint64_t kWideMinusInf = 0x000FFFFFFFFFFFFFull;
 constexpr double kInf64 = __builtin_huge_val();
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// Greatest key over L lanes and the lowest index that has it.  (Names of their
-// own: one more lane_max here would hide those for 32 bits.)
-template <int L>
-__device__ inline uint32_t best_index(uint32_t own, uint32_t at, uint32_t& best) {
-  best = lane_max<L>(own);
-  return lane_min<L>(own == best ? at : 0xFFFFFFFFu);
-}
 template <int L>
 __device__ inline uint32_t best_index(uint64_t own, uint32_t at, uint64_t& best) {
   const uint32_t high = lane_max<L>(static_cast<uint32_t>(own >> 32));
@@ -119,17 +112,17 @@ __device__ inline bool choose_exactly(const RouteArgs& a, const T* row, const fl
   const int lane = threadIdx.x % L;
   double m = -kInf64, total = 0.0;
   if (!a.sigmoid) {
-#pragma unroll 1
+#pragma unroll 2
     for (int e = lane; e < a.experts; e += L) m = fmax(m, static_cast<double>(static_cast<float>(row[e])));
     for (int d = 1; d < L; d <<= 1) m = fmax(m, __shfl_xor(m, d, L));
-#pragma unroll 1
+#pragma unroll 2
     for (int e = lane; e < a.experts; e += L) {
       const float x = static_cast<float>(row[e]);
       if (x != -INFINITY) total += exp(static_cast<double>(x) - m);
     }
     for (int d = 1; d < L; d <<= 1) total += __shfl_xor(total, d, L);
   }
-#pragma unroll 1
+#pragma unroll 2
   for (int e = lane; e < a.experts; e += L) {
     const float x = static_cast<float>(row[e]), b = bias != nullptr ? bias[e] : 0.0f;
     const double score = a.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x)))
@@ -148,7 +141,7 @@ __device__ inline bool choose_exactly(const RouteArgs& a, const T* row, const fl
       rank += other > key || (other == key && o < lanes.group);
     }
     const uint64_t open = lanes.bits(a, rank < a.top_groups);
-#pragma unroll 1
+#pragma unroll 2
     for (int e = lane; e < a.experts; e += L)
       if (!((open >> (e / lanes.size)) & 1u)) values[e] = -kInf64;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -157,7 +150,7 @@ __device__ inline bool choose_exactly(const RouteArgs& a, const T* row, const fl
   for (int q = 0; q < a.k; ++q) {
     uint64_t own = 0, best;
     uint32_t at = 0xFFFFFFFFu;
-#pragma unroll 1
+#pragma unroll 2
     for (int e = lane; e < a.experts; e += L) {
       const uint64_t key = key_of(values[e]);
       if (key > own) {
@@ -174,25 +167,49 @@ __device__ inline bool choose_exactly(const RouteArgs& a, const T* row, const fl
 }
 
 // How far apart two selection values in 32 bits have to be for their order to be
-// the exact one: a score is off by less than 2^-20 (of sums of up to 1024 terms),
-// a value by its own rounding more; four times that for a pair of group sums.
-__device__ inline float margin_of(float v) { return 0x1p-19f * fmaxf(1.0f, fabsf(v)); }
+// the exact one.  With e = 2^-24: 2^y has a relative error of 1.25 |y ln 2| e + 2 e.
+// A sigmoid s = 1 / (1 + 2^y) is then off by s (1 - s) times that (at most 0.8 e)
+// and 3 e for its two roundings, a softmax p by p (1.25 |z| + H + 16) e with
+// p |z| < 0.4 and an entropy H of at most 7, 24 e in all; the sum with the bias
+// rounds by e |v|.  Twice that is below 2^-20 and 2^-18 of max(1, |v|); a pair of
+// group sums has twice as much again.
+__device__ inline float margin_of(const RouteArgs& a, float v) {
+  return (a.sigmoid ? 0x1p-20f : 0x1p-18f) * fmaxf(1.0f, fabsf(v));
+}
+
+// Rows of whole pieces; rows whose last piece is moved back to end with them;
+// rows narrower than a piece.
+enum class RowShape { kWhole, kMoved, kNarrow };
+
+// The keys in which a row's best are found, the greatest first and of equal ones
+// the lowest index.  kPacked: value and index in one word, so that a maximum
+// finds both.
+//  - logits of 16 bits: the upper 19 bits of their order hold all of them, 13 are
+//    left for the index;
+//  - values with a bias: steps of 2^-22 of the row's range (which margin_of's
+//    check counts in), and 10 bits for the index.
+// Logits of 32 bits without a bias take a word for the value alone, and the index
+// is looked for.
+constexpr uint32_t kFine = 0x1FFF, kCoarse = 0x3FF;
+constexpr float kSteps = 4194300.0f;  // below 2^22
 
 // L lanes a row, which hold I pieces of 16 bytes of it each.  The k best are taken
-// one after another, each the greatest key of the row's lanes and the lowest index
-// that has it.  Without a bias the logits are the keys, and exact.  With one
+// one after another.  Without a bias the logits are the keys, and exact.  With one
 // (Biased) the keys are selection values in 32 bits, and two more than k are
 // taken: where neighbours among them are closer than margin_of, and not of the
-// same logit and bias, or groups are as close, the row's choice is made again in
-// 64 bits.  (All in 64 bits: 132 us for 65536 rows of 256 experts in 8 groups,
-// k = 8; one wave a row 233.)
-template <typename T, int L, int I, bool Narrow, bool Biased, bool Grouped>
+// same logit and bias, or the groups at the border are as close, the row's choice
+// is made again in 64 bits.  Bound by vector instructions, most of them of the k
+// rounds.  65536 rows of 256 experts in 8 groups, k = 8: all in 64 bits 132 us,
+// one wave a row 233, value and index apart 113.
+template <typename T, int L, int I, RowShape Shape, bool Biased, bool Grouped>
 __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* __restrict__ logits,
                                                        const float* __restrict__ bias, float* __restrict__ weights,
                                                        int32_t* __restrict__ chosen, float* stats) {
+  constexpr bool Narrow = Shape == RowShape::kNarrow, Whole = Shape == RowShape::kWhole;
   using Piece = RowPiece<T, Narrow>;
   constexpr int V = kPiece<T>, kGroups = kThreads / L;
-  constexpr bool kChecked = Biased || Grouped;
+  constexpr bool kChecked = Biased || Grouped, kPacked = Biased || sizeof(T) == 2;
+  constexpr uint32_t kIndex = Biased ? kCoarse : kFine, kNone = Biased ? kCoarse : kKeyOfMinusInf;
   extern __shared__ double lds[];
   // The row's values, and its choices' ids and scores.
   double* exact = lds + (threadIdx.x / L) * a.experts;
@@ -203,85 +220,171 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
   int begin[I], first[I];
 #pragma unroll
   for (int i = 0; i < I; ++i) {
-    begin[i] = static_cast<int>(Piece::begin((i * L + lane) * V, a.experts));
-    // Elements before it are another piece's.
-    first[i] = Narrow ? 0 : Piece::shift((i * L + lane) * V, a.experts);
+    const int column = (i * L + lane) * V;
+    begin[i] = Whole ? column : static_cast<int>(Piece::begin(column, a.experts));
+    // Elements before it are another piece's, or past the row.
+    first[i] = Narrow ? 0 : Whole ? (column < a.experts ? 0 : V) : Piece::shift(column, a.experts);
   }
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L; r < a.rows; r += step) {
-    const T* row = logits + r * a.stride;
-    float x[I][V], m = -FLT_MAX, ls = 0.0f, c = 0.0f, l2s = 0.0f;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L;
+  if (r >= a.rows) return;
+  const T* row = logits + r * a.stride;
+  float x[I][V], m = -FLT_MAX, ls = 0.0f, c = 0.0f, l2s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < I; ++i) {
-      const piece_t<T> raw = Piece::load(row, (i * L + lane) * V, a.experts);
+  for (int i = 0; i < I; ++i) {
+    const piece_t<T> raw = Piece::load(row, (i * L + lane) * V, a.experts);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const bool in = Whole ? first[i] == 0 : j >= first[i] && (!Narrow || begin[i] + j < a.experts);
+      x[i][j] = in ? static_cast<float>(raw[j]) : -INFINITY;
+      m = fmaxf(m, x[i][j]);
+    }
+  }
+  if (!a.sigmoid && (kChecked || !a.renormalize)) m = lane_max<L>(m);
+  if (!a.sigmoid && !a.renormalize) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += expf(x[i][j] - m);
+    ls = logf(lane_sum<L>(s));
+  }
+  if (kChecked && !a.sigmoid) {
+    float s = 0.0f;
+    c = m * kLog2e;
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], kLog2e, -c));
+    l2s = __builtin_amdgcn_logf(lane_sum<L>(s));
+  }
+  // A score in 32 bits: of the choice alone, not of the weights.
+  auto sigmoid = [&](float v) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v * kLog2e)); };
+  auto softmax = [&](float v) { return __builtin_amdgcn_exp2f(__builtin_fmaf(v, kLog2e, -c) - l2s); };
+  auto score = [&](float v) { return a.sigmoid ? sigmoid(v) : softmax(v); };
+  auto selected = [&](float s, float v, float b) { return v == -INFINITY || b == -INFINITY ? -INFINITY : s + b; };
+  auto selection = [&](float v, float b) { return selected(score(v), v, b); };
+  float v[I][V], least = INFINITY, most = -INFINITY;
+  bool close = false;
+  float seen = 0.0f;
+  if constexpr (Biased) {
+    float b[I][V];
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; j += 4) {
+        if constexpr (Narrow) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) b[i][j + u] = bias[begin[i] + j + u < a.experts ? begin[i] + j + u : 0];
+        } else {
+          const piece_t<float> four = *reinterpret_cast<const piece_t<float>*>(bias + (Whole && first[i] != 0 ? 0 : begin[i]) + j);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) b[i][j + u] = four[u];
+        }
+      }
+    if (a.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i][j] = sigmoid(x[i][j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i][j] = softmax(x[i][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < I; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const bool in = j >= first[i] && (!Narrow || begin[i] + j < a.experts);
-        x[i][j] = in ? static_cast<float>(raw[j]) : -INFINITY;
-        m = fmaxf(m, x[i][j]);
+        v[i][j] = selected(v[i][j], x[i][j], b[i][j]);
+        close |= v[i][j] != v[i][j];
+        least = fminf(least, v[i][j] == -INFINITY ? INFINITY : v[i][j]);
+        most = fmaxf(most, v[i][j]);
       }
-    }
-    if (!a.sigmoid && (kChecked || !a.renormalize)) m = lane_max<L>(m);
-    if (!a.sigmoid && !a.renormalize) {
-      float s = 0.0f;
-#pragma unroll
-      for (int i = 0; i < I; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) s += expf(x[i][j] - m);
-      ls = logf(lane_sum<L>(s));
-    }
-    if (kChecked && !a.sigmoid) {
-      float s = 0.0f;
-      c = m * kLog2e;
-#pragma unroll
-      for (int i = 0; i < I; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) s += __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], kLog2e, -c));
-      l2s = __builtin_amdgcn_logf(lane_sum<L>(s));
-    }
-    // A score in 32 bits: of the choice alone, not of the weights.
-    auto score = [&](float v) {
-      return a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v * kLog2e))
-                       : __builtin_amdgcn_exp2f(__builtin_fmaf(v, kLog2e, -c) - l2s);
-    };
-    auto selection = [&](float v, float b) { return v == -INFINITY || b == -INFINITY ? -INFINITY : score(v) + b; };
-    float v[I][V];
+  } else {
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        v[i][j] = Biased ? selection(x[i][j], bias[Narrow && begin[i] + j >= a.experts ? 0 : begin[i] + j]) : x[i][j];
-    uint32_t key[I][V];
+      for (int j = 0; j < V; ++j) v[i][j] = x[i][j];
+  }
+  uint32_t key[I][V];
+  float step_of_key = 0.0f;
+  if constexpr (Biased) {
+    least = lane_min_value<L>(least);
+    most = lane_max<L>(most);
+    const float range = most - least, steps = range > 0.0f ? kSteps / range : 0.0f;
+    step_of_key = range > 0.0f ? range / kSteps : 0.0f;
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) key[i][j] = key_of(v[i][j]);
-    bool close = false;
-    float seen = 0.0f;
-    if constexpr (Grouped) {
+      for (int j = 0; j < V; ++j) {
+        const uint32_t place = static_cast<uint32_t>(fmaxf((v[i][j] - least) * steps, 0.0f)) + 1;
+        key[i][j] = v[i][j] == -INFINITY ? 0 : (place << 10) | (kCoarse - (begin[i] + j));
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        key[i][j] = key_of(v[i][j]);
+        if constexpr (kPacked) key[i][j] = (key[i][j] & ~kFine) | (kFine - (begin[i] + j));
+      }
+  }
+  if constexpr (Grouped) {
+    const int size = a.experts / a.groups;
+    if constexpr (Whole) {
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+        if (first[i] == 0)
+#pragma unroll
+          for (int j = 0; j < V; j += 4)
+            *reinterpret_cast<f32x4*>(values + begin[i] + j) = f32x4{v[i][j], v[i][j + 1], v[i][j + 2], v[i][j + 3]};
+    } else {
 #pragma unroll
       for (int i = 0; i < I; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j)
           if (j >= first[i] && begin[i] + j < a.experts) values[begin[i] + j] = v[i][j];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      const GroupLanes<L> lanes(a);
-      const BestTwo<float> best = lanes.best(a, values);
-      // Without a bias the two best logits have the two best scores.
-      const float one = Biased || best.first == -INFINITY ? best.first : score(best.first);
-      const float two = best.second == -INFINITY ? 0.0f : Biased ? best.second : score(best.second);
-      const float sum = best.nan ? NAN : one == -INFINITY ? -INFINITY : one + two;
-      int rank = 0;
-      for (int o = 0; o < a.groups; ++o) {
-        const float other = __shfl(sum, o * lanes.each, L);
-        const bool same = !Biased && __shfl(best.first, o * lanes.each, L) == best.first &&
-                          __shfl(best.second, o * lanes.each, L) == best.second;
-        const bool none = other == -INFINITY && sum == -INFINITY;
-        rank += other > sum || ((same || none) && o < lanes.group);
-        close |= o != lanes.group && lanes.group < a.groups && !same && !none &&
-                 !(fabsf(other - sum) > 4.0f * margin_of(sum));
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const GroupLanes<L> lanes(a);
+    const BestTwo<float> best = lanes.best(a, values);
+    // Without a bias the two best logits have the two best scores.
+    const float one = Biased || best.first == -INFINITY ? best.first : score(best.first);
+    const float two = best.second == -INFINITY ? 0.0f : Biased ? best.second : score(best.second);
+    const float sum = best.nan ? NAN : one == -INFINITY ? -INFINITY : one + two;
+    // The sums take the place of the values.
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (lanes.group < a.groups && lane % lanes.each == 0) values[lanes.group] = sum;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    int rank = 0;
+    for (int o = 0; o < a.groups; ++o) {
+      const float other = values[o];
+      rank += other > sum || (other == sum && o < lanes.group);
+      close |= other != other;
+    }
+    const uint64_t open = lanes.bits(a, rank < a.top_groups);
+    if (a.top_groups < a.groups) {
+      // The last open group and the first closed one: ranks differ, unless a sum is no number.
+      const uint64_t in = lanes.bits(a, rank == a.top_groups - 1), out = lanes.bits(a, rank == a.top_groups);
+      const int g = in != 0 ? __builtin_ctzll(in) : 0, h = out != 0 ? __builtin_ctzll(out) : 0;
+      const bool same = !Biased && __shfl(best.first, g * lanes.each, L) == __shfl(best.first, h * lanes.each, L) &&
+                        __shfl(best.second, g * lanes.each, L) == __shfl(best.second, h * lanes.each, L);
+      close |= !same && values[h] != -INFINITY &&
+               !(values[g] - values[h] > 4.0f * (margin_of(a, values[g]) + step_of_key));
+      // Behind two that are the same, a third could be greater by less than 32 bits show.
+      for (int o = 0; o < a.groups; ++o)
+        close |= same && o != g && o != h && values[o] != -INFINITY &&
+                 !(fabsf(values[o] - values[g]) > 4.0f * margin_of(a, values[g]));
+    }
+    if (Whole && size % V == 0) {
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        const bool in = (open >> ((static_cast<uint32_t>(begin[i]) / static_cast<uint32_t>(size)) & 63u)) & 1u;
+#pragma unroll
+        for (int j = 0; j < V; ++j) key[i][j] = in ? key[i][j] : 0;
       }
-      const uint64_t open = lanes.bits(a, rank < a.top_groups);
+    } else {
       const float inverse = static_cast<float>(a.groups) / static_cast<float>(a.experts);
 #pragma unroll
       for (int i = 0; i < I; ++i)
@@ -292,20 +395,34 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
           if (!((open >> (g & 63)) & 1u)) key[i][j] = 0;
         }
     }
-    const int rounds = Biased ? (a.k + 2 < a.experts ? a.k + 2 : a.experts) : a.k;
+  }
+  const int rounds = Biased ? (a.k + 2 < a.experts ? a.k + 2 : a.experts) : a.k;
+  uint32_t best = 0;
 #pragma unroll 1
-    for (int q = 0; q < rounds; ++q) {
-      uint32_t own = 0, at = 0xFFFFFFFFu, best;
+  for (int q = 0; q < rounds; ++q) {
+    uint32_t win;
+    if constexpr (kPacked) {
+      // No two keys are equal: the next one is the nearest below the last, the greatest
+      // difference to it modulo 2^32 (from zero at first), and none has to be struck out.
+      uint32_t next = 0;
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) next = key[i][j] - best > next ? key[i][j] - best : next;
+      best = q > 0 && best == 0 ? 0 : best + lane_max<L>(next);  // zero: none is left
+      win = kIndex - (best & kIndex);
+    } else {
+      uint32_t own = 0, at = 0xFFFFFFFFu;
 #pragma unroll
       for (int i = 0; i < I; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) own = key[i][j] > own ? key[i][j] : own;
+      best = lane_max<L>(own);
 #pragma unroll
       for (int i = I - 1; i >= 0; --i)
 #pragma unroll
-        for (int j = V - 1; j >= 0; --j) at = key[i][j] == own ? begin[i] + j : at;
-      const uint32_t win = best_index<L>(own, at, best);
-      if (lane == 0) ids[q] = best > kKeyOfMinusInf ? static_cast<int32_t>(win) : -1;
+        for (int j = V - 1; j >= 0; --j) at = key[i][j] == best ? begin[i] + j : at;
+      win = lane_min<L>(at);
 #pragma unroll
       for (int i = 0; i < I; ++i) {
         const uint32_t j0 = win - begin[i];
@@ -313,60 +430,68 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
         for (int j = 0; j < V; ++j) key[i][j] = j0 == static_cast<uint32_t>(j) ? 0 : key[i][j];
       }
     }
-    // A wave's LDS accesses are performed in order, and a row's lanes are of one wave.
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if constexpr (Biased) {
-      // Neighbours among the k and the next one have to be clear of each other, or the same.
-      for (int q = lane; q < a.k && q + 1 < rounds; q += L) {
-        const int32_t i = ids[q], j = ids[q + 1];
-        if (j < 0) continue;  // none is left
-        const float vi = selection(static_cast<float>(row[i]), bias[i]);
-        const float vj = selection(static_cast<float>(row[j]), bias[j]);
-        close |= !(vi - vj > margin_of(vi)) && !(row[i] == row[j] && bias[i] == bias[j]);
-      }
-      // Where the last chosen and the next one are the same, one behind them could yet be greater.
-      if (rounds == a.k + 2 && ids[a.k + 1] >= 0) {
-        const int32_t i = ids[a.k - 1], j = ids[a.k], n = ids[a.k + 1];
-        const float vj = selection(static_cast<float>(row[j]), bias[j]);
-        const float vn = selection(static_cast<float>(row[n]), bias[n]);
-        close |= row[i] == row[j] && bias[i] == bias[j] && !(vj - vn > margin_of(vj));
-      }
-    } else if constexpr (Grouped) {
-      // Where logits differ and their scores in 64 bits do not (1, or 0), the scores decide.
-      for (int q = lane; q < a.k; q += L) {
-        const float xq = ids[q] < 0 ? 0.0f : static_cast<float>(row[ids[q]]);
-        close |= ids[q] >= 0 && (a.sigmoid ? !(xq < 30.0f && xq > -700.0f) : !(xq - m > -700.0f));
-      }
+    if (lane == 0) ids[q] = best > kNone ? static_cast<int32_t>(win) : -1;
+  }
+  // A wave's LDS accesses are performed in order, and a row's lanes are of one wave.
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  if constexpr (Biased) {
+    // Neighbours among the k and the next one have to be clear of each other, or the same.
+    for (int q = lane; q < a.k && q + 1 < rounds; q += L) {
+      const int32_t i = ids[q], j = ids[q + 1];
+      if (j < 0) continue;  // none is left
+      const float vi = selection(static_cast<float>(row[i]), bias[i]);
+      const float vj = selection(static_cast<float>(row[j]), bias[j]);
+      close |= !(vi - vj > margin_of(a, vi) + 4.0f * step_of_key) && !(row[i] == row[j] && bias[i] == bias[j]);
     }
-    if constexpr (kChecked) {
-      // Any row of the wave: all do it, those that were decided with the same result.
-      // With values that are no numbers, the chosen may be others than the NaN: it is to be seen all the same.
-      if (__ballot(close) != 0 && choose_exactly<T, L>(a, row, bias, exact, ids)) seen = NAN;
+    // Where the last chosen and the next one are the same, one behind them could yet be greater.
+    if (rounds == a.k + 2 && ids[a.k + 1] >= 0) {
+      const int32_t i = ids[a.k - 1], j = ids[a.k], n = ids[a.k + 1];
+      const float vj = selection(static_cast<float>(row[j]), bias[j]);
+      const float vn = selection(static_cast<float>(row[n]), bias[n]);
+      close |= row[i] == row[j] && bias[i] == bias[j] && !(vj - vn > margin_of(a, vj) + 4.0f * step_of_key);
     }
-    float most = -INFINITY, sum = 0.0f;
-#pragma unroll 1
+  } else if constexpr (Grouped) {
+    // Where logits differ and their scores in 64 bits do not (1, or 0), the scores decide.
     for (int q = lane; q < a.k; q += L) {
-      const int32_t id = ids[q];
-      const float xj = id < 0 ? 0.0f : static_cast<float>(row[id]);
-      scores[q] = a.sigmoid ? log_sigmoid(xj) : a.renormalize ? xj : (xj - m) - ls;
-      if (id >= 0) most = fmaxf(most, scores[q]);
+      const float xq = ids[q] < 0 ? 0.0f : static_cast<float>(row[ids[q]]);
+      close |= ids[q] >= 0 && (a.sigmoid ? !(xq < 30.0f && xq > -700.0f) : !(xq - m > -700.0f));
     }
-    most = lane_max<L>(most);
+  }
+  if constexpr (kChecked) {
+    // Any row of the wave: all do it, those that were decided with the same result.
+    // With values that are no numbers, the chosen may be others than the NaN: it is to be seen all the same.
+    if (__ballot(close) != 0 && choose_exactly<T, L>(a, row, bias, exact, ids)) seen = NAN;
+  }
+  most = -INFINITY;
+  float sum = 0.0f;
 #pragma unroll 1
-    for (int q = lane; q < a.k; q += L) {
-      scores[q] = ids[q] < 0 ? 0.0f : expf(a.renormalize ? scores[q] - most : scores[q]) + seen;
-      sum += scores[q];
-    }
-    const float over = a.renormalize ? lane_sum<L>(sum) : 1.0f;
+  for (int q = lane; q < a.k; q += L) {
+    const int32_t id = ids[q];
+    scores[q] = id < 0 ? -INFINITY : static_cast<float>(row[id]);
+    most = fmaxf(most, scores[q]);
+  }
+  most = lane_max<L>(most);
+  // Sigmoids that are all tiny keep their ratios as logarithms.
+  const bool tiny = a.sigmoid && a.renormalize && most < -80.0f;
+  if (tiny) most = log_sigmoid(most);
 #pragma unroll 1
-    for (int q = lane; q < a.k; q += L) {
-      weights[r * a.k + q] = ids[q] < 0 ? 0.0f : a.scale * (scores[q] / over);
-      chosen[r * a.k + q] = ids[q];
-    }
-    if (stats != nullptr && lane == 0) {
-      stats[2 * r] = m;
-      stats[2 * r + 1] = ls;
-    }
+  for (int q = lane; q < a.k; q += L) {
+    const float xj = scores[q];
+    float e;
+    if (a.sigmoid && !tiny) e = 1.0f / (1.0f + expf(-xj));
+    else e = expf(a.sigmoid ? log_sigmoid(xj) - most : a.renormalize ? xj - most : (xj - m) - ls);
+    scores[q] = ids[q] < 0 ? 0.0f : e + seen;
+    sum += scores[q];
+  }
+  const float over = a.renormalize ? lane_sum<L>(sum) : 1.0f;
+#pragma unroll 1
+  for (int q = lane; q < a.k; q += L) {
+    weights[r * a.k + q] = ids[q] < 0 ? 0.0f : a.scale * (scores[q] / over);
+    chosen[r * a.k + q] = ids[q];
+  }
+  if (stats != nullptr && lane == 0) {
+    stats[2 * r] = m;
+    stats[2 * r + 1] = ls;
   }
 }
 
@@ -480,48 +605,54 @@ template <typename T>
 spmm_status run_route(const spmm_route_desc* d, const void* logits, const float* bias, float* weights, int32_t* chosen,
                       float* stats, hipStream_t s) {
   const RouteArgs a = route_args(d);
-  auto launch = [&](auto L, auto I, auto Narrow) {
-    constexpr int kGroups = kThreads / decltype(L)::value;
-    const int64_t blocks = ceil_div(d->rows, kGroups);
-    const dim3 grid(static_cast<unsigned>(blocks < 16384 ? blocks : 16384));
+  constexpr int V = kPiece<T>;
+  auto launch = [&](auto L, auto I, auto Shape) {
+    constexpr int kL = decltype(L)::value, kI = decltype(I)::value, kGroups = kThreads / kL;
+    constexpr RowShape kShape = decltype(Shape)::value;
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.rows, kGroups)));
     const size_t values = bias != nullptr || a.groups > 1 ? static_cast<size_t>(a.experts) * 8 : 0;
     const size_t lds = kGroups * (values + (2 * static_cast<size_t>(a.k) + 2) * 4);
     const T* x = static_cast<const T*>(logits);
-    constexpr int kL = decltype(L)::value, kI = decltype(I)::value;
-    constexpr bool kNarrow = decltype(Narrow)::value;
     if (bias != nullptr && a.groups > 1)
-      hipLaunchKernelGGL((route_rows<T, kL, kI, kNarrow, true, true>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
+      hipLaunchKernelGGL((route_rows<T, kL, kI, kShape, true, true>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
                          chosen, stats);
     else if (bias != nullptr)
-      hipLaunchKernelGGL((route_rows<T, kL, kI, kNarrow, true, false>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
+      hipLaunchKernelGGL((route_rows<T, kL, kI, kShape, true, false>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
                          chosen, stats);
     else if (a.groups > 1)
-      hipLaunchKernelGGL((route_rows<T, kL, kI, kNarrow, false, true>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
+      hipLaunchKernelGGL((route_rows<T, kL, kI, kShape, false, true>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
                          chosen, stats);
     else
-      hipLaunchKernelGGL((route_rows<T, kL, kI, kNarrow, false, false>), grid, dim3(kThreads), lds, s, a, x, bias,
-                         weights, chosen, stats);
+      hipLaunchKernelGGL((route_rows<T, kL, kI, kShape, false, false>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
+                         chosen, stats);
   };
   using std::integral_constant;
-  constexpr int V = kPiece<T>;
+  // The fewest lanes that hold the row in one piece each, or in 16 logits each, and a lane a group at least.
+  auto with_shape = [&](auto L, auto I) {
+    if (d->experts % V == 0) launch(L, I, integral_constant<RowShape, RowShape::kWhole>());
+    else launch(L, I, integral_constant<RowShape, RowShape::kMoved>());
+  };
   const int64_t pieces = ceil_div(d->experts, V);
-  // A lane a group at least.
-  if (d->experts < V && d->groups <= 4)
-    launch(integral_constant<int, 4>(), integral_constant<int, 1>(), std::true_type());
-  else if (d->experts < V)
-    launch(integral_constant<int, 8>(), integral_constant<int, 1>(), std::true_type());
-  else if (pieces <= 4 && d->groups <= 4)
-    launch(integral_constant<int, 4>(), integral_constant<int, 1>(), std::false_type());
-  else if (pieces <= 8 && d->groups <= 8)
-    launch(integral_constant<int, 8>(), integral_constant<int, 1>(), std::false_type());
-  else if (pieces <= 16 && d->groups <= 16)
-    launch(integral_constant<int, 16>(), integral_constant<int, 1>(), std::false_type());
-  else if (pieces <= 16 * (16 / V) && d->groups <= 16)
-    launch(integral_constant<int, 16>(), integral_constant<int, 16 / V>(), std::false_type());
-  else if (pieces <= 64)
-    launch(integral_constant<int, 64>(), integral_constant<int, 1>(), std::false_type());
-  else
-    launch(integral_constant<int, 64>(), integral_constant<int, 16 / V>(), std::false_type());
+  // A launch has fewer than 2^32 work-items.
+  constexpr int64_t kMost = int64_t(1) << 24;
+  if (d->rows > kMost) {
+    for (int64_t r = 0; r < d->rows; r += kMost) {
+      spmm_route_desc part = *d;
+      part.rows = d->rows - r < kMost ? d->rows - r : kMost;
+      if (spmm_status st = run_route<T>(&part, static_cast<const T*>(logits) + r * d->logits_stride, bias,
+                                        weights + r * d->top_k, chosen + r * d->top_k,
+                                        stats == nullptr ? nullptr : stats + 2 * r, s))
+        return st;
+    }
+    return SPMM_OK;
+  }
+  if (d->experts < V) launch(integral_constant<int, 8>(), integral_constant<int, 1>(), integral_constant<RowShape, RowShape::kNarrow>());
+  else if (pieces <= 4 && d->groups <= 4) with_shape(integral_constant<int, 4>(), integral_constant<int, 1>());
+  else if (pieces <= 8 && d->groups <= 8) with_shape(integral_constant<int, 8>(), integral_constant<int, 1>());
+  else if (pieces <= 16 && d->groups <= 16) with_shape(integral_constant<int, 16>(), integral_constant<int, 1>());
+  else if (pieces <= 16 * (16 / V) && d->groups <= 16) with_shape(integral_constant<int, 16>(), integral_constant<int, 16 / V>());
+  else if (pieces <= 64) with_shape(integral_constant<int, 64>(), integral_constant<int, 1>());
+  else with_shape(integral_constant<int, 64>(), integral_constant<int, 16 / V>());
   return check_launch("route");
 }
 
