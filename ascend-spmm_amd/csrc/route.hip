@@ -101,35 +101,36 @@ struct GroupLanes {
   }
 };
 
-// Exact choice of the rows of a wave, in 64 bits: for rows whose choice 32 bits
-// do not decide.  It takes a row's logits and leaves ids[0..k) (-1 where no
-// expert is left); values: `experts` doubles of LDS for each row.  Compact rather
-// than fast: about one row in 2000 of random logits comes here.  Returns whether
-// a softmax's values are no numbers, as a NaN or an infinity is among its logits.
-template <typename T, int L>
+// Exact choice of one row by a wave, in 64 bits: for rows whose choice 32 bits do
+// not decide, about one in 2000 of random logits.  It takes the row's logits and
+// leaves ids[0..k) (-1 where no expert is left); values: `experts` doubles of the
+// wave's own LDS.  Returns whether a softmax's values are no numbers, as a NaN or
+// an infinity is among its logits.
+template <typename T>
 __device__ inline bool choose_exactly(const RouteArgs& a, const T* row, const float* bias, double* values,
                                             int32_t* ids) {
+  constexpr int L = 64;
   const int lane = threadIdx.x % L;
   double m = -kInf64, total = 0.0;
   if (!a.sigmoid) {
-#pragma unroll 2
+#pragma unroll 4
     for (int e = lane; e < a.experts; e += L) m = fmax(m, static_cast<double>(static_cast<float>(row[e])));
     for (int d = 1; d < L; d <<= 1) m = fmax(m, __shfl_xor(m, d, L));
-#pragma unroll 2
+#pragma unroll 4
     for (int e = lane; e < a.experts; e += L) {
       const float x = static_cast<float>(row[e]);
       if (x != -INFINITY) total += exp(static_cast<double>(x) - m);
     }
     for (int d = 1; d < L; d <<= 1) total += __shfl_xor(total, d, L);
   }
-#pragma unroll 2
+#pragma unroll 4
   for (int e = lane; e < a.experts; e += L) {
     const float x = static_cast<float>(row[e]), b = bias != nullptr ? bias[e] : 0.0f;
     const double score = a.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x)))
                                    : exp(static_cast<double>(x) - m) / total;
     values[e] = x == -INFINITY || b == -INFINITY ? -kInf64 : score + b;
   }
-  // A wave's LDS accesses are performed in order, and a row's lanes are of one wave.
+  // A wave's LDS accesses are performed in order.
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   if (a.groups > 1) {
     const GroupLanes<L> lanes(a);
@@ -141,7 +142,7 @@ __device__ inline bool choose_exactly(const RouteArgs& a, const T* row, const fl
       rank += other > key || (other == key && o < lanes.group);
     }
     const uint64_t open = lanes.bits(a, rank < a.top_groups);
-#pragma unroll 2
+#pragma unroll 4
     for (int e = lane; e < a.experts; e += L)
       if (!((open >> (e / lanes.size)) & 1u)) values[e] = -kInf64;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -150,7 +151,7 @@ __device__ inline bool choose_exactly(const RouteArgs& a, const T* row, const fl
   for (int q = 0; q < a.k; ++q) {
     uint64_t own = 0, best;
     uint32_t at = 0xFFFFFFFFu;
-#pragma unroll 2
+#pragma unroll 4
     for (int e = lane; e < a.experts; e += L) {
       const uint64_t key = key_of(values[e]);
       if (key > own) {
@@ -211,10 +212,13 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
   constexpr bool kChecked = Biased || Grouped, kPacked = Biased || sizeof(T) == 2;
   constexpr uint32_t kIndex = Biased ? kCoarse : kFine, kNone = Biased ? kCoarse : kKeyOfMinusInf;
   extern __shared__ double lds[];
-  // The row's values, and its choices' ids and scores.
-  double* exact = lds + (threadIdx.x / L) * a.experts;
-  float* values = reinterpret_cast<float*>(exact);
-  int32_t* ids = reinterpret_cast<int32_t*>(lds + (kChecked ? kGroups * a.experts : 0)) + (threadIdx.x / L) * (2 * a.k + 2);
+  // 64-bit values for one row of each wave; the row's own values where there are groups; its choices' ids and scores.
+  double* exact = lds + (threadIdx.x >> 6) * a.experts;
+  float* all_values = reinterpret_cast<float*>(lds + (kChecked ? kThreads / 64 * a.experts : 0));
+  const int per_row = Grouped ? (a.experts + 3) / 4 * 4 : 0;
+  float* values = all_values + (threadIdx.x / L) * per_row;
+  int32_t* all_ids = reinterpret_cast<int32_t*>(all_values + kGroups * per_row);
+  int32_t* ids = all_ids + (threadIdx.x / L) * (2 * a.k + 2);
   float* scores = reinterpret_cast<float*>(ids + a.k + 2);
   const int lane = threadIdx.x % L;
   int begin[I], first[I];
@@ -226,8 +230,8 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
     first[i] = Narrow ? 0 : Whole ? (column < a.experts ? 0 : V) : Piece::shift(column, a.experts);
   }
   const int64_t r = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / L;
-  if (r >= a.rows) return;
-  const T* row = logits + r * a.stride;
+  const bool live = r < a.rows;  // lanes without a row go along with the last one
+  const T* row = logits + (live ? r : a.rows - 1) * a.stride;
   float x[I][V], m = -FLT_MAX, ls = 0.0f, c = 0.0f, l2s = 0.0f;
 #pragma unroll
   for (int i = 0; i < I; ++i) {
@@ -458,9 +462,16 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
     }
   }
   if constexpr (kChecked) {
-    // Any row of the wave: all do it, those that were decided with the same result.
-    // With values that are no numbers, the chosen may be others than the NaN: it is to be seen all the same.
-    if (__ballot(close) != 0 && choose_exactly<T, L>(a, row, bias, exact, ids)) seen = NAN;
+    uint64_t rows = __ballot(close && live);
+    while (rows != 0) {
+      // The whole wave takes one such row after another.
+      const int group = __builtin_ctzll(rows) / L;
+      rows &= ~((~uint64_t(0) >> (64 - L)) << (group * L));
+      const int64_t which = static_cast<int64_t>(blockIdx.x) * kGroups + (threadIdx.x >> 6) * (64 / L) + group;
+      int32_t* into = all_ids + ((threadIdx.x >> 6) * (64 / L) + group) * (2 * a.k + 2);
+      // With values that are no numbers, the chosen may be others than the NaN: it is to be seen all the same.
+      if (choose_exactly(a, logits + which * a.stride, bias, exact, into) && (threadIdx.x & 63) / L == group) seen = NAN;
+    }
   }
   most = -INFINITY;
   float sum = 0.0f;
@@ -485,11 +496,11 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
   }
   const float over = a.renormalize ? lane_sum<L>(sum) : 1.0f;
 #pragma unroll 1
-  for (int q = lane; q < a.k; q += L) {
+  for (int q = lane; q < a.k && live; q += L) {
     weights[r * a.k + q] = ids[q] < 0 ? 0.0f : a.scale * (scores[q] / over);
     chosen[r * a.k + q] = ids[q];
   }
-  if (stats != nullptr && lane == 0) {
+  if (stats != nullptr && lane == 0 && live) {
     stats[2 * r] = m;
     stats[2 * r + 1] = ls;
   }
@@ -610,8 +621,9 @@ spmm_status run_route(const spmm_route_desc* d, const void* logits, const float*
     constexpr int kL = decltype(L)::value, kI = decltype(I)::value, kGroups = kThreads / kL;
     constexpr RowShape kShape = decltype(Shape)::value;
     const dim3 grid(static_cast<unsigned>(ceil_div(a.rows, kGroups)));
-    const size_t values = bias != nullptr || a.groups > 1 ? static_cast<size_t>(a.experts) * 8 : 0;
-    const size_t lds = kGroups * (values + (2 * static_cast<size_t>(a.k) + 2) * 4);
+    const size_t exact = bias != nullptr || a.groups > 1 ? static_cast<size_t>(a.experts) * 8 * (kThreads / 64) : 0;
+    const size_t values = a.groups > 1 ? align_up(static_cast<size_t>(a.experts), 4) * 4 : 0;
+    const size_t lds = exact + kGroups * (values + (2 * static_cast<size_t>(a.k) + 2) * 4);
     const T* x = static_cast<const T*>(logits);
     if (bias != nullptr && a.groups > 1)
       hipLaunchKernelGGL((route_rows<T, kL, kI, kShape, true, true>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
