@@ -419,16 +419,18 @@ __global__ __launch_bounds__(64) void log_probs_join(LogArgs a, const T* __restr
                                                      const void* __restrict__ targets, RowOut out, int parts,
                                                      const Part* __restrict__ part_sums,
                                                      const uint64_t* __restrict__ part_best) {
+  extern __shared__ uint64_t heads[];  // the parts' lists
   const int64_t r = blockIdx.x;
   const int lane = threadIdx.x;
+  for (int k = lane; k < parts * a.top; k += 64) heads[k] = part_best[r * parts * a.top + k];
   const int64_t target = target_of(targets, a.index64, r);
   const bool named = static_cast<uint64_t>(target) < static_cast<uint64_t>(a.classes);
   const float xt = named ? static_cast<float>(x[r * a.stride + target]) : 0.0f;
   Part mine = {-FLT_MAX, 0.0f, 0.0f};
   if (lane < parts) mine = part_sums[r * parts + lane];
-  const uint64_t* heads = part_best + (r * parts + lane) * a.top;
+  __syncthreads();
   int taken = 0;
-  uint64_t head = lane < parts && a.top > 0 ? heads[0] : 0;
+  uint64_t head = lane < parts && a.top > 0 ? heads[lane * a.top] : 0;
   const Origin o(lane_max<64>(mine.m));
   const float shift = origin_shift(Origin(mine.m), o), f = __builtin_amdgcn_exp2f(shift);
   const float t = lane_sum<64>(f * __builtin_fmaf(mine.s, fmaxf(shift, kFloor), mine.t)), s = lane_sum<64>(mine.s * f);
@@ -443,7 +445,7 @@ __global__ __launch_bounds__(64) void log_probs_join(LogArgs a, const T* __restr
           key > kKeyOfMinusInf ? static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(pair)) : -1;
     }
     // Pairs differ by their index: one lane at most has this one, but for the empty pair.
-    if (head == pair && pair != 0) head = ++taken < a.top ? heads[taken] : 0;
+    if (head == pair && pair != 0) head = ++taken < a.top ? heads[lane * a.top + taken] : 0;
   }
 }
 
@@ -599,8 +601,8 @@ spmm_status run_forward(const spmm_log_probs_desc* d, const void* logits, const 
     if (spmm_status st = check_launch("log_probs")) return st;
   }
   if (parts == 1) return SPMM_OK;
-  hipLaunchKernelGGL(log_probs_join<T>, dim3(static_cast<unsigned>(d->rows)), dim3(64), 0, s, a, x, targets, out, parts,
-                     sums, best);
+  hipLaunchKernelGGL(log_probs_join<T>, dim3(static_cast<unsigned>(d->rows)), dim3(64),
+                     static_cast<size_t>(parts) * a.top * sizeof(uint64_t), s, a, x, targets, out, parts, sums, best);
   return check_launch("log_probs join");
 }
 

@@ -13,7 +13,7 @@ using torch::autograd::variable_list;
 // `t` as `rows` rows of its last dimension: a view where its rows are contiguous
 // and evenly apart, else a copy.
 at::Tensor flat_rows(const at::Tensor& t, int64_t rows) {
-  const at::Tensor flat = t.reshape({rows, t.size(-1)});
+  const at::Tensor flat = t.dim() == 2 ? t : t.reshape({rows, t.size(-1)});
   const int64_t width = flat.size(1);
   if ((flat.stride(1) == 1 || width <= 1) && (flat.stride(0) >= width || rows <= 1)) return flat;
   return flat.contiguous();
@@ -31,6 +31,10 @@ std::vector<int64_t> leading_sizes(const at::Tensor& t, int64_t last) {
   sizes.push_back(last);
   return sizes;
 }
+
+// Scratch of the library's calls, and its address: none where none is needed.
+at::Tensor scratch(const at::Tensor& like, size_t bytes) { return bytes > 0 ? workspace(like, bytes) : at::Tensor(); }
+void* scratch_data(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 void check_differentiable_once(const char* op) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op, ": its gradient is not differentiable");
@@ -77,8 +81,8 @@ struct Embedding : torch::autograd::Function<Embedding> {
                                                  ctx->saved_data["scale"].toDouble());
     size_t bytes = 0;
     raise_status(spmm_embedding_grad_workspace(&d, &bytes), "embedding");
-    at::Tensor ws = workspace(grad, bytes);
-    raise_status(spmm_embedding_grad_run(&d, ids.data_ptr(), grad.data_ptr(), dweight.data_ptr(), ws.data_ptr(), bytes,
+    at::Tensor ws = scratch(grad, bytes);
+    raise_status(spmm_embedding_grad_run(&d, ids.data_ptr(), grad.data_ptr(), dweight.data_ptr(), scratch_data(ws), bytes,
                                          current_stream(grad)),
                  "embedding");
     return {dweight, at::Tensor(), at::Tensor()};
@@ -202,9 +206,9 @@ std::tuple<at::Tensor, at::Tensor> expert_plan(const at::Tensor& experts, int64_
   const auto i32 = ids.options().dtype(at::kInt);
   at::Tensor offsets = at::empty({count + 1}, i32);
   at::Tensor place = at::empty({ids.size(0), ids.dim() == 2 ? ids.size(1) : 1}, i32);
-  at::Tensor ws = workspace(ids, bytes);
+  at::Tensor ws = scratch(ids, bytes);
   raise_status(spmm_expert_plan_run(type, ids.data_ptr(), ids.numel(), count, offsets.data_ptr<int32_t>(),
-                                    place.data_ptr<int32_t>(), ws.data_ptr(), bytes, current_stream(ids)),
+                                    place.data_ptr<int32_t>(), scratch_data(ws), bytes, current_stream(ids)),
                "ExpertPlan");
   return {offsets, place};
 }
@@ -342,10 +346,10 @@ variable_list log_probs_forward(const at::Tensor& logits, const at::Tensor& targ
   at::Tensor values = at::empty(leading_sizes(logits, top), f32);
   at::Tensor ids = at::empty(leading_sizes(logits, top), f32.dtype(at::kInt));
   if (stats != nullptr) *stats = at::empty({d.rows, 2}, f32);
-  at::Tensor ws = workspace(logits, bytes);
+  at::Tensor ws = scratch(logits, bytes);
   raise_status(spmm_log_probs_run(&d, rows.data_ptr(), t.data_ptr(), logp.data_ptr<float>(), entropy.data_ptr<float>(),
                                   values.data_ptr<float>(), ids.data_ptr<int32_t>(),
-                                  stats != nullptr ? stats->data_ptr<float>() : nullptr, ws.data_ptr(), bytes,
+                                  stats != nullptr ? stats->data_ptr<float>() : nullptr, scratch_data(ws), bytes,
                                   current_stream(logits)),
                "log_probs");
   return {logp, entropy, values, ids};
@@ -432,13 +436,8 @@ void bind_expert_ops(pybind11::module_& m) {
     the target and the entropy are differentiable with respect to logits.
     )doc",
         pybind11::arg("logits"), pybind11::arg("targets"), pybind11::arg("top") = 0);
-  m.def("route", &route, "Experts of rows from a router's logits (GPU)", pybind11::arg("logits"), pybind11::arg("top_k"),
-        pybind11::arg("score"), pybind11::arg("bias"), pybind11::arg("groups"), pybind11::arg("top_groups"),
-        pybind11::arg("renormalize"), pybind11::arg("scale"));
-  m.def("expert_plan", &expert_plan, "Offsets and places of rows sorted by expert (GPU)", pybind11::arg("experts"),
-        pybind11::arg("count"));
-  m.def("expert_pack", &expert_pack, "Rows at the places of their choices (GPU)", pybind11::arg("x"),
-        pybind11::arg("place"), pybind11::arg("offsets"));
-  m.def("expert_restore", &expert_restore, "Weighted sums of the choices' rows (GPU)", pybind11::arg("results"),
-        pybind11::arg("weights"), pybind11::arg("place"), pybind11::arg("offsets"));
+  m.def("route", &route, "Experts of rows from a router's logits (GPU)");
+  m.def("expert_plan", &expert_plan, "Offsets and places of rows sorted by expert (GPU)");
+  m.def("expert_pack", &expert_pack, "Rows at the places of their choices (GPU)");
+  m.def("expert_restore", &expert_restore, "Weighted sums of the choices' rows (GPU)");
 }

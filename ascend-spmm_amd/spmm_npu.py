@@ -256,11 +256,10 @@ def route(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, 
     compared in 64 bits.  The weights are differentiable with respect to
     ``logits``; ``bias`` has no gradient.
     """
-    if score not in _SCORES:
+    code = _SCORES.get(score)
+    if code is None:
         raise ValueError("score must be one of " + ", ".join(sorted(_SCORES)))
-    groups = int(groups)
-    return _route(logits, int(top_k), _SCORES[score], bias, groups, groups if top_groups is None else int(top_groups),
-                  bool(renormalize), float(scale))
+    return _route(logits, top_k, code, bias, groups, groups if top_groups is None else top_groups, renormalize, scale)
 
 
 class ExpertPlan:
@@ -280,7 +279,7 @@ class ExpertPlan:
     """
 
     def __init__(self, experts, count):
-        self.offsets, self.place = _expert_plan(experts, int(count))
+        self.offsets, self.place = _expert_plan(experts, count)
 
     def pack(self, x):
         """Each row of ``x`` at the places of its choices: [rows * top_k, width],
