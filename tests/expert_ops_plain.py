@@ -61,14 +61,11 @@ def log_probs(x, targets, top, a=None, h=None):
     logp = (z - ls).gather(1, at[:, None])[:, 0]
     logp = torch.where(empty, torch.full_like(logp, -INF), logp)
     logp = torch.where(named, logp, torch.zeros_like(logp))
-    values = torch.full((rows, top), -INF, dtype=torch.float64)
-    ids = torch.full((rows, top), -1, dtype=torch.int32)
-    for r in range(rows):
-        usable = [i for i in range(n) if x[r, i] > -INF] if n <= 4096 else \
-            torch.nonzero(x[r] > -INF)[:, 0].tolist()
-        order = sorted(usable, key=lambda i: (-float(x[r, i]), i))[:top]
-        for q, i in enumerate(order):
-            values[r, q], ids[r, q] = (z - ls)[r, i], i
+    # A stable sort keeps equal ones in the order of their indices; NaN is none of them.
+    best = torch.where(torch.isnan(x), torch.full_like(x, -INF), x).sort(dim=1, descending=True, stable=True)
+    ids, found = best.indices[:, :top], best.values[:, :top] > -INF
+    values = torch.where(found, (z - ls).gather(1, ids), torch.full_like(found, -INF, dtype=torch.float64))
+    ids = torch.where(found, ids, torch.full_like(ids, -1)).to(torch.int32)
     out = dict(logp=logp, entropy=H, values=values, ids=ids)
     if a is not None:
         ga = torch.where(named & ~empty, a.double().cpu(), torch.zeros_like(logp))[:, None]

@@ -182,3 +182,36 @@ def test_refusals(spmm_npu):
         dual = torch.autograd.forward_ad.make_dual(w.detach(), torch.ones_like(w))
         with pytest.raises(RuntimeError, match="forward-mode"):
             spmm_npu.embedding(dual, ids)
+
+
+@pytest.mark.parametrize("count,table,width,dtype", [(262144, 3000, 512, torch.bfloat16), (140001, 70000, 512, torch.float16),
+                                                     (300000, 100, 128, torch.float32), (1200001, 5000, 4, torch.float16)])
+def test_many_ids(spmm_npu, count, table, width, dtype):
+    """Longer ranges of positions, runs over hundreds of them, several rounds of the sort's tiles;
+    against 64-bit sums on the GPU, bounds as above."""
+    g = torch.Generator(device="cuda").manual_seed(count)
+    weight = torch.randn(table, width, generator=g, device="cuda").to(dtype).requires_grad_(True)
+    grad = torch.randn(count, width, generator=g, device="cuda").to(dtype)
+    for kind in ("zipf", "uniform"):
+        ids = ids_of(kind, count, table)
+        out = spmm_npu.embedding(weight, ids, scale=0.25)
+        assert torch.equal(out, (weight.detach().float()[ids] * 0.25).to(dtype))
+        (dw,) = torch.autograd.grad(out, weight, grad)
+        total = torch.zeros(table, width, dtype=torch.float64, device="cuda").index_add_(0, ids, grad.double())
+        size = torch.zeros(table, width, dtype=torch.float64, device="cuda").index_add_(0, ids, grad.double().abs())
+        named = torch.bincount(ids, minlength=table).double()[:, None]
+        check(dw, total * 0.25, ((named + 2) * E32 * size * 0.25).cpu(), kind)
+        assert torch.equal(dw, torch.autograd.grad(spmm_npu.embedding(weight, ids, scale=0.25), weight, grad)[0])
+
+
+def test_tables_of_more_than_2_31_elements(spmm_npu):
+    rows, width = (1 << 21) + 7, 1032
+    weight = torch.zeros(rows, width, device="cuda", dtype=torch.bfloat16)
+    weight[-1], weight[-2], weight[3] = 3.0, 2.0, 1.0
+    ids = torch.tensor([rows - 1, 3, rows - 2, rows, 0, rows - 1], device="cuda")
+    leaf = weight.requires_grad_(True)
+    out = spmm_npu.embedding(leaf, ids)
+    assert out[:, 0].tolist() == [3.0, 1.0, 2.0, 0.0, 0.0, 3.0] and out[:, -1].tolist() == out[:, 0].tolist()
+    (dw,) = torch.autograd.grad(out, leaf, torch.ones_like(out))
+    assert dw[[rows - 1, rows - 2, 3, 0], -1].tolist() == [2.0, 1.0, 1.0, 1.0]
+    assert float(dw.float().sum(1).sum()) == 5 * width

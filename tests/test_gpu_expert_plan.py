@@ -173,3 +173,48 @@ def test_graph_replays(spmm_npu):
         x.copy_(normal((700, 72), torch.bfloat16, 40 + k).cuda())
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.parametrize("rows,k,count,width,dtype", [(70000, 2, 40, 520, torch.bfloat16), (300000, 3, 2000, 8, torch.float16),
+                                                      (140000, 1, 3, 33, torch.float32)])
+def test_many_rows(spmm_npu, rows, k, count, width, dtype):
+    """Several rows a group of lanes and more than 512 tiles of the sort; against the GPU's stable sort
+    and 64-bit sums, bounds as above."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    ids = torch.randint(-1, count + 1, (rows, k), generator=g, device="cuda", dtype=torch.int32)
+    key = torch.where((ids >= 0) & (ids < count), ids, torch.full_like(ids, count)).reshape(-1).long()
+    place = torch.empty_like(key)
+    place[key.argsort(stable=True)] = torch.arange(rows * k, device="cuda")
+    p = spmm_npu.ExpertPlan(ids, count)
+    assert torch.equal(p.place.reshape(-1).long(), place)
+    assert torch.equal(p.offsets.long(), torch.searchsorted(key.sort().values, torch.arange(count + 1, device="cuda")))
+    kept = (key < count).view(rows, k, 1)
+    x = torch.randn(rows, width, generator=g, device="cuda").to(dtype).requires_grad_(True)
+    y = torch.randn(rows * k, width, generator=g, device="cuda").to(dtype).requires_grad_(True)
+    w = torch.randn(rows, k, generator=g, device="cuda").requires_grad_(True)
+    grad = torch.randn(rows, width, generator=g, device="cuda").to(dtype)
+    packed, out = p.pack(x), p.restore(y, w)
+    want = (x.detach()[:, None, :] * kept).reshape(rows * k, width)
+    assert torch.equal(packed.detach()[place], want)
+    yd = torch.where(kept, y.detach().double()[place].view(rows, k, width), 0.0)
+    wd = torch.where(kept, w.detach().double()[:, :, None], 0.0)
+    check(out, (yd * wd).sum(1), ((k + 1) * E32 * (yd * wd).abs().sum(1)).cpu(), "out")
+    (dx,) = torch.autograd.grad(packed, x, y.detach())
+    check(dx, yd.sum(1), ((k + 1) * E32 * yd.abs().sum(1)).cpu(), "dx")
+    dy, dw = torch.autograd.grad(out, (y, w), grad)
+    gd = grad.double()[:, None, :]
+    check(dy[place], (wd * gd).reshape(rows * k, width), (E32 * (wd * gd).abs().reshape(rows * k, width)).cpu(), "dy")
+    check(dw, (yd * gd).sum(2), ((width / 32 + 64) * E32 * (yd * gd).abs().sum(2)).cpu(), "dw")
+
+
+def test_packed_rows_of_more_than_2_31_elements(spmm_npu):
+    rows, k, width = 1 << 20, 2, 1032
+    ids = torch.tensor([[1, 0]], device="cuda").expand(rows, k)
+    p = spmm_npu.ExpertPlan(ids, 2)
+    x = torch.zeros(rows, width, device="cuda", dtype=torch.bfloat16)
+    x[-1], x[0] = 2.0, 1.0
+    packed = p.pack(x)
+    assert packed[[0, rows - 1, rows, 2 * rows - 1], -1].tolist() == [1.0, 2.0, 1.0, 2.0]
+    assert float(packed[:, 0].float().sum()) == 6.0
+    out = p.restore(packed, torch.tensor([[3.0, 4.0]], device="cuda").expand(rows, k))
+    assert out[[0, -1], -1].tolist() == [7.0, 14.0] and not out[1:-1, 0].any()

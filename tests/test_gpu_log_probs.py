@@ -64,6 +64,18 @@ def test_masked_rows(spmm_npu, n, dtype):
     run(spmm_npu, x, t, min(n, 7))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pieces", [1, 3, 7, 12, 15, 27, 50, 90, 200])
+def test_many_rows(spmm_npu, pieces, dtype):
+    """Enough rows for fewer lanes and several pieces a lane, with ties and masks."""
+    piece = 16 // dtype.itemsize
+    n = pieces * piece - (pieces % 2) * (piece // 2)
+    x, t = make(17001, n, dtype, seed=pieces)
+    x[::7] = (x[::7] * 2).round()
+    x[3::11, ::3] = -INF
+    run(spmm_npu, x, t, min(n, 6))
+
+
 @pytest.mark.parametrize("n", [40, 3000, 9000, 70000])
 def test_ties_go_to_the_lowest_index(spmm_npu, n):
     for dtype in DTYPES:
@@ -177,3 +189,18 @@ def test_refusals(spmm_npu):
     assert out[0].requires_grad and out[1].requires_grad and not out[2].requires_grad and not out[3].requires_grad
     with pytest.raises(RuntimeError, match="not differentiable"):
         torch.autograd.grad(out[0].square().sum(), leaf, create_graph=True)
+
+
+def test_more_elements_and_rows_than_32_bits_or_one_launch(spmm_npu):
+    """2^22 + 3 rows of 2056: over 2^33 bytes, and more rows than one launch of the wide kernel takes."""
+    rows, n = (1 << 22) + 3, 2056
+    x = torch.zeros(rows, n, device="cuda", dtype=torch.float16)
+    x[-1, n - 1] = 3.0
+    x[(1 << 22) - 1, 5] = 2.0
+    t = torch.full((rows,), n - 1, dtype=torch.int32, device="cuda")
+    logp, entropy, values, ids = spmm_npu.log_probs(x, t, top=1)
+    even = -float(np.log(n))
+    assert abs(float(logp[0]) - even) < 1e-5 and float((logp[: (1 << 22) - 1] - logp[0]).abs().max()) == 0.0
+    assert abs(float(logp[-1]) - (3.0 - float(np.log(n - 1 + np.exp(3.0))))) < 1e-5
+    assert int(ids[-1, 0]) == n - 1 and int(ids[(1 << 22) - 1, 0]) == 5 and int(ids[-2, 0]) == 0
+    assert abs(float(logp[(1 << 22) - 1]) + float(np.log(n - 1 + np.exp(2.0)))) < 1e-5

@@ -221,3 +221,14 @@ def test_choices_that_32_bits_do_not_decide(spmm_npu, dtype):
                 for bias in (None, torch.zeros(experts, device="cuda"), coarse, tiny, 1000.0 + coarse):
                     if bias is not None or groups > 1:
                         run(spmm_npu, x, 5, score, bias=bias, groups=groups, top_groups=kept)
+
+
+def test_more_rows_than_one_launch(spmm_npu):
+    rows = (1 << 24) + 5
+    x = torch.zeros(rows, 2, device="cuda", dtype=torch.float16)
+    x[1::3, 1] = 1.0
+    x[-1, 1] = 2.0
+    w, e = spmm_npu.route(x, 1, renormalize=False)
+    assert torch.equal(e[:, 0].long(), (x[:, 1] > 0).long())
+    p = torch.softmax(x.double(), 1).amax(1)
+    assert float((w[:, 0].double() - p).abs().max()) < 1e-6 and abs(float(w[-1, 0]) - float(p[-1])) < 1e-6
