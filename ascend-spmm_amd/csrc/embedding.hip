@@ -5,6 +5,9 @@
 // An id outside the table gives a row of zeros and adds to none.  The gradient's
 // sums are fp32, in the order of the positions, so that they repeat exactly: the
 // ids are sorted (stably) and each run of equal ones is summed.
+#include <cfloat>
+#include <cmath>
+
 #include "lane_reduce.h"
 #include "row_pieces.h"
 #include "sort_ids.h"
@@ -318,7 +321,8 @@ spmm_status check_embedding_desc(const spmm_embedding_desc* d) {
     return fail(SPMM_ERR_CONTRACT, "embedding: ids and rows of the table must be below 2^30, the width below 2^22");
   if (d->table_rows > 1 && d->weight_stride < d->width)
     return fail(SPMM_ERR_CONTRACT, "embedding: rows of weight overlap");
-  if (!(d->scale - d->scale == 0.0)) return fail(SPMM_ERR_INVALID_ARGUMENT, "embedding: scale must be finite");
+  if (!(std::fabs(d->scale) <= FLT_MAX))
+    return fail(SPMM_ERR_INVALID_ARGUMENT, "embedding: scale must be finite in FP32");
   return SPMM_OK;
 }
 

@@ -168,15 +168,17 @@ __device__ inline bool choose_exactly(const RouteArgs& a, const T* row, const fl
 }
 
 // How far apart two selection values in 32 bits have to be for their order to be
-// the exact one.  With e = 2^-24: 2^y has a relative error of 1.25 |y ln 2| e + 2 e.
+// the exact one.  With e = 2^-24, 2^y has a relative error of 1.25 |y ln 2| e + 2 e.
 // A sigmoid s = 1 / (1 + 2^y) is then off by s (1 - s) times that (at most 0.8 e)
-// and 3 e for its two roundings, a softmax p by p (1.25 |z| + H + 16) e with
-// p |z| < 0.4 and an entropy H of at most 7, 24 e in all; the sum with the bias
-// rounds by e |v|.  Twice that is below 2^-20 and 2^-18 of max(1, |v|); a pair of
-// group sums has twice as much again.
-__device__ inline float margin_of(const RouteArgs& a, float v) {
-  return (a.sigmoid ? 0x1p-20f : 0x1p-18f) * fmaxf(1.0f, fabsf(v));
+// and 3 e for its two roundings; a softmax p by p (1.25 |z| + H + 16) e with
+// p |z| < 0.4 and an entropy H of at most 7, 25 p e in all; the sum with the bias
+// rounds by e times the row's greatest value.  Two values: twice that.  Two sums of
+// two: the softmax's four scores are at most 1 together, and there are three
+// roundings more.
+__device__ inline float pair_margin(bool sigmoid, float scores, float most) {
+  return (sigmoid ? 0x1p-20f : 0x1p-19f * scores) + 0x1p-22f * most;
 }
+__device__ inline float group_margin(float most) { return 0x1p-19f + 0x1p-20f * most; }
 
 // Rows of whole pieces; rows whose last piece is moved back to end with them;
 // rows narrower than a piece.
@@ -187,8 +189,8 @@ enum class RowShape { kWhole, kMoved, kNarrow };
 // finds both.
 //  - logits of 16 bits: the upper 19 bits of their order hold all of them, 13 are
 //    left for the index;
-//  - values with a bias: steps of 2^-22 of the row's range (which margin_of's
-//    check counts in), and 10 bits for the index.
+//  - values with a bias: steps of 2^-22 of the row's range (which the
+//    check of neighbours counts in), and 10 bits for the index.
 // Logits of 32 bits without a bias take a word for the value alone, and the index
 // is looked for.
 constexpr uint32_t kFine = 0x1FFF, kCoarse = 0x3FF;
@@ -197,7 +199,7 @@ constexpr float kSteps = 4194300.0f;  // below 2^22
 // L lanes a row, which hold I pieces of 16 bytes of it each.  The k best are taken
 // one after another.  Without a bias the logits are the keys, and exact.  With one
 // (Biased) the keys are selection values in 32 bits, and two more than k are
-// taken: where neighbours among them are closer than margin_of, and not of the
+// taken: where neighbours among them are closer than pair_margin, and not of the
 // same logit and bias, or the groups at the border are as close, the row's choice
 // is made again in 64 bits.  Bound by vector instructions, most of them of the k
 // rounds.  65536 rows of 256 experts in 8 groups, k = 8: all in 64 bits 132 us,
@@ -266,7 +268,6 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
   auto softmax = [&](float v) { return __builtin_amdgcn_exp2f(__builtin_fmaf(v, kLog2e, -c) - l2s); };
   auto score = [&](float v) { return a.sigmoid ? sigmoid(v) : softmax(v); };
   auto selected = [&](float s, float v, float b) { return v == -INFINITY || b == -INFINITY ? -INFINITY : s + b; };
-  auto selection = [&](float v, float b) { return selected(score(v), v, b); };
   float v[I][V], least = INFINITY, most = -INFINITY;
   bool close = false;
   float seen = 0.0f;
@@ -312,10 +313,11 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
       for (int j = 0; j < V; ++j) v[i][j] = x[i][j];
   }
   uint32_t key[I][V];
-  float step_of_key = 0.0f;
+  float step_of_key = 0.0f, largest = 1.0f;  // the row's greatest value by size
   if constexpr (Biased) {
     least = lane_min_value<L>(least);
     most = lane_max<L>(most);
+    largest = fmaxf(fabsf(least), fabsf(most));
     const float range = most - least, steps = range > 0.0f ? kSteps / range : 0.0f;
     step_of_key = range > 0.0f ? range / kSteps : 0.0f;
 #pragma unroll
@@ -374,12 +376,11 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
       const int g = in != 0 ? __builtin_ctzll(in) : 0, h = out != 0 ? __builtin_ctzll(out) : 0;
       const bool same = !Biased && __shfl(best.first, g * lanes.each, L) == __shfl(best.first, h * lanes.each, L) &&
                         __shfl(best.second, g * lanes.each, L) == __shfl(best.second, h * lanes.each, L);
-      close |= !same && values[h] != -INFINITY &&
-               !(values[g] - values[h] > 4.0f * (margin_of(a, values[g]) + step_of_key));
+      close |= !same && values[h] != -INFINITY && !(values[g] - values[h] > group_margin(largest));
       // Behind two that are the same, a third could be greater by less than 32 bits show.
       for (int o = 0; o < a.groups; ++o)
         close |= same && o != g && o != h && values[o] != -INFINITY &&
-                 !(fabsf(values[o] - values[g]) > 4.0f * margin_of(a, values[g]));
+                 !(fabsf(values[o] - values[g]) > group_margin(largest));
     }
     if (Whole && size % V == 0) {
 #pragma unroll
@@ -439,20 +440,21 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
   // A wave's LDS accesses are performed in order, and a row's lanes are of one wave.
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   if constexpr (Biased) {
+    auto clear = [&](int32_t i, int32_t j) {
+      const float xi = static_cast<float>(row[i]), xj = static_cast<float>(row[j]), si = score(xi), sj = score(xj);
+      return selected(si, xi, bias[i]) - selected(sj, xj, bias[j]) >
+             pair_margin(a.sigmoid, si + sj, largest) + 4.0f * step_of_key;
+    };
     // Neighbours among the k and the next one have to be clear of each other, or the same.
     for (int q = lane; q < a.k && q + 1 < rounds; q += L) {
       const int32_t i = ids[q], j = ids[q + 1];
       if (j < 0) continue;  // none is left
-      const float vi = selection(static_cast<float>(row[i]), bias[i]);
-      const float vj = selection(static_cast<float>(row[j]), bias[j]);
-      close |= !(vi - vj > margin_of(a, vi) + 4.0f * step_of_key) && !(row[i] == row[j] && bias[i] == bias[j]);
+      close |= !clear(i, j) && !(row[i] == row[j] && bias[i] == bias[j]);
     }
     // Where the last chosen and the next one are the same, one behind them could yet be greater.
     if (rounds == a.k + 2 && ids[a.k + 1] >= 0) {
       const int32_t i = ids[a.k - 1], j = ids[a.k], n = ids[a.k + 1];
-      const float vj = selection(static_cast<float>(row[j]), bias[j]);
-      const float vn = selection(static_cast<float>(row[n]), bias[n]);
-      close |= row[i] == row[j] && bias[i] == bias[j] && !(vj - vn > margin_of(a, vj) + 4.0f * step_of_key);
+      close |= row[i] == row[j] && bias[i] == bias[j] && !clear(j, n);
     }
   } else if constexpr (Grouped) {
     // Where logits differ and their scores in 64 bits do not (1, or 0), the scores decide.
@@ -517,7 +519,7 @@ __global__ __launch_bounds__(kThreads) void route_grad(RouteArgs a, const T* __r
                                                        T* __restrict__ dlogits) {
   using Piece = RowPiece<T, Narrow>;
   constexpr int V = kPiece<T>;
-  __shared__ float out[kTile + V];
+  alignas(16) __shared__ float out[kTile + V];
   __shared__ float parts[kTile], sums[kTile];  // by choice, by row
   const int tile = kTile / a.experts;
   const bool dense = !a.sigmoid && !a.renormalize;
@@ -595,8 +597,8 @@ spmm_status check_route_desc(const spmm_route_desc* d) {
   if (d->top_k < 1 || d->top_k > kMaxTopK || d->top_k > open)
     return fail(SPMM_ERR_INVALID_ARGUMENT, "route: top_k must be 1 to 64 and at most the experts of top_groups groups (" +
                                                std::to_string(open) + "), but got " + std::to_string(d->top_k));
-  if (!(d->scale > 0.0) || !(d->scale <= FLT_MAX))
-    return fail(SPMM_ERR_INVALID_ARGUMENT, "route: scale must be finite and positive");
+  if (!(d->scale >= FLT_MIN) || !(d->scale <= FLT_MAX))
+    return fail(SPMM_ERR_INVALID_ARGUMENT, "route: scale must be a positive FP32 number");
   return SPMM_OK;
 }
 
@@ -663,6 +665,7 @@ spmm_status run_route(const spmm_route_desc* d, const void* logits, const float*
   else if (pieces <= 8 && d->groups <= 8) with_shape(integral_constant<int, 8>(), integral_constant<int, 1>());
   else if (pieces <= 16 && d->groups <= 16) with_shape(integral_constant<int, 16>(), integral_constant<int, 1>());
   else if (pieces <= 16 * (16 / V) && d->groups <= 16) with_shape(integral_constant<int, 16>(), integral_constant<int, 16 / V>());
+  else if (pieces <= 32 * (16 / V) && d->groups <= 32) with_shape(integral_constant<int, 32>(), integral_constant<int, 16 / V>());
   else if (pieces <= 64) with_shape(integral_constant<int, 64>(), integral_constant<int, 1>());
   else with_shape(integral_constant<int, 64>(), integral_constant<int, 16 / V>());
   return check_launch("route");

@@ -521,7 +521,7 @@ typedef struct spmm_embedding_desc {
   int64_t width;
   int64_t weight_stride;  /* elements between rows of weight               */
   int64_t grad_stride;    /* elements between rows of grad (gradient only) */
-  double scale;           /* finite                                        */
+  double scale;           /* finite in fp32                                */
   int32_t index_type;
   int32_t value_type;
 } spmm_embedding_desc;
@@ -556,7 +556,7 @@ typedef struct spmm_route_desc {
   int64_t top_k;          /* 1 to 64                                       */
   int64_t groups;         /* 1 to 64, divides the experts                  */
   int64_t top_groups;
-  double scale;           /* finite and positive                           */
+  double scale;           /* positive, a normal fp32 number                */
   int32_t score;          /* spmm_score                                    */
   int32_t renormalize;
   int32_t value_type;     /* logits and dlogits                            */

@@ -61,7 +61,7 @@ def test_embedding_refusals(lib):
                           (emb(count=-1), 4, b"negative extent"), (emb(count=1 << 30), 4, b"below 2^30"),
                           (emb(table=1 << 30), 4, b"below 2^30"), (emb(width=1 << 22), 4, b"below 2^22"),
                           (emb(stride=15), 4, b"rows of weight overlap"), (emb(scale=float("inf")), 1, b"finite"),
-                          (emb(scale=float("nan")), 1, b"finite")):
+                          (emb(scale=float("nan")), 1, b"finite"), (emb(scale=-1e39), 1, b"finite")):
         assert run(d) == code and text in lib.spmm_last_error()
     assert run(emb(), ids=None) == 1 and run(emb(), out=None) == 1
     assert run(emb(count=0), ids=None, out=None) == 0 and run(emb(width=0), ids=None, out=None) == 0
@@ -101,7 +101,7 @@ def test_route_refusals(lib):
                           (rt(experts=1024, groups=128), 1, b"groups"), (rt(groups=8, top_groups=9), 1, b"top_groups"),
                           (rt(groups=8, top_groups=0), 1, b"top_groups"), (rt(groups=8, top_groups=1, k=9), 1, b"top_k"),
                           (rt(scale=0.0), 1, b"scale"), (rt(scale=float("nan")), 1, b"scale"),
-                          (rt(scale=1e39), 1, b"scale"), (rt(score=2), 1, b"score")):
+                          (rt(scale=1e39), 1, b"scale"), (rt(scale=1e-39), 1, b"scale"), (rt(score=2), 1, b"score")):
         assert run(d) == code and text in lib.spmm_last_error(), lib.spmm_last_error()
     assert run(rt(), x=None) == 1 and run(rt(), w=None) == 1 and run(rt(rows=0), x=None) == 0
 
