@@ -108,7 +108,7 @@ struct GroupLanes {
 // an infinity is among its logits.
 template <typename T>
 __device__ inline bool choose_exactly(const RouteArgs& a, const T* row, const float* bias, double* values,
-                                            int32_t* ids) {
+                                      int32_t* ids) {
   constexpr int L = 64;
   const int lane = threadIdx.x % L;
   double m = -kInf64, total = 0.0;
@@ -168,17 +168,20 @@ __device__ inline bool choose_exactly(const RouteArgs& a, const T* row, const fl
 }
 
 // How far apart two selection values in 32 bits have to be for their order to be
-// the exact one.  With e = 2^-24, 2^y has a relative error of 1.25 |y ln 2| e + 2 e.
-// A sigmoid s = 1 / (1 + 2^y) is then off by s (1 - s) times that (at most 0.8 e)
-// and 3 e for its two roundings; a softmax p by p (1.25 |z| + H + 16) e with
-// p |z| < 0.4 and an entropy H of at most 7, 25 p e in all; the sum with the bias
-// rounds by e times the row's greatest value.  Two values: twice that.  Two sums of
-// two: the softmax's four scores are at most 1 together, and there are three
-// roundings more.
+// the exact one.  With e = 2^-24: y = x log2(e) is off by 1.25 |x| e (in units of
+// log e), 2^y by 2 e more.  A sigmoid 1 / (1 + 2^y) is then off by s (1 - s) times
+// that, 0.8 e at most, and by 3 e for its two roundings.  A softmax's sum of up to
+// 1024 terms is off by 1.25 sum p |z| e + 24 e, below 32 e; its logarithm, of up
+// to 10, by 11 e; p = 2^(y - log2 s) in all by (52 + 2.25 |z|) e of itself, with
+// p |z| < 0.4.  A value with its bias rounds by e times the row's greatest value.
+// Two values: twice that.  Two sums of two: a softmax's four scores are at most 1
+// together, and there are three roundings more.
 __device__ inline float pair_margin(bool sigmoid, float scores, float most) {
-  return (sigmoid ? 0x1p-20f : 0x1p-19f * scores) + 0x1p-22f * most;
+  return (sigmoid ? 0x1p-20f : 0x1p-18f * scores) + 0x1p-22f * most;
 }
-__device__ inline float group_margin(float most) { return 0x1p-19f + 0x1p-20f * most; }
+__device__ inline float group_margin(bool sigmoid, float most) {
+  return (sigmoid ? 0x1p-19f : 0x1p-18f) + 0x1p-20f * most;
+}
 
 // Rows of whole pieces; rows whose last piece is moved back to end with them;
 // rows narrower than a piece.
@@ -202,12 +205,12 @@ constexpr float kSteps = 4194300.0f;  // below 2^22
 // taken: where neighbours among them are closer than pair_margin, and not of the
 // same logit and bias, or the groups at the border are as close, the row's choice
 // is made again in 64 bits.  Bound by vector instructions, most of them of the k
-// rounds.  65536 rows of 256 experts in 8 groups, k = 8: all in 64 bits 132 us,
-// one wave a row 233, value and index apart 113.
+// rounds.  65536 rows of 256 experts in 8 groups, k = 8: 53 us (1.3 TB/s); all in
+// 64 bits 132, one wave a row 233, value and index apart 113.
 template <typename T, int L, int I, RowShape Shape, bool Biased, bool Grouped>
 __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* __restrict__ logits,
-                                                       const float* __restrict__ bias, float* __restrict__ weights,
-                                                       int32_t* __restrict__ chosen, float* stats) {
+                                                          const float* __restrict__ bias, float* __restrict__ weights,
+                                                          int32_t* __restrict__ chosen, float* stats) {
   constexpr bool Narrow = Shape == RowShape::kNarrow, Whole = Shape == RowShape::kWhole;
   using Piece = RowPiece<T, Narrow>;
   constexpr int V = kPiece<T>, kGroups = kThreads / L;
@@ -376,11 +379,11 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
       const int g = in != 0 ? __builtin_ctzll(in) : 0, h = out != 0 ? __builtin_ctzll(out) : 0;
       const bool same = !Biased && __shfl(best.first, g * lanes.each, L) == __shfl(best.first, h * lanes.each, L) &&
                         __shfl(best.second, g * lanes.each, L) == __shfl(best.second, h * lanes.each, L);
-      close |= !same && values[h] != -INFINITY && !(values[g] - values[h] > group_margin(largest));
+      close |= !same && values[h] != -INFINITY && !(values[g] - values[h] > group_margin(a.sigmoid, largest));
       // Behind two that are the same, a third could be greater by less than 32 bits show.
       for (int o = 0; o < a.groups; ++o)
         close |= same && o != g && o != h && values[o] != -INFINITY &&
-                 !(fabsf(values[o] - values[g]) > group_margin(largest));
+                 !(fabsf(values[o] - values[g]) > group_margin(a.sigmoid, largest));
     }
     if (Whole && size % V == 0) {
 #pragma unroll
@@ -476,16 +479,18 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
     }
   }
   most = -INFINITY;
+  least = INFINITY;
   float sum = 0.0f;
 #pragma unroll 1
   for (int q = lane; q < a.k; q += L) {
     const int32_t id = ids[q];
     scores[q] = id < 0 ? -INFINITY : static_cast<float>(row[id]);
     most = fmaxf(most, scores[q]);
+    if (id >= 0) least = fminf(least, scores[q]);
   }
   most = lane_max<L>(most);
-  // Sigmoids that are all tiny keep their ratios as logarithms.
-  const bool tiny = a.sigmoid && a.renormalize && most < -80.0f;
+  // Sigmoids that fp32 does not hold keep their ratios as logarithms.
+  const bool tiny = a.sigmoid && a.renormalize && lane_min_value<L>(least) < -80.0f;
   if (tiny) most = log_sigmoid(most);
 #pragma unroll 1
   for (int q = lane; q < a.k; q += L) {

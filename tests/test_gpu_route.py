@@ -89,6 +89,8 @@ def test_masked_experts(spmm_npu, score, renormalize):
         x[1, experts - 1] = 3.0          # one left
         x[2, 0] = 200.0                  # one far above
         x[3] = -300.0                    # scores that vanish in fp32
+        x[5] = -95.0                     # and beside some that do not
+        x[5, ::2] = -78.0
         x[4] = torch.finfo(torch.float32).min  # the type's lowest value is a logit as any other
         bias = normal((experts,), torch.float32, 10, 0.1).cuda()
         bias[experts // 2] = -INF
