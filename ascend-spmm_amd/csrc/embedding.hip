@@ -172,7 +172,8 @@ __global__ __launch_bounds__(kThreads) void sum_runs(SumArgs s, const T* __restr
     if (head || tail) {
       float* slot = s.slots + ((2 * range + (head ? 0 : 1)) * s.pieces + p) * V;
 #pragma unroll
-      for (int j = 0; j < V; j += 4) *reinterpret_cast<f32x4*>(slot + j) = f32x4{sum[j], sum[j + 1], sum[j + 2], sum[j + 3]};
+      for (int j = 0; j < V; j += 4)
+        *reinterpret_cast<f32x4*>(slot + j) = f32x4{sum[j], sum[j + 1], sum[j + 2], sum[j + 3]};
       if (!head && p == 0) s.runs[1 + atomicAdd(s.runs, 1u)] = static_cast<uint32_t>(range);
     } else {
       float v[V];

@@ -155,7 +155,8 @@ __global__ __launch_bounds__(kThreads) void add_choices(RowsArgs a, const T* __r
             for (int q = 0; q < V; ++q) sum[i][q] = __builtin_fmaf(w[u], static_cast<float>(raw[u][i][q]), sum[i][q]);
       }
 #pragma unroll
-      for (int i = 0; i < I; ++i) Tile::Piece::template store<true>(out + r * a.width, Tile::column(c0, i), a.width, sum[i]);
+      for (int i = 0; i < I; ++i)
+        Tile::Piece::template store<true>(out + r * a.width, Tile::column(c0, i), a.width, sum[i]);
     }
 }
 
@@ -239,8 +240,8 @@ spmm_status check_experts_desc(const spmm_experts_desc* d) {
 }
 
 RowsArgs rows_args(const spmm_experts_desc* d) {
-  return {d->rows, d->width, d->stride, d->grad_stride, static_cast<int32_t>(d->top_k), static_cast<int32_t>(d->experts),
-          d->rows * d->top_k};
+  return {d->rows, d->width, d->stride, d->grad_stride, static_cast<int32_t>(d->top_k),
+          static_cast<int32_t>(d->experts), d->rows * d->top_k};
 }
 
 // f(L, I, Narrow) for rows of `width`.
@@ -277,7 +278,8 @@ spmm_status run_add(const spmm_experts_desc* d, const void* y, const float* weig
   return with_type(d->value_type, [&](auto zero) {
     using T = decltype(zero);
     with_row<T>(d->width, [&](auto L, auto I, auto Narrow) {
-      hipLaunchKernelGGL((add_choices<T, decltype(L)::value, decltype(I)::value, decltype(Narrow)::value, Weighted>), row_grid<decltype(L)::value>(d->rows),
+      constexpr int Lanes = decltype(L)::value, Each = decltype(I)::value;
+      hipLaunchKernelGGL((add_choices<T, Lanes, Each, decltype(Narrow)::value, Weighted>), row_grid<Lanes>(d->rows),
                          dim3(kThreads), 0, s, rows_args(d), static_cast<const T*>(y), weights, place, offsets,
                          static_cast<T*>(out));
     });
@@ -332,8 +334,9 @@ spmm_status spmm_expert_pack_run(const spmm_experts_desc* d, const void* x, cons
   return with_type(d->value_type, [&](auto zero) {
     using T = decltype(zero);
     with_row<T>(d->width, [&](auto L, auto I, auto Narrow) {
-      hipLaunchKernelGGL((pack_choices<T, decltype(L)::value, decltype(I)::value, decltype(Narrow)::value>), row_grid<decltype(L)::value>(d->rows), dim3(kThreads), 0,
-                         as_stream(stream), rows_args(d), static_cast<const T*>(x), place, offsets,
+      constexpr int Lanes = decltype(L)::value, Each = decltype(I)::value;
+      hipLaunchKernelGGL((pack_choices<T, Lanes, Each, decltype(Narrow)::value>), row_grid<Lanes>(d->rows),
+                         dim3(kThreads), 0, as_stream(stream), rows_args(d), static_cast<const T*>(x), place, offsets,
                          static_cast<T*>(packed));
     });
     return check_launch("expert_pack");
@@ -373,8 +376,9 @@ spmm_status spmm_expert_restore_grad_run(const spmm_experts_desc* d, const void*
   return with_type(d->value_type, [&](auto zero) {
     using T = decltype(zero);
     with_row<T>(d->width, [&](auto L, auto I, auto Narrow) {
-      hipLaunchKernelGGL((restore_grad<T, decltype(L)::value, decltype(I)::value, decltype(Narrow)::value>), row_grid<decltype(L)::value>(d->rows), dim3(kThreads), 0,
-                         as_stream(stream), rows_args(d), static_cast<const T*>(y), weights, place, offsets,
+      constexpr int Lanes = decltype(L)::value, Each = decltype(I)::value;
+      hipLaunchKernelGGL((restore_grad<T, Lanes, Each, decltype(Narrow)::value>), row_grid<Lanes>(d->rows),
+                         dim3(kThreads), 0, as_stream(stream), rows_args(d), static_cast<const T*>(y), weights, place, offsets,
                          static_cast<const T*>(grad), static_cast<T*>(dy), dweights);
     });
     return check_launch("expert_restore_grad");

@@ -92,6 +92,5 @@ __device__ inline float key_value(uint32_t key) {
   return as_float(key ^ ((key & 0x80000000u) != 0 ? 0x80000000u : 0xFFFFFFFFu));
 }
 constexpr uint32_t kKeyOfMinusInf = 0x007FFFFFu;
-constexpr uint32_t kKeyOfInf = 0xFF800000u;
 
 }  // namespace spmm

@@ -113,7 +113,8 @@ __global__ __launch_bounds__(kThreads) void log_probs_rows(LogArgs a, const T* _
 #pragma unroll
     for (int i = 0; i < I; ++i) raw[i] = Piece::load(x + row * a.stride, column(i), a.classes);
     target = target_of(targets, a.index64, row);
-    xt = static_cast<float>(x[row * a.stride + (static_cast<uint64_t>(target) < static_cast<uint64_t>(a.classes) ? target : 0)]);
+    const bool named = static_cast<uint64_t>(target) < static_cast<uint64_t>(a.classes);
+    xt = static_cast<float>(x[row * a.stride + (named ? target : 0)]);
   };
   fetch(r);
   for (; r < a.rows; r += step) {
@@ -529,18 +530,21 @@ __global__ __launch_bounds__(kThreads) void log_probs_grad(LogArgs a, const T* _
 
 spmm_status check_log_desc(const spmm_log_probs_desc* d) {
   if (d == nullptr) return fail(SPMM_ERR_INVALID_ARGUMENT, "null descriptor");
-  if (!dense_type(d->value_type)) return fail(SPMM_ERR_CONTRACT, "log_probs supports only FP16, BF16 and FP32 tensors");
+  if (!dense_type(d->value_type))
+    return fail(SPMM_ERR_CONTRACT, "log_probs supports only FP16, BF16 and FP32 tensors");
   if (d->index_type != SPMM_INDEX_I32 && d->index_type != SPMM_INDEX_I64)
     return fail(SPMM_ERR_CONTRACT, "log_probs: targets must be int32 or int64");
   if (d->rows < 0 || d->rows > INT32_MAX)
-    return fail(SPMM_ERR_CONTRACT, "log_probs: rows must be at least 0 and below 2^31, but got " + std::to_string(d->rows));
+    return fail(SPMM_ERR_CONTRACT,
+                "log_probs: rows must be at least 0 and below 2^31, but got " + std::to_string(d->rows));
   if (d->classes < 1 || d->classes > INT32_MAX)
     return fail(SPMM_ERR_CONTRACT, "log_probs requires 1 <= classes < 2^31, but got " + std::to_string(d->classes));
   if (d->rows > 1 && d->logits_stride < d->classes)
     return fail(SPMM_ERR_CONTRACT, "log_probs: rows of logits overlap");
   if (d->top < 0 || d->top > kMaxTop || d->top > d->classes)
-    return fail(SPMM_ERR_INVALID_ARGUMENT, "log_probs: top must be at least 0, at most 64 and at most the classes, but got " +
-                                               std::to_string(d->top));
+    return fail(SPMM_ERR_INVALID_ARGUMENT,
+                "log_probs: top must be at least 0, at most 64 and at most the classes, but got " +
+                    std::to_string(d->top));
   return SPMM_OK;
 }
 

@@ -284,7 +284,8 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
 #pragma unroll
           for (int u = 0; u < 4; ++u) b[i][j + u] = bias[begin[i] + j + u < a.experts ? begin[i] + j + u : 0];
         } else {
-          const piece_t<float> four = *reinterpret_cast<const piece_t<float>*>(bias + (Whole && first[i] != 0 ? 0 : begin[i]) + j);
+          const float* from = bias + (Whole && first[i] != 0 ? 0 : begin[i]) + j;
+          const piece_t<float> four = *reinterpret_cast<const piece_t<float>*>(from);
 #pragma unroll
           for (int u = 0; u < 4; ++u) b[i][j + u] = four[u];
         }
@@ -646,7 +647,6 @@ spmm_status run_route(const spmm_route_desc* d, const void* logits, const float*
                          chosen, stats);
   };
   using std::integral_constant;
-  // The fewest lanes that hold the row in one piece each, or in 16 logits each, and a lane a group at least.
   auto with_shape = [&](auto L, auto I) {
     if (d->experts % V == 0) launch(L, I, integral_constant<RowShape, RowShape::kWhole>());
     else launch(L, I, integral_constant<RowShape, RowShape::kMoved>());
@@ -665,14 +665,17 @@ spmm_status run_route(const spmm_route_desc* d, const void* logits, const float*
     }
     return SPMM_OK;
   }
-  if (d->experts < V) launch(integral_constant<int, 8>(), integral_constant<int, 1>(), integral_constant<RowShape, RowShape::kNarrow>());
-  else if (pieces <= 4 && d->groups <= 4) with_shape(integral_constant<int, 4>(), integral_constant<int, 1>());
-  else if (pieces <= 8 && d->groups <= 8) with_shape(integral_constant<int, 8>(), integral_constant<int, 1>());
-  else if (pieces <= 16 && d->groups <= 16) with_shape(integral_constant<int, 16>(), integral_constant<int, 1>());
-  else if (pieces <= 16 * (16 / V) && d->groups <= 16) with_shape(integral_constant<int, 16>(), integral_constant<int, 16 / V>());
-  else if (pieces <= 32 * (16 / V) && d->groups <= 32) with_shape(integral_constant<int, 32>(), integral_constant<int, 16 / V>());
-  else if (pieces <= 64) with_shape(integral_constant<int, 64>(), integral_constant<int, 1>());
-  else with_shape(integral_constant<int, 64>(), integral_constant<int, 16 / V>());
+  // The fewest lanes that hold the row in one piece each, or in 16 logits each, and a lane a group at least.
+  constexpr integral_constant<int, 1> one;
+  constexpr integral_constant<int, 16 / V> more;
+  if (d->experts < V) launch(integral_constant<int, 8>(), one, integral_constant<RowShape, RowShape::kNarrow>());
+  else if (pieces <= 4 && d->groups <= 4) with_shape(integral_constant<int, 4>(), one);
+  else if (pieces <= 8 && d->groups <= 8) with_shape(integral_constant<int, 8>(), one);
+  else if (pieces <= 16 && d->groups <= 16) with_shape(integral_constant<int, 16>(), one);
+  else if (pieces <= 16 * more.value && d->groups <= 16) with_shape(integral_constant<int, 16>(), more);
+  else if (pieces <= 32 * more.value && d->groups <= 32) with_shape(integral_constant<int, 32>(), more);
+  else if (pieces <= 64) with_shape(integral_constant<int, 64>(), one);
+  else with_shape(integral_constant<int, 64>(), more);
   return check_launch("route");
 }
 
