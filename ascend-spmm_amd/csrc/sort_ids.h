@@ -3,31 +3,46 @@
 //
 // Up to kRankMost keys take one launch, in which each key's place is counted:
 // the keys below it, and the equal ones before it.  More keys are counted and
-// placed digit by digit, three launches each: count_digits counts the digits of
-// each tile of keys, add_digits adds each digit's counts up over the tiles, and
-// place_digits finds each key's place.  Within a tile a wave takes 64
-// consecutive keys at a time, in order, and ranks each among the equal ones by
-// ballots over the digit's bits: no atomic decides an order.
+// placed digit by digit: count_digits counts the digits of each tile of keys,
+// add_digits adds each digit's counts up over the tiles (of few tiles
+// place_digits does that by itself, two launches for three), and place_digits
+// finds each key's place.  Within a tile a wave takes 64 consecutive keys at a
+// time, in order, and ranks each among the equal ones by ballots over the
+// digit's bits: no atomic decides an order.
 #pragma once
 
 #include "lane_reduce.h"
 
 namespace spmm {
 
-constexpr int kSortThreads = 256;
-constexpr int kSortWaves = kSortThreads / 64;
+constexpr int kRankThreads = 256;
+constexpr int kManyWaves = 4, kFewWaves = 16;    // of a tile's work-group
 constexpr int kSortBits = 11;                    // most bits of one digit of several
 constexpr int kSortBins = (1 << kSortBits) + 1;  // most values of a single digit
 constexpr int64_t kRankMost = 4096;
 
+// Few tiles of many waves, so that place_digits adds up the counts of the tiles
+// before by itself: as many as leave it 32768 counts to read, and each wave at
+// most 4 rounds of 64 keys, 2 where it has many counts to read.  Beyond, that
+// costs more than the launch of add_digits.  A plan for 64 experts: 16384
+// choices 7.5 us against 9.0, 524288 11.3 against 14.4, 1048576 (8 rounds) 15.8
+// against 18.3; for 511: 100000 choices 10.6 against 12.4, 524288 (8 rounds) 18.3
+// against 16.0; for 2048: 16384 choices 13.9 against 17.0, 49143 (4 rounds) 19.0
+// against 18.4.
+inline int64_t few_most(int bins) { return bins > 256 ? 32768 / bins : 128; }
+inline bool few_tiles(int64_t n, int bins) { return n <= few_most(bins) * kFewWaves * 64 * (bins > 256 ? 2 : 4); }
+
 // Keys of a wave in one tile, in rounds of 64: as few as leave 512 tiles at
-// most, as a round waits for the one before it.
-inline int sort_rounds(int64_t n) {
+// most (few_most of the few), as a round waits for the one before it.
+inline int sort_rounds(int64_t n, int bins) {
+  if (few_tiles(n, bins)) return static_cast<int>(ceil_div(n > 0 ? n : 1, few_most(bins) * kFewWaves * 64));
   int rounds = 1;
-  while (rounds < 16 && n > int64_t(512) * kSortThreads * rounds) rounds *= 2;
+  while (rounds < 16 && n > int64_t(512) * kManyWaves * 64 * rounds) rounds *= 2;
   return rounds;
 }
-inline int64_t sort_tiles(int64_t n) { return ceil_div(n > 0 ? n : 1, kSortThreads * sort_rounds(n)); }
+inline int64_t sort_tiles(int64_t n, int bins) {
+  return ceil_div(n > 0 ? n : 1, (few_tiles(n, bins) ? kFewWaves : kManyWaves) * 64 * sort_rounds(n, bins));
+}
 
 // Bits of the values 0 to `most`.
 inline int bits_of(int64_t most) {
@@ -43,12 +58,12 @@ struct Digit {
 };
 
 // Counts by wave of the tile's digits in LDS: hist[wave][bins].
-template <typename Keys>
+template <int W, typename Keys>
 __device__ inline void count_tile(uint32_t* hist, Digit d, int64_t n, int rounds, Keys keys) {
-  for (int k = threadIdx.x; k < kSortWaves * d.bins; k += kSortThreads) hist[k] = 0;
+  for (int k = threadIdx.x; k < W * d.bins; k += W * 64) hist[k] = 0;
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kSortWaves + wave) * rounds * 64 + lane;
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * W + wave) * rounds * 64 + lane;
   for (int q = 0; q < rounds; ++q)
     if (first + q * 64 < n) atomicAdd(&hist[wave * d.bins + d.of(keys(first + q * 64))], 1u);
   __syncthreads();
@@ -57,22 +72,22 @@ __device__ inline void count_tile(uint32_t* hist, Digit d, int64_t n, int rounds
 // counts: [tiles][bins].  keys(i) gives key i.  (Counting the next digit in
 // place_digits, by atomics, costs more than this launch: 10.4 and 22.9 us for
 // 6.6 + 2.7 and 9.2 + 4.8.)
-template <typename Keys>
-__global__ __launch_bounds__(kSortThreads) void count_digits(Digit d, int64_t n, int rounds, Keys keys,
-                                                             uint32_t* counts) {
-  __shared__ uint32_t hist[kSortWaves * kSortBins];
-  count_tile(hist, d, n, rounds, keys);
-  for (int b = threadIdx.x; b < d.bins; b += kSortThreads) {
+template <int W, typename Keys>
+__global__ __launch_bounds__(W * 64) void count_digits(Digit d, int64_t n, int rounds, Keys keys, uint32_t* counts) {
+  __shared__ uint32_t hist[W * kSortBins];
+  count_tile<W>(hist, d, n, rounds, keys);
+  for (int b = threadIdx.x; b < d.bins; b += W * 64) {
     uint32_t sum = 0;
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) sum += hist[w * d.bins + b];
+    for (int w = 0; w < W; ++w) sum += hist[w * d.bins + b];
     counts[static_cast<int64_t>(blockIdx.x) * d.bins + b] = sum;
   }
 }
 
 // Exclusive sums of values[0..bins) in LDS over the work-group, in place.
+template <int W>
 __device__ inline void scan_bins(uint32_t* values, int bins, uint32_t* sums) {
-  const int per = (bins + kSortThreads - 1) / kSortThreads, tid = threadIdx.x;
+  const int per = (bins + W * 64 - 1) / (W * 64), tid = threadIdx.x;
   uint32_t own = 0;
   for (int k = 0; k < per; ++k)
     if (tid * per + k < bins) own += values[tid * per + k];
@@ -110,20 +125,42 @@ __device__ inline uint64_t same_digit(uint32_t digit, int bits, bool valid) {
 
 // put(i, key, place) for each key; base_of(bin, start) for each digit, with the
 // place of its first key, by the first work-group.
-template <typename Keys, typename Put, typename Bases>
-__global__ __launch_bounds__(kSortThreads) void place_digits(Digit d, int64_t n, int rounds, Keys keys,
-                                                             const uint32_t* counts, const uint32_t* totals, Put put,
-                                                             Bases base_of) {
-  __shared__ uint32_t hist[kSortWaves * kSortBins], base[kSortBins], sums[kSortWaves];
-  for (int b = threadIdx.x; b < d.bins; b += kSortThreads) base[b] = totals[b];
-  count_tile(hist, d, n, rounds, keys);  // with barriers
-  scan_bins(base, d.bins, sums);
-  for (int b = threadIdx.x; b < d.bins; b += kSortThreads) {
+template <int W, typename Keys, typename Put, typename Bases>
+__global__ __launch_bounds__(W * 64) void place_digits(Digit d, int64_t n, int rounds, Keys keys,
+                                                       const uint32_t* counts, const uint32_t* totals, Put put,
+                                                       Bases base_of) {
+  constexpr int kThreads = W * 64;
+  constexpr bool kFew = W == kFewWaves;
+  __shared__ uint32_t hist[W * kSortBins], base[kSortBins], before[kFew ? kSortBins : 1], sums[W];
+  if constexpr (kFew) {
+    for (int b = threadIdx.x; b < d.bins; b += kThreads) base[b] = before[b] = 0;
+    __syncthreads();
+    const int tiles = static_cast<int>(gridDim.x), own = static_cast<int>(blockIdx.x);
+    const int shares = d.bins < kThreads ? kThreads / d.bins : 1;
+    for (int k = threadIdx.x; k < shares * d.bins; k += kThreads) {
+      const int share = k / d.bins, b = k - share * d.bins;
+      uint32_t all = 0, lower = 0;
+#pragma unroll 8
+      for (int t = share; t < tiles; t += shares) {
+        const uint32_t c = counts[static_cast<int64_t>(t) * d.bins + b];
+        all += c;
+        lower += t < own ? c : 0;
+      }
+      atomicAdd(&base[b], all);
+      atomicAdd(&before[b], lower);
+    }
+  } else {
+    for (int b = threadIdx.x; b < d.bins; b += kThreads) base[b] = totals[b];
+  }
+  count_tile<W>(hist, d, n, rounds, keys);  // with barriers
+  scan_bins<W>(base, d.bins, sums);
+  for (int b = threadIdx.x; b < d.bins; b += kThreads) {
     uint32_t at = base[b];
     if (blockIdx.x == 0) base_of(b, at);
-    at += counts[static_cast<int64_t>(blockIdx.x) * d.bins + b];
+    if constexpr (kFew) at += before[b];
+    else at += counts[static_cast<int64_t>(blockIdx.x) * d.bins + b];
 #pragma unroll
-    for (int w = 0; w < kSortWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       const uint32_t c = hist[w * d.bins + b];
       hist[w * d.bins + b] = at;
       at += c;
@@ -132,7 +169,7 @@ __global__ __launch_bounds__(kSortThreads) void place_digits(Digit d, int64_t n,
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   volatile uint32_t* next = hist + wave * d.bins;  // the place of the wave's next key of each digit
-  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kSortWaves + wave) * rounds * 64 + lane;
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * W + wave) * rounds * 64 + lane;
   for (int q = 0; q < rounds; ++q) {
     const int64_t i = first + q * 64;
     const bool valid = i < n;
@@ -154,14 +191,14 @@ __global__ __launch_bounds__(kSortThreads) void place_digits(Digit d, int64_t n,
 // 4096 keys: 5 us, against 27 for two digits.
 constexpr int kRankKeys = 16;
 template <typename Keys, typename Put, typename Bases>
-__global__ __launch_bounds__(kSortThreads) void rank_keys(int n, int bins, Keys keys, Put put, Bases base_of) {
+__global__ __launch_bounds__(kRankThreads) void rank_keys(int n, int bins, Keys keys, Put put, Bases base_of) {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   __shared__ u32x4 all[kRankMost / 4 + 64];
-  __shared__ uint32_t part[kSortWaves][kRankKeys];
+  __shared__ uint32_t part[kRankThreads / 64][kRankKeys];
   uint32_t* words = reinterpret_cast<uint32_t*>(all);
   // Filled up with keys above all others, which no key counts.
   const int padded = (n + 63) / 64 * 64;
-  for (int k = threadIdx.x; k < padded; k += kSortThreads) words[k] = k < n ? keys(k) : ~0u;
+  for (int k = threadIdx.x; k < padded; k += kRankThreads) words[k] = k < n ? keys(k) : ~0u;
   __syncthreads();
   const int own = threadIdx.x % kRankKeys, share = threadIdx.x / kRankKeys, wave = threadIdx.x >> 6;
   const int q = blockIdx.x * kRankKeys + own;
@@ -169,7 +206,7 @@ __global__ __launch_bounds__(kSortThreads) void rank_keys(int n, int bins, Keys 
   const uint32_t key = q < n ? words[q] : static_cast<uint32_t>(q - n);
   const int index = q < n ? q : 0;
   uint32_t rank = 0;
-  for (int k = share; k < padded / 4; k += kSortThreads / kRankKeys) {
+  for (int k = share; k < padded / 4; k += kRankThreads / kRankKeys) {
     const u32x4 v = all[k];
 #pragma unroll
     for (int j = 0; j < 4; ++j) rank += v[j] < key + (4 * k + j < index ? 1u : 0u);
@@ -181,13 +218,13 @@ __global__ __launch_bounds__(kSortThreads) void rank_keys(int n, int bins, Keys 
   if (threadIdx.x >= kRankKeys || q >= n + bins) return;
   rank = 0;
 #pragma unroll
-  for (int w = 0; w < kSortWaves; ++w) rank += part[w][own];
+  for (int w = 0; w < kRankThreads / 64; ++w) rank += part[w][own];
   if (q < n) put(q, key, rank);
   else base_of(q - n, rank);
 }
 
 // Words of the counts and totals of n keys.
-inline int64_t sort_words(int64_t n, int bins) { return n <= kRankMost ? 0 : (sort_tiles(n) + 1) * bins; }
+inline int64_t sort_words(int64_t n, int bins) { return n <= kRankMost ? 0 : (sort_tiles(n, bins) + 1) * bins; }
 
 // Turns each digit's counts into those of the tiles before, and totals[bins]
 // into the counts of all.
@@ -196,23 +233,29 @@ spmm_status launch_add_digits(int bins, int64_t tiles, uint32_t* counts, uint32_
 template <typename Keys, typename Put, typename Bases>
 spmm_status sort_by_rank(int64_t n, int bins, Keys keys, Put put, Bases base_of, hipStream_t s) {
   hipLaunchKernelGGL((rank_keys<Keys, Put, Bases>), dim3(static_cast<unsigned>(ceil_div(n + bins, kRankKeys))),
-                     dim3(kSortThreads), 0, s, static_cast<int>(n), bins, keys, put, base_of);
+                     dim3(kRankThreads), 0, s, static_cast<int>(n), bins, keys, put, base_of);
   return check_launch("rank_keys");
 }
 
-// One digit's three launches.  `counts` holds sort_words(n, d.bins) words.
+// One digit's launches.  `counts` holds sort_words(n, d.bins) words.
 template <typename Keys, typename Put, typename Bases>
 spmm_status sort_digit(Digit d, int64_t n, Keys keys, uint32_t* counts, Put put, Bases base_of, hipStream_t s) {
-  const int64_t tiles = sort_tiles(n);
-  const int rounds = sort_rounds(n);
+  const int64_t tiles = sort_tiles(n, d.bins);
+  const int rounds = sort_rounds(n, d.bins);
   uint32_t* totals = counts + tiles * d.bins;
   const dim3 grid(static_cast<unsigned>(tiles));
-  hipLaunchKernelGGL(count_digits<Keys>, grid, dim3(kSortThreads), 0, s, d, n, rounds, keys, counts);
-  if (spmm_status st = check_launch("count_digits")) return st;
-  if (spmm_status st = launch_add_digits(d.bins, tiles, counts, totals, s)) return st;
-  hipLaunchKernelGGL((place_digits<Keys, Put, Bases>), grid, dim3(kSortThreads), 0, s, d, n, rounds, keys, counts,
-                     totals, put, base_of);
-  return check_launch("place_digits");
+  auto launch = [&](auto waves) {
+    constexpr int W = decltype(waves)::value;
+    hipLaunchKernelGGL((count_digits<W, Keys>), grid, dim3(W * 64), 0, s, d, n, rounds, keys, counts);
+    if (spmm_status st = check_launch("count_digits")) return st;
+    if (W == kManyWaves)
+      if (spmm_status st = launch_add_digits(d.bins, tiles, counts, totals, s)) return st;
+    hipLaunchKernelGGL((place_digits<W, Keys, Put, Bases>), grid, dim3(W * 64), 0, s, d, n, rounds, keys, counts,
+                       totals, put, base_of);
+    return check_launch("place_digits");
+  };
+  if (few_tiles(n, d.bins)) return launch(std::integral_constant<int, kFewWaves>());
+  return launch(std::integral_constant<int, kManyWaves>());
 }
 
 }  // namespace spmm

@@ -84,6 +84,16 @@ def test_sort_of_many_choices(spmm_npu, count):
     assert torch.equal(one.offsets.cpu(), offsets)
 
 
+@pytest.mark.parametrize("count,few", [(1, 128), (255, 128), (256, 127), (2048, 15)])
+def test_sort_of_few_and_many_tiles(spmm_npu, count, few):
+    """From one key beyond a launch's to one beyond the most of the few tiles, in 1 to 4 rounds a wave."""
+    for n in (4097, 1024 * few, 1024 * few + 1, 2048 * few, 2048 * few + 1, 3000 * few, 4096 * few, 4096 * few + 1):
+        ids = choices(n, 1, count, seed=n, dropped=0.05)
+        offsets, place = plan(ids, count)
+        p = spmm_npu.ExpertPlan(ids.cuda(), count)
+        assert torch.equal(p.offsets.cpu(), offsets) and torch.equal(p.place.cpu().reshape(-1), place)
+
+
 def test_strided_tensors(spmm_npu):
     ids = choices(60, 2, 4)
     big = normal((130, 100), torch.float16, 5).cuda()
