@@ -91,3 +91,43 @@ def test_rows_without_an_expert_pass_through(spmm_npu):
     grad[::3] = float("nan")
     (dw,) = torch.autograd.grad(out, w, grad)
     assert bool(torch.isfinite(dw).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_layer_captured_with_its_gradients(spmm_npu, dtype):
+    """A training step of the layer in one graph: every replay, with other inputs and eager
+    steps in between, gives what an eager step gives."""
+    g = torch.Generator().manual_seed(2)
+    rows, count, width, classes = 5000, 5, 48, 3000
+    normal = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda()  # noqa: E731
+    table, router, w = normal(700, width), normal(1, width, count), normal(count, width, width)
+    head = normal(1, width, classes)
+    every = torch.tensor([0, rows], device="cuda")
+    ids = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    labels = torch.zeros(rows, dtype=torch.int64, device="cuda")
+
+    def step():
+        leaves = [t.detach().requires_grad_(True) for t in (table, router, w, head)]
+        t, r, e, h = leaves
+        x = spmm_npu.embedding(t, ids)
+        weights, experts = spmm_npu.route(spmm_npu.grouped_matmul(x, r, every), 2, renormalize=False)
+        plan = spmm_npu.ExpertPlan(experts, count)
+        y = plan.restore(spmm_npu.grouped_matmul(plan.pack(x), e, plan.offsets), weights)
+        logp, entropy, _, top = spmm_npu.log_probs(spmm_npu.grouped_matmul(y, h, every), labels, top=2)
+        return (logp.detach(), entropy.detach(), top) + torch.autograd.grad((logp, entropy), leaves, (up, up))
+
+    up = torch.randn(rows, generator=g).cuda()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(4):
+        ids.copy_(torch.randint(-1, 700, (rows,), generator=g) if k % 2 else torch.full((rows,), 3))
+        labels.copy_(torch.randint(-1, classes, (rows,), generator=g))
+        table.copy_(normal(700, width))
+        graph.replay()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
