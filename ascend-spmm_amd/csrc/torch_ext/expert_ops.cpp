@@ -147,11 +147,13 @@ struct Route : torch::autograd::Function<Route> {
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["bias"] = bias.has_value();
     ctx->mark_non_differentiable({experts});
+    ctx->set_materialize_grads(false);  // the ids' would be zeros, filled by a launch
     return {weights, experts};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_differentiable_once("route");
+    if (!grads[0].defined()) return variable_list(8);
     const variable_list saved = ctx->get_saved_variables();
     const at::Tensor& logits = saved[0];
     c10::DeviceGuard guard(logits.device());
@@ -367,6 +369,7 @@ struct LogProbs : torch::autograd::Function<LogProbs> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     check_differentiable_once("log_probs");
+    if (!grads[0].defined() && !grads[1].defined()) return variable_list(3);
     const variable_list saved = ctx->get_saved_variables();
     const at::Tensor& logits = saved[0];
     c10::DeviceGuard guard(logits.device());

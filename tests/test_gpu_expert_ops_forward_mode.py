@@ -61,3 +61,28 @@ def test_many_streams_at_once(spmm_npu):
     torch.cuda.synchronize()
     for k, result in enumerate(got):
         assert all(torch.equal(a, b) for a, b in zip(result, want[k % 4]))
+
+
+class Ends(torch.autograd.Function):
+    """Gives no gradient."""
+
+    @staticmethod
+    def forward(ctx, *xs):
+        return xs[0].sum()
+
+    @staticmethod
+    def backward(ctx, grad):
+        return None, None
+
+
+def test_no_gradient_comes_in(spmm_npu):
+    x = torch.randn(5, 12, device="cuda", requires_grad=True)
+    ids = torch.zeros(5, dtype=torch.int64, device="cuda")
+    weights, _ = spmm_npu.route(x, 2)
+    logp, entropy, _, _ = spmm_npu.log_probs(x, ids)
+    for a, b in ((weights, weights), (logp, entropy)):
+        (dx,) = torch.autograd.grad(Ends.apply(a, b), x, allow_unused=True)
+        assert dx is None or not dx.any()
+    rows = spmm_npu.embedding(x, ids)
+    (dx,) = torch.autograd.grad(Ends.apply(rows, rows), x, allow_unused=True)
+    assert dx is None or not dx.any()
