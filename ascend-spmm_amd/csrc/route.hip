@@ -168,7 +168,8 @@ __device__ inline bool choose_exactly(const RouteArgs& a, const T* row, const fl
   if (a.groups > 1) {
     const GroupLanes<L> lanes(a);
     const BestTwo<double> best = lanes.best(a, values);
-    const uint64_t key = best.nan ? ~uint64_t(0) : key_of(best.second == -kInf64 ? best.first : best.first + best.second);
+    const double sum = best.second == -kInf64 ? best.first : best.first + best.second;
+    const uint64_t key = best.nan ? ~uint64_t(0) : key_of(sum);
     int rank = 0;
     for (int o = 0; o < a.groups; ++o) {
       const uint64_t other = __shfl(key, o * lanes.each, L);
@@ -522,7 +523,8 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
       const int64_t which = static_cast<int64_t>(blockIdx.x) * kGroups + (threadIdx.x >> 6) * (64 / L) + group;
       int32_t* into = all_ids + ((threadIdx.x >> 6) * (64 / L) + group) * (2 * a.k + 2);
       // With values that are no numbers, the chosen may be others than the NaN: it is to be seen all the same.
-      if (choose_exactly(a, logits + which * a.stride, bias, exact, into) && (threadIdx.x & 63) / L == group) seen = NAN;
+      if (choose_exactly(a, logits + which * a.stride, bias, exact, into) && (threadIdx.x & 63) / L == group)
+        seen = NAN;
     }
   }
   most = -INFINITY;
@@ -577,7 +579,8 @@ __global__ __launch_bounds__(kThreads) void route_grad(RouteArgs a, const T* __r
   __shared__ float parts[kTile], sums[kTile];  // by choice, by row
   const int tile = kTile / a.experts;
   const bool dense = !a.sigmoid && !a.renormalize;
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * tile; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * tile) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * tile;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * tile; r0 < a.rows; r0 += step) {
     const int rows = static_cast<int>(a.rows - r0 < tile ? a.rows - r0 : tile);
     const int choices = rows * a.k, all = rows * a.experts;
     for (int q = threadIdx.x; q < choices; q += kThreads) {
@@ -682,17 +685,17 @@ spmm_status run_route(const spmm_route_desc* d, const void* logits, const float*
     const size_t lds = exact + kGroups * (values + (2 * static_cast<size_t>(a.k) + 2) * 4);
     const T* x = static_cast<const T*>(logits);
     if (bias != nullptr && a.groups > 1)
-      hipLaunchKernelGGL((route_rows<T, kL, kI, kShape, true, true>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
-                         chosen, stats);
+      hipLaunchKernelGGL((route_rows<T, kL, kI, kShape, true, true>), grid, dim3(kThreads), lds, s, a, x, bias,
+                         weights, chosen, stats);
     else if (bias != nullptr)
-      hipLaunchKernelGGL((route_rows<T, kL, kI, kShape, true, false>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
-                         chosen, stats);
+      hipLaunchKernelGGL((route_rows<T, kL, kI, kShape, true, false>), grid, dim3(kThreads), lds, s, a, x, bias,
+                         weights, chosen, stats);
     else if (a.groups > 1)
-      hipLaunchKernelGGL((route_rows<T, kL, kI, kShape, false, true>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
-                         chosen, stats);
+      hipLaunchKernelGGL((route_rows<T, kL, kI, kShape, false, true>), grid, dim3(kThreads), lds, s, a, x, bias,
+                         weights, chosen, stats);
     else
-      hipLaunchKernelGGL((route_rows<T, kL, kI, kShape, false, false>), grid, dim3(kThreads), lds, s, a, x, bias, weights,
-                         chosen, stats);
+      hipLaunchKernelGGL((route_rows<T, kL, kI, kShape, false, false>), grid, dim3(kThreads), lds, s, a, x, bias,
+                         weights, chosen, stats);
   };
   using std::integral_constant;
   auto with_shape = [&](auto L, auto I) {
