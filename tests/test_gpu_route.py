@@ -64,6 +64,27 @@ def test_groups(spmm_npu, experts, groups, top_groups, k, score, dtype):
     run(spmm_npu, x, k, score, groups=groups, top_groups=top_groups, renormalize=False)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1, 3, 4, 8, 12, 16, 20, 32, 64, 128, 252])
+def test_every_shape_of_groups(spmm_npu, size, dtype):
+    """Groups of few and many pieces on few and many lanes, biases of -inf and masked logits among them."""
+    for groups in (2, 3, 4, 5, 8, 16, 17, 32, 63, 64):
+        experts = groups * size
+        if experts > 1024:
+            continue
+        x = normal((9, experts), dtype, experts).cuda()
+        x[1, ::3] = -INF
+        x[2, : experts - size] = -INF
+        bias = normal((experts,), torch.float32, groups, 0.2).cuda()
+        top_groups = max(1, groups // 3)
+        k = min(5, top_groups * size)
+        run(spmm_npu, x, k, "sigmoid", bias=bias, groups=groups, top_groups=top_groups)
+        bias[::7] = -INF
+        run(spmm_npu, x, k, "sigmoid", bias=bias, groups=groups, top_groups=top_groups)
+        run(spmm_npu, x, k, "softmax", bias=bias)
+        run(spmm_npu, x, k, "softmax", groups=groups, top_groups=top_groups)
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_ties_go_to_the_lowest_index(spmm_npu, score):
     for experts in (5, 64, 300):
