@@ -9,8 +9,9 @@
 //
 // All of it is fp32 and in powers of two: y = fma(x, log2(e), -c), c = m log2(e)
 // rounded, rounds once for each logit.  c need not be exact, as every y has the
-// same c: it is taken out again as a whole.  Where c would overflow (|m| above
-// 1e37, so rows of a type's lowest value), y = (x - m) log2(e).
+// same c: it is taken out again as a whole.  But y of the maximum is what c was
+// rounded by, so c has to be small enough that this is next to nothing: beyond
+// |m| = 2^20, y = (x - m) log2(e), which rounds twice.
 #include <cfloat>
 #include <cmath>
 
@@ -26,7 +27,9 @@ constexpr int kMaxTop = 64;
 constexpr int kMaxParts = 64;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.693147180559945309417f;
-constexpr float kFar = 1e37f;     // of a maximum whose c would not do
+// A greater maximum has a c that will not do.  Up to it c is below 2^21, and
+// rounded by 2^-4 at most.
+constexpr float kFar = 0x1p20f;
 constexpr float kFloor = -300.0f;  // below it 2^y is zero; a finite stand-in for an infinite y
 
 // The product by itself: contracted with a difference of two of them it would
@@ -225,10 +228,12 @@ struct Part {
   float m, s, t;
 };
 
-// 2^(y of one origin - y of another): the factor that takes sums from `from` to
-// `to`, and the shift that t takes besides.  Sums from far below vanish.
+// y of one origin - y of another: 2^shift is the factor that takes sums from
+// `from` to `to`, the shift what t takes besides.  Sums from far below vanish.  A
+// far origin is m log2(e) itself, the others are c.
 __device__ inline float origin_shift(const Origin& from, const Origin& to) {
-  return to.far ? (from.m - to.m) * kLog2e : from.c - to.c;
+  if (to.far) return from.far ? (from.m - to.m) * kLog2e : -from.near(to.m);
+  return from.far ? to.near(from.m) : from.c - to.c;
 }
 
 // Wider rows: a work-group streams one part of a row, each thread with a
@@ -265,7 +270,7 @@ __global__ __launch_bounds__(kWideThreads) void log_probs_wide(LogArgs a, const 
   const int64_t p0 = pieces * part / parts, p1 = pieces * (part + 1) / parts;
   const int tid = threadIdx.x;
 
-  // Sums relative to a maximum no lower than -kFar, so that lower logits alone leave s zero.
+  // Sums relative to a maximum no lower than -kFar: logits far below it alone leave s zero.
   float m = -INFINITY, s = 0.0f, t = 0.0f;
   auto add = [&](auto N, const float (&v)[decltype(N)::value]) {
     float top = m;
