@@ -232,6 +232,7 @@ enum class RowShape { kWhole, kMoved, kNarrow };
 // is looked for.
 constexpr uint32_t kFine = 0x1FFF, kCoarse = 0x3FF;
 constexpr float kSteps = 4194300.0f;  // below 2^22
+constexpr float kLargest = 1e38f;
 
 // L lanes a row, which hold I pieces of 16 bytes of it each.  The k best are taken
 // one after another.  Without a bias the logits are the keys, and exact.  With one
@@ -367,6 +368,8 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
       least = lane_min_value<L>(least);
     }
     largest = fmaxf(fabsf(least), fabsf(most));
+    // Greater values' range, or the sum of two, may overflow: 64 bits decide.
+    close |= !(largest <= kLargest);
     const float range = most - least, steps = range > 0.0f ? kSteps / range : 0.0f;
     step_of_key = range > 0.0f ? range / kSteps : 0.0f;
 #pragma unroll
