@@ -372,6 +372,8 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
     close |= !(largest <= kLargest);
     const float range = most - least, steps = range > 0.0f ? kSteps / range : 0.0f;
     step_of_key = range > 0.0f ? range / kSteps : 0.0f;
+    // A range so small that this overflows has no keys.
+    close |= !(steps <= FLT_MAX);
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
