@@ -233,6 +233,7 @@ enum class RowShape { kWhole, kMoved, kNarrow };
 constexpr uint32_t kFine = 0x1FFF, kCoarse = 0x3FF;
 constexpr float kSteps = 4194300.0f;  // below 2^22
 constexpr float kLargest = 1e38f;
+constexpr float kFar = 0x1p20f;
 
 // L lanes a row, which hold I pieces of 16 bytes of it each.  The k best are taken
 // one after another.  Without a bias the logits are the keys, and exact.  With one
@@ -292,9 +293,13 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
       for (int j = 0; j < V; ++j) s += expf(x[i][j] - m);
     ls = logf(lane_sum<L>(s));
   }
+  bool close = false;
   if (kChecked && !a.sigmoid) {
     float s = 0.0f;
     c = m * kLog2e;
+    // 64 bits decide where c is rounded by more than 2^-4.  (Of -FLT_MAX, which is also the maximum
+    // of a row without any expert, the scores are NaN, which no check below lets pass.)
+    close = !(fabsf(m) <= kFar) && m > -FLT_MAX;
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
@@ -307,7 +312,6 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
   auto score = [&](float v) { return a.sigmoid ? sigmoid(v) : softmax(v); };
   auto selected = [&](float s, float v, float b) { return v == -INFINITY || b == -INFINITY ? -INFINITY : s + b; };
   float v[I][V], least = INFINITY, most = -INFINITY;
-  bool close = false;
   float seen = 0.0f;
   if constexpr (Biased) {
     float b[I][V];
