@@ -240,9 +240,11 @@ constexpr float kFar = 0x1p20f;
 // (Biased) the keys are selection values in 32 bits, and two more than k are
 // taken: where neighbours among them are closer than pair_margin, and not of the
 // same logit and bias, or the groups at the border are as close, the row's choice
-// is made again in 64 bits.  Bound by vector instructions, most of them of the k
-// rounds.  65536 rows of 256 experts in 8 groups, k = 8: 45 us (1.6 TB/s, vector
-// units always busy); all in 64 bits 132, one wave a row 233, value and index apart 113.
+// is made again in 64 bits.  In groups without a bias the keys are the logits, and
+// 64 bits decide where two that differ may have the same score.  Bound by vector
+// instructions, most of them of the k rounds.  65536 rows of 256 experts in 8
+// groups, k = 8: 45 us (1.6 TB/s, vector units always busy); all in 64 bits 132, one
+// wave a row 233, value and index apart 113.
 template <typename T, int L, int I, RowShape Shape, bool Biased, bool Grouped>
 __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* __restrict__ logits,
                                                           const float* __restrict__ bias, float* __restrict__ weights,
@@ -497,6 +499,33 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
     }
     if (lane == 0) ids[q] = best > kNone ? static_cast<int32_t>(win) : -1;
   }
+  // Of groups without a bias: whether a logit below x may differ from it and have its score in 64 bits.
+  // The nearest is |x| 2^-24 away or more.  Over a gap in x a softmax changes by gap of itself, and its
+  // x - m is rounded besides, a sigmoid by (1 - s) gap, at least min(1, e^-x) gap / 2: beyond x = 2^-24
+  // and up to 14, where x e^-x is 2^-24 at least, that is more than a few roundings.
+  auto may_tie = [&](float x) {
+    return a.sigmoid ? !(x < 14.0f && fabsf(x) > 0x1p-24f) : !(fabsf(x) > 0x1p-24f * (1.0f + (m - x)));
+  };
+  auto ties = [&](float x, float gap) {
+    return !(a.sigmoid ? gap * fminf(expf(-x), 1.0f) > 0x1p-49f : gap > 0x1p-49f * (1.0f + (m - x)));
+  };
+  float below = -INFINITY;  // the greatest logit that is lower than the last one chosen, where it may tie
+  if constexpr (Grouped && !Biased) {
+    constexpr uint32_t kValue = kPacked ? ~kFine : ~0u;
+    auto logit = [&](uint32_t key) { return key_value(kPacked && key < 0x80000000u ? key | kFine : key & kValue); };
+    if (__ballot(best > kNone && may_tie(logit(best))) != 0) {
+      uint32_t own = 0;
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const uint32_t value = key[i][j] & kValue;
+          own = value < (best & kValue) && value > own ? value : own;
+        }
+      own = lane_max<L>(own);
+      if (own > (kNone & kValue)) below = logit(own);
+    }
+  }
   // A wave's LDS accesses are performed in order, and a row's lanes are of one wave.
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   if constexpr (Biased) {
@@ -517,10 +546,15 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
       close |= row[i] == row[j] && bias[i] == bias[j] && !clear(j, n);
     }
   } else if constexpr (Grouped) {
-    // Where logits differ and their scores in 64 bits do not (1, or 0), the scores decide.
+    // Where logits differ and their scores in 64 bits do not, the scores decide: those next to zero, and
+    // neighbours among the k and the next one.
+    for (int q = lane; q < a.k; q += L) scores[q] = ids[q] < 0 ? -INFINITY : static_cast<float>(row[ids[q]]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     for (int q = lane; q < a.k; q += L) {
-      const float xq = ids[q] < 0 ? 0.0f : static_cast<float>(row[ids[q]]);
-      close |= ids[q] >= 0 && (a.sigmoid ? !(xq < 30.0f && xq > -700.0f) : !(xq - m > -700.0f));
+      const float x0 = scores[q], x1 = q + 1 == a.k ? below : scores[q + 1];
+      if (x0 == -INFINITY) continue;  // none is left
+      close |= !((a.sigmoid ? x0 : x0 - m) > -700.0f);
+      if (may_tie(x0) && x0 != x1 && ties(x0, x0 - x1)) close = true;
     }
   }
   if constexpr (kChecked) {
