@@ -374,8 +374,9 @@ spmm_status spmm_expert_restore_grad_run(const spmm_experts_desc* d, const void*
   if (spmm_status st = check_experts_desc(d)) return st;
   if (d->rows > 1 && d->grad_stride < d->width) return fail(SPMM_ERR_CONTRACT, "ExpertPlan: rows of grad overlap");
   if (d->rows == 0 || (dy == nullptr && dweights == nullptr)) return SPMM_OK;
-  if (place == nullptr || offsets == nullptr ||
-      (d->width > 0 && (y == nullptr || weights == nullptr || grad == nullptr)))
+  // The kernel reads the weights of rows of no columns too.
+  if (place == nullptr || offsets == nullptr || weights == nullptr ||
+      (d->width > 0 && (y == nullptr || grad == nullptr)))
     return fail(SPMM_ERR_INVALID_ARGUMENT, "ExpertPlan: null device pointer");
   return with_type(d->value_type, [&](auto zero) {
     using T = decltype(zero);
