@@ -254,7 +254,7 @@ __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* 
   constexpr int V = kPiece<T>, kGroups = kThreads / L;
   constexpr bool kChecked = Biased || Grouped, kPacked = Biased || sizeof(T) == 2;
   constexpr uint32_t kIndex = Biased ? kCoarse : kFine, kNone = Biased ? kCoarse : kKeyOfMinusInf;
-  extern __shared__ double lds[];
+  extern __shared__ __align__(16) double lds[];  // read as pieces of 16 bytes too
   // 64-bit values for one row of each wave; the row's own values where there are groups; its choices' ids and scores.
   double* exact = lds + (threadIdx.x >> 6) * a.experts;
   float* all_values = reinterpret_cast<float*>(lds + (kChecked ? kThreads / 64 * a.experts : 0));
