@@ -288,40 +288,43 @@ __global__ __launch_bounds__(kWideThreads) void log_probs_wide(LogArgs a, const 
       t = __builtin_fmaf(e, fmaxf(y, kFloor), t);
     }
   };
-  int64_t p = p0 + tid;
-  const int64_t end = p1 < whole ? p1 : whole;
-  for (; p + (U - 1) * kWideThreads < end; p += U * kWideThreads) {
-    piece_t<T> raw[U];
-    float v[U * V];
+  // take(N, v) for the part's logits, N at a time.
+  auto stream = [&](auto take) {
+    int64_t p = p0 + tid;
+    const int64_t end = p1 < whole ? p1 : whole;
+    for (; p + (U - 1) * kWideThreads < end; p += U * kWideThreads) {
+      piece_t<T> raw[U];
+      float v[U * V];
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = Piece::template load<true>(row, (p + u * kWideThreads) * V, a.classes);
+      for (int u = 0; u < U; ++u) raw[u] = Piece::template load<true>(row, (p + u * kWideThreads) * V, a.classes);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[u * V + j] = static_cast<float>(raw[u][j]);
-    add(std::integral_constant<int, U * V>(), v);
-  }
-  for (; p < p1; p += kWideThreads) {
-    const piece_t<T> raw = Piece::template load<true>(row, p * V, a.classes);
-    const int first = Piece::shift(p * V, a.classes);
-    float v[V];
+        for (int j = 0; j < V; ++j) v[u * V + j] = static_cast<float>(raw[u][j]);
+      take(std::integral_constant<int, U * V>(), v);
+    }
+    for (; p < p1; p += kWideThreads) {
+      const piece_t<T> raw = Piece::template load<true>(row, p * V, a.classes);
+      const int first = Piece::shift(p * V, a.classes);
+      float v[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = j >= first ? static_cast<float>(raw[j]) : -INFINITY;
-    add(std::integral_constant<int, V>(), v);
-  }
+      for (int j = 0; j < V; ++j) v[j] = j >= first ? static_cast<float>(raw[j]) : -INFINITY;
+      take(std::integral_constant<int, V>(), v);
+    }
+  };
+  stream(add);
 
   const Origin o(fmaxf(block_max<W>(m, red[0]), -FLT_MAX));
   if (o.far) {
     s = t = 0.0f;
-    for (p = p0 + tid; p < p1; p += kWideThreads) {
-      const piece_t<T> raw = Piece::load(row, p * V, a.classes);
-      const int first = Piece::shift(p * V, a.classes);
-      for (int j = first; j < V; ++j) {
-        const float y = o(static_cast<float>(raw[j])), e = __builtin_amdgcn_exp2f(y);
+    stream([&](auto N, const float (&v)[decltype(N)::value]) {
+#pragma unroll
+      for (int j = 0; j < decltype(N)::value; ++j) {
+        const float y = o(v[j]), e = __builtin_amdgcn_exp2f(y);
         s += e;
         t = __builtin_fmaf(e, fmaxf(y, kFloor), t);
       }
-    }
+    });
   } else {
     const float shift = origin_of(m) - o.c, f = __builtin_amdgcn_exp2f(shift);
     t = f * __builtin_fmaf(s, fmaxf(shift, kFloor), t);
