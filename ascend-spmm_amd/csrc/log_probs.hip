@@ -99,7 +99,7 @@ __device__ inline uint32_t class_key(float v) { return v != v ? 0u : order_key(v
 
 // The rows that fit the registers of L lanes, I pieces of 16 bytes each.  The
 // next row's loads are under way while a row is summed.  100000 x 47 fp32, top 1:
-// 8.3 us (2.6 TB/s; 5.9 where the logits are in cache), bound by latency.
+// 8.5 us (2.6 TB/s; 5.9 where the logits are in cache), bound by latency.
 template <typename T, int L, int I, bool Narrow>
 __global__ __launch_bounds__(kThreads) void log_probs_rows(LogArgs a, const T* __restrict__ x,
                                                            const void* __restrict__ targets, RowOut out) {
@@ -247,9 +247,10 @@ __device__ inline float origin_shift(const Origin& from, const Origin& to) {
 // the buffer holds (many equal logits), the row is gone through once for each
 // best class instead.
 //
-// 4096 x 131072 bf16, top 4: 196 us (5.5 TB/s), vector units 86% busy: the
-// exponential, and six instructions more for each logit.  One such row: 6.6 us,
-// and 4.4 of the join.
+// 4096 x 131072 bf16, top 4: 197 us (5.5 TB/s), vector units 87% busy: the
+// exponential, and six instructions more for each logit.  One such row: 6.4 us,
+// and 4.5 of the join.  Rows far from zero are read a second time for their sums:
+// 328 us for 168 with top 0.
 constexpr int kCandidates = 1024;
 
 template <typename T>
@@ -488,7 +489,7 @@ __global__ __launch_bounds__(64) void log_probs_join(LogArgs a, const T* __restr
 
 // dlogits, each group of L lanes (256: the work-group) walking the pieces
 // [p0, p1) of a row; rows over blockIdx.x, parts of a row over blockIdx.y.  Bound
-// by memory: 4096 x 131072 bf16 395 us (5.4 TB/s), 100000 x 47 fp32 10.8 (3.5).
+// by memory: 4096 x 131072 bf16 396 us (5.4 TB/s), 100000 x 47 fp32 11.0 (3.4).
 template <typename T, int L, bool Narrow>
 __global__ __launch_bounds__(kThreads) void log_probs_grad(LogArgs a, const T* __restrict__ x,
                                                            const void* __restrict__ targets,

@@ -135,10 +135,12 @@ struct GroupLanes {
 };
 
 // Exact choice of one row by a wave, in 64 bits: for rows whose choice 32 bits do
-// not decide, about one in 2000 of random logits.  It takes the row's logits and
-// leaves ids[0..k) (-1 where no expert is left); values: `experts` doubles of the
-// wave's own LDS.  Returns whether a softmax's values are no numbers, as a NaN or
-// an infinity is among its logits.
+// not decide, about one in 2000 of random logits with biases of the scores' size,
+// and nearly all where a bias is far beyond them or all values are equal (the
+// kernel's 42 us below are 182 then).  It takes the row's logits and leaves
+// ids[0..k) (-1 where no expert is left); values: `experts` doubles of the wave's
+// own LDS.  Returns whether a softmax's values are no numbers, as a NaN or an
+// infinity is among its logits.
 template <typename T>
 __device__ inline bool choose_exactly(const RouteArgs& a, const T* row, const float* bias, double* values,
                                       int32_t* ids) {
@@ -232,8 +234,8 @@ enum class RowShape { kWhole, kMoved, kNarrow };
 // is looked for.
 constexpr uint32_t kFine = 0x1FFF, kCoarse = 0x3FF;
 constexpr float kSteps = 4194300.0f;  // below 2^22
-constexpr float kLargest = 1e38f;
-constexpr float kFar = 0x1p20f;
+constexpr float kLargest = 1e38f;     // of a value in 32 bits: two of them add up to a finite one
+constexpr float kFar = 0x1p20f;       // of a logit that a softmax in 32 bits starts from
 
 // L lanes a row, which hold I pieces of 16 bytes of it each.  The k best are taken
 // one after another.  Without a bias the logits are the keys, and exact.  With one
@@ -242,9 +244,9 @@ constexpr float kFar = 0x1p20f;
 // same logit and bias, or the groups at the border are as close, the row's choice
 // is made again in 64 bits.  In groups without a bias the keys are the logits, and
 // 64 bits decide where two that differ may have the same score.  Bound by vector
-// instructions, most of them of the k rounds.  65536 rows of 256 experts in 8
-// groups, k = 8: 45 us (1.6 TB/s, vector units always busy); all in 64 bits 132, one
-// wave a row 233, value and index apart 113.
+// instructions, most of them of the k rounds.  65536 rows of 256 fp32 logits in 8
+// groups, bias, k = 8: 42 to 45 us (1.6 TB/s, vector units always busy); all in 64
+// bits 132, one wave a row 233, value and index apart 113.
 template <typename T, int L, int I, RowShape Shape, bool Biased, bool Grouped>
 __global__ __launch_bounds__(kThreads, 4) void route_rows(RouteArgs a, const T* __restrict__ logits,
                                                           const float* __restrict__ bias, float* __restrict__ weights,

@@ -424,7 +424,8 @@ void bind_expert_ops(pybind11::module_& m) {
     [width], and a row of zeros for an id outside of the table.  weight [rows,
     width] FP16, BF16 or FP32, ids int32 or int64.  Differentiable with respect
     to weight; its gradient adds in FP32 in the order of the ids, so that it
-    repeats exactly.
+    repeats exactly.  A weight whose rows are not contiguous is copied whole by
+    each call.
     )doc",
         pybind11::arg("weight"), pybind11::arg("ids"), pybind11::arg("scale") = 1.0);
   m.def("log_probs", &log_probs,

@@ -253,8 +253,10 @@ def route(logits, top_k, score="softmax", bias=None, groups=1, top_groups=None, 
     An expert whose logit or bias is -inf is never chosen: where fewer than
     ``top_k`` are left, the rest are -1 with weight 0, which ``ExpertPlan`` leaves
     out.  A NaN counts as greatest, so that it is seen in the weights.  Values are
-    compared in 64 bits.  The weights are differentiable with respect to
-    ``logits``; ``bias`` has no gradient.
+    compared in 64 bits, without a bias and groups the logits themselves.  To
+    switch an expert off, give it a bias of -inf: one far beyond the scores (-1e4)
+    has nearly every row compared in 64 bits indeed, at four times the time.  The
+    weights are differentiable with respect to ``logits``; ``bias`` has no gradient.
     """
     code = _SCORES.get(score)
     if code is None:

@@ -29,7 +29,8 @@ def run(f, x, t, top):
     (dx,) = torch.autograd.grad((logp, entropy), leaf, (a.cuda(), h.cuda()))
     check(dx, want["dx"], want["err_dx"], "dx")
 
-SIZES = [2.0 ** 20 - 1, 2.0 ** 20, 2.0 ** 20 + 3, 3e6, 1e7, 2.0 ** 24, 1e9, 2e9, 3e9, 1e10, 1e15, 1e20, 1e30, 1e37, 3e38]
+SIZES = [2.0 ** 20 - 1, 2.0 ** 20, 2.0 ** 20 + 3, 3e6, 1e7, 2.0 ** 24, 1e9, 2e9, 3e9, 1e10, 1e15, 1e20, 1e30, 1e37,
+         3e38]
 
 
 def targets(rows, n):
@@ -54,7 +55,7 @@ def test_maxima_of_any_size(spmm_npu, n, dtype):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,n", [(1, 40000), (3, 70001), (40, 9000)])
 def test_parts_on_both_sides(spmm_npu, rows, n, dtype):
-    """Maxima of a row's parts and threads around where the origin changes, in parts of one row and of one work-group."""
+    """Maxima of a row's parts and threads around where the origin changes."""
     gen = torch.Generator().manual_seed(n)
     for edge in (2.0 ** 20, -2.0 ** 20):
         spans = torch.randint(-6, 7, (rows, n // 2048 + 1), generator=gen).repeat_interleave(2048, 1)[:, :n]
